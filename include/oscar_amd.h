@@ -508,6 +508,87 @@ int oscar_step_forward(const oscar_mtp_layer* layer, const void* rot_k_operand, 
                        const int32_t* seq_lens, int32_t num_requests, int32_t max_short, void* out_bf16,
                        void* workspace, size_t workspace_size, oscar_stream_t stream);
 
+/* ---------------------------------------------------------------- plain paged caches and positions
+ * What the layers around the INT2 ones need: the position rotation of queries
+ * and keys (which the INT2 write takes rotated as well), and caches that hold
+ * keys and values as they are.  These entries take head sizes other than 256.
+ */
+enum oscar_dtype { OSCAR_BF16 = 0, OSCAR_FP16 = 1, OSCAR_FP32 = 2 };
+
+/* A layer's K and V pages: value f of head h of token t of page p lies at byte
+ * p * stride_page + t * stride_token + h * stride_head + f * size of its type.
+ * Base addresses and strides are multiples of 16 bytes and tokens and heads do
+ * not overlap; the pages of K and V may interleave in one tensor. */
+typedef struct oscar_plain_cache {
+  void* k;
+  void* v;
+  int64_t num_pages;
+  int64_t k_stride_page;
+  int64_t k_stride_token;
+  int64_t k_stride_head;
+  int64_t v_stride_page;
+  int64_t v_stride_token;
+  int64_t v_stride_head;
+  int32_t block_size;
+  int32_t num_kv_heads;
+  int32_t head_size;
+  int32_t dtype; /* oscar_dtype */
+} oscar_plain_cache;
+
+/* How positions turn a head's first rotary_dim features, in pairs: feature j
+ * and j + rotary_dim / 2 (adjacent = 0) or 2j and 2j + 1 (adjacent = 1).  Pair
+ * j turns by row positions[axis of j][token] of the table, whose rows hold the
+ * rotary_dim / 2 cosines, then the sines:
+ *   y1 = x1 cos - x2 sin, y2 = x2 cos + x1 sin.
+ * axes: 1 for text, 3 for the time, height and width of images and video
+ * (at most 4); pair_axis: two bits per pair, pair 0 lowest. */
+typedef struct oscar_rotary {
+  const float* table; /* [positions][rotary_dim] fp32, 16-byte aligned */
+  int64_t positions;
+  int32_t rotary_dim; /* even, 2 .. 256 */
+  int32_t adjacent;
+  int32_t axes;
+  int32_t reserved; /* 0 */
+  uint64_t pair_axis[4];
+} oscar_rotary;
+
+/* Heads of a batch of tokens: value f of head h of token t lies at element
+ * t * token_stride + h * head_stride + f of `data`. */
+typedef struct oscar_heads {
+  void* data;
+  int64_t token_stride;
+  int64_t head_stride;
+  int32_t num_heads; /* 0: none */
+  int32_t reserved;  /* 0 */
+} oscar_heads;
+
+/* Queries and keys turned by their positions (inverse = 1: turned back, which
+ * is also the gradient), in fp32, rounded once to their type.  An output may be
+ * its input (same address and strides); otherwise the two do not overlap.
+ *   positions: int64, axis a of token t at a * position_axis_stride + t.
+ * A token with a position outside [0, rotary->positions) on any axis is left
+ * out: its output rows keep what they held.  dtype: of all rows; head_size any
+ * multiple of 2 from rotary_dim to 256.
+ */
+int oscar_rotate_positions(const oscar_rotary* rotary, const int64_t* positions, int64_t position_axis_stride,
+                           int64_t num_tokens, const oscar_heads* query, const oscar_heads* query_out,
+                           const oscar_heads* key, const oscar_heads* key_out, int32_t head_size, int32_t dtype,
+                           int32_t inverse, oscar_stream_t stream);
+
+/* The write of a step's keys and values to a plain cache, one launch: queries
+ * turned into query_out, keys turned on the way to their slots, values written
+ * as they are.  The cache's type (bf16 or fp16), head size and kv heads are the
+ * rows'.
+ *   slot_mapping: [num_tokens] int64; slots < 0 or at or beyond num_pages *
+ *     block_size are skipped (the token's query is still turned).  Slots of a
+ *     call are distinct: of two tokens that name one, each 16 bytes are either's.
+ * A token with a position outside the table is left out whole.
+ */
+int oscar_append_rotated(const oscar_rotary* rotary, const int64_t* positions, int64_t position_axis_stride,
+                         int64_t num_tokens, const oscar_heads* query, const oscar_heads* query_out,
+                         const oscar_heads* key, const oscar_heads* value, const oscar_plain_cache* cache,
+                         const int64_t* slot_mapping, oscar_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

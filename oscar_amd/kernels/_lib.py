@@ -82,6 +82,9 @@ SIGNATURES = {
                                           _c_p, _c_p, _c_i32, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64,
                                           _c_i64, _c_i64, _c_i32, _c_i32, _c_p, _c_p, _c_i32, _c_i32, _c_i32,
                                           _c_i32, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p]),
+    "oscar_rotate_positions": (_c_i32, [_c_p, _c_p, _c_i64, _c_i64, _c_p, _c_p, _c_p, _c_p, _c_i32, _c_i32, _c_i32,
+                                        _c_p]),
+    "oscar_append_rotated": (_c_i32, [_c_p, _c_p, _c_i64, _c_i64, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p]),
 }
 
 STATUS = {
@@ -121,6 +124,16 @@ def call(name: str, *args) -> None:
     status = getattr(load(), name)(*args)
     if status != 0:
         raise OscarKernelError(f"{name} failed: {STATUS.get(status, status)}")
+
+
+def call_on(device: torch.device, name: str, *args) -> None:
+    """call() with the device's current stream appended, the device made the
+    current one around it where it is another."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        call(name, *args, stream_handle(device))
+    else:
+        with torch.cuda.device(device):
+            call(name, *args, stream_handle(device))
 
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)

@@ -1,0 +1,157 @@
+"""Position rotation of query and key heads (oscar_rotate_positions).
+
+The INT2 write and the attention impl take queries and keys that already carry
+their positions; this is the rotation that puts them there, on one axis for
+text or on several (time, height, width) for image and video prompts.  The
+heads' first ``rotary_dim`` features turn in pairs by the cosines and sines of
+a table (one row per position, cosines first: the layout serving engines keep),
+in fp32 with one rounding; the rest pass through.  The map is orthogonal, so
+``inverse=True`` both takes positions off and gives the gradient.
+"""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import _lib
+
+DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+MAX_ROTARY_DIM = 256
+MAX_AXES = 4
+
+_p, _i32, _i64 = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64
+
+
+class RotaryArgs(ctypes.Structure):
+    """struct oscar_rotary (include/oscar_amd.h)."""
+    _fields_ = [("table", _p), ("positions", _i64), ("rotary_dim", _i32), ("adjacent", _i32), ("axes", _i32),
+                ("reserved", _i32), ("pair_axis", ctypes.c_uint64 * 4)]
+
+
+class HeadsArgs(ctypes.Structure):
+    """struct oscar_heads (include/oscar_amd.h)."""
+    _fields_ = [("data", _p), ("token_stride", _i64), ("head_stride", _i64), ("num_heads", _i32), ("reserved", _i32)]
+
+
+def rotary_table(positions: int, rotary_dim: int, base: float = 10000.0, device=None) -> torch.Tensor:
+    """fp32 [positions, rotary_dim]: the cosines, then the sines, of position *
+    base^(-2j / rotary_dim), from angles in 64 bits (in 32, positions past 2^17
+    would be off by more than the table's own rounding)."""
+    if rotary_dim < 2 or rotary_dim % 2:
+        raise ValueError("rotary_dim must be even")
+    turn = base ** (-torch.arange(0, rotary_dim, 2, dtype=torch.float64) / rotary_dim)
+    angle = torch.arange(positions, dtype=torch.float64)[:, None] * turn
+    return torch.cat((angle.cos(), angle.sin()), -1).to(device=device, dtype=torch.float32)
+
+
+def section_axes(sections, interleaved: bool = False) -> list:
+    """The position axis of every feature pair, from how many pairs each axis
+    has: in blocks (all of the first axis, then the next), or interleaved (the
+    axes in turn until an axis but the first has had its share, the rest on the
+    first)."""
+    sections = [int(s) for s in sections]
+    if not 1 <= len(sections) <= MAX_AXES or any(s < 0 for s in sections) or sum(sections) < 1:
+        raise ValueError(f"sections are 1 to {MAX_AXES} pair counts")
+    pairs, n = sum(sections), len(sections)
+    if not interleaved:
+        return [axis for axis, count in enumerate(sections) for _ in range(count)]
+    axes = [j % n if j // n < sections[j % n] else 0 for j in range(pairs)]
+    if any(axes.count(axis) != count for axis, count in enumerate(sections)):
+        raise ValueError(f"sections {sections} cannot be interleaved: an axis but the first has too many pairs")
+    return axes
+
+
+class Rotary:
+    """A model's position rotation, checked and packed once: the table (fp32
+    [positions, rotary_dim]), whether pairs are adjacent features or halves of
+    the rotary part, and, for positions on several axes, the axis of every pair
+    (``section_axes``)."""
+
+    def __init__(self, table: torch.Tensor, adjacent: bool = False, axes=None):
+        if table.ndim != 2 or table.dtype != torch.float32 or not table.is_contiguous() or table.shape[0] < 1:
+            raise ValueError("the rotary table must be a contiguous fp32 [positions, rotary_dim] tensor")
+        rd = table.shape[1]
+        if rd < 2 or rd % 2 or rd > MAX_ROTARY_DIM:
+            raise ValueError(f"rotary_dim {rd} must be even, 2 to {MAX_ROTARY_DIM}")
+        axes = [0] * (rd // 2) if axes is None else [int(a) for a in axes]
+        if len(axes) != rd // 2 or min(axes) < 0 or max(axes) >= MAX_AXES:
+            raise ValueError(f"axes must name one of {MAX_AXES} position axes for each of the {rd // 2} pairs")
+        self.table = table
+        self.device = table.device
+        self.rotary_dim = rd
+        self.axes = max(axes) + 1
+        words = [0] * 4
+        for j, a in enumerate(axes):
+            words[j // 32] |= a << (2 * (j % 32))
+        self.args = RotaryArgs(table.data_ptr(), table.shape[0], rd, int(adjacent), self.axes, 0,
+                               (ctypes.c_uint64 * 4)(*words))
+        self.address = ctypes.addressof(self.args)
+
+
+def heads(x: torch.Tensor, tokens: int, d: int, dtype, device, what: str) -> HeadsArgs:
+    """The first tokens of x [N, heads, d]."""
+    if x.ndim != 3 or x.shape[0] < tokens or x.shape[2] != d:
+        raise ValueError(f"{what} must be [tokens, heads, {d}] with a row per token")
+    if x.dtype != dtype or x.device != device:
+        raise ValueError(f"{what} must be {dtype} on {device} as the other rows are")
+    token, head, feature = x.stride()
+    if feature != 1:
+        raise ValueError(f"{what}: a head's features must be contiguous")
+    return HeadsArgs(x.data_ptr(), token, head, x.shape[1], 0)
+
+
+def positions_of(positions: torch.Tensor, rotary: Rotary, tokens: int, device) -> tuple[torch.Tensor, int]:
+    """int64 positions [N], or [axes, N], and the stride between axes."""
+    if positions.dtype != torch.int64:
+        if positions.dtype not in (torch.int32, torch.int16):
+            raise ValueError(f"positions must be integers, got {positions.dtype}")
+        positions = positions.to(torch.int64)
+    if positions.device != device or rotary.device != device:
+        raise ValueError("positions and rotary table must be on the rows' device")
+    if positions.ndim == 1:
+        positions = positions[None]
+    if positions.ndim != 2 or positions.shape[0] != rotary.axes or positions.shape[1] < tokens:
+        raise ValueError(f"positions must be [{rotary.axes}, tokens] with an entry per token"
+                         + (" (or [tokens])" if rotary.axes == 1 else ""))
+    if positions.stride(1) != 1 and tokens > 1:
+        positions = positions.contiguous()
+    return positions, positions.stride(0)
+
+
+def rotate(query: torch.Tensor, key: torch.Tensor | None, positions: torch.Tensor, rotary: Rotary, query_out=None,
+           key_out=None, inverse: bool = False):
+    """query [N, Hq, D] and key [N, Hk, D] (or None) turned by their positions
+    (int64 [N], or [axes, N]), bf16, fp16 or fp32 alike, with any token and head
+    strides.  Returns (query_out, key_out): new tensors, or the ones given, which
+    may be the inputs themselves.  A token with a position outside the table is
+    left out: its output rows keep what they held."""
+    dtype, device = query.dtype, query.device
+    if dtype not in DTYPES:
+        raise ValueError(f"rotate takes bf16, fp16 or fp32 rows, got {dtype}")
+    if query.ndim != 3:
+        raise ValueError("query must be [tokens, heads, head size]")
+    n, _, d = query.shape
+    if d < rotary.rotary_dim or d % 2 or d > 256:
+        raise ValueError(f"head size {d} must be even, {rotary.rotary_dim} (rotary_dim) to 256")
+    q = heads(query, n, d, dtype, device, "query")
+    if query_out is None:
+        query_out = torch.empty(query.shape, dtype=dtype, device=device)
+    qo = heads(query_out, n, d, dtype, device, "query_out")
+    k = ko = None
+    if key is not None:
+        k = heads(key, n, d, dtype, device, "key")
+        if key_out is None:
+            key_out = torch.empty((n, *key.shape[1:]), dtype=dtype, device=device)
+        ko = heads(key_out, n, d, dtype, device, "key_out")
+    if qo.num_heads != q.num_heads or (k is not None and ko.num_heads != k.num_heads):
+        raise ValueError("outputs must have their inputs' heads")
+    positions, axis_stride = positions_of(positions, rotary, n, device)
+    if not query.is_cuda:
+        raise ValueError("OSCAR kernels take device tensors")
+    if n:
+        ref = ctypes.byref
+        _lib.call_on(device, "oscar_rotate_positions", rotary.address, positions.data_ptr(), axis_stride, n, ref(q),
+                     ref(qo), None if k is None else ref(k), None if ko is None else ref(ko), d, DTYPES[dtype],
+                     int(inverse))
+    return query_out, key_out if key is not None else None

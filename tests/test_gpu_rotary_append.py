@@ -1,0 +1,241 @@
+"""Position rotation and the plain cache's write on the GPU, against the formula
+in 64 bits.
+
+Tolerance of a turned value y = x1 c - x2 s (the table's entries taken as they
+are): three fp32 roundings of terms no larger than |x1| + |x2|, then one
+rounding to the type: 2^-23 (|x1| + |x2|) + eps / 2 |y|, and half of the type's
+smallest step.  Values that pass through, and caches' untouched slots, are equal
+bit for bit."""
+import pytest
+import torch
+
+from oscar_amd.kernels import append, rotary
+
+pytestmark = pytest.mark.gpu
+TYPES = [torch.bfloat16, torch.float16, torch.float32]
+
+
+def turned(x, positions, turn, adjacent, axes, inverse=False):
+    """(y, bound) in 64 bits of x [N, H, D] on the CPU; positions [axes, N]."""
+    rd = turn.rotary_dim
+    half = rd // 2
+    x64, table = x.double().cpu(), turn.table.double().cpu()
+    pos = positions.cpu().reshape(-1, x.shape[0])
+    y, reach = x64.clone(), torch.zeros_like(x64)
+    for j in range(half):
+        row = table[pos[axes[j] if axes is not None else 0]]
+        c, s = row[:, j, None], row[:, half + j, None] * (-1 if inverse else 1)
+        a, b = (2 * j, 2 * j + 1) if adjacent else (j, j + half)
+        y[..., a], y[..., b] = x64[..., a] * c - x64[..., b] * s, x64[..., b] * c + x64[..., a] * s
+        reach[..., a] = reach[..., b] = x64[..., a].abs() + x64[..., b].abs()
+    info = torch.finfo(x.dtype)
+    step = info.smallest_normal * info.eps / 2
+    bound = torch.where(reach > 0, 2.0 ** -23 * reach + info.eps / 2 * y.abs() + step, 0.0)
+    return y, bound
+
+
+def close(got, want):
+    y, bound = want
+    off = (got.double().cpu() - y).abs() - bound
+    assert off.max().item() <= 0, f"off by {off.max().item():.3e} more than the bound"
+
+
+def rows(g, n, hq, hk, d, dtype, fused):
+    x = torch.randn(n, hq + 2 * hk, d, generator=g, device="cuda:0") * 3
+    parts = x.to(dtype).split((hq, hk, hk), 1)
+    return parts if fused else [p.contiguous() for p in parts]
+
+
+# (head size, rotary_dim): 16-byte pieces and, where halves or heads are no
+# multiple of them, single pairs
+SHAPES = [(256, 64), (128, 128), (64, 32), (96, 48), (80, 80), (64, 24), (66, 6), (2, 2), (256, 256)]
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("d, rd", SHAPES)
+@pytest.mark.parametrize("adjacent", [False, True])
+def test_rotate(device, dtype, d, rd, adjacent):
+    g = torch.Generator(device=device).manual_seed(d * rd + adjacent)
+    for n, hq, hk, fused, axes in ((1, 6, 1, False, None), (5, 3, 2, True, None), (1037, 2, 1, True, None),
+                                   (33, 12, 4, False, 3)):
+        pair_axes = None if axes is None else [int(a) for a in torch.randint(0, 3, (rd // 2,))]
+        if pair_axes is not None:
+            pair_axes[0] = 2
+        turn = rotary.Rotary(rotary.rotary_table(5000, rd, device=device), adjacent, pair_axes)
+        q, k, _ = rows(g, n, hq, hk, d, dtype, fused)
+        pos = torch.randint(0, 5000, (turn.axes, n), generator=g, device=device)
+        for inverse in (False, True):
+            got = rotary.rotate(q, k, pos[0] if turn.axes == 1 else pos, turn, inverse=inverse)
+            close(got[0], turned(q, pos, turn, adjacent, pair_axes, inverse))
+            close(got[1], turned(k, pos, turn, adjacent, pair_axes, inverse))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_in_place_equals_new_tensors(device, dtype):
+    g = torch.Generator(device=device).manual_seed(3)
+    for d, rd, adjacent in ((256, 64, False), (64, 64, True), (66, 6, False), (66, 6, True)):
+        turn = rotary.Rotary(rotary.rotary_table(300, rd, device=device), adjacent)
+        q, k, _ = rows(g, 211, 5, 2, d, dtype, True)
+        pos = torch.arange(211, device=device)
+        want_q, want_k = rotary.rotate(q, k, pos, turn)
+        got_q, got_k = rotary.rotate(q, k, pos, turn, query_out=q, key_out=k)
+        assert got_q is q and got_k is k and torch.equal(q, want_q) and torch.equal(k, want_k)
+
+
+def test_gradient_is_the_inverse(device):
+    """d/dx of sum(g . rotate(x)): the formula's, autograd's of the plain form in
+    64 bits, and central differences of the kernel in fp32."""
+    g = torch.Generator(device=device).manual_seed(4)
+    turn = rotary.Rotary(rotary.rotary_table(100, 32, device=device), axes=rotary.section_axes((6, 5, 5)))
+    pos = torch.randint(0, 100, (3, 7), generator=g, device=device)
+    x = torch.randn(7, 2, 48, generator=g, device=device)
+    w = torch.randn(7, 2, 48, generator=g, device=device)
+    grad, _ = rotary.rotate(w, None, pos, turn, inverse=True)
+    axes = rotary.section_axes((6, 5, 5))
+    close(grad, turned(w, pos, turn, False, axes, inverse=True))
+    leaf = x.double().cpu().requires_grad_()
+    table = turn.table.double().cpu()
+    index = torch.arange(16)
+    token = pos.cpu()[torch.tensor(axes)].t()
+    c, s = table[token, index][:, None], table[token, index + 16][:, None]
+    a, b = leaf[..., :16], leaf[..., 16:32]
+    y = torch.cat((a * c - b * s, b * c + a * s, leaf[..., 32:]), -1)
+    (y * w.double().cpu()).sum().backward()
+    reach = torch.ones_like(leaf) * 2.0 ** -22 * w.abs().max().item() * 2
+    assert ((grad.double().cpu() - leaf.grad).abs() <= reach).all()
+    # the map is linear, so a difference of step 1 has only the sums' roundings:
+    # 7 * 2 * 48 terms below 4 * 4 = 16 each, in fp32 products
+    for at in ((0, 0, 0), (3, 1, 17), (6, 0, 31), (2, 1, 40)):
+        up, down = x.clone(), x.clone()
+        up[at] += 0.5
+        down[at] -= 0.5
+        diff = sum(sign * (rotary.rotate(z, None, pos, turn)[0].double() * w.double()).sum().item()
+                   for sign, z in ((1, up), (-1, down)))
+        assert diff == pytest.approx(grad[at].item(), abs=4 * 16 * 2.0 ** -23)
+
+
+def test_positions_outside_the_table_leave_rows_alone(device):
+    turn = rotary.Rotary(rotary.rotary_table(10, 32, device=device), axes=[0, 1] * 8)
+    pos = torch.tensor([[0, 9, 10, 3, -1, 2], [0, 9, 3, 1 << 40, 4, 9]], device=device)
+    q = torch.randn(6, 3, 64, device=device).bfloat16()
+    out = torch.full_like(q, 7.0)
+    rotary.rotate(q, None, pos, turn, query_out=out)
+    bad = torch.tensor([2, 3, 4])
+    assert (out[bad] == 7.0).all()
+    good = torch.tensor([0, 1, 5])
+    close(out[good], turned(q[good], pos[:, good], turn, False, [0, 1] * 8))
+
+
+@pytest.mark.parametrize("dtype", TYPES[:2], ids=str)
+@pytest.mark.parametrize("layout", ["apart", "joint", "heads_first", "stacked"])
+@pytest.mark.parametrize("n, hq, hk, d, rd, page", [(1, 6, 1, 256, 64, 128), (4, 6, 1, 256, 64, 128),
+                                                   (301, 8, 8, 64, 64, 16), (77, 12, 2, 128, 96, 48),
+                                                   (50, 3, 3, 72, 12, 32), (1500, 7, 1, 128, 128, 1)])
+def test_append(device, dtype, layout, n, hq, hk, d, rd, page):
+    g = torch.Generator(device=device).manual_seed(n + d)
+    pages = n // page + 5
+    if layout == "joint":
+        both = torch.randn(pages, 2, page, hk, d, generator=g, device=device).to(dtype)
+        caches = [both[:, 0], both[:, 1]]
+    elif layout == "heads_first":
+        caches = [torch.randn(pages, hk, page, d, generator=g, device=device).to(dtype).transpose(1, 2)
+                  for _ in range(2)]
+    elif layout == "stacked":
+        caches = list(torch.randn(2, pages, page, hk, d, generator=g, device=device).to(dtype))
+    else:
+        caches = [torch.randn(pages, page, hk, d, generator=g, device=device).to(dtype) for _ in range(2)]
+    before = [c.clone() for c in caches]
+    turn = rotary.Rotary(rotary.rotary_table(4096, rd, device=device), adjacent=layout == "joint")
+    q, k, v = rows(g, n + 3, hq, hk, d, dtype, layout != "apart")       # three padding rows
+    pos = torch.randint(0, 4096, (n,), generator=g, device=device)
+    slots = torch.randperm(pages * page, generator=g, device=device)[:n]
+    if n > 4:
+        slots[::7] = -1
+        slots[1], slots[2], slots[3] = pages * page, (1 << 40) + 5, -(1 << 40)
+    got = append.append_rotated(q, k, v, pos, turn, append.PagedCache(*caches), slots)
+    assert got.shape == (n, hq, d)
+    close(got, turned(q[:n], pos, turn, turn.args.adjacent, None))
+    live = (slots >= 0) & (slots < pages * page)
+    at = slots[live]
+    keys = caches[0].reshape(-1, hk, d)[at]
+    y, bound = turned(k[:n], pos, turn, turn.args.adjacent, None)
+    close(keys, (y[live.cpu()], bound[live.cpu()]))
+    assert torch.equal(caches[1].reshape(-1, hk, d)[at], v[:n][live])
+    rest = torch.ones(pages * page, dtype=torch.bool, device=device)
+    rest[at] = False
+    for c, b in zip(caches, before):
+        assert torch.equal(c.reshape(-1, hk, d)[rest], b.reshape(-1, hk, d)[rest])
+
+
+def test_append_leaves_out_tokens_without_a_position(device):
+    turn = rotary.Rotary(rotary.rotary_table(10, 64, device=device))
+    cache = append.PagedCache(*(torch.zeros(2, 16, 1, 64, device=device, dtype=torch.bfloat16) for _ in range(2)))
+    x = torch.ones(4, 1, 64, device=device, dtype=torch.bfloat16)
+    out = torch.full_like(x, 5.0)
+    append.append_rotated(x, x, x, torch.tensor([1, 10, -1, 9], device=device), turn, cache,
+                          torch.tensor([3, 4, 5, 6], device=device), query_out=out)
+    written = cache.v_cache.view(32, 64)[:, 0] != 0
+    assert written.nonzero().flatten().tolist() == [3, 6]
+    assert (cache.k_cache.view(32, 64)[4:6] == 0).all() and (out[1:3] == 5.0).all() and (out[0] != 5.0).any()
+
+
+def test_append_without_query_and_without_tokens(device):
+    turn = rotary.Rotary(rotary.rotary_table(10, 64, device=device))
+    cache = append.PagedCache(*(torch.zeros(2, 16, 1, 64, device=device, dtype=torch.float16) for _ in range(2)))
+    x = torch.ones(4, 1, 64, device=device, dtype=torch.float16)
+    none = torch.zeros(0, dtype=torch.int64, device=device)
+    assert append.append_rotated(None, x, x, none, turn, cache, none) is None
+    assert append.append_rotated(x, x, x, none, turn, cache, none).shape == (0, 1, 64)
+    assert (cache.v_cache == 0).all()
+    # int32 positions and slots, every other entry of longer tensors
+    pos = torch.arange(8, device=device, dtype=torch.int32)[::2]
+    append.append_rotated(None, x, x, pos, turn, cache, torch.arange(8, device=device, dtype=torch.int32)[::2])
+    assert (cache.v_cache.view(32, 64)[:8:2] == 1).all() and (cache.v_cache.view(32, 64)[1:8:2] == 0).all()
+    assert rotary.rotate(x[:0], None, none, turn)[0].shape == (0, 1, 64)
+
+
+def test_offsets_past_32_bits(device):
+    """Pages more than 2^32 bytes apart (one tensor of 6 GB of which two pages are used)."""
+    base = torch.empty(3 << 30, dtype=torch.bfloat16, device=device)
+    page = 16 * 64
+    pages = base.numel() // page
+    caches = [base.view(pages, 16, 1, 64), torch.zeros(8, 16, 1, 64, dtype=torch.bfloat16, device=device)]
+    with pytest.raises(ValueError, match="share"):
+        append.PagedCache(*caches)
+    joint = base.view(pages // 2, 2, 16, 1, 64)
+    cache = append.PagedCache(joint[:, 0], joint[:, 1])
+    turn = rotary.Rotary(rotary.rotary_table(10, 64, device=device))
+    x = torch.randn(2, 1, 64, device=device).bfloat16()
+    slots = torch.tensor([0, pages // 2 * 16 - 1], device=device)
+    joint[0], joint[-1] = 0, 0
+    append.append_rotated(None, x, x, torch.tensor([0, 0], device=device), turn, cache, slots)
+    assert torch.equal(joint[0, 1, 0], x[0]) and torch.equal(joint[-1, 1, 15], x[1])
+    assert torch.equal(joint[-1, 0, 15], x[1])          # position 0 turns nothing
+
+
+def test_streams_and_replays(device):
+    g = torch.Generator(device=device).manual_seed(9)
+    turn = rotary.Rotary(rotary.rotary_table(600, 64, device=device))
+    caches = [torch.zeros(40, 16, 2, 64, device=device, dtype=torch.bfloat16) for _ in range(2)]
+    cache = append.PagedCache(*caches)
+    q, k, v = rows(g, 500, 4, 2, 64, torch.bfloat16, True)
+    pos = torch.arange(500, device=device)
+    slots = torch.randperm(640, generator=g, device=device)[:500]
+    want = append.append_rotated(q, k, v, pos, turn, cache, slots)
+    want_caches = [c.clone() for c in caches]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = append.append_rotated(q, k, v, pos, turn, cache, slots)
+    side.synchronize()
+    assert torch.equal(got, want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = append.append_rotated(q, k, v, pos, turn, cache, slots)
+    for _ in range(3):
+        for c in caches:
+            c.zero_()
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and all(torch.equal(a, b) for a, b in zip(caches, want_caches))

@@ -1,0 +1,251 @@
+"""Position rotation and the plain cache's write without a GPU: tables, axis
+layouts, cache geometry, and what is refused before anything is launched."""
+import ctypes
+import math
+
+import pytest
+import torch
+
+from oscar_amd.kernels import _lib, append, rotary
+
+
+def test_table_holds_cosines_then_sines_of_64_bit_angles():
+    table = rotary.rotary_table(70001, 8, base=100.0)
+    assert table.shape == (70001, 8) and table.dtype == torch.float32
+    for pos in (0, 1, 777, 70000):
+        for j in range(4):
+            angle = pos * 100.0 ** (-2 * j / 8)
+            assert table[pos, j].item() == pytest.approx(math.cos(angle), abs=2.0 ** -24)
+            assert table[pos, 4 + j].item() == pytest.approx(math.sin(angle), abs=2.0 ** -24)
+    with pytest.raises(ValueError, match="even"):
+        rotary.rotary_table(4, 7)
+
+
+def test_section_axes():
+    assert rotary.section_axes((2, 1, 1)) == [0, 0, 1, 2]
+    assert rotary.section_axes((4, 2, 2), interleaved=True) == [0, 1, 2, 0, 1, 2, 0, 0]
+    assert rotary.section_axes((11, 11, 10), interleaved=True)[-3:] == [2, 0, 1]
+    assert rotary.section_axes((5,)) == [0] * 5
+    for bad in ((), (1, 2, 3, 4, 5), (0, 0), (3, -1)):
+        with pytest.raises(ValueError, match="sections"):
+            rotary.section_axes(bad)
+    with pytest.raises(ValueError, match="interleaved"):
+        rotary.section_axes((1, 5, 2), interleaved=True)
+
+
+def test_rotary_packs_two_bits_a_pair():
+    turn = rotary.Rotary(rotary.rotary_table(4, 128), axes=rotary.section_axes((16, 24, 24)))
+    got = [(turn.args.pair_axis[j // 32] >> (2 * (j % 32))) & 3 for j in range(64)]
+    assert got == [0] * 16 + [1] * 24 + [2] * 24 and turn.axes == 3
+    assert rotary.Rotary(rotary.rotary_table(4, 128)).axes == 1
+
+
+@pytest.mark.parametrize("table, axes", [
+    (torch.zeros(4), None), (torch.zeros(4, 7), None), (torch.zeros(4, 258), None), (torch.zeros(0, 8), None),
+    (torch.zeros(4, 8, dtype=torch.float16), None), (torch.zeros(8, 4).t(), None),
+    (torch.zeros(4, 8), [0, 1]), (torch.zeros(4, 8), [0, 1, 2, 4]), (torch.zeros(4, 8), [0, 0, -1, 0])])
+def test_rotary_refuses(table, axes):
+    with pytest.raises(ValueError):
+        rotary.Rotary(table, axes=axes)
+
+
+def _cache(shape=(3, 16, 2, 64), dtype=torch.bfloat16):
+    return torch.zeros(shape, dtype=dtype)
+
+
+def test_cache_geometries():
+    c = append.PagedCache(_cache(), _cache())
+    assert (c.args.k_stride_page, c.args.k_stride_token, c.args.k_stride_head) == (16 * 256, 256, 128)
+    both = _cache((3, 2, 16, 2, 64))
+    c = append.PagedCache(both[:, 0], both[:, 1])
+    assert c.args.k_stride_page == 2 * 16 * 256 and c.args.v == both.data_ptr() + 16 * 256
+    heads_first = _cache((3, 2, 16, 64)).transpose(1, 2)
+    c = append.PagedCache(heads_first, heads_first)
+    assert (c.args.k_stride_token, c.args.k_stride_head) == (128, 16 * 128)
+    one = append.PagedCache(_cache((1, 1, 1, 64)), _cache((1, 1, 1, 64)))
+    assert min(one.args.k_stride_page, one.args.k_stride_token, one.args.k_stride_head) >= 128
+
+
+@pytest.mark.parametrize("k, v, match", [
+    (_cache(), _cache((3, 16, 2, 128)), "share"), (_cache()[0], _cache()[0], "share"),
+    (_cache(), _cache(dtype=torch.float16), "alike"),
+    (_cache(dtype=torch.float32), _cache(dtype=torch.float32), "bf16 or fp16"),
+    (_cache((3, 16, 2, 60)), _cache((3, 16, 2, 60)), "multiple of 8"),
+    (_cache((3, 16, 2, 264)), _cache((3, 16, 2, 264)), "at most 256"),
+    (_cache((3, 16, 2, 128))[..., ::2], _cache(), "16 bytes"),
+    (_cache((3, 16, 2, 65))[..., 1:], _cache(), "16 bytes"),
+    (_cache((3, 1, 2, 64)).expand(3, 16, 2, 64), _cache(), "16 bytes"),
+    (_cache((1, 16, 2, 64)).expand(3, 16, 2, 64), _cache(), "16 bytes"),
+    (torch.zeros(40000, dtype=torch.bfloat16).as_strided((3, 16, 2, 64), (4096, 64, 64, 1)), _cache(), "overlap"),
+    (torch.zeros(40000, dtype=torch.bfloat16).as_strided((3, 16, 2, 64), (1024, 128, 64, 1)), _cache(), "overlap"),
+])
+def test_cache_refuses(k, v, match):
+    with pytest.raises(ValueError, match=match):
+        append.PagedCache(k, v)
+
+
+def _rotate_args(**over):
+    args = dict(query=torch.zeros(5, 4, 64), key=torch.zeros(5, 2, 64), positions=torch.zeros(5, dtype=torch.int64),
+                rotary=rotary.Rotary(rotary.rotary_table(8, 32)))
+    args.update(over)
+    return args
+
+
+@pytest.mark.parametrize("over, match", [
+    ({"query": torch.zeros(5, 4, 64, dtype=torch.float64)}, "bf16, fp16 or fp32"),
+    ({"query": torch.zeros(5, 256)}, "heads"),
+    ({"query": torch.zeros(5, 4, 30), "key": None}, "head size"),
+    ({"query": torch.zeros(5, 4, 258), "key": None}, "head size"),
+    ({"query": torch.zeros(5, 4, 128)[..., ::2]}, "contiguous"),
+    ({"key": torch.zeros(4, 2, 64)}, "key"), ({"key": torch.zeros(5, 2, 128)}, "key"),
+    ({"key": torch.zeros(5, 2, 64, dtype=torch.float16)}, "key"),
+    ({"query_out": torch.zeros(5, 3, 64)}, "heads"), ({"query_out": torch.zeros(4, 4, 64)}, "query_out"),
+    ({"key_out": torch.zeros(5, 1, 64)}, "heads"),
+    ({"positions": torch.zeros(4, dtype=torch.int64)}, "positions"),
+    ({"positions": torch.zeros(5)}, "integers"), ({"positions": torch.zeros(3, 5, dtype=torch.int64)}, "positions"),
+    ({"positions": torch.zeros(5, dtype=torch.int64), "rotary": rotary.Rotary(rotary.rotary_table(8, 32),
+                                                                              axes=[0, 1] * 8)}, "positions"),
+    ({}, "device tensors"),
+])
+def test_rotate_refuses(over, match):
+    with pytest.raises(ValueError, match=match):
+        rotary.rotate(**_rotate_args(**over))
+
+
+def _append_args(**over):
+    bf = torch.bfloat16
+    args = dict(query=torch.zeros(5, 4, 64, dtype=bf), key=torch.zeros(5, 2, 64, dtype=bf),
+                value=torch.zeros(5, 2, 64, dtype=bf), positions=torch.zeros(5, dtype=torch.int64),
+                rotary=rotary.Rotary(rotary.rotary_table(8, 32)), cache=append.PagedCache(_cache(), _cache()),
+                slot_mapping=torch.zeros(5, dtype=torch.int64))
+    args.update(over)
+    return args
+
+
+@pytest.mark.parametrize("over, match", [
+    ({"slot_mapping": torch.zeros(5, 1, dtype=torch.int64)}, "slot_mapping"),
+    ({"slot_mapping": torch.zeros(5)}, "integers"),
+    ({"slot_mapping": torch.zeros(6, dtype=torch.int64)}, "key"),
+    ({"key": torch.zeros(5, 2, 64)}, "key"), ({"value": torch.zeros(5, 2, 64, dtype=torch.float16)}, "value"),
+    ({"key": torch.zeros(5, 1, 64, dtype=torch.bfloat16)}, "2 heads"),
+    ({"value": torch.zeros(5, 3, 64, dtype=torch.bfloat16)}, "2 heads"),
+    ({"query": torch.zeros(4, 4, 64, dtype=torch.bfloat16)}, "query"),
+    ({"query_out": torch.zeros(5, 5, 64, dtype=torch.bfloat16)}, "query's heads"),
+    ({"positions": torch.zeros(4, dtype=torch.int64)}, "positions"),
+    ({"rotary": rotary.Rotary(rotary.rotary_table(8, 128))}, "rotary_dim"),
+    ({}, "device tensors"),
+])
+def test_append_refuses(over, match):
+    with pytest.raises(ValueError, match=match):
+        append.append_rotated(**_append_args(**over))
+
+
+# ------------------------------------------------------------------ the C entries' own checks (nothing is launched)
+FAKE = 1 << 20
+
+
+def _c_rotary(**over):
+    args = rotary.RotaryArgs(FAKE, 8, 32, 0, 1, 0, (ctypes.c_uint64 * 4)())
+    for name, value in over.items():
+        if name == "pair_axis":
+            args.pair_axis[0] = value
+        else:
+            setattr(args, name, value)
+    return args
+
+
+def _c_heads(n, data=FAKE):
+    return rotary.HeadsArgs(data, n * 64, 64, n, 0)
+
+
+def _c_cache(**over):
+    args = append.PlainCacheArgs(FAKE, FAKE, 3, 4096, 256, 128, 4096, 256, 128, 16, 2, 64, 0)
+    for name, value in over.items():
+        setattr(args, name, value)
+    return args
+
+
+def _status(fn, *args):
+    keep = [ctypes.byref(a) if isinstance(a, ctypes.Structure) else a for a in args]
+    return getattr(_lib.load(), fn)(*keep)
+
+
+INVALID, HEAD, GEOMETRY = -1, -2, -5
+
+
+@pytest.mark.parametrize("over, head_size, dtype, status", [
+    ({"rotary_dim": 31}, 64, 0, INVALID), ({"rotary_dim": 0}, 64, 0, INVALID), ({"rotary_dim": 258}, 256, 0, INVALID),
+    ({"axes": 0}, 64, 0, INVALID), ({"axes": 5}, 64, 0, INVALID), ({"positions": 0}, 64, 0, INVALID),
+    ({"table": None}, 64, 0, INVALID), ({"pair_axis": 4}, 64, 0, INVALID), ({}, 64, 3, INVALID), ({}, 64, -1, INVALID),
+    ({}, 30, 0, HEAD), ({}, 258, 0, HEAD), ({}, 63, 0, HEAD)])
+def test_rotate_entry_refuses(over, head_size, dtype, status):
+    q = _c_heads(2)
+    assert _status("oscar_rotate_positions", _c_rotary(**over), FAKE, 0, 5, q, q, None, None, head_size, dtype, 0,
+                   None) == status
+
+
+def test_rotate_entry_refuses_rows():
+    q, r = _c_heads(2), _c_rotary()
+    for query, out, key, key_out in ((q, None, None, None), (q, _c_heads(3), None, None), (q, q, q, None),
+                                     (_c_heads(2, None), q, None, None), (q, _c_heads(2, None), None, None),
+                                     (_c_heads(-1), _c_heads(-1), None, None)):
+        assert _status("oscar_rotate_positions", r, FAKE, 0, 5, query, out, key, key_out, 64, 0, 0, None) == INVALID
+    assert _status("oscar_rotate_positions", r, None, 0, 5, q, q, None, None, 64, 0, 0, None) == INVALID
+    assert _status("oscar_rotate_positions", r, FAKE, 0, -1, q, q, None, None, 64, 0, 0, None) == INVALID
+    assert _status("oscar_rotate_positions", None, FAKE, 0, 5, q, q, None, None, 64, 0, 0, None) == INVALID
+    assert _status("oscar_rotate_positions", r, FAKE, 0, 0, q, q, None, None, 64, 0, 0, None) == 0
+    assert _status("oscar_rotate_positions", r, FAKE, 0, 5, None, None, None, None, 64, 0, 0, None) == 0
+
+
+@pytest.mark.parametrize("over, status", [
+    ({"k": None}, INVALID), ({"num_pages": 0}, INVALID), ({"block_size": 0}, INVALID), ({"num_kv_heads": 0}, INVALID),
+    ({"dtype": 2}, INVALID), ({"head_size": 60}, HEAD), ({"head_size": 264}, HEAD), ({"k": FAKE + 8}, GEOMETRY),
+    ({"k_stride_token": 264}, GEOMETRY), ({"v_stride_head": 64}, GEOMETRY), ({"k_stride_token": 128}, GEOMETRY),
+    ({"v_stride_page": 2048}, GEOMETRY), ({"v_stride_page": 1 << 33, "v_stride_token": 1 << 28}, GEOMETRY),
+    ({"num_kv_heads": 3}, INVALID)])
+def test_append_entry_refuses(over, status):
+    h = _c_heads(2)
+    if over == {"num_kv_heads": 3}:
+        over = {"num_kv_heads": 3, "k_stride_token": 384, "v_stride_token": 384, "k_stride_page": 6144,
+                "v_stride_page": 6144}
+    assert _status("oscar_append_rotated", _c_rotary(), FAKE, 0, 5, None, None, h, h, _c_cache(**over), FAKE,
+                   None) == status
+
+
+def test_append_entry_refuses_rows():
+    h, c, r = _c_heads(2), _c_cache(), _c_rotary()
+    for query, out, key, value, slots in ((None, None, None, h, FAKE), (None, None, h, None, FAKE),
+                                          (None, None, h, h, None), (h, None, h, h, FAKE),
+                                          (None, None, _c_heads(1), h, FAKE)):
+        assert _status("oscar_append_rotated", r, FAKE, 0, 5, query, out, key, value, c, slots, None) == INVALID
+    assert _status("oscar_append_rotated", r, FAKE, 0, 5, None, None, h, h, None, FAKE, None) == INVALID
+    assert _status("oscar_append_rotated", _c_rotary(rotary_dim=128), FAKE, 0, 5, None, None, h, h, c, FAKE,
+                   None) == HEAD
+    assert _status("oscar_append_rotated", r, FAKE, 0, 0, None, None, h, h, c, None, None) == 0
+
+
+def test_argument_structs_match_the_header(tmp_path):
+    import re
+    import subprocess
+    from pathlib import Path
+
+    header = Path(__file__).resolve().parents[1] / "include" / "oscar_amd.h"
+    structs = {"oscar_rotary": rotary.RotaryArgs, "oscar_heads": rotary.HeadsArgs,
+               "oscar_plain_cache": append.PlainCacheArgs}
+    text = re.sub(r"/\*.*?\*/", "", header.read_text(), flags=re.S)
+    lines = ['#include <stdio.h>', '#include <stddef.h>', '#include "oscar_amd.h"', "int main(void) {"]
+    want = []
+    for cname, cls in structs.items():
+        body = re.search(r"typedef struct " + cname + r" \{(.*?)\} " + cname + ";", text, flags=re.S).group(1)
+        declared = [re.findall(r"\w+", d.split("[")[0])[-1] for d in body.split(";") if d.strip()]
+        assert declared == [f for f, _ in cls._fields_], cname
+        lines.append(f'  printf("%zu\\n", sizeof({cname}));')
+        want.append(ctypes.sizeof(cls))
+        for field, _ in cls._fields_:
+            lines.append(f'  printf("%zu\\n", offsetof({cname}, {field}));')
+            want.append(getattr(cls, field).offset)
+    (tmp_path / "layout.c").write_text("\n".join(lines + ["  return 0;", "}"]) + "\n")
+    subprocess.run(["gcc", "-std=c99", "-Wall", "-Werror", "-I", str(header.parent), str(tmp_path / "layout.c"), "-o",
+                    str(tmp_path / "layout")], check=True)
+    got = subprocess.run([str(tmp_path / "layout")], check=True, capture_output=True, text=True).stdout.split()
+    assert [int(x) for x in got] == want
