@@ -589,6 +589,49 @@ int oscar_append_rotated(const oscar_rotary* rotary, const int64_t* positions, i
                          const oscar_heads* key, const oscar_heads* value, const oscar_plain_cache* cache,
                          const int64_t* slot_mapping, oscar_stream_t stream);
 
+/* ---------------------------------------------------------------- chunk attention over a plain cache
+ * Causal attention of a step's new tokens over a plain paged cache that holds
+ * their keys and values already (oscar_append_rotated's).  Token j of request
+ * i's n = qsl[i + 1] - qsl[i], at position p = seq_lens[i] - n + j, sees the
+ * keys at positions max(0, p - window + 1) .. p (window 0: from 0 on).
+ *
+ * oscar_chunk_plan cuts a step's work into items, on the host, for every layer
+ * of the step whose cache has this geometry (its pointers are not used): call
+ * it with items = NULL for the sizes in *step, then with a host buffer of
+ * items_size bytes, which the caller copies to the device.  query_start_loc
+ * [num_requests + 1] and seq_lens [num_requests] are HOST arrays.
+ *
+ * oscar_chunk_attention runs a plan:
+ *   items: the device copy, 16-byte aligned; block_table [num_requests]
+ *     [block_table_stride] int32, of whose rows the first table_cols entries at
+ *     most are read: keys on pages outside [0, num_pages) are left out, like
+ *     keys that a row does not see, and a row that sees none becomes zeros;
+ *   query, out: 16-byte aligned rows of the cache's type (strides multiples of 8)
+ *     from token 0 of the step on; rows of no request are left as they were;
+ *   workspace: workspace_size bytes, 16-byte aligned; scale: positive.
+ * head_size 64, 128 or 256; block_size a multiple of 16.
+ */
+typedef struct oscar_chunk_step {
+  int32_t num_requests;
+  int32_t num_tokens;
+  int32_t num_heads;
+  int32_t window;
+  int32_t table_cols;
+  int32_t narrow;
+  int32_t joins;
+  int32_t reserved;
+  int64_t items_size;
+  int64_t workspace_size;
+} oscar_chunk_step;
+
+int oscar_chunk_plan(const int32_t* query_start_loc, const int32_t* seq_lens, int32_t num_requests,
+                     int32_t num_heads, int32_t window, const oscar_plain_cache* cache, void* items,
+                     size_t items_size, oscar_chunk_step* step);
+int oscar_chunk_attention(const oscar_chunk_step* step, const void* items, const int32_t* block_table,
+                          int64_t block_table_stride, const oscar_plain_cache* cache, const oscar_heads* query,
+                          const oscar_heads* out, float scale, void* workspace, size_t workspace_size,
+                          oscar_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

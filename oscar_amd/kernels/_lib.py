@@ -85,6 +85,8 @@ SIGNATURES = {
     "oscar_rotate_positions": (_c_i32, [_c_p, _c_p, _c_i64, _c_i64, _c_p, _c_p, _c_p, _c_p, _c_i32, _c_i32, _c_i32,
                                         _c_p]),
     "oscar_append_rotated": (_c_i32, [_c_p, _c_p, _c_i64, _c_i64, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p]),
+    "oscar_chunk_plan": (_c_i32, [_c_p, _c_p, _c_i32, _c_i32, _c_i32, _c_p, _c_p, _c_sz, _c_p]),
+    "oscar_chunk_attention": (_c_i32, [_c_p, _c_p, _c_p, _c_i64, _c_p, _c_p, _c_p, _c_f32, _c_p, _c_sz, _c_p]),
 }
 
 STATUS = {

@@ -1,0 +1,127 @@
+"""Attention of a step's new tokens over a plain paged cache
+(oscar_chunk_attention): decode, MTP verification, prompts and chunks of them,
+in any mixture, for layers whose keys and values are kept as they are
+(``append.PagedCache``).  What ``append.append_rotated`` has written of the
+step's own tokens is part of what they see.
+"""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import _lib, decode, rotary as _rotary
+from .append import PagedCache
+
+HEAD_SIZES = (64, 128, 256)
+
+_i32, _i64 = ctypes.c_int32, ctypes.c_int64
+
+
+class ChunkStepArgs(ctypes.Structure):
+    """struct oscar_chunk_step (include/oscar_amd.h)."""
+    _fields_ = [("num_requests", _i32), ("num_tokens", _i32), ("num_heads", _i32), ("window", _i32),
+                ("table_cols", _i32), ("narrow", _i32), ("joins", _i32), ("reserved", _i32), ("items_size", _i64),
+                ("workspace_size", _i64)]
+
+
+class ChunkStep:
+    """A step's request layout and how its work is cut, for every layer of the
+    step whose cache has the geometry of `cache`, whose heads are num_heads and
+    whose window is the same (0: none): built once per step, like the block
+    table.
+
+    qsl [requests + 1] and seqs [requests] are host lists (query starts from the
+    step's token 0; keys after the step); block_tables int32 [requests, pages] on
+    the cache's device.  A step is not built under graph capture; a captured call
+    keeps this step's lengths (its block table is read at every replay) and needs
+    the step to live as long as the graph."""
+
+    def __init__(self, qsl, seqs, block_tables: torch.Tensor, num_heads: int, cache: PagedCache, window: int = 0):
+        layout = decode.request_layout(qsl, seqs)
+        requests = len(layout.lengths)
+        if num_heads < 1 or num_heads % cache.num_kv_heads:
+            raise ValueError(f"{num_heads} query heads do not share {cache.num_kv_heads} kv heads")
+        if window < 0:
+            raise ValueError("the window must be positive, or 0 for none")
+        if cache.head_size not in HEAD_SIZES:
+            raise ValueError(f"chunk attention takes head sizes {HEAD_SIZES}, got {cache.head_size}")
+        if cache.block_size % 16:
+            raise ValueError("chunk attention needs a cache block size that is a multiple of 16")
+        if layout.qsl and layout.qsl[0] < 0:
+            raise ValueError("query starts are counted from the step's token 0")
+        args = ChunkStepArgs()
+        plan = [ctypes.addressof(layout.qstart), ctypes.addressof(layout.seq_t), requests, num_heads, window,
+                cache.address]
+        _lib.call("oscar_chunk_plan", *plan, None, 0, ctypes.byref(args))
+        if block_tables.ndim != 2 or block_tables.shape[0] < requests or block_tables.shape[1] < args.table_cols:
+            raise ValueError(f"block table must be [requests, pages] with the {args.table_cols} pages of the longest")
+        if block_tables.device != cache.device:
+            raise ValueError("the block table must be on the cache's device")
+        device = cache.device
+        if device.type != "cuda":
+            raise ValueError("OSCAR kernels take device tensors")
+        if block_tables.dtype != torch.int32 or block_tables.stride(1) != 1:
+            block_tables = block_tables.to(torch.int32).contiguous()
+        if torch.cuda.is_current_stream_capturing():
+            raise ValueError("a step is built before its calls are captured")
+        with torch.cuda.device(device):
+            host = torch.empty(max(args.items_size, 16), dtype=torch.uint8, pin_memory=True)
+            _lib.call("oscar_chunk_plan", *plan, host.data_ptr(), host.numel(), ctypes.byref(args))
+            self.items = host.to(device, non_blocking=True)
+            self.ready = torch.cuda.Event()
+            self.ready.record()
+            self.stream = _lib.stream_handle(device)
+        self.args = args
+        self.address = ctypes.addressof(args)
+        self.tokens = args.num_tokens
+        self.num_heads = num_heads
+        self.workspace_size = args.workspace_size
+        self.geometry = (cache.num_kv_heads, cache.head_size, cache.block_size)
+        self.device = device
+        self.block_tables = block_tables
+        self.items_ptr, self.table_ptr, self.table_stride = (self.items.data_ptr(), block_tables.data_ptr(),
+                                                             block_tables.stride(0))
+
+    def _join(self, device) -> None:
+        """Order this step's arrays before the current stream, which is not the one it was built on."""
+        stream = torch.cuda.current_stream(device)
+        if not torch.cuda.is_current_stream_capturing():        # (a capture begins with the device idle)
+            stream.wait_event(self.ready)
+        self.items.record_stream(stream)
+        self.block_tables.record_stream(stream)
+
+
+def chunk_attention(query: torch.Tensor, cache: PagedCache, step: ChunkStep, scale: float, out=None) -> torch.Tensor:
+    """Causal attention of query [N, Hq, D] (the cache's type; token t of the
+    step in row t) over the cache; returns [N, Hq, D] of that type, a new tensor
+    or `out`, whose rows past the step's tokens (and of tokens of no request) are
+    left as they were.  scale must be positive.  Keys on pages outside the cache
+    are left out; a row that sees no key becomes zeros."""
+    device = cache.device
+    if (cache.num_kv_heads, cache.head_size, cache.block_size) != step.geometry or device != step.device:
+        raise ValueError("the step was built for another cache geometry or device")
+    d = cache.head_size
+    if not 0.0 < scale < 3.0e38:
+        raise ValueError("scale must be positive and finite")
+    q = _rotary.heads(query, step.tokens, d, cache.dtype, device, "query")
+    if q.num_heads != step.num_heads:
+        raise ValueError(f"query must have the step's {step.num_heads} heads")
+    if (q.data | 2 * q.token_stride | 2 * q.head_stride) % 16:
+        query = query.contiguous()
+        q = _rotary.heads(query, step.tokens, d, cache.dtype, device, "query")
+    if out is None:
+        out = torch.empty(query.shape, dtype=query.dtype, device=device)
+    o = _rotary.heads(out, step.tokens, d, cache.dtype, device, "out")
+    if o.num_heads != step.num_heads or (o.data | 2 * o.token_stride | 2 * o.head_stride) % 16:
+        raise ValueError("out must have the query's heads, rows at multiples of 16 bytes")
+    if step.tokens == 0:
+        return out
+    if _lib.stream_handle(device) != step.stream:
+        step._join(device)
+    need = step.workspace_size
+    ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    ref = ctypes.byref
+    _lib.call_on(device, "oscar_chunk_attention", step.address, step.items_ptr, step.table_ptr, step.table_stride,
+                 cache.address, ref(q), ref(o), scale, _lib.ptr(ws), need)
+    return out

@@ -1,0 +1,277 @@
+"""Chunk attention over a plain paged cache, against the formula in 64 bits.
+
+Tolerance of an output o = sum p_t v_t (p the normalised weights, inputs taken
+as they are), eps the type's, B = sum p_t |v_t|:
+  the weights are rounded to the type before the product and summed as rounded:
+    each is off by eps / 2 relative, the mean by eps / 2 (B + |o|) at most;
+  the scores are fp32 sums of D products, off by at most (D + 2) 2^-24 sum |q k|
+    scale; a weight by that, relatively, and the mean by twice that times B;
+    the exponential and the lazy maximum (weights up to 2^8 of the largest
+    possible 1) add 2^-21 of a weight;
+  fp16 weights below 2^-14 of the maximum are subnormal: off by 2^-25 each, of a
+    sum that is at least 1: t 2^-25 max |v|;
+  the output's own rounding: eps / 2 |o| and half a subnormal step."""
+import math
+
+import pytest
+import torch
+
+from oscar_amd.kernels import append, chunk, rotary
+
+pytestmark = pytest.mark.gpu
+
+
+def expected(q, keys, values, first, window, scale, hidden=None):
+    """(o, bound) of one request: q [n, Hq, D] at positions first .., keys / values
+    [t, Hk, D]; hidden [t]: keys that no row sees."""
+    n, hq, d = q.shape
+    hk = keys.shape[1]
+    dtype = q.dtype
+    eps = torch.finfo(dtype).eps
+    q, keys, values = q.double(), keys.double(), values.double()
+    pos = first + torch.arange(n, device=q.device)
+    at = torch.arange(keys.shape[0], device=q.device)
+    seen = at[None] <= pos[:, None]
+    if window:
+        seen &= at[None] > pos[:, None] - window
+    if hidden is not None:
+        seen &= ~hidden[None]
+    out, bound = torch.zeros_like(q), torch.zeros_like(q)
+    for h in range(hq):
+        k, v = keys[:, h // (hq // hk)], values[:, h // (hq // hk)]
+        s = (q[:, h] @ k.t()) * scale
+        reach = (q[:, h].abs() @ k.abs().t()) * scale
+        s = s.masked_fill(~seen, -math.inf)
+        top = s.amax(-1, keepdim=True)
+        p = torch.where(seen, (s - torch.where(top.isinf(), 0.0, top)).exp(), 0.0)
+        total = p.sum(-1, keepdim=True)
+        p = p / torch.where(total > 0, total, 1.0)
+        v = torch.where(seen.any(0)[:, None], v, 0.0)
+        o = p @ v
+        mean = p @ v.abs()
+        off = (torch.where(seen, reach, 0.0).amax(-1, keepdim=True)) * (d + 2) * 2.0 ** -24
+        b = eps / 2 * (mean + o.abs()) + (2 * off + 2.0 ** -20) * mean + eps / 2 * o.abs() * (1 + eps)
+        b += torch.finfo(dtype).smallest_normal * eps / 2
+        if dtype == torch.float16:
+            b += seen.sum(-1, keepdim=True) * 2.0 ** -25 * v.abs().amax()
+        out[:, h], bound[:, h] = o, b
+    return out, bound
+
+
+def make(g, reqs, hq, hk, d, page, dtype, layout="apart", spread=1.0):
+    """Caches with shuffled pages, block table, queries of a step of (new, history) requests."""
+    need = [max(1, -(-(n + h) // page)) for n, h in reqs]
+    pages = sum(need) + 2
+    shape = (page, hk, d)
+    if layout == "joint":
+        both = torch.randn(pages, 2, *shape, generator=g, device="cuda:0").to(dtype)
+        caches = [both[:, 0], both[:, 1]]
+    elif layout == "heads_first":
+        caches = [torch.randn(pages, hk, page, d, generator=g, device="cuda:0").to(dtype).transpose(1, 2)
+                  for _ in range(2)]
+    else:
+        caches = [torch.randn(pages, *shape, generator=g, device="cuda:0").to(dtype) for _ in range(2)]
+    order = torch.randperm(pages, generator=g, device="cuda:0").to(torch.int32)
+    table = torch.full((len(reqs), max(need)), -1, dtype=torch.int32, device="cuda:0")
+    at = 0
+    for i, c in enumerate(need):
+        table[i, :c] = order[at:at + c]
+        at += c
+    q = (torch.randn(sum(n for n, _ in reqs), hq, d, generator=g, device="cuda:0") * spread).to(dtype)
+    starts = [0]
+    for n, _ in reqs:
+        starts.append(starts[-1] + n)
+    return q, caches, table, starts, [n + h for n, h in reqs]
+
+
+def gather(caches, row, seq, page):
+    at = torch.arange(seq, device=row.device)
+    slot = row[at // page].long() * page + at % page
+    return [c.reshape(-1, *c.shape[2:])[slot] for c in caches]
+
+
+def check(got, q, caches, table, starts, seqs, window, scale, page):
+    for i, seq in enumerate(seqs):
+        a, b = starts[i], starts[i + 1]
+        if a == b:
+            continue
+        keys, values = gather(caches, table[i], seq, page)
+        o, bound = expected(q[a:b], keys, values, seq - (b - a), window, scale)
+        off = (got[a:b].double() - o).abs() - bound
+        assert off.max().item() <= 0, f"request {i}: off by {off.max().item():.3e} more than the bound"
+
+
+DECODE = [[(1, 0)], [(1, 1)], [(1, 31)], [(1, 32)], [(1, 4099)], [(4, 700), (1, 15), (3, 0), (2, 5000)],
+          [(16, 33), (0, 100), (5, 127), (1, 128), (7, 1000)], [(1, 40 * i) for i in range(70)]]
+PROMPTS = [[(17, 0)], [(33, 1)], [(257, 0)], [(300, 777)], [(129, 2000), (1, 900), (64, 0)], [(1100, 333)]]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("case", range(len(DECODE + PROMPTS)))
+def test_against_the_formula(device, dtype, d, case):
+    reqs = (DECODE + PROMPTS)[case]
+    g = torch.Generator(device=device).manual_seed(100 * case + d)
+    for hq, hk, page, window, layout in ((6, 1, 128, 0, "apart"), (4, 4, 16, 0, "joint"), (8, 2, 48, 100, "heads_first"),
+                                         (16, 1, 32, 1, "apart"), (7, 1, 64, 33, "joint")):
+        q, caches, table, starts, seqs = make(g, reqs, hq, hk, d, page, dtype, layout, spread=2.0)
+        cache = append.PagedCache(*caches)
+        step = chunk.ChunkStep(starts, seqs, table, hq, cache, window)
+        got = chunk.chunk_attention(q, cache, step, d ** -0.5)
+        check(got, q, caches, table, starts, seqs, window, d ** -0.5, page)
+
+
+def test_scores_of_any_size(device):
+    """One key dominates, or all weigh alike; maxima that rise along the keys."""
+    g = torch.Generator(device=device).manual_seed(5)
+    for scale, spread in ((1.0, 8.0), (1e-6, 1.0), (0.3, 30.0)):
+        q, caches, table, starts, seqs = make(g, [(3, 900), (40, 300)], 8, 2, 128, 32, torch.bfloat16, spread=spread)
+        ramp = torch.linspace(0, 4, 32, device=device)[None, :, None, None]
+        caches[0].mul_(ramp.to(torch.bfloat16))
+        cache = append.PagedCache(*caches)
+        got = chunk.chunk_attention(q, cache, chunk.ChunkStep(starts, seqs, table, 8, cache), scale)
+        check(got, q, caches, table, starts, seqs, 0, scale, 32)
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_what_lies_in_unseen_slots_does_not_matter(device, d):
+    """Slots past a request's keys, other requests' pages: NaN and infinities."""
+    g = torch.Generator(device=device).manual_seed(6)
+    reqs = [(1, 40), (4, 90), (50, 100), (1, 0), (130, 3)]
+    q, caches, table, starts, seqs = make(g, reqs, 6, 1, d, 64, torch.bfloat16)
+    cache = append.PagedCache(*caches)
+    step = chunk.ChunkStep(starts, seqs, table, 6, cache)
+    want = chunk.chunk_attention(q, cache, step, 0.1)
+    used = torch.zeros(caches[0].shape[0] * 64, dtype=torch.bool, device=device)
+    for i, seq in enumerate(seqs):
+        at = torch.arange(seq, device=device)
+        used[table[i][at // 64].long() * 64 + at % 64] = True
+    for c, bad in zip(caches, (math.nan, math.inf)):
+        c.view(-1, 1, d)[~used] = bad
+    assert torch.equal(chunk.chunk_attention(q, cache, step, 0.1), want)
+    check(want, q, caches, table, starts, seqs, 0, 0.1, 64)
+
+
+def test_unmapped_pages_are_left_out(device):
+    g = torch.Generator(device=device).manual_seed(7)
+    reqs = [(2, 200), (40, 200), (1, 10), (3, 300)]
+    q, caches, table, starts, seqs = make(g, reqs, 4, 2, 128, 32, torch.float16)
+    bad = table.clone()
+    bad[0, 2], bad[1, 0], bad[1, 6], bad[2, 0], bad[3, 9] = -1, caches[0].shape[0], 1 << 30, -(1 << 31), -7
+    cache = append.PagedCache(*caches)
+    got = chunk.chunk_attention(q, cache, chunk.ChunkStep(starts, seqs, bad, 4, cache), 0.09)
+    for i, seq in enumerate(seqs):
+        hidden = torch.zeros(seq, dtype=torch.bool, device=device)
+        for c in range(-(-seq // 32)):
+            if bad[i, c] != table[i, c]:
+                hidden[32 * c:32 * (c + 1)] = True
+        keys, values = gather(caches, table[i], seq, 32)
+        o, bound = expected(q[starts[i]:starts[i + 1]], keys, values, reqs[i][1], 0, 0.09, hidden)
+        assert ((got[starts[i]:starts[i + 1]].double() - o).abs() <= bound).all()
+    assert (got[starts[2]:starts[3]] == 0).all()          # nothing left to see
+
+
+def test_rows_of_no_request_are_left_alone(device):
+    g = torch.Generator(device=device).manual_seed(8)
+    q, caches, table, _, seqs = make(g, [(4, 50), (3, 60)], 6, 1, 64, 16, torch.bfloat16)
+    cache = append.PagedCache(*caches)
+    starts = [0, 4, 7]
+    padded = torch.cat((q, torch.full((5, 6, 64), math.nan, device=device).bfloat16()))
+    out = torch.full((14, 6, 64), 3.0, device=device).bfloat16()[:12]
+    step = chunk.ChunkStep(starts, seqs, table, 6, cache)
+    assert chunk.chunk_attention(padded, cache, step, 0.125, out=out) is out
+    assert (out[7:] == 3.0).all()
+    check(out, q, caches, table, starts, seqs, 0, 0.125, 16)
+    # a step that begins past token 0 (rows before it are another call's)
+    out2 = torch.full_like(out, 3.0)
+    shifted = torch.cat((padded[:2], padded))
+    chunk.chunk_attention(shifted[:9], cache, chunk.ChunkStep([2, 6, 9], seqs, table, 6, cache), 0.125, out=out2[:9])
+    assert (out2[:2] == 3.0).all() and torch.equal(out2[2:9], out[:7])
+
+
+def test_strided_queries_and_outputs(device):
+    g = torch.Generator(device=device).manual_seed(9)
+    q, caches, table, starts, seqs = make(g, [(40, 50), (1, 600)], 6, 2, 64, 16, torch.float16)
+    cache = append.PagedCache(*caches)
+    step = chunk.ChunkStep(starts, seqs, table, 6, cache)
+    want = chunk.chunk_attention(q, cache, step, 0.125)
+    fused = torch.zeros(41, 10, 64, device=device, dtype=torch.float16)
+    fused[:, 2:8] = q
+    out = torch.zeros(41, 9, 64, device=device, dtype=torch.float16)
+    chunk.chunk_attention(fused[:, 2:8], cache, step, 0.125, out=out[:, 1:7])
+    assert torch.equal(out[:, 1:7], want) and (out[:, 0] == 0).all() and (out[:, 7:] == 0).all()
+    heads_first = q.transpose(0, 1).contiguous().transpose(0, 1)
+    assert torch.equal(chunk.chunk_attention(heads_first, cache, step, 0.125), want)
+    odd = torch.zeros(41, 6, 65, device=device, dtype=torch.float16)[..., 1:]
+    odd.copy_(q)
+    assert torch.equal(chunk.chunk_attention(odd, cache, step, 0.125), want)
+    with pytest.raises(ValueError, match="16 bytes"):
+        chunk.chunk_attention(q, cache, step, 0.125, out=odd)
+
+
+def test_streams_and_replays(device):
+    g = torch.Generator(device=device).manual_seed(10)
+    q, caches, table, starts, seqs = make(g, [(4, 5000), (100, 900)], 6, 1, 128, 128, torch.bfloat16)
+    cache = append.PagedCache(*caches)
+    step = chunk.ChunkStep(starts, seqs, table, 6, cache)
+    assert step.workspace_size > 0
+    want = chunk.chunk_attention(q, cache, step, 0.1)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = chunk.chunk_attention(q, cache, step, 0.1)
+        own = chunk.chunk_attention(q, cache, chunk.ChunkStep(starts, seqs, table, 6, cache), 0.1)
+    side.synchronize()
+    assert torch.equal(got, want) and torch.equal(own, want)
+    graphs = []
+    for _ in range(2):                # two graphs of one step
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = chunk.chunk_attention(q, cache, step, 0.1)
+        graphs.append((graph, out))
+    for _ in range(3):
+        for graph, out in graphs:
+            out.zero_()
+            graph.replay()
+        junk = chunk.chunk_attention(q, cache, step, 0.2)
+        torch.cuda.synchronize()
+        assert all(torch.equal(out, want) for _, out in graphs) and not torch.equal(junk, want)
+    with torch.cuda.graph(torch.cuda.CUDAGraph()):
+        with pytest.raises(ValueError, match="before its calls are captured"):
+            chunk.ChunkStep(starts, seqs, table, 6, cache)
+        out.zero_()
+
+
+def test_append_then_attend(device):
+    """A prompt, its follow-up chunk and MTP steps of two requests, rotated on
+    image positions, written and read; against the formula over all tokens."""
+    g = torch.Generator(device=device).manual_seed(11)
+    hq, hk, d, page, rd, dtype = 6, 2, 128, 32, 64, torch.bfloat16
+    axes = rotary.section_axes((11, 11, 10), interleaved=True)
+    turn = rotary.Rotary(rotary.rotary_table(2000, rd, device=device), axes=axes)
+    caches = [torch.full((40, page, hk, d), math.nan, dtype=dtype, device=device) for _ in range(2)]
+    cache = append.PagedCache(*caches)
+    table = torch.randperm(40, generator=g, device=device).to(torch.int32).view(2, 20)
+    total = [0, 0]
+    kept = [[[], []], [[], []]]
+    for lengths in ((100, 37), (200, 1), (4, 4), (1, 130), (4, 2)):
+        n = sum(lengths)
+        x = torch.randn(n, hq + 2 * hk, d, generator=g, device=device).to(dtype)
+        q, k, v = x.split((hq, hk, hk), 1)
+        pos = torch.randint(0, 2000, (3, n), generator=g, device=device)
+        slots = []
+        for i, m in enumerate(lengths):
+            at = torch.arange(total[i], total[i] + m, device=device)
+            slots.append(table[i][at // page].long() * page + at % page)
+        q_turned = append.append_rotated(q, k, v, pos, turn, cache, torch.cat(slots))
+        k_turned = rotary.rotate(k, None, pos, turn)[0]
+        starts, seqs = [0, lengths[0], n], [t + m for t, m in zip(total, lengths)]
+        got = chunk.chunk_attention(q_turned, cache, chunk.ChunkStep(starts, seqs, table, hq, cache), d ** -0.5)
+        for i, m in enumerate(lengths):
+            a, b = starts[i], starts[i + 1]
+            kept[i][0].append(k_turned[a:b])
+            kept[i][1].append(v[a:b])
+            o, bound = expected(rotary.rotate(q, None, pos, turn)[0][a:b], torch.cat(kept[i][0]), torch.cat(kept[i][1]),
+                                total[i], 0, d ** -0.5)
+            assert ((got[a:b].double() - o).abs() <= bound).all()
+            total[i] += m
