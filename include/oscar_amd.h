@@ -618,8 +618,8 @@ typedef struct oscar_chunk_step {
   int32_t window;
   int32_t table_cols;
   int32_t narrow;
+  int32_t wide;
   int32_t joins;
-  int32_t reserved;
   int64_t items_size;
   int64_t workspace_size;
 } oscar_chunk_step;

@@ -22,6 +22,8 @@
 #include "plain_cache.h"
 
 #include <algorithm>
+#include <cstring>
+#include <functional>
 #include <type_traits>
 #include <vector>
 
@@ -33,6 +35,7 @@ constexpr int kTileRows = 32;
 constexpr int kWaves = 4;
 constexpr int kThreads = 64 * kWaves;
 constexpr int kCus = 256;
+constexpr int32_t kMostKeys = 1 << 30;     // of a request, and rows: positions and windows add without overflow
 constexpr float kNone = -3.0e38f;          // running maximum before any key
 constexpr float kLazy = 8.f;               // a maximum is raised when a score exceeds it by 2^8
 
@@ -107,6 +110,7 @@ struct ChunkArgs {
   float* partials;         // slots of 32 rows: [32][D], then m[32], l[32]
   float scale_log2;
   int32_t group, block_size, window;
+  int32_t wide0;           // first piece of the wide kernel
   FastDiv group_div, block_div;
 };
 
@@ -342,6 +346,7 @@ __global__ __launch_bounds__(kThreads, 1) void narrow_kernel(ChunkArgs a) {
 
   if (first < last) {
     load_tile(first, std::false_type{}, kt);
+    __builtin_amdgcn_sched_barrier(0);      // (the waits below count K's loads before V's)
     load_tile(first, std::true_type{}, vt);
   }
   // One tile.  (The two places as parameters that do not alias: the compiler
@@ -414,6 +419,269 @@ __global__ __launch_bounds__(kThreads, 1) void narrow_kernel(ChunkArgs a) {
   }
 }
 
+// ---------------------------------------------------------------- 256 rows
+// A wide row tile: kW waves of kR times 32 rows each, over tiles of 32 keys that
+// all of them read from LDS.  The scores of a tile are computed one tile ahead,
+// so that products and softmax overlap inside a wave: iteration t runs
+//   A:  S(t + 1) = K Q^T        beside the weights of the tile's first 16 keys,
+//   B1: O += V^T P^T, 16 keys   beside the weights of the other 16,
+//   B2: O += V^T P^T, 16 keys   beside the maximum of S(t + 1),
+// each step of a product followed by its share of the arithmetic (the order is
+// the schedule: scheduling barriers keep it).  K and V tiles come through rings
+// of four places, requested two iterations ahead; one barrier an iteration, in
+// the middle of B, where the K tile just used and the V tile before this one
+// are given up.
+constexpr int kWideRows = 256;
+constexpr int kRing = 4;
+
+template <int D>
+constexpr int wide_lds() { return 2 * kRing * kTileKeys * 2 * D; }
+
+template <typename T, int D, int kR, int kW, int kWgs>
+__global__ __launch_bounds__(64 * kW, kW * kWgs / 4) void wide_kernel(ChunkArgs a) {
+  extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+  typedef typename Num<T>::V8 V8;
+  constexpr int kTileBytes = kTileKeys * 2 * D;
+  constexpr int kLoads = kTileBytes / 1024 / kW;       // of a tile and wave
+  constexpr int kKeys = kTileKeys / kW;                // keys of a tile that a wave loads
+  constexpr int kSteps = D / 16, kBlocks = D / 32;
+  constexpr int kAhead = D == 256 ? 2 : 4;
+  static_assert(kLoads * 1024 * kW == kTileBytes && kR * kW * 32 == kWideRows, "whole kilobytes a wave");
+  const int tid = (int)threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const Piece p = a.pieces[a.wide0 + blockIdx.x];
+  uint8_t* const kring = smem;
+  uint8_t* const vring = smem + kRing * kTileBytes;
+  const int tiles = (p.key1 - p.key0 + kTileKeys - 1) / kTileKeys;
+  const int group0 = p.key0 / 16;
+
+  int page_base = group0;
+  int pages = load_pages(a, p, page_base, lane);
+  RowState<T, D> s[kR];
+#pragma unroll
+  for (int r = 0; r < kR; ++r) load_rows<T, D>(a, p, p.row0 + 32 * (kR * wave + r), lane, s[r]);
+  const int first = s[0].first, last = s[kR - 1].last;
+
+  // Tile u's page of this wave's keys (kept until its V is requested, two tiles
+  // later), and which halves of the tiles from the last requested one back are
+  // unmapped, two bits each.
+  int page_next = 0, page_after = 0;
+  uint32_t unmapped = 0;
+  auto request_k = [&](int u) {
+    const int g = group0 + 2 * u - page_base;
+    if (g >= 64) {
+      page_base += g;
+      pages = load_pages(a, p, page_base, lane);
+    }
+    const int at = group0 + 2 * u - page_base;
+    const int lo = __builtin_amdgcn_readlane(pages, at), hi = __builtin_amdgcn_readlane(pages, at + 1);
+    const int page = kKeys * wave < 16 ? lo : hi;
+    unmapped = (unmapped << 2) | (lo < 0 ? 1u : 0u) | (hi < 0 ? 2u : 0u);
+    load_keys<D, false, kLoads>(a, p, p.key0 + u * kTileKeys + kKeys * wave, kKeys * wave, page,
+                                kring + (u % kRing) * kTileBytes, lane);
+    return page;
+  };
+  auto request_v = [&](int u, int page) {
+    load_keys<D, true, kLoads>(a, p, p.key0 + u * kTileKeys + kKeys * wave, kKeys * wave, page,
+                               vring + (u % kRing) * kTileBytes, lane);
+  };
+  // (the waits below count these in this order)
+  const int p0 = request_k(0);
+  __builtin_amdgcn_sched_barrier(0);
+  const int p1 = request_k(1);
+  page_next = request_k(2);
+  request_v(0, p0);
+  __builtin_amdgcn_sched_barrier(0);
+  page_after = request_k(3);
+  request_v(1, p1);
+  __builtin_amdgcn_sched_barrier(0);
+
+  const int k_addr = k_read<D>(lane), v_addr = v_read<D>(lane);
+  auto k_operand = [&](const uint8_t* kt, int i) {
+    return *reinterpret_cast<const V8*>(kt + (k_addr ^ (32 * i)));
+  };
+  auto v_operand = [&](const uint8_t* vt, int h, int b) {
+    const uint8_t* at = vt + (v_addr ^ (64 * b)) + h * 32 * D;
+    const shortx4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)at);
+    const shortx4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(at + 16 * D));
+    return __builtin_bit_cast(V8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+  };
+  // The running maxima, raised where a tile's scores ask for it.
+  auto raise_max = [&](float (&top)[kR]) {
+    bool raise[kR], any = false;
+#pragma unroll
+    for (int r = 0; r < kR; ++r) {
+      top[r] = max_halves(top[r]) * a.scale_log2;
+      raise[r] = top[r] > s[r].m + kLazy;
+      any = any || raise[r];
+    }
+    if (__ballot(any)) {
+#pragma unroll
+      for (int r = 0; r < kR; ++r) {
+        const float m = raise[r] ? top[r] : s[r].m, f = __builtin_amdgcn_exp2f(s[r].m - m);
+#pragma unroll
+        for (int b = 0; b < kBlocks; ++b) s[r].acc[b] *= f;
+        s[r].l *= f;
+        s[r].m = m;
+      }
+    }
+  };
+  // Rows that do not see the whole of tile u lose what they do not see.
+  auto mask_tile = [&](floatx16 (&x)[kR], int u, uint32_t gone) {
+    const int key0 = p.key0 + u * kTileKeys;
+    if (key0 + kTileKeys - 1 <= first && (a.window == 0 || key0 > last - a.window) && gone == 0u) return;
+#pragma unroll
+    for (int r = 0; r < kR; ++r) {
+      const int hi = s[r].pos - key0 - 4 * (lane >> 5);
+      const int lo = a.window == 0 ? INT32_MIN : hi - a.window;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int key = 8 * (i >> 2) + (i & 3);
+        x[r][i] = key <= hi && key > lo && ((gone >> (i >> 3)) & 1u) == 0u ? x[r][i] : -__builtin_inff();
+      }
+    }
+  };
+
+  // ---- first scores ----
+  floatx16 xa[kR], xb[kR];
+  wait_vmcnt<5 * kLoads>();                 // K(0) is there
+  asm volatile("s_barrier" ::: "memory");
+#pragma unroll
+  for (int r = 0; r < kR; ++r) xa[r] = floatx16{};
+#pragma unroll
+  for (int i = 0; i < kSteps; ++i) {
+    const V8 k = k_operand(kring, i);
+#pragma unroll
+    for (int r = 0; r < kR; ++r) xa[r] = Num<T>::mfma(k, s[r].q[i], xa[r]);
+  }
+  mask_tile(xa, 0, (unmapped >> 6) & 3u);
+  float top[kR];
+#pragma unroll
+  for (int r = 0; r < kR; ++r) {
+    top[r] = xa[r][0];
+#pragma unroll
+    for (int i = 1; i < 16; ++i) top[r] = fmaxf(top[r], xa[r][i]);
+  }
+  raise_max(top);
+  wait_vmcnt<2 * kLoads>();                 // K(1), K(2), V(0) are there
+  asm volatile("s_barrier" ::: "memory");
+  {
+    const int page = request_k(4);
+    request_v(2, page_next);
+    page_next = page_after;
+    page_after = page;
+  }
+
+  // One iteration: tile t's scores are in x, tile t + 1's come to y.
+  auto iterate = [&](int t, floatx16 (&x)[kR], floatx16 (&y)[kR], uint8_t* __restrict__ kr,
+                     uint8_t* __restrict__ vr) __attribute__((always_inline)) {
+    const uint8_t* kt = kr + ((t + 1) % kRing) * kTileBytes;
+    const uint8_t* vt = vr + (t % kRing) * kTileBytes;
+    V8 w[kR][2];                            // [rows][key half]
+    auto weight = [&](int e) {
+#pragma unroll
+      for (int r = 0; r < kR; ++r) x[r][e] = __builtin_amdgcn_exp2f(x[r][e] * a.scale_log2 - s[r].m);
+    };
+    auto round = [&](int h) {
+#pragma unroll
+      for (int r = 0; r < kR; ++r) {
+        floatx8 f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = x[r][8 * h + i];
+        w[r][h] = __builtin_convertvector(f, V8);
+        s[r].l = Num<T>::sum8(w[r][h], s[r].l);
+      }
+    };
+    // A
+    V8 k[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) k[i] = k_operand(kt, i);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+#pragma unroll
+      for (int r = 0; r < kR; ++r) y[r] = Num<T>::mfma(k[i % kAhead], s[r].q[i], i == 0 ? floatx16{} : y[r]);
+      if (i + kAhead < kSteps) k[i % kAhead] = k_operand(kt, i + kAhead);
+#pragma unroll
+      for (int e = i * 8 / kSteps; e < (i + 1) * 8 / kSteps; ++e) weight(e);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    V8 v[kAhead];
+    constexpr int kPv = 2 * kBlocks;
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) v[i] = v_operand(vt, i / kBlocks, i % kBlocks);
+    round(0);
+    __builtin_amdgcn_sched_barrier(0);
+    mask_tile(y, t + 1, (unmapped >> 6) & 3u);
+    // B1, B2
+    float top[kR];
+#pragma unroll
+    for (int i = 0; i < kPv; ++i) {
+      const int h = i / kBlocks, b = i % kBlocks;
+      if (i == kBlocks) {
+        round(1);
+        wait_vmcnt<2 * kLoads>();           // K(t + 2), V(t + 1) are there
+        asm volatile("s_barrier" ::: "memory");
+        const int page = request_k(t + 5);
+        request_v(t + 3, page_next);
+        page_next = page_after;
+        page_after = page;
+      }
+#pragma unroll
+      for (int r = 0; r < kR; ++r) s[r].acc[b] = Num<T>::mfma(v[i % kAhead], w[r][h], s[r].acc[b]);
+      if (i + kAhead < kPv) v[i % kAhead] = v_operand(vt, (i + kAhead) / kBlocks, (i + kAhead) % kBlocks);
+      if (h == 0) {
+#pragma unroll
+        for (int e = 8 + b * 8 / kBlocks; e < 8 + (b + 1) * 8 / kBlocks; ++e) weight(e);
+      } else {
+#pragma unroll
+        for (int r = 0; r < kR; ++r) {
+          if (b == 0) top[r] = y[r][0];
+#pragma unroll
+          for (int e = b * 16 / kBlocks; e < (b + 1) * 16 / kBlocks; ++e) top[r] = fmaxf(top[r], y[r][e]);
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    raise_max(top);
+  };
+  for (int t = 0; t < tiles; t += 2) {
+    iterate(t, xa, xb, kring, vring);
+    if (t + 1 < tiles) iterate(t + 1, xb, xa, kring, vring);
+  }
+  arrive_all();                             // (loads to LDS that nobody waits for)
+
+#pragma unroll
+  for (int r = 0; r < kR; ++r) {
+    const float l = sum_halves(s[r].l);
+    const int at = 32 * (kR * wave + r) + (lane & 31);
+    if (at >= p.rows) continue;
+    if (p.slot < 0) {
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      uint8_t* o = out_row(a, p.token0, p.kv_head, p.row0 + at) + 8 * (lane >> 5);
+#pragma unroll
+      for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          store4<T>(o + 64 * b + 16 * i, floatx4{s[r].acc[b][4 * i], s[r].acc[b][4 * i + 1], s[r].acc[b][4 * i + 2],
+                                                 s[r].acc[b][4 * i + 3]} * inv);
+    } else {
+      float* part = a.partials + (int64_t)(p.slot + kR * wave + r) * (kTileRows * (D + 2));
+      float* o = part + (lane & 31) * D + 4 * (lane >> 5);
+#pragma unroll
+      for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          *reinterpret_cast<floatx4*>(o + 32 * b + 8 * i) =
+              floatx4{s[r].acc[b][4 * i], s[r].acc[b][4 * i + 1], s[r].acc[b][4 * i + 2], s[r].acc[b][4 * i + 3]};
+      if (lane < 32) {
+        part[kTileRows * D + (lane & 31)] = s[r].m;
+        part[kTileRows * D + kTileRows + (lane & 31)] = l;
+      }
+    }
+  }
+}
+
 // ---------------------------------------------------------------- join
 // One row and 64 of its features a workgroup: 16 threads across the features,
 // 16 across the partials.
@@ -460,76 +728,133 @@ __global__ __launch_bounds__(256) void join_kernel(ChunkArgs a) {
 
 // ---------------------------------------------------------------- the plan
 struct Plan {
-  std::vector<Piece> narrow;
+  std::vector<Piece> narrow, wide;
   std::vector<Join> joins;
   int32_t slots = 0;
 };
 
-// Keys that rows of tokens [first, last] of a request see: [lo, hi).
-void visible(int32_t pos0, int32_t first, int32_t last, int32_t window, int32_t& lo, int32_t& hi) {
-  hi = pos0 + last + 1;
-  lo = window > 0 ? std::max(0, pos0 + first - window + 1) : 0;
-  lo = lo / kTileKeys * kTileKeys;
-}
+struct RowTile {
+  Piece piece;
+  int32_t tiles;           // of 32 keys
+};
 
-int make_plan(const int32_t* qsl, const int32_t* seqs, int32_t num_requests, int32_t group, int32_t kv_heads,
-              int32_t head_size, int32_t window, Plan& plan) {
-  struct Tile {
-    Piece piece;
-    int32_t tiles;
-  };
-  std::vector<Tile> rows;
-  int64_t total = 0;
-  int32_t most = 0;
-  for (int32_t i = 0; i < num_requests; ++i) {
-    const int32_t n = qsl[i + 1] - qsl[i];
-    const int64_t request_rows = (int64_t)n * group;
-    for (int64_t r = 0; r < request_rows; r += kTileRows) {
-      Piece p{};
-      p.token0 = qsl[i];
-      p.pos0 = seqs[i] - n;
-      p.table_row = i;
-      p.row0 = (int32_t)r;
-      p.rows = (int32_t)std::min<int64_t>(kTileRows, request_rows - r);
-      visible(p.pos0, p.row0 / group, (p.row0 + p.rows - 1) / group, window, p.key0, p.key1);
-      const int32_t tiles = (p.key1 - p.key0 + kTileKeys - 1) / kTileKeys;
-      for (int32_t h = 0; h < kv_heads; ++h) {
-        p.kv_head = h;
-        rows.push_back(Tile{p, tiles});
-      }
-      total += (int64_t)tiles * kv_heads;
-      most = std::max(most, tiles);
+// The row tiles of a request, `rows` rows each, with the keys that they see.
+void row_tiles(int32_t token0, int32_t n, int32_t seq, int32_t table_row, int32_t group, int32_t kv_heads,
+               int32_t window, int32_t rows, std::vector<RowTile>& out) {
+  const int32_t all = n * group;
+  for (int32_t r = 0; r < all; r += rows) {
+    Piece p{};
+    p.token0 = token0;
+    p.pos0 = seq - n;
+    p.table_row = table_row;
+    p.row0 = r;
+    p.rows = std::min(rows, all - r);
+    p.slot = -1;
+    const int32_t lo = window > 0 ? std::max(0, p.pos0 + r / group - window + 1) : 0;
+    p.key0 = lo / kTileKeys * kTileKeys;
+    p.key1 = p.pos0 + (r + p.rows - 1) / group + 1;
+    for (int32_t h = 0; h < kv_heads; ++h) {
+      p.kv_head = h;
+      out.push_back(RowTile{p, (p.key1 - p.key0 + kTileKeys - 1) / kTileKeys});
     }
   }
-  // Key tiles of a piece: the fewest with which the pieces fit the workgroups
-  // that are resident at once.
-  const int64_t resident = (int64_t)kCus * std::max(1, 256 / head_size);
+}
+
+// A row tile in n pieces of equal parts of its keys.
+void cut(const RowTile& x, int32_t n, Plan& plan, std::vector<Piece>& out) {
+  if (n <= 1) {
+    out.push_back(x.piece);
+    return;
+  }
+  const int32_t groups = (x.piece.rows + kTileRows - 1) / kTileRows;
+  for (int32_t g = 0; g < groups; ++g)
+    plan.joins.push_back(Join{x.piece.token0, x.piece.kv_head, x.piece.row0 + g * kTileRows,
+                              std::min(kTileRows, x.piece.rows - g * kTileRows), plan.slots + g, groups, n, 0});
+  for (int32_t s = 0; s < n; ++s) {
+    Piece p = x.piece;
+    p.key0 = x.piece.key0 + kTileKeys * (int32_t)((int64_t)x.tiles * s / n);
+    p.key1 = std::min<int32_t>(x.piece.key1, x.piece.key0 + kTileKeys * (int32_t)((int64_t)x.tiles * (s + 1) / n));
+    p.slot = plan.slots;
+    plan.slots += groups;
+    out.push_back(p);
+  }
+}
+
+int32_t pieces_of(const RowTile& x, int64_t per) { return (int32_t)((x.tiles + per - 1) / per); }
+
+// Narrow tiles: the fewest key tiles a piece with which the pieces fit the
+// workgroups that are resident at once.
+void plan_narrow(const std::vector<RowTile>& rows, int32_t head_size, Plan& plan) {
+  int64_t total = 0;
+  int32_t most = 0;
+  for (const RowTile& x : rows) {
+    total += x.tiles;
+    most = std::max(most, x.tiles);
+  }
+  const int64_t resident = (int64_t)kCus * (256 / head_size);
   int64_t per = std::max<int64_t>(kWaves, (total + resident - 1) / resident);
   auto count = [&](int64_t t) {
     int64_t c = 0;
-    for (const Tile& x : rows) c += (x.tiles + t - 1) / t;
+    for (const RowTile& x : rows) c += pieces_of(x, t);
     return c;
   };
   if ((int64_t)rows.size() >= resident) per = std::max<int64_t>(per, most);
-  else
-    while (per < most && count(per) > resident) ++per;
-  for (const Tile& x : rows) {
-    const int32_t n = (int32_t)((x.tiles + per - 1) / per);
-    if (n <= 1) {
-      plan.narrow.push_back(x.piece);
-      plan.narrow.back().slot = -1;
-      continue;
+  while (per < most && count(per) > resident) ++per;
+  for (const RowTile& x : rows) cut(x, pieces_of(x, per), plan, plan.narrow);
+}
+
+// Wide tiles: workgroups take pieces as they come free, the longest first.  Of
+// a few piece lengths the one whose pieces, dealt out to the workgroups that
+// are resident at once, end first.
+constexpr int32_t kPieceCost = 5;          // of a piece beside its tiles, in tiles' time
+void plan_wide(const std::vector<RowTile>& rows, int32_t head_size, Plan& plan) {
+  int64_t total = 0;
+  int32_t most = 0;
+  for (const RowTile& x : rows) {
+    total += x.tiles;
+    most = std::max(most, x.tiles);
+  }
+  const int64_t resident = (int64_t)kCus * (head_size == 64 ? 2 : 1);
+  int64_t best = most, best_end = INT64_MAX;
+  std::vector<int32_t> length;
+  std::vector<int64_t> load;
+  for (int64_t k = 0; k <= 4; ++k) {
+    const int64_t per = k == 0 ? most : std::max<int64_t>(8, (total + resident * k - 1) / (resident * k));
+    if (per > most || (k > 0 && (int64_t)rows.size() > 4 * resident)) continue;
+    length.clear();
+    for (const RowTile& x : rows) {
+      const int32_t n = pieces_of(x, per);
+      for (int32_t i = 0; i < n; ++i) length.push_back((x.tiles + n - 1) / n + kPieceCost * (n > 1 ? 2 : 1));
     }
-    plan.joins.push_back(Join{x.piece.token0, x.piece.kv_head, x.piece.row0, x.piece.rows, plan.slots, 1, n, 0});
-    for (int32_t s = 0; s < n; ++s) {
-      Piece p = x.piece;
-      p.key0 = x.piece.key0 + kTileKeys * (int32_t)((int64_t)x.tiles * s / n);
-      p.key1 = std::min<int32_t>(x.piece.key1, x.piece.key0 + kTileKeys * (int32_t)((int64_t)x.tiles * (s + 1) / n));
-      p.slot = plan.slots++;
-      plan.narrow.push_back(p);
+    std::sort(length.begin(), length.end(), std::greater<int32_t>());
+    load.assign((size_t)resident, 0);
+    for (size_t i = 0; i < length.size(); ++i) {
+      const size_t at = i % (size_t)resident;
+      load[(i / (size_t)resident) % 2 ? (size_t)resident - 1 - at : at] += length[i];
+    }
+    const int64_t end = *std::max_element(load.begin(), load.end());
+    if (end < best_end) {
+      best_end = end;
+      best = per;
     }
   }
-  return kOk;
+  for (const RowTile& x : rows) cut(x, pieces_of(x, best), plan, plan.wide);
+  std::stable_sort(plan.wide.begin(), plan.wide.end(),
+                   [](const Piece& x, const Piece& y) { return x.key1 - x.key0 > y.key1 - y.key0; });
+}
+
+void make_plan(const int32_t* qsl, const int32_t* seqs, int32_t num_requests, int32_t group, int32_t kv_heads,
+               int32_t head_size, int32_t window, Plan& plan) {
+  std::vector<RowTile> narrow, wide;
+  for (int32_t i = 0; i < num_requests; ++i) {
+    const int32_t n = qsl[i + 1] - qsl[i];
+    if (n * (int64_t)group <= kTileRows)
+      row_tiles(qsl[i], n, seqs[i], i, group, kv_heads, window, kTileRows, narrow);
+    else
+      row_tiles(qsl[i], n, seqs[i], i, group, kv_heads, window, kWideRows, wide);
+  }
+  if (!narrow.empty()) plan_narrow(narrow, head_size, plan);
+  if (!wide.empty()) plan_wide(wide, head_size, plan);
 }
 
 constexpr size_t narrow_lds(int d) { return (size_t)kWaves * kTileRows * d * 4 + kWaves * 64 * 4; }
@@ -541,6 +866,14 @@ int launch(const ChunkArgs& a, const oscar_chunk_step& step, hipStream_t stream)
     const int st = set_dynamic_lds(reinterpret_cast<const void*>(&narrow_kernel<T, D>), (int)narrow_lds(D), done);
     if (st != kOk) return st;
     narrow_kernel<T, D><<<step.narrow, kThreads, narrow_lds(D), stream>>>(a);
+  }
+  if (step.wide > 0) {
+    static std::atomic<uint64_t> done{0};
+    constexpr int kR = D == 256 ? 1 : 2, kW = 8 / kR, kWgs = D == 64 ? 2 : 1;
+    const auto kernel = &wide_kernel<T, D, kR, kW, kWgs>;
+    const int st = set_dynamic_lds(reinterpret_cast<const void*>(kernel), wide_lds<D>(), done);
+    if (st != kOk) return st;
+    kernel<<<step.wide, 64 * kW, wide_lds<D>(), stream>>>(a);
   }
   if (step.joins > 0) join_kernel<T, D><<<dim3(step.joins, kTileRows, D / 64), 256, 0, stream>>>(a);
   return hipGetLastError() == hipSuccess ? kOk : kErrLaunch;
@@ -576,31 +909,33 @@ extern "C" int oscar_chunk_plan(const int32_t* query_start_loc, const int32_t* s
   int32_t pages = 0;
   for (int32_t i = 0; i < num_requests; ++i) {
     const int64_t n = (int64_t)query_start_loc[i + 1] - query_start_loc[i];
-    if (query_start_loc[i] < 0 || n < 0 || seq_lens[i] < n || n * group > INT32_MAX - kTileRows ||
-        seq_lens[i] > INT32_MAX - 4096)
+    if (query_start_loc[i] < 0 || n < 0 || seq_lens[i] < n || n * group > kMostKeys ||
+        seq_lens[i] > kMostKeys)
       return kErrInvalidArgument;
     if (n > 0) pages = std::max(pages, (seq_lens[i] - 1) / cache->block_size + 1);
   }
   try {
     Plan plan;
-    const int st = make_plan(query_start_loc, seq_lens, num_requests, group, cache->num_kv_heads, cache->head_size,
-                             window, plan);
-    if (st != kOk) return st;
-    const size_t narrow = plan.narrow.size() * sizeof(Piece), joins = plan.joins.size() * sizeof(Join);
-    if (plan.narrow.size() > INT32_MAX || plan.joins.size() > INT32_MAX) return kErrInvalidArgument;
+    make_plan(query_start_loc, seq_lens, num_requests, group, cache->num_kv_heads, cache->head_size, window, plan);
+    const size_t narrow = plan.narrow.size() * sizeof(Piece), wide = plan.wide.size() * sizeof(Piece);
+    const size_t joins = plan.joins.size() * sizeof(Join);
+    if (plan.narrow.size() + plan.wide.size() > INT32_MAX || plan.joins.size() > INT32_MAX) return kErrInvalidArgument;
     step->num_requests = num_requests;
     step->num_tokens = num_requests > 0 ? query_start_loc[num_requests] : 0;
     step->num_heads = num_heads;
-    step->window = window;
+    step->window = std::min(window, kMostKeys);
     step->table_cols = pages;
     step->narrow = (int32_t)plan.narrow.size();
+    step->wide = (int32_t)plan.wide.size();
     step->joins = (int32_t)plan.joins.size();
-    step->items_size = (int64_t)(narrow + joins);
+    step->items_size = (int64_t)(narrow + wide + joins);
     step->workspace_size = (int64_t)plan.slots * kTileRows * (cache->head_size + 2) * 4;
     if (items == nullptr) return kOk;
-    if (items_size < narrow + joins) return kErrWorkspaceTooSmall;
-    if (narrow > 0) __builtin_memcpy(items, plan.narrow.data(), narrow);
-    if (joins > 0) __builtin_memcpy(static_cast<uint8_t*>(items) + narrow, plan.joins.data(), joins);
+    if (items_size < narrow + wide + joins) return kErrWorkspaceTooSmall;
+    uint8_t* to = static_cast<uint8_t*>(items);
+    if (narrow > 0) std::memcpy(to, plan.narrow.data(), narrow);
+    if (wide > 0) std::memcpy(to + narrow, plan.wide.data(), wide);
+    if (joins > 0) std::memcpy(to + narrow + wide, plan.joins.data(), joins);
   } catch (...) {
     return kErrInvalidArgument;
   }
@@ -618,7 +953,8 @@ extern "C" int oscar_chunk_attention(const oscar_chunk_step* step, const void* i
       out->num_heads != step->num_heads || step->num_heads < 1 || step->num_heads % cache->num_kv_heads ||
       !(scale > 0.f) || !(scale <= 3.0e38f))
     return kErrInvalidArgument;
-  if (step->narrow <= 0) return kOk;
+  if (step->narrow < 0 || step->wide < 0 || step->joins < 0) return kErrInvalidArgument;
+  if (step->narrow + step->wide == 0) return kOk;
   if (items == nullptr || block_table == nullptr || query->data == nullptr || out->data == nullptr ||
       block_table_stride < step->table_cols)
     return kErrInvalidArgument;
@@ -646,7 +982,8 @@ extern "C" int oscar_chunk_attention(const oscar_chunk_step* step, const void* i
   a.table = block_table;
   a.table_stride = block_table_stride;
   a.pieces = static_cast<const Piece*>(items);
-  a.joins = reinterpret_cast<const Join*>(a.pieces + step->narrow);
+  a.wide0 = step->narrow;
+  a.joins = reinterpret_cast<const Join*>(a.pieces + step->narrow + step->wide);
   a.partials = static_cast<float*>(workspace);
   a.scale_log2 = scale * 1.4426950408889634f;
   a.group = step->num_heads / cache->num_kv_heads;

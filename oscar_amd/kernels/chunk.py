@@ -21,7 +21,7 @@ _i32, _i64 = ctypes.c_int32, ctypes.c_int64
 class ChunkStepArgs(ctypes.Structure):
     """struct oscar_chunk_step (include/oscar_amd.h)."""
     _fields_ = [("num_requests", _i32), ("num_tokens", _i32), ("num_heads", _i32), ("window", _i32),
-                ("table_cols", _i32), ("narrow", _i32), ("joins", _i32), ("reserved", _i32), ("items_size", _i64),
+                ("table_cols", _i32), ("narrow", _i32), ("wide", _i32), ("joins", _i32), ("items_size", _i64),
                 ("workspace_size", _i64)]
 
 
