@@ -620,6 +620,8 @@ typedef struct oscar_chunk_step {
   int32_t narrow;
   int32_t wide;
   int32_t joins;
+  int32_t few_joins;
+  int32_t reserved; /* 0 */
   int64_t items_size;
   int64_t workspace_size;
 } oscar_chunk_step;

@@ -31,6 +31,10 @@ COMMON = [
 PER_FILE = {
     "quant_write.hip": ["-ffp-contract=off"],
     "step_write.hip": ["-ffp-contract=off"],
+    # Matrix products leave their results in plain registers, where the softmax
+    # reads them (by default kernels of more than 256 registers get them in
+    # accumulation registers and a move per score).
+    "chunk_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
 }
 
 

@@ -22,9 +22,11 @@
 #include "plain_cache.h"
 
 #include <algorithm>
+#include <cstddef>
 #include <cstring>
 #include <functional>
 #include <type_traits>
+#include <utility>
 #include <vector>
 
 namespace oscar {
@@ -42,6 +44,7 @@ constexpr float kLazy = 8.f;               // a maximum is raised when a score e
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 typedef float floatx8 __attribute__((ext_vector_type(8)));
+typedef uint16_t ushortx2 __attribute__((ext_vector_type(2)));
 typedef short shortx4 __attribute__((ext_vector_type(4)));
 typedef short shortx8 __attribute__((ext_vector_type(8)));
 typedef __attribute__((address_space(3))) void lds_void;
@@ -52,6 +55,15 @@ struct Num;
 template <>
 struct Num<__bf16> {
   typedef bf16x8 V8;
+  static __device__ __forceinline__ V8 round8(const float (&f)[8]) {
+    // (settled here, in pairs: left to it, the compiler rounds value by value for
+    // the comparisons that follow and again for the product)
+    u32x4 w = __builtin_bit_cast(
+        u32x4, __builtin_convertvector((floatx8{f[0], f[1], f[2], f[3], f[4], f[5], f[6], f[7]}), V8));
+    asm volatile("" : "+v"(w));
+    return __builtin_bit_cast(V8, w);
+  }
+  static constexpr uint16_t kLazyBits = 0x4380;      // 2^kLazy
   static __device__ __forceinline__ floatx16 mfma(V8 a, V8 b, floatx16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
   }
@@ -66,6 +78,15 @@ struct Num<__bf16> {
 template <>
 struct Num<_Float16> {
   typedef half8 V8;
+  static __device__ __forceinline__ V8 round8(const float (&f)[8]) {
+    // (settled here, in pairs: left to it, the compiler rounds value by value for
+    // the comparisons that follow and again for the product)
+    u32x4 w = __builtin_bit_cast(
+        u32x4, __builtin_convertvector((floatx8{f[0], f[1], f[2], f[3], f[4], f[5], f[6], f[7]}), V8));
+    asm volatile("" : "+v"(w));
+    return __builtin_bit_cast(V8, w);
+  }
+  static constexpr uint16_t kLazyBits = 0x5C00;
   static __device__ __forceinline__ floatx16 mfma(V8 a, V8 b, floatx16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
   }
@@ -101,7 +122,8 @@ struct ChunkArgs {
   int64_t q_token, q_head, out_token, out_head;      // bytes
   const uint8_t* k;
   const uint8_t* v;
-  int64_t k_page, v_page, num_pages;
+  int64_t num_pages;
+  uint32_t k_page, v_page;                           // bytes
   int32_t k_token, v_token, k_head, v_head;          // bytes
   const int32_t* table;
   int64_t table_stride;
@@ -110,9 +132,34 @@ struct ChunkArgs {
   float* partials;         // slots of 32 rows: [32][D], then m[32], l[32]
   float scale_log2;
   int32_t group, block_size, window;
-  int32_t wide0;           // first piece of the wide kernel
+  int32_t narrow, wide;    // pieces, narrow ones first
+  int32_t few_joins;       // joins of few partials come first
   FastDiv group_div, block_div;
 };
+
+// f(0), f(1), .. f(N - 1) with constants.
+template <typename F, int... kI>
+__device__ __forceinline__ void each_of(F&& f, std::integer_sequence<int, kI...>) {
+  (f(std::integral_constant<int, kI>{}), ...);
+}
+template <int N, typename F>
+__device__ __forceinline__ void each(F&& f) { each_of(f, std::make_integer_sequence<int, N>{}); }
+
+// x, opaque to the compiler: what is computed from it stays where it is written,
+// instead of in registers through a loop.
+__device__ __forceinline__ int opaque(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+
+// A product stays before what is written after it.
+__device__ __forceinline__ void pin(floatx16& x) { asm volatile("" : "+v"(x)); }
+// The instructions before this stay before those after it: a product's steps are
+// written in the order in which they are to be issued.
+__device__ __forceinline__ void keep_order() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+}
 
 template <int N>
 __device__ __forceinline__ void wait_vmcnt() {
@@ -122,10 +169,6 @@ __device__ __forceinline__ void wait_vmcnt() {
 __device__ __forceinline__ void arrive_all() {
   __builtin_amdgcn_s_waitcnt(0x0070);       // vmcnt(0), lgkmcnt(0), expcnt left at its maximum
   asm volatile("s_barrier" ::: "memory");
-}
-__device__ __forceinline__ float other_half(float x) {       // lane ^ 32's
-  const auto s = __builtin_amdgcn_permlane32_swap(__float_as_int(x), __float_as_int(x), false, false);
-  return (threadIdx.x & 32) != 0 ? __int_as_float(s[0]) : __int_as_float(s[1]);
 }
 __device__ __forceinline__ float max_halves(float x) {
   const auto s = __builtin_amdgcn_permlane32_swap(__float_as_int(x), __float_as_int(x), false, false);
@@ -157,30 +200,45 @@ __device__ __forceinline__ int load_pages(const ChunkArgs& a, const Piece& p, in
   return page;
 }
 
-// Load kCount KB of consecutive keys from `key` on (inside one group of 16)
-// to LDS: K or V rows of one kv head.  Keys past the piece's and unmapped pages
-// arrive as zeros (records past the end).
+// Where a lane's 16 bytes lie in the first load of a run of keys: its key's row,
+// and its chunk.  The loads that follow are some keys further on, and xor-ed with
+// those keys' swizzle (their bits and the lane's are apart).
+struct LanePlace {
+  int row, chunk;          // bytes
+};
+template <int D, bool kV>
+__device__ __forceinline__ LanePlace lane_place(const ChunkArgs& a, int lane) {
+  constexpr int kLaneRow = D / 8;           // lanes of a row
+  const int key = lane / kLaneRow, place = lane % kLaneRow;
+  return LanePlace{key * (kV ? a.v_token : a.k_token),
+                   16 * (place ^ (kV ? v_swizzle<D>(key) : k_swizzle<D>(key)))};
+}
+
+// Load kCount KB of consecutive keys from `key` on (inside one group of 16, at
+// place in_page of `page`) to LDS: K or V rows of one kv head.  Keys past the
+// piece's and unmapped pages arrive as zeros (records past the end).
 template <int D, bool kV, int kCount>
 __device__ __forceinline__ void load_keys(const ChunkArgs& a, const Piece& p, int key, int key_in_tile, int page,
-                                          uint8_t* lds, int lane) {
-  constexpr int kLaneRow = D / 8;           // lanes of a row
+                                          int in_page, uint8_t* lds, const LanePlace& at) {
   constexpr int kStep = 512 / D;            // keys of a load
   const int stride = kV ? a.v_token : a.k_token;
-  const uint8_t* base = kV ? a.v : a.k;
-  const int in_page = (int)fast_mod((uint32_t)key, a.block_div);
   const int live = page < 0 ? 0 : min(16, p.key1 - key);
-  base += (int64_t)max(page, 0) * (kV ? a.v_page : a.k_page) + (int64_t)in_page * stride +
-          (int64_t)p.kv_head * (kV ? a.v_head : a.k_head);
+  const uint8_t* base = (kV ? a.v : a.k) + (int64_t)p.kv_head * (kV ? a.v_head : a.k_head) +
+                        (uint64_t)(uint32_t)max(page, 0) * (kV ? a.v_page : a.k_page) + (uint32_t)(in_page * stride);
   const uint32_t records = live > 0 ? (uint32_t)((live - 1) * stride + 2 * D) : 0u;
   const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)base, (short)0, records, 0x00020000);
-  const int lane_key = lane / kLaneRow, place = lane % kLaneRow;
 #pragma unroll
   for (int n = 0; n < kCount; ++n) {
-    const int r = n * kStep + lane_key;     // key of this lane, from `key` on
-    const int chunk = place ^ (kV ? v_swizzle<D>(key_in_tile + r) : k_swizzle<D>(key_in_tile + r));
+    const int first = key_in_tile + n * kStep;
+    const int turn = 16 * (kV ? v_swizzle<D>(first) : k_swizzle<D>(first));
     __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_void*)(lds + key_in_tile * 2 * D + n * 1024), 16,
-                                             r * stride + 16 * chunk, 0, 0, 0);
+                                             at.row + n * kStep * stride + (at.chunk ^ turn), 0, 0, 0);
   }
+}
+// A key's place in its page.  (The high product is a vector instruction: back to
+// a scalar, or the loads would loop over the descriptors of the lanes.)
+__device__ __forceinline__ int place_in_page(const ChunkArgs& a, int key) {
+  return __builtin_amdgcn_readfirstlane((int)fast_mod((uint32_t)key, a.block_div));
 }
 
 // A wave's 32 rows: queries, output sums, maximum and sum of weights.
@@ -212,73 +270,28 @@ __device__ __forceinline__ void load_rows(const ChunkArgs& a, const Piece& p, in
   s.last = p.pos0 + (int)fast_div((uint32_t)min(row0 + kTileRows - 1, end), a.group_div);
 }
 
-// S^T = K Q^T of one tile.
-template <typename T, int D>
-__device__ __forceinline__ floatx16 scores(const uint8_t* kt, int k_addr, const RowState<T, D>& s) {
-  floatx16 x{};
+// The first kCount scores a lane holds (register i: key 8 (i / 4) + 4 g + i % 4
+// of the tile) that its row, at `pos`, does not see become -inf.  `unmapped`: bit
+// h for keys 16h .. 16h + 15.
+template <int kCount>
+__device__ __forceinline__ void mask_scores(const ChunkArgs& a, floatx16& x, int key0, uint32_t unmapped, int lane,
+                                            int pos) {
+  const int hi = pos - key0 - 4 * (lane >> 5);
+  const int lo = a.window == 0 ? INT32_MIN : hi - a.window;
 #pragma unroll
-  for (int i = 0; i < D / 16; ++i)
-    x = Num<T>::mfma(*reinterpret_cast<const typename Num<T>::V8*>(kt + (k_addr ^ (32 * i))), s.q[i], x);
-  return x;
-}
-
-// Weights of one tile: exp2(score - m), rounded to T for the product and summed
-// as rounded, so that the output stays a mean of the values.  `unmapped`: bit h
-// for keys 16h .. 16h + 15.
-template <typename T, int D>
-__device__ __forceinline__ void weights(const ChunkArgs& a, floatx16& x, int key0, uint32_t unmapped, int lane,
-                                        RowState<T, D>& s, typename Num<T>::V8 (&p)[2]) {
-  const bool whole = key0 + kTileKeys - 1 <= s.first && (a.window == 0 || key0 > s.last - a.window) && unmapped == 0u;
-  if (!whole) {
-    const int g4 = 4 * (lane >> 5);
-    const int hi = s.pos - key0 - g4;       // register i holds key 8 (i / 4) + 4 g + i % 4
-    const int lo = a.window == 0 ? INT32_MIN : hi - a.window;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const int key = 8 * (i >> 2) + (i & 3);
-      const bool seen = key <= hi && key > lo && ((unmapped >> (i >> 3)) & 1u) == 0u;
-      x[i] = seen ? x[i] : -__builtin_inff();
-    }
-  }
-  float top = x[0];
-#pragma unroll
-  for (int i = 1; i < 16; ++i) top = fmaxf(top, x[i]);
-  top = max_halves(top) * a.scale_log2;
-  const bool raise = top > s.m + kLazy;
-  if (__ballot(raise)) {
-    const float m = raise ? top : s.m;
-    const float alpha = __builtin_amdgcn_exp2f(s.m - m);
-#pragma unroll
-    for (int i = 0; i < D / 32; ++i) s.acc[i] *= alpha;
-    s.l *= alpha;
-    s.m = m;
-  }
-#pragma unroll
-  for (int i = 0; i < 16; ++i) x[i] = __builtin_amdgcn_exp2f(x[i] * a.scale_log2 - s.m);
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    floatx8 w;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) w[i] = x[8 * h + i];
-    p[h] = __builtin_convertvector(w, typename Num<T>::V8);
-    s.l = Num<T>::sum8(p[h], s.l);
+  for (int i = 0; i < kCount; ++i) {
+    const int key = 8 * (i >> 2) + (i & 3);
+    x[i] = key <= hi && key > lo && ((unmapped >> (i >> 3)) & 1u) == 0u ? x[i] : -__builtin_inff();
   }
 }
 
-// O^T += V^T P^T of one tile: feature block b of keys 16 h + 8 (u / 4) + 4 g + u % 4.
+// V^T operand of feature block b and keys 16 h + 8 (u / 4) + 4 g + u % 4.
 template <typename T, int D>
-__device__ __forceinline__ void values(const uint8_t* vt, int v_addr, const typename Num<T>::V8 (&p)[2],
-                                       RowState<T, D>& s) {
-#pragma unroll
-  for (int h = 0; h < 2; ++h)
-#pragma unroll
-    for (int b = 0; b < D / 32; ++b) {
-      const uint8_t* at = vt + (v_addr ^ (64 * b)) + h * 32 * D;
-      const shortx4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)at);
-      const shortx4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(at + 16 * D));
-      const shortx8 v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-      s.acc[b] = Num<T>::mfma(__builtin_bit_cast(typename Num<T>::V8, v), p[h], s.acc[b]);
-    }
+__device__ __forceinline__ typename Num<T>::V8 v_operand_at(const uint8_t* vt, int v_addr, int h, int b) {
+  const uint8_t* at = vt + (v_addr ^ (64 * b)) + h * 32 * D;
+  const shortx4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)at);
+  const shortx4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(at + 16 * D));
+  return __builtin_bit_cast(typename Num<T>::V8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
 }
 
 // This lane's place in the reads of a K tile (key lane % 32, chunk 2 i + lane /
@@ -313,384 +326,450 @@ __device__ __forceinline__ uint8_t* out_row(const ChunkArgs& a, int token0, int 
 // their own (no barrier until they combine): few rows, so memory bounds it, and
 // what matters is loads in flight.  A wave's K and V tile each have one place
 // in LDS; the next K tile is requested when the scores are done, the next V
-// tile when its sums are, so that one or two tiles (32 D .. 128 D bytes a wave)
-// are always on their way.
-template <typename T, int D>
-__global__ __launch_bounds__(kThreads, 1) void narrow_kernel(ChunkArgs a) {
-  extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
-  constexpr int kTileBytes = kTileKeys * 2 * D;
-  constexpr int kLoads = D / 16;            // of a tile
+// tile when its sums are, so that one or two tiles are always on their way.
+// Tiles are 32 keys, or, beside wide pieces at D = 256, 16 (the upper half of the
+// score tile is then the lower one's again and not used), so that two workgroups
+// fit a CU's LDS; alone they are slower (32 users' 4 tokens over 2K to 16K keys
+// 61.8 us with 32 keys, 64.7 with 16).
+constexpr int beside_keys(int d) { return d == 256 ? 16 : 32; }
+constexpr int narrow_lds(int d, int keys) { return kWaves * 2 * keys * 2 * d + kWaves * 2 * kTileRows * 4; }
+
+template <typename T, int D, int kKeys>
+__device__ __forceinline__ void narrow_piece(const ChunkArgs& a, const Piece p, uint8_t* smem) {
+  typedef typename Num<T>::V8 V8;
+  constexpr int kHalves = kKeys / 16;
+  constexpr int kTileBytes = kKeys * 2 * D;
+  constexpr int kLoads = kTileBytes / 1024;
+  constexpr int kBlocks = D / 32;
   const int tid = (int)threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const Piece p = a.pieces[blockIdx.x];
-  uint8_t* kt = smem + wave * 2 * kTileBytes;
-  uint8_t* vt = kt + kTileBytes;
 
-  const int tiles = (p.key1 - p.key0 + kTileKeys - 1) / kTileKeys;
-  const int first = p.key0 / kTileKeys + tiles * wave / kWaves;
-  const int last = p.key0 / kTileKeys + tiles * (wave + 1) / kWaves;
+  const int tiles = (p.key1 - p.key0 + kKeys - 1) / kKeys;
+  const int first = p.key0 / kKeys + tiles * wave / kWaves;
+  const int last = p.key0 / kKeys + tiles * (wave + 1) / kWaves;
 
-  int page_base = 2 * first;
+  int page_base = kHalves * first;
   int pages = load_pages(a, p, page_base, lane);
   RowState<T, D> s;
   load_rows<T, D>(a, p, p.row0, lane, s);
+  const int whole_from = a.window == 0 ? 0 : s.last - a.window + 1, whole_to = s.first - kKeys + 1;
 
-  auto page_of = [&](int t, int h) { return __builtin_amdgcn_readlane(pages, 2 * t + h - page_base); };
+  const LanePlace k_place = lane_place<D, false>(a, lane), v_place = lane_place<D, true>(a, lane);
+  auto page_of = [&](int t, int h) { return __builtin_amdgcn_readlane(pages, kHalves * t + h - page_base); };
   auto load_tile = [&](int t, auto v_tag, uint8_t* lds) {
     constexpr bool kV = decltype(v_tag)::value;
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
-      load_keys<D, kV, kLoads / 2>(a, p, t * kTileKeys + 16 * h, 16 * h, page_of(t, h), lds, lane);
+    for (int h = 0; h < kHalves; ++h)
+      load_keys<D, kV, kLoads / kHalves>(a, p, t * kKeys + 16 * h, 16 * h, page_of(t, h),
+                                         place_in_page(a, t * kKeys + 16 * h), lds, kV ? v_place : k_place);
   };
-  const int k_addr = k_read<D>(lane), v_addr = v_read<D>(lane);
+  const int k_addr = k_read<D>(lane & (32 + kKeys - 1)), v_addr = v_read<D>(lane);
 
-  if (first < last) {
-    load_tile(first, std::false_type{}, kt);
-    __builtin_amdgcn_sched_barrier(0);      // (the waits below count K's loads before V's)
-    load_tile(first, std::true_type{}, vt);
-  }
   // One tile.  (The two places as parameters that do not alias: the compiler
   // then sees that a V read does not wait for the K tile that is on its way.)
   auto tile = [&](int t, uint8_t* __restrict__ kt, uint8_t* __restrict__ vt) __attribute__((always_inline)) {
-    const uint32_t unmapped = (page_of(t, 0) < 0 ? 1u : 0u) | (page_of(t, 1) < 0 ? 2u : 0u);
+    uint32_t unmapped = 0;
+#pragma unroll
+    for (int h = 0; h < kHalves; ++h) unmapped |= page_of(t, h) < 0 ? 1u << h : 0u;
     const bool more = t + 1 < last;
-    if (more && 2 * (t + 1) - page_base >= 64) {
-      page_base = 2 * (t + 1);
+    if (more && kHalves * (t + 1) - page_base >= 64) {
+      page_base = kHalves * (t + 1);
       pages = load_pages(a, p, page_base, lane);
     }
     wait_vmcnt<kLoads>();                   // K is there, V on its way
     asm volatile("" ::: "memory");
-    floatx16 x = scores<T, D>(kt, k_addr, s);
+    floatx16 x{};
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i)
+      x = Num<T>::mfma(*reinterpret_cast<const V8*>(kt + (k_addr ^ (32 * i))), s.q[i], x);
     asm volatile("" ::: "memory");
     if (more) load_tile(t + 1, std::false_type{}, kt);
-    typename Num<T>::V8 w[2];
-    weights<T, D>(a, x, t * kTileKeys, unmapped, lane, s, w);
+
+    const int key0 = t * kKeys;
+    if (!(key0 >= whole_from && key0 <= whole_to && unmapped == 0u)) mask_scores<8 * kHalves>(a, x, key0, unmapped, lane, s.pos);
+    float top = x[0];
+#pragma unroll
+    for (int i = 1; i < 8 * kHalves; ++i) top = fmaxf(top, x[i]);
+    top = max_halves(top) * a.scale_log2;
+    const bool raise = top > s.m + kLazy;
+    if (__ballot(raise)) {
+      const float m = raise ? top : s.m, f = __builtin_amdgcn_exp2f(s.m - m);
+#pragma unroll
+      for (int b = 0; b < kBlocks; ++b) s.acc[b] *= f;
+      s.l *= f;
+      s.m = m;
+    }
+    V8 w[kHalves];
+#pragma unroll
+    for (int h = 0; h < kHalves; ++h) {
+      float f[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[i] = __builtin_amdgcn_exp2f(x[8 * h + i] * a.scale_log2 - s.m);
+      w[h] = Num<T>::round8(f);
+      s.l = Num<T>::sum8(w[h], s.l);
+    }
+
     if (more) wait_vmcnt<kLoads>();
     else wait_vmcnt<0>();
     asm volatile("" ::: "memory");
-    values<T, D>(vt, v_addr, w, s);
+#pragma unroll
+    for (int h = 0; h < kHalves; ++h)
+#pragma unroll
+      for (int b = 0; b < kBlocks; ++b)
+        s.acc[b] = Num<T>::mfma(v_operand_at<T, D>(vt, v_addr, h, b), w[h], s.acc[b]);
     asm volatile("" ::: "memory");
     if (more) load_tile(t + 1, std::true_type{}, vt);
   };
-  for (int t = first; t < last; ++t) tile(t, kt, vt);
-
-  // Combine: every wave's sums to LDS (16-byte pieces, the row xor-ed in).
-  float* sums = reinterpret_cast<float*>(smem);
-  float* ml = sums + kWaves * kTileRows * D;          // [wave][m | l][32]
-  s.l = sum_halves(s.l);
-  arrive_all();
-  const int row = lane & 31;
-  if (row < p.rows) {
-#pragma unroll
-    for (int b = 0; b < D / 32; ++b)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int piece = 8 * b + 2 * i + (lane >> 5);
-        *reinterpret_cast<floatx4*>(sums + (wave * kTileRows + row) * D + 4 * (piece ^ (row & 15))) =
-            floatx4{s.acc[b][4 * i], s.acc[b][4 * i + 1], s.acc[b][4 * i + 2], s.acc[b][4 * i + 3]};
-      }
-    ml[wave * 64 + (lane >> 5) * 32 + row] = lane < 32 ? s.m : s.l;
+  uint8_t* const kt = smem + wave * 2 * kTileBytes;
+  if (first < last) {
+    load_tile(first, std::false_type{}, kt);
+    __builtin_amdgcn_sched_barrier(0);      // (the waits count K's loads before V's)
+    load_tile(first, std::true_type{}, kt + kTileBytes);
   }
-  __syncthreads();
-  for (int i = tid; i < p.rows * (D / 4); i += kThreads) {
-    const int r = i / (D / 4), piece = i % (D / 4);
-    float m = ml[r];
+  for (int t = first; t < last; ++t) tile(t, kt, kt + kTileBytes);
+
+  // Combine: the waves' sums through LDS, D / kRounds features at a time (16-byte
+  // pieces, the row xor-ed in).
+  constexpr int kRounds = 32 / kKeys, kPart = D / kRounds;
+  float* const sums = reinterpret_cast<float*>(smem);
+  float* const ml = sums + kWaves * kTileRows * kPart;          // [wave][m | l][32]
+  s.l = sum_halves(s.l);
+  const int row = lane & 31;
 #pragma unroll
-    for (int w = 1; w < kWaves; ++w) m = fmaxf(m, ml[w * 64 + r]);
-    floatx4 o{};
-    float l = 0.f;
+  for (int round = 0; round < kRounds; ++round) {
+    arrive_all();
+    if (row < p.rows) {
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
-      const float f = __builtin_amdgcn_exp2f(ml[w * 64 + r] - m);
-      l += f * ml[w * 64 + 32 + r];
-      o += f * *reinterpret_cast<const floatx4*>(sums + (w * kTileRows + r) * D + 4 * (piece ^ (r & 15)));
+      for (int b = 0; b < kPart / 32; ++b)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int piece = 8 * b + 2 * i + (lane >> 5);
+          const floatx16& acc = s.acc[round * kPart / 32 + b];
+          *reinterpret_cast<floatx4*>(sums + (wave * kTileRows + row) * kPart + 4 * (piece ^ (row & 15))) =
+              floatx4{acc[4 * i], acc[4 * i + 1], acc[4 * i + 2], acc[4 * i + 3]};
+        }
+      ml[wave * 64 + (lane >> 5) * 32 + row] = lane < 32 ? s.m : s.l;
     }
-    if (p.slot < 0) {
-      const float inv = l == 0.f ? 0.f : 1.f / l;
-      store4<T>(out_row(a, p.token0, p.kv_head, p.row0 + r) + 8 * piece, o * inv);
-    } else {
-      float* part = a.partials + (int64_t)p.slot * (kTileRows * (D + 2));
-      *reinterpret_cast<floatx4*>(part + r * D + 4 * piece) = o;
-      if (piece == 0) {
-        part[kTileRows * D + r] = m;
-        part[kTileRows * D + kTileRows + r] = l;
+    __syncthreads();
+    for (int i = tid; i < p.rows * (kPart / 4); i += kThreads) {
+      const int r = i / (kPart / 4), piece = i % (kPart / 4), feature = round * kPart + 4 * piece;
+      float m = ml[r];
+#pragma unroll
+      for (int w = 1; w < kWaves; ++w) m = fmaxf(m, ml[w * 64 + r]);
+      floatx4 o{};
+      float l = 0.f;
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) {
+        const float f = __builtin_amdgcn_exp2f(ml[w * 64 + r] - m);
+        l += f * ml[w * 64 + 32 + r];
+        o += f * *reinterpret_cast<const floatx4*>(sums + (w * kTileRows + r) * kPart + 4 * (piece ^ (r & 15)));
+      }
+      if (p.slot < 0) {
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        store4<T>(out_row(a, p.token0, p.kv_head, p.row0 + r) + 2 * feature, o * inv);
+      } else {
+        float* part = a.partials + (int64_t)p.slot * (kTileRows * (D + 2));
+        *reinterpret_cast<floatx4*>(part + r * D + feature) = o;
+        if (feature == 0) {
+          part[kTileRows * D + r] = m;
+          part[kTileRows * D + kTileRows + r] = l;
+        }
       }
     }
   }
 }
 
-// ---------------------------------------------------------------- 256 rows
-// A wide row tile: kW waves of kR times 32 rows each, over tiles of 32 keys that
-// all of them read from LDS.  The scores of a tile are computed one tile ahead,
-// so that products and softmax overlap inside a wave: iteration t runs
-//   A:  S(t + 1) = K Q^T        beside the weights of the tile's first 16 keys,
-//   B1: O += V^T P^T, 16 keys   beside the weights of the other 16,
-//   B2: O += V^T P^T, 16 keys   beside the maximum of S(t + 1),
-// each step of a product followed by its share of the arithmetic (the order is
-// the schedule: scheduling barriers keep it).  K and V tiles come through rings
-// of four places, requested two iterations ahead; one barrier an iteration, in
-// the middle of B, where the K tile just used and the V tile before this one
-// are given up.
-constexpr int kWideRows = 256;
-constexpr int kRing = 4;
+// ---------------------------------------------------------------- 128 rows
+// A wide row tile: four waves of 32 rows each, over stages of keys in LDS that
+// all four read, two stages in turn: while one is computed, the next is on its
+// way.  A wave does a tile's products and softmax one after the other; the
+// matrix unit is kept busy by the waves of the other workgroups on the CU, which
+// no barrier ties to this one.
+constexpr int kWideRows = 32 * kWaves;
+constexpr int kWideWgs = 2;                                      // workgroups a CU
+constexpr int stage_tiles(int d) { return d == 256 ? 1 : 2; }    // 32-key tiles of a stage
 
 template <int D>
-constexpr int wide_lds() { return 2 * kRing * kTileKeys * 2 * D; }
+constexpr int wide_lds() { return 2 * 2 * stage_tiles(D) * kTileKeys * 2 * D; }
 
-template <typename T, int D, int kR, int kW, int kWgs>
-__global__ __launch_bounds__(64 * kW, kW * kWgs / 4) void wide_kernel(ChunkArgs a) {
-  extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+template <typename T, int D>
+__device__ __forceinline__ void wide_piece(const ChunkArgs& a, const Piece p, uint8_t* smem) {
   typedef typename Num<T>::V8 V8;
+  constexpr int kTiles = stage_tiles(D);
   constexpr int kTileBytes = kTileKeys * 2 * D;
-  constexpr int kLoads = kTileBytes / 1024 / kW;       // of a tile and wave
-  constexpr int kKeys = kTileKeys / kW;                // keys of a tile that a wave loads
-  constexpr int kSteps = D / 16, kBlocks = D / 32;
-  constexpr int kAhead = D == 256 ? 2 : 4;
-  static_assert(kLoads * 1024 * kW == kTileBytes && kR * kW * 32 == kWideRows, "whole kilobytes a wave");
+  constexpr int kStageBytes = 2 * kTiles * kTileBytes;           // K tiles, then V tiles
+  constexpr int kLoads = kTiles * kTileBytes / 1024 / kWaves;    // of a stage's K, a wave
+  constexpr int kKeys = kTiles * kTileKeys / kWaves;             // that it loads: inside a group of 16
+  constexpr int kSteps = D / 16, kBlocks = D / 32, kPv = 2 * kBlocks;
+  constexpr int kAheadK = D == 128 ? 6 : 4, kAheadV = D == 256 ? 2 : D == 128 ? 6 : 4;     // operands read ahead
+  constexpr bool kKeepAddresses = D <= 128;      // of the operand reads in registers (D = 256 has none left)
   const int tid = (int)threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const Piece p = a.pieces[a.wide0 + blockIdx.x];
-  uint8_t* const kring = smem;
-  uint8_t* const vring = smem + kRing * kTileBytes;
   const int tiles = (p.key1 - p.key0 + kTileKeys - 1) / kTileKeys;
   const int group0 = p.key0 / 16;
 
   int page_base = group0;
   int pages = load_pages(a, p, page_base, lane);
-  RowState<T, D> s[kR];
-#pragma unroll
-  for (int r = 0; r < kR; ++r) load_rows<T, D>(a, p, p.row0 + 32 * (kR * wave + r), lane, s[r]);
-  const int first = s[0].first, last = s[kR - 1].last;
+  RowState<T, D> s;
+  load_rows<T, D>(a, p, p.row0 + kTileRows * wave, lane, s);
 
-  // Tile u's page of this wave's keys (kept until its V is requested, two tiles
-  // later), and which halves of the tiles from the last requested one back are
-  // unmapped, two bits each.
-  int page_next = 0, page_after = 0;
-  uint32_t unmapped = 0;
-  auto request_k = [&](int u) {
-    const int g = group0 + 2 * u - page_base;
-    if (g >= 64) {
-      page_base += g;
-      pages = load_pages(a, p, page_base, lane);
-    }
-    const int at = group0 + 2 * u - page_base;
-    const int lo = __builtin_amdgcn_readlane(pages, at), hi = __builtin_amdgcn_readlane(pages, at + 1);
-    const int page = kKeys * wave < 16 ? lo : hi;
-    unmapped = (unmapped << 2) | (lo < 0 ? 1u : 0u) | (hi < 0 ? 2u : 0u);
-    load_keys<D, false, kLoads>(a, p, p.key0 + u * kTileKeys + kKeys * wave, kKeys * wave, page,
-                                kring + (u % kRing) * kTileBytes, lane);
-    return page;
-  };
-  auto request_v = [&](int u, int page) {
-    load_keys<D, true, kLoads>(a, p, p.key0 + u * kTileKeys + kKeys * wave, kKeys * wave, page,
-                               vring + (u % kRing) * kTileBytes, lane);
-  };
-  // (the waits below count these in this order)
-  const int p0 = request_k(0);
-  __builtin_amdgcn_sched_barrier(0);
-  const int p1 = request_k(1);
-  page_next = request_k(2);
-  request_v(0, p0);
-  __builtin_amdgcn_sched_barrier(0);
-  page_after = request_k(3);
-  request_v(1, p1);
-  __builtin_amdgcn_sched_barrier(0);
-
+  LanePlace k_place = lane_place<D, false>(a, lane), v_place = lane_place<D, true>(a, lane);
   const int k_addr = k_read<D>(lane), v_addr = v_read<D>(lane);
+  // A stage's keys of this wave: their page and place in it (found with K's
+  // request, V's are the same), and which groups of 16 keys are unmapped.
+  int page = 0, in_page = place_in_page(a, p.key0 + kKeys * wave);
+  const int advance = place_in_page(a, kTiles * kTileKeys);
+  uint32_t gone_next = 0;
+  auto request_k = [&](int stage, uint8_t* to) __attribute__((always_inline)) {
+    const int group = group0 + 2 * kTiles * stage;
+    if (group - page_base >= 64) {
+      page_base = group;
+      pages = load_pages(a, p, page_base, opaque(lane));
+    }
+    const int at = group - page_base;
+    gone_next = 0;
+#pragma unroll
+    for (int h = 0; h < 2 * kTiles; ++h) {
+      const int g = __builtin_amdgcn_readlane(pages, at + h);
+      gone_next |= g < 0 ? 1u << h : 0u;
+      page = h == 0 || kKeys * wave >= 16 * h ? g : page;
+    }
+    if (stage > 0) {
+      in_page += advance;
+      in_page -= in_page >= a.block_size ? a.block_size : 0;
+    }
+    load_keys<D, false, kLoads>(a, p, p.key0 + kTiles * kTileKeys * stage + kKeys * wave, kKeys * wave, page, in_page,
+                                to, k_place);
+  };
+  auto request_v = [&](int stage, uint8_t* to) __attribute__((always_inline)) {
+    load_keys<D, true, kLoads>(a, p, p.key0 + kTiles * kTileKeys * stage + kKeys * wave, kKeys * wave, page, in_page,
+                               to + kTiles * kTileBytes, v_place);
+  };
   auto k_operand = [&](const uint8_t* kt, int i) {
-    return *reinterpret_cast<const V8*>(kt + (k_addr ^ (32 * i)));
+    const int at = kKeepAddresses ? k_addr : opaque(k_addr);
+    return *reinterpret_cast<const V8*>(kt + (at ^ (32 * i)));
   };
-  auto v_operand = [&](const uint8_t* vt, int h, int b) {
-    const uint8_t* at = vt + (v_addr ^ (64 * b)) + h * 32 * D;
-    const shortx4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)at);
-    const shortx4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(at + 16 * D));
-    return __builtin_bit_cast(V8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+  auto v_operand = [&](const uint8_t* vt, int i) {
+    return v_operand_at<T, D>(vt, kKeepAddresses ? v_addr : opaque(v_addr), i / kBlocks, i % kBlocks);
   };
-  // The running maxima, raised where a tile's scores ask for it.
-  auto raise_max = [&](float (&top)[kR]) {
-    bool raise[kR], any = false;
+  // Rows that do not see the whole of a tile lose what they do not see.
+  const int whole_from = a.window == 0 ? 0 : s.last - a.window + 1, whole_to = s.first - kTileKeys + 1;
+  auto mask = [&](floatx16& x, int key0, uint32_t gone) {
+    if (__builtin_expect(key0 >= whole_from && key0 <= whole_to && gone == 0u, 1)) return;
+    mask_scores<16>(a, x, key0, gone, lane, s.pos);
+  };
+  auto weigh = [&](const floatx16& x, V8 (&w)[2]) {
 #pragma unroll
-    for (int r = 0; r < kR; ++r) {
-      top[r] = max_halves(top[r]) * a.scale_log2;
-      raise[r] = top[r] > s[r].m + kLazy;
-      any = any || raise[r];
-    }
-    if (__ballot(any)) {
+    for (int h = 0; h < 2; ++h) {
+      float f[8];
 #pragma unroll
-      for (int r = 0; r < kR; ++r) {
-        const float m = raise[r] ? top[r] : s[r].m, f = __builtin_amdgcn_exp2f(s[r].m - m);
-#pragma unroll
-        for (int b = 0; b < kBlocks; ++b) s[r].acc[b] *= f;
-        s[r].l *= f;
-        s[r].m = m;
-      }
+      for (int i = 0; i < 8; ++i) f[i] = __builtin_amdgcn_exp2f(x[8 * h + i] * a.scale_log2 - s.m);
+      w[h] = Num<T>::round8(f);
+      __builtin_amdgcn_sched_barrier(0);    // (eight at a time: registers)
     }
   };
-  // Rows that do not see the whole of tile u lose what they do not see.
-  auto mask_tile = [&](floatx16 (&x)[kR], int u, uint32_t gone) {
-    const int key0 = p.key0 + u * kTileKeys;
-    if (key0 + kTileKeys - 1 <= first && (a.window == 0 || key0 > last - a.window) && gone == 0u) return;
+  // Some weight is above 2^kLazy (or no number).  Positive numbers compare as
+  // their bits do, so this takes nine operations for a tile, where the maximum of
+  // the scores takes one for each.
+  auto beyond = [&](const V8 (&w)[2]) {
+    typedef uint16_t ushortx8 __attribute__((ext_vector_type(8)));
+    ushortx8 u = __builtin_elementwise_max(__builtin_bit_cast(ushortx8, w[0]), __builtin_bit_cast(ushortx8, w[1]));
+    const ushortx2 top = __builtin_elementwise_max(
+        __builtin_elementwise_max(__builtin_shufflevector(u, u, 0, 1), __builtin_shufflevector(u, u, 2, 3)),
+        __builtin_elementwise_max(__builtin_shufflevector(u, u, 4, 5), __builtin_shufflevector(u, u, 6, 7)));
+    const ushortx2 most{Num<T>::kLazyBits, Num<T>::kLazyBits};
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_sub_sat(top, most)) != 0u;
+  };
+  // Raises the running maximum to that of the tile's scores where a weight was
+  // too large (always so for the first keys of a row), and rescales the sums.
+  auto raise = [&](const floatx16& x) __attribute__((always_inline)) {
+    float top = x[0];
 #pragma unroll
-    for (int r = 0; r < kR; ++r) {
-      const int hi = s[r].pos - key0 - 4 * (lane >> 5);
-      const int lo = a.window == 0 ? INT32_MIN : hi - a.window;
+    for (int i = 1; i < 16; ++i) top = fmaxf(top, x[i]);
+    top = max_halves(top) * a.scale_log2;
+    const float m = top > s.m + kLazy ? top : s.m, f = __builtin_amdgcn_exp2f(s.m - m);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int key = 8 * (i >> 2) + (i & 3);
-        x[r][i] = key <= hi && key > lo && ((gone >> (i >> 3)) & 1u) == 0u ? x[r][i] : -__builtin_inff();
-      }
-    }
+    for (int b = 0; b < kBlocks; ++b) s.acc[b] *= f;
+    s.l *= f;
+    s.m = m;
   };
 
-  // ---- first scores ----
-  floatx16 xa[kR], xb[kR];
-  wait_vmcnt<5 * kLoads>();                 // K(0) is there
-  asm volatile("s_barrier" ::: "memory");
-#pragma unroll
-  for (int r = 0; r < kR; ++r) xa[r] = floatx16{};
-#pragma unroll
-  for (int i = 0; i < kSteps; ++i) {
-    const V8 k = k_operand(kring, i);
-#pragma unroll
-    for (int r = 0; r < kR; ++r) xa[r] = Num<T>::mfma(k, s[r].q[i], xa[r]);
-  }
-  mask_tile(xa, 0, (unmapped >> 6) & 3u);
-  float top[kR];
-#pragma unroll
-  for (int r = 0; r < kR; ++r) {
-    top[r] = xa[r][0];
-#pragma unroll
-    for (int i = 1; i < 16; ++i) top[r] = fmaxf(top[r], xa[r][i]);
-  }
-  raise_max(top);
-  wait_vmcnt<2 * kLoads>();                 // K(1), K(2), V(0) are there
-  asm volatile("s_barrier" ::: "memory");
-  {
-    const int page = request_k(4);
-    request_v(2, page_next);
-    page_next = page_after;
-    page_after = page;
-  }
-
-  // One iteration: tile t's scores are in x, tile t + 1's come to y.
-  auto iterate = [&](int t, floatx16 (&x)[kR], floatx16 (&y)[kR], uint8_t* __restrict__ kr,
-                     uint8_t* __restrict__ vr) __attribute__((always_inline)) {
-    const uint8_t* kt = kr + ((t + 1) % kRing) * kTileBytes;
-    const uint8_t* vt = vr + (t % kRing) * kTileBytes;
-    V8 w[kR][2];                            // [rows][key half]
-    auto weight = [&](int e) {
-#pragma unroll
-      for (int r = 0; r < kR; ++r) x[r][e] = __builtin_amdgcn_exp2f(x[r][e] * a.scale_log2 - s[r].m);
-    };
-    auto round = [&](int h) {
-#pragma unroll
-      for (int r = 0; r < kR; ++r) {
-        floatx8 f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] = x[r][8 * h + i];
-        w[r][h] = __builtin_convertvector(f, V8);
-        s[r].l = Num<T>::sum8(w[r][h], s[r].l);
-      }
-    };
-    // A
-    V8 k[kAhead];
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i) k[i] = k_operand(kt, i);
-    __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-    for (int i = 0; i < kSteps; ++i) {
-#pragma unroll
-      for (int r = 0; r < kR; ++r) y[r] = Num<T>::mfma(k[i % kAhead], s[r].q[i], i == 0 ? floatx16{} : y[r]);
-      if (i + kAhead < kSteps) k[i % kAhead] = k_operand(kt, i + kAhead);
-#pragma unroll
-      for (int e = i * 8 / kSteps; e < (i + 1) * 8 / kSteps; ++e) weight(e);
-      __builtin_amdgcn_sched_barrier(0);
+  // One tile; `requests(i)` goes out beside step i of its first product.
+  auto tile = [&](const uint8_t* __restrict__ kt, const uint8_t* __restrict__ vt, int key0, uint32_t gone,
+                  auto&& requests) __attribute__((always_inline)) {
+    if constexpr (!kKeepAddresses) {
+      k_place = LanePlace{opaque(k_place.row), opaque(k_place.chunk)};
+      v_place = LanePlace{opaque(v_place.row), opaque(v_place.chunk)};
     }
-    V8 v[kAhead];
-    constexpr int kPv = 2 * kBlocks;
+    // S^T = K Q^T
+    V8 k[kAheadK];
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) v[i] = v_operand(vt, i / kBlocks, i % kBlocks);
-    round(0);
-    __builtin_amdgcn_sched_barrier(0);
-    mask_tile(y, t + 1, (unmapped >> 6) & 3u);
-    // B1, B2
-    float top[kR];
+    for (int i = 0; i < kAheadK; ++i) k[i] = k_operand(kt, i);
+    keep_order();
+    __builtin_amdgcn_s_setprio(1);
+    floatx16 x;
+    each<kSteps>([&](auto step) {
+      constexpr int i = decltype(step)::value;
+      x = Num<T>::mfma(k[i % kAheadK], s.q[i], i == 0 ? floatx16{} : x);
+      pin(x);
+      if constexpr (i + kAheadK < kSteps) k[i % kAheadK] = k_operand(kt, i + kAheadK);
+      keep_order();
+      requests(i);
+      keep_order();
+    });
+    V8 v[kAheadV];
 #pragma unroll
-    for (int i = 0; i < kPv; ++i) {
-      const int h = i / kBlocks, b = i % kBlocks;
-      if (i == kBlocks) {
-        round(1);
-        wait_vmcnt<2 * kLoads>();           // K(t + 2), V(t + 1) are there
-        asm volatile("s_barrier" ::: "memory");
-        const int page = request_k(t + 5);
-        request_v(t + 3, page_next);
-        page_next = page_after;
-        page_after = page;
-      }
-#pragma unroll
-      for (int r = 0; r < kR; ++r) s[r].acc[b] = Num<T>::mfma(v[i % kAhead], w[r][h], s[r].acc[b]);
-      if (i + kAhead < kPv) v[i % kAhead] = v_operand(vt, (i + kAhead) / kBlocks, (i + kAhead) % kBlocks);
-      if (h == 0) {
-#pragma unroll
-        for (int e = 8 + b * 8 / kBlocks; e < 8 + (b + 1) * 8 / kBlocks; ++e) weight(e);
-      } else {
-#pragma unroll
-        for (int r = 0; r < kR; ++r) {
-          if (b == 0) top[r] = y[r][0];
-#pragma unroll
-          for (int e = b * 16 / kBlocks; e < (b + 1) * 16 / kBlocks; ++e) top[r] = fmaxf(top[r], y[r][e]);
-        }
-      }
-      __builtin_amdgcn_sched_barrier(0);
+    for (int i = 0; i < kAheadV; ++i) v[i] = v_operand(vt, i);
+    __builtin_amdgcn_s_setprio(0);
+    mask(x, key0, gone);
+    V8 w[2];
+    weigh(x, w);
+    if (__ballot(beyond(w))) {
+      raise(x);
+      weigh(x, w);
     }
-    raise_max(top);
+    keep_order();
+    __builtin_amdgcn_s_setprio(1);
+    // O^T += V^T P^T
+    each<kPv>([&](auto step) {
+      constexpr int i = decltype(step)::value, h = i / kBlocks, b = i % kBlocks;
+      s.acc[b] = Num<T>::mfma(v[i % kAheadV], w[h], s.acc[b]);
+      pin(s.acc[b]);
+      if constexpr (i + kAheadV < kPv) v[i % kAheadV] = v_operand(vt, i + kAheadV);
+      if constexpr (b == 0) s.l = Num<T>::sum8(w[h], s.l);
+      keep_order();
+    });
+    __builtin_amdgcn_s_setprio(0);
   };
-  for (int t = 0; t < tiles; t += 2) {
-    iterate(t, xa, xb, kring, vring);
-    if (t + 1 < tiles) iterate(t + 1, xb, xa, kring, vring);
+
+  request_k(0, smem);
+  request_v(0, smem);
+#pragma unroll
+  for (int i = 0; i < kSteps; ++i) {        // the queries are in registers before the sums take theirs
+    u32x4 q = __builtin_bit_cast(u32x4, s.q[i]);
+    asm volatile("" : "+v"(q));
+    s.q[i] = __builtin_bit_cast(V8, q);
+  }
+  keep_order();
+#pragma unroll
+  for (int b = 0; b < kBlocks; ++b) s.acc[b] = floatx16{};
+  int stage = 0;
+  auto run = [&](uint8_t* __restrict__ now, uint8_t* __restrict__ next) __attribute__((always_inline)) {
+    wait_vmcnt<0>();                        // this stage is there,
+    asm volatile("s_barrier" ::: "memory"); // and nobody reads the place of the next one
+    const uint32_t gone = gone_next;
+    const int key0 = p.key0 + kTiles * kTileKeys * stage;
+    ++stage;
+#pragma unroll
+    for (int u = 0; u < kTiles; ++u) {
+      if (u > 0 && kTiles * (stage - 1) + u >= tiles) break;
+      tile(now + u * kTileBytes, now + (kTiles + u) * kTileBytes, key0 + u * kTileKeys, (gone >> (2 * u)) & 3u,
+           [&](int i) __attribute__((always_inline)) {
+             if (u == 0 && i == 0) request_k(stage, next);
+             if (u == 0 && i == (kSteps > 4 ? 3 : 1)) request_v(stage, next);
+           });
+    }
+  };
+  // (two stages a turn, so that their places are constants of the reads)
+  while (kTiles * stage < tiles) {
+    run(smem, smem + kStageBytes);
+    if (kTiles * stage >= tiles) break;
+    run(smem + kStageBytes, smem);
   }
   arrive_all();                             // (loads to LDS that nobody waits for)
 
+  const float l = sum_halves(s.l);
+  const int at = kTileRows * wave + (lane & 31);
+  if (at >= p.rows) return;
+  if (p.slot < 0) {
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    uint8_t* o = out_row(a, p.token0, p.kv_head, p.row0 + at) + 8 * (lane >> 5);
 #pragma unroll
-  for (int r = 0; r < kR; ++r) {
-    const float l = sum_halves(s[r].l);
-    const int at = 32 * (kR * wave + r) + (lane & 31);
-    if (at >= p.rows) continue;
-    if (p.slot < 0) {
-      const float inv = l == 0.f ? 0.f : 1.f / l;
-      uint8_t* o = out_row(a, p.token0, p.kv_head, p.row0 + at) + 8 * (lane >> 5);
+    for (int b = 0; b < kBlocks; ++b)
 #pragma unroll
-      for (int b = 0; b < kBlocks; ++b)
+      for (int i = 0; i < 4; ++i)
+        store4<T>(o + 64 * b + 16 * i,
+                  floatx4{s.acc[b][4 * i], s.acc[b][4 * i + 1], s.acc[b][4 * i + 2], s.acc[b][4 * i + 3]} * inv);
+  } else {
+    float* part = a.partials + (int64_t)(p.slot + wave) * (kTileRows * (D + 2));
+    float* o = part + (lane & 31) * D + 4 * (lane >> 5);
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          store4<T>(o + 64 * b + 16 * i, floatx4{s[r].acc[b][4 * i], s[r].acc[b][4 * i + 1], s[r].acc[b][4 * i + 2],
-                                                 s[r].acc[b][4 * i + 3]} * inv);
-    } else {
-      float* part = a.partials + (int64_t)(p.slot + kR * wave + r) * (kTileRows * (D + 2));
-      float* o = part + (lane & 31) * D + 4 * (lane >> 5);
+    for (int b = 0; b < kBlocks; ++b)
 #pragma unroll
-      for (int b = 0; b < kBlocks; ++b)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          *reinterpret_cast<floatx4*>(o + 32 * b + 8 * i) =
-              floatx4{s[r].acc[b][4 * i], s[r].acc[b][4 * i + 1], s[r].acc[b][4 * i + 2], s[r].acc[b][4 * i + 3]};
-      if (lane < 32) {
-        part[kTileRows * D + (lane & 31)] = s[r].m;
-        part[kTileRows * D + kTileRows + (lane & 31)] = l;
-      }
+      for (int i = 0; i < 4; ++i)
+        *reinterpret_cast<floatx4*>(o + 32 * b + 8 * i) =
+            floatx4{s.acc[b][4 * i], s.acc[b][4 * i + 1], s.acc[b][4 * i + 2], s.acc[b][4 * i + 3]};
+    if (lane < 32) {
+      part[kTileRows * D + (lane & 31)] = s.m;
+      part[kTileRows * D + kTileRows + (lane & 31)] = l;
     }
   }
 }
 
-// ---------------------------------------------------------------- join
-// One row and 64 of its features a workgroup: 16 threads across the features,
-// 16 across the partials.
+// ---------------------------------------------------------------- kernels
+constexpr int narrow_wgs(int d) { return 256 / d; }             // workgroups a CU
 template <typename T, int D>
-__global__ __launch_bounds__(256) void join_kernel(ChunkArgs a) {
-  const Join j = a.joins[blockIdx.x];
-  const int row = (int)blockIdx.y;
+__global__ __launch_bounds__(kThreads, narrow_wgs(D)) void narrow_kernel(ChunkArgs a) {
+  extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+  narrow_piece<T, D, kTileKeys>(a, a.pieces[blockIdx.x], smem);
+}
+template <typename T, int D>
+__global__ __launch_bounds__(kThreads, kWideWgs) void wide_kernel(ChunkArgs a) {
+  extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+  wide_piece<T, D>(a, a.pieces[blockIdx.x], smem);
+}
+// A step with both: the wide pieces first, the narrow ones where they leave room
+// (1024 tokens beside seven users' 4, D = 128: 159 us; two launches 163, the narrow
+// ones first 161, eight of each in turn 193: reads at full rate leave the wide
+// pieces' next stage late).
+template <typename T, int D>
+__global__ __launch_bounds__(kThreads, kWideWgs) void mixed_kernel(ChunkArgs a) {
+  extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+  const int i = (int)blockIdx.x;
+  if (i < a.wide) wide_piece<T, D>(a, a.pieces[a.narrow + i], smem);
+  else narrow_piece<T, D, beside_keys(D)>(a, a.pieces[i - a.wide], smem);
+}
+
+// ---------------------------------------------------------------- join
+// The partials of cut row tiles.  A 32-row group of few partials (kFewParts): a
+// thread to four features of a row, 256 to a workgroup, every partial in turn.  Of
+// more: a workgroup to 64 features of a row, 16 threads across the features and
+// 16 across the partials, whose sums meet in LDS.
+constexpr int kFewParts = 8;
+
+template <typename T, int D>
+__device__ __forceinline__ void join_few(const ChunkArgs& a, const Join j, int block) {
+  const int i = block * 256 + (int)threadIdx.x, row = i / (D / 4), feature = 4 * (i % (D / 4));
   if (row >= j.rows) return;
-  const int tid = (int)threadIdx.x, feature = 64 * (int)blockIdx.z + 4 * (tid & 15), part = tid >> 4;
+  const float* const first = a.partials + (int64_t)j.slot0 * (kTileRows * (D + 2));
+  const int64_t step = (int64_t)j.step * (kTileRows * (D + 2));
+  float m[kFewParts], top = kNone;
+  floatx4 x[kFewParts];
+#pragma unroll
+  for (int s = 0; s < kFewParts; ++s) {
+    m[s] = kNone;
+    if (s < j.count) {
+      m[s] = first[s * step + kTileRows * D + row];
+      x[s] = *reinterpret_cast<const floatx4*>(first + s * step + row * D + feature);
+    }
+    top = fmaxf(top, m[s]);
+  }
+  floatx4 o{};
+  float l = 0.f;
+#pragma unroll
+  for (int s = 0; s < kFewParts; ++s)
+    if (s < j.count) {
+      const float w = __builtin_amdgcn_exp2f(m[s] - top);
+      l += w * first[s * step + kTileRows * D + kTileRows + row];
+      o += w * x[s];
+    }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  store4<T>(out_row(a, j.token0, j.kv_head, j.row0 + row) + 2 * feature, o * inv);
+}
+
+template <typename T, int D>
+__device__ __forceinline__ void join_many(const ChunkArgs& a, const Join j, int row, int part64) {
+  const int tid = (int)threadIdx.x, feature = 64 * part64 + 4 * (tid & 15), part = tid >> 4;
   __shared__ float red[16][64 + 4];
   __shared__ float red_m[16], red_l[16];
   auto slot = [&](int i) { return a.partials + (int64_t)(j.slot0 + i * j.step) * (kTileRows * (D + 2)); };
@@ -724,6 +803,20 @@ __global__ __launch_bounds__(256) void join_kernel(ChunkArgs a) {
   }
   const float inv = lsum == 0.f ? 0.f : 1.f / lsum;
   store4<T>(out_row(a, j.token0, j.kv_head, j.row0 + row) + 2 * feature, sum * inv);
+}
+
+// Groups of few partials first, D / 32 workgroups each; then 32 x D / 64 a group.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void join_kernel(ChunkArgs a) {
+  constexpr int kFewBlocks = D / 32, kManyBlocks = kTileRows * D / 64;
+  const int block = (int)blockIdx.x, few = a.few_joins * kFewBlocks;
+  if (block < few) {
+    join_few<T, D>(a, a.joins[block / kFewBlocks], block % kFewBlocks);
+    return;
+  }
+  const int many = (block - few) / kManyBlocks, at = (block - few) % kManyBlocks;
+  const Join j = a.joins[a.few_joins + many];
+  if (at / (D / 64) < j.rows) join_many<T, D>(a, j, at / (D / 64), at % (D / 64));
 }
 
 // ---------------------------------------------------------------- the plan
@@ -760,8 +853,9 @@ void row_tiles(int32_t token0, int32_t n, int32_t seq, int32_t table_row, int32_
   }
 }
 
-// A row tile in n pieces of equal parts of its keys.
-void cut(const RowTile& x, int32_t n, Plan& plan, std::vector<Piece>& out) {
+// A row tile in pieces between the key tiles `cuts` (from 0 to its last).
+void cut(const RowTile& x, const std::vector<int32_t>& cuts, Plan& plan, std::vector<Piece>& out) {
+  const int32_t n = (int32_t)cuts.size() - 1;
   if (n <= 1) {
     out.push_back(x.piece);
     return;
@@ -772,8 +866,8 @@ void cut(const RowTile& x, int32_t n, Plan& plan, std::vector<Piece>& out) {
                               std::min(kTileRows, x.piece.rows - g * kTileRows), plan.slots + g, groups, n, 0});
   for (int32_t s = 0; s < n; ++s) {
     Piece p = x.piece;
-    p.key0 = x.piece.key0 + kTileKeys * (int32_t)((int64_t)x.tiles * s / n);
-    p.key1 = std::min<int32_t>(x.piece.key1, x.piece.key0 + kTileKeys * (int32_t)((int64_t)x.tiles * (s + 1) / n));
+    p.key0 = x.piece.key0 + kTileKeys * cuts[s];
+    p.key1 = std::min<int32_t>(x.piece.key1, x.piece.key0 + kTileKeys * cuts[s + 1]);
     p.slot = plan.slots;
     plan.slots += groups;
     out.push_back(p);
@@ -784,14 +878,14 @@ int32_t pieces_of(const RowTile& x, int64_t per) { return (int32_t)((x.tiles + p
 
 // Narrow tiles: the fewest key tiles a piece with which the pieces fit the
 // workgroups that are resident at once.
-void plan_narrow(const std::vector<RowTile>& rows, int32_t head_size, Plan& plan) {
+void plan_narrow(const std::vector<RowTile>& rows, int32_t head_size, bool alone, Plan& plan) {
   int64_t total = 0;
   int32_t most = 0;
   for (const RowTile& x : rows) {
     total += x.tiles;
     most = std::max(most, x.tiles);
   }
-  const int64_t resident = (int64_t)kCus * (256 / head_size);
+  const int64_t resident = (int64_t)kCus * (alone ? narrow_wgs(head_size) : 2);
   int64_t per = std::max<int64_t>(kWaves, (total + resident - 1) / resident);
   auto count = [&](int64_t t) {
     int64_t c = 0;
@@ -800,13 +894,29 @@ void plan_narrow(const std::vector<RowTile>& rows, int32_t head_size, Plan& plan
   };
   if ((int64_t)rows.size() >= resident) per = std::max<int64_t>(per, most);
   while (per < most && count(per) > resident) ++per;
-  for (const RowTile& x : rows) cut(x, pieces_of(x, per), plan, plan.narrow);
+  std::vector<int32_t> cuts;
+  for (const RowTile& x : rows) {
+    const int32_t n = pieces_of(x, per);
+    cuts.clear();
+    for (int32_t i = 0; i <= n; ++i) cuts.push_back((int32_t)((int64_t)x.tiles * i / n));
+    cut(x, cuts, plan, plan.narrow);
+  }
 }
 
-// Wide tiles: workgroups take pieces as they come free, the longest first.  Of
-// a few piece lengths the one whose pieces, dealt out to the workgroups that
-// are resident at once, end first.
-constexpr int32_t kPieceCost = 5;          // of a piece beside its tiles, in tiles' time
+// Wide tiles.  Workgroups take pieces as they come free, two to a CU.  Tiles are
+// left whole, or the line of all tiles' keys is cut in equal shares, two a CU:
+// whichever is estimated to end first.  In units of a key tile's time on a busy
+// CU (D = 256 1.05 us, 128 0.47, 64 0.27): a piece costs 4 beside its tiles, one
+// of a cut row tile 15 (its partials are written and read again: the same at any
+// D, as both go with D); a workgroup alone on its CU takes 1.07, 1.45 or 1.5 units
+// a tile; the join is a launch of 5 us; shares end a tenth later than their mean,
+// as they are not dealt out as they were cut.  Measured, whole / cut, us:
+//   D = 256, 6 heads: 9256 tokens over 15360 1208 / 1242, 4096 over 28672 1165 /
+//   790, 3001 alone 109 / 60, 1024 alone 45 / 33;
+//   D = 128, 32 heads: 8192 alone 514 / 567, 1024 over 4096 119 / 103, 8 prompts
+//   of 300 over 500 51 / 56;  D = 64, 16 heads: 8192 over 8192 427 / 461, 1024
+//   over 1024 37 / 27.
+constexpr int32_t kPieceCost = 4, kCutCost = 15, kLeastPiece = 8, kShares = kCus * kWideWgs;
 void plan_wide(const std::vector<RowTile>& rows, int32_t head_size, Plan& plan) {
   int64_t total = 0;
   int32_t most = 0;
@@ -814,33 +924,39 @@ void plan_wide(const std::vector<RowTile>& rows, int32_t head_size, Plan& plan) 
     total += x.tiles;
     most = std::max(most, x.tiles);
   }
-  const int64_t resident = (int64_t)kCus * (head_size == 64 ? 2 : 1);
-  int64_t best = most, best_end = INT64_MAX;
+  const double alone = head_size == 256 ? 1.07 : head_size == 128 ? 1.45 : 1.5;
+  const double join = head_size == 256 ? 5.0 : head_size == 128 ? 11.0 : 18.0;
+  // Whole tiles, dealt out to the CUs longest first, there and back.
   std::vector<int32_t> length;
-  std::vector<int64_t> load;
-  for (int64_t k = 0; k <= 4; ++k) {
-    const int64_t per = k == 0 ? most : std::max<int64_t>(8, (total + resident * k - 1) / (resident * k));
-    if (per > most || (k > 0 && (int64_t)rows.size() > 4 * resident)) continue;
-    length.clear();
-    for (const RowTile& x : rows) {
-      const int32_t n = pieces_of(x, per);
-      for (int32_t i = 0; i < n; ++i) length.push_back((x.tiles + n - 1) / n + kPieceCost * (n > 1 ? 2 : 1));
+  length.reserve(rows.size());
+  for (const RowTile& x : rows) length.push_back(x.tiles + kPieceCost);
+  std::sort(length.begin(), length.end(), std::greater<int32_t>());
+  std::vector<int64_t> load(kCus, 0);
+  for (size_t i = 0; i < length.size(); ++i) load[(i / kCus) % 2 ? kCus - 1 - i % kCus : i % kCus] += length[i];
+  const double whole = std::max((double)*std::max_element(load.begin(), load.end()), alone * most);
+  const double share = std::max((double)total / kShares, (double)kLeastPiece);
+  const double pieces = (double)rows.size() + std::min((double)kShares, total / share);
+  const double parted = std::max(1.1 * (total + kCutCost * pieces) / kCus, alone * share + kCutCost) + join;
+  const int64_t shares = parted < whole ? kShares : 0;
+  int64_t at = 0;                           // on the line
+  for (const RowTile& x : rows) {
+    std::vector<int32_t> cuts{0};
+    if (shares > 0) {
+      // the share's ends inside this tile, but for slivers
+      for (int64_t s = at * shares / total; s <= (at + x.tiles) * shares / total; ++s) {
+        const int64_t end = s * total / shares - at;
+        if (end >= cuts.back() + kLeastPiece && end <= x.tiles - kLeastPiece) cuts.push_back((int32_t)end);
+      }
     }
-    std::sort(length.begin(), length.end(), std::greater<int32_t>());
-    load.assign((size_t)resident, 0);
-    for (size_t i = 0; i < length.size(); ++i) {
-      const size_t at = i % (size_t)resident;
-      load[(i / (size_t)resident) % 2 ? (size_t)resident - 1 - at : at] += length[i];
-    }
-    const int64_t end = *std::max_element(load.begin(), load.end());
-    if (end < best_end) {
-      best_end = end;
-      best = per;
-    }
+    cuts.push_back(x.tiles);
+    cut(x, cuts, plan, plan.wide);
+    at += x.tiles;
   }
-  for (const RowTile& x : rows) cut(x, pieces_of(x, best), plan, plan.wide);
   std::stable_sort(plan.wide.begin(), plan.wide.end(),
                    [](const Piece& x, const Piece& y) { return x.key1 - x.key0 > y.key1 - y.key0; });
+  // The first two rounds of workgroups share CUs in order: the longest pieces,
+  // shortest first, meet the next ones, longest first.
+  std::reverse(plan.wide.begin(), plan.wide.begin() + (std::ptrdiff_t)std::min<size_t>(kCus, plan.wide.size()));
 }
 
 void make_plan(const int32_t* qsl, const int32_t* seqs, int32_t num_requests, int32_t group, int32_t kv_heads,
@@ -853,29 +969,25 @@ void make_plan(const int32_t* qsl, const int32_t* seqs, int32_t num_requests, in
     else
       row_tiles(qsl[i], n, seqs[i], i, group, kv_heads, window, kWideRows, wide);
   }
-  if (!narrow.empty()) plan_narrow(narrow, head_size, plan);
+  if (!narrow.empty()) plan_narrow(narrow, head_size, wide.empty(), plan);
   if (!wide.empty()) plan_wide(wide, head_size, plan);
+  std::stable_partition(plan.joins.begin(), plan.joins.end(), [](const Join& j) { return j.count <= kFewParts; });
 }
-
-constexpr size_t narrow_lds(int d) { return (size_t)kWaves * kTileRows * d * 4 + kWaves * 64 * 4; }
 
 template <typename T, int D>
 int launch(const ChunkArgs& a, const oscar_chunk_step& step, hipStream_t stream) {
-  if (step.narrow > 0) {
-    static std::atomic<uint64_t> done{0};
-    const int st = set_dynamic_lds(reinterpret_cast<const void*>(&narrow_kernel<T, D>), (int)narrow_lds(D), done);
-    if (st != kOk) return st;
-    narrow_kernel<T, D><<<step.narrow, kThreads, narrow_lds(D), stream>>>(a);
-  }
-  if (step.wide > 0) {
-    static std::atomic<uint64_t> done{0};
-    constexpr int kR = D == 256 ? 1 : 2, kW = 8 / kR, kWgs = D == 64 ? 2 : 1;
-    const auto kernel = &wide_kernel<T, D, kR, kW, kWgs>;
-    const int st = set_dynamic_lds(reinterpret_cast<const void*>(kernel), wide_lds<D>(), done);
-    if (st != kOk) return st;
-    kernel<<<step.wide, 64 * kW, wide_lds<D>(), stream>>>(a);
-  }
-  if (step.joins > 0) join_kernel<T, D><<<dim3(step.joins, kTileRows, D / 64), 256, 0, stream>>>(a);
+  static std::atomic<uint64_t> done[3];
+  constexpr int kLds[3] = {narrow_lds(D, kTileKeys), wide_lds<D>(),
+                           std::max(narrow_lds(D, beside_keys(D)), wide_lds<D>())};
+  static_assert(kLds[2] <= 80 * 1024, "two workgroups' LDS must fit the CU's 160 KiB");
+  void (*const kernels[3])(ChunkArgs) = {&narrow_kernel<T, D>, &wide_kernel<T, D>, &mixed_kernel<T, D>};
+  const int which = step.wide == 0 ? 0 : step.narrow == 0 ? 1 : 2;
+  const int st = set_dynamic_lds(reinterpret_cast<const void*>(kernels[which]), kLds[which], done[which]);
+  if (st != kOk) return st;
+  kernels[which]<<<step.narrow + step.wide, kThreads, kLds[which], stream>>>(a);
+  const int64_t blocks = (int64_t)step.few_joins * (D / 32) + (int64_t)(step.joins - step.few_joins) * (kTileRows * D / 64);
+  if (blocks > INT32_MAX) return kErrInvalidArgument;
+  if (blocks > 0) join_kernel<T, D><<<(uint32_t)blocks, 256, 0, stream>>>(a);
   return hipGetLastError() == hipSuccess ? kOk : kErrLaunch;
 }
 
@@ -890,7 +1002,8 @@ int check_chunk_cache(const oscar_plain_cache* c) {
   const int status = check_plain_cache(c);
   if (status != kOk) return status;
   if (c->head_size != 64 && c->head_size != 128 && c->head_size != 256) return kErrUnsupportedHeadDim;
-  return c->block_size % 16 == 0 ? kOk : kErrUnsupportedGeometry;
+  const bool near = c->k_stride_page <= UINT32_MAX && c->v_stride_page <= UINT32_MAX;
+  return c->block_size % 16 == 0 && near ? kOk : kErrUnsupportedGeometry;
 }
 
 }  // namespace
@@ -928,6 +1041,8 @@ extern "C" int oscar_chunk_plan(const int32_t* query_start_loc, const int32_t* s
     step->narrow = (int32_t)plan.narrow.size();
     step->wide = (int32_t)plan.wide.size();
     step->joins = (int32_t)plan.joins.size();
+    step->few_joins = (int32_t)std::count_if(plan.joins.begin(), plan.joins.end(),
+                                             [](const Join& j) { return j.count <= kFewParts; });
     step->items_size = (int64_t)(narrow + wide + joins);
     step->workspace_size = (int64_t)plan.slots * kTileRows * (cache->head_size + 2) * 4;
     if (items == nullptr) return kOk;
@@ -953,7 +1068,8 @@ extern "C" int oscar_chunk_attention(const oscar_chunk_step* step, const void* i
       out->num_heads != step->num_heads || step->num_heads < 1 || step->num_heads % cache->num_kv_heads ||
       !(scale > 0.f) || !(scale <= 3.0e38f))
     return kErrInvalidArgument;
-  if (step->narrow < 0 || step->wide < 0 || step->joins < 0) return kErrInvalidArgument;
+  if (step->narrow < 0 || step->wide < 0 || step->few_joins < 0 || step->joins < step->few_joins)
+    return kErrInvalidArgument;
   if (step->narrow + step->wide == 0) return kOk;
   if (items == nullptr || block_table == nullptr || query->data == nullptr || out->data == nullptr ||
       block_table_stride < step->table_cols)
@@ -972,8 +1088,8 @@ extern "C" int oscar_chunk_attention(const oscar_chunk_step* step, const void* i
   a.out_head = 2 * out->head_stride;
   a.k = static_cast<const uint8_t*>(cache->k);
   a.v = static_cast<const uint8_t*>(cache->v);
-  a.k_page = cache->k_stride_page;
-  a.v_page = cache->v_stride_page;
+  a.k_page = (uint32_t)cache->k_stride_page;
+  a.v_page = (uint32_t)cache->v_stride_page;
   a.num_pages = cache->num_pages;
   a.k_token = (int32_t)cache->k_stride_token;
   a.v_token = (int32_t)cache->v_stride_token;
@@ -982,7 +1098,9 @@ extern "C" int oscar_chunk_attention(const oscar_chunk_step* step, const void* i
   a.table = block_table;
   a.table_stride = block_table_stride;
   a.pieces = static_cast<const Piece*>(items);
-  a.wide0 = step->narrow;
+  a.narrow = step->narrow;
+  a.wide = step->wide;
+  a.few_joins = step->few_joins;
   a.joins = reinterpret_cast<const Join*>(a.pieces + step->narrow + step->wide);
   a.partials = static_cast<float*>(workspace);
   a.scale_log2 = scale * 1.4426950408889634f;

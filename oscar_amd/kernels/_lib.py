@@ -128,17 +128,10 @@ def call(name: str, *args) -> None:
         raise OscarKernelError(f"{name} failed: {STATUS.get(status, status)}")
 
 
-def call_on(device: torch.device, name: str, *args) -> None:
-    """call() with the device's current stream appended, the device made the
-    current one around it where it is another."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        call(name, *args, stream_handle(device))
-    else:
-        with torch.cuda.device(device):
-            call(name, *args, stream_handle(device))
-
-
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
 def stream_handle(device: torch.device) -> int:
@@ -148,6 +141,19 @@ def stream_handle(device: torch.device) -> int:
         idx = device.index
         return _raw_stream(torch.cuda.current_device() if idx is None else idx)
     return torch.cuda.current_stream(device).cuda_stream
+
+
+def call_on(device: torch.device, name: str, *args) -> None:
+    """call() with the device's current stream appended, the device made the
+    current one around it where it is another."""
+    index = device.index
+    if index is None or index == _current_device():
+        status = getattr(_lib or load(), name)(*args, stream_handle(device))
+    else:
+        with torch.cuda.device(device):
+            status = getattr(_lib or load(), name)(*args, stream_handle(device))
+    if status != 0:
+        raise OscarKernelError(f"{name} failed: {STATUS.get(status, status)}")
 
 
 def ptr(t) -> int:

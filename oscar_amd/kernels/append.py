@@ -56,11 +56,12 @@ class PagedCache:
                 raise ValueError("a cache page must span less than 2 GiB")
             strides += [2 * page, 2 * token, 2 * head]
         self.k_cache, self.v_cache = k_cache, v_cache
-        self.device, self.dtype = k_cache.device, k_cache.dtype
+        self.device, self.dtype, self.on_gpu = k_cache.device, k_cache.dtype, k_cache.is_cuda
         self.pages, self.block_size, self.num_kv_heads, self.head_size = pages, bs, hk, d
         self.args = PlainCacheArgs(k_cache.data_ptr(), v_cache.data_ptr(), pages, *strides, bs, hk, d,
                                    _rotary.DTYPES[k_cache.dtype])
         self.address = ctypes.addressof(self.args)
+        self.geometry = (hk, d, bs)
 
 
 def append_rotated(query: torch.Tensor | None, key: torch.Tensor, value: torch.Tensor, positions: torch.Tensor,
@@ -77,28 +78,27 @@ def append_rotated(query: torch.Tensor | None, key: torch.Tensor, value: torch.T
     n, d, dtype, device = slot_mapping.shape[0], cache.head_size, cache.dtype, cache.device
     if d < rotary.rotary_dim:
         raise ValueError(f"head size {d} is below rotary_dim {rotary.rotary_dim}")
-    k = _rotary.heads(key, n, d, dtype, device, "key")
-    v = _rotary.heads(value, n, d, dtype, device, "value")
-    if k.num_heads != cache.num_kv_heads or v.num_heads != cache.num_kv_heads:
+    k, hk = _rotary.heads(key, n, d, dtype, device, "key")
+    v, hv = _rotary.heads(value, n, d, dtype, device, "value")
+    if hk != cache.num_kv_heads or hv != cache.num_kv_heads:
         raise ValueError(f"key and value must have the cache's {cache.num_kv_heads} heads")
     q = qo = None
     if query is not None:
-        q = _rotary.heads(query, n, d, dtype, device, "query")
+        q, hq = _rotary.heads(query, n, d, dtype, device, "query")
         if query_out is None:
-            query_out = torch.empty((n, *query.shape[1:]), dtype=dtype, device=device)
-        qo = _rotary.heads(query_out, n, d, dtype, device, "query_out")
-        if qo.num_heads != q.num_heads:
-            raise ValueError("query_out must have the query's heads")
-    if slot_mapping.dtype != torch.int64 or (n > 1 and slot_mapping.stride(0) != 1):
+            query_out, qo = _rotary.new_heads(query, n, hq, d)
+        else:
+            qo, count = _rotary.heads(query_out, n, d, dtype, device, "query_out")
+            if count != hq:
+                raise ValueError("query_out must have the query's heads")
+    if slot_mapping.dtype is not torch.int64 or (n > 1 and slot_mapping.stride(0) != 1):
         if slot_mapping.dtype not in (torch.int64, torch.int32):
             raise ValueError(f"slot_mapping must be integers, got {slot_mapping.dtype}")
         slot_mapping = slot_mapping.to(torch.int64).contiguous()
     positions, axis_stride = _rotary.positions_of(positions, rotary, n, device)
-    if not cache.k_cache.is_cuda:
+    if not cache.on_gpu:
         raise ValueError("OSCAR kernels take device tensors")
     if n:
-        ref = ctypes.byref
-        _lib.call_on(device, "oscar_append_rotated", rotary.address, positions.data_ptr(), axis_stride, n,
-                     None if q is None else ref(q), None if qo is None else ref(qo), ref(k), ref(v), cache.address,
-                     slot_mapping.data_ptr())
+        _lib.call_on(device, "oscar_append_rotated", rotary.address, positions.data_ptr(), axis_stride, n, q, qo, k, v,
+                     cache.address, slot_mapping.data_ptr())
     return query_out if query is not None else None

@@ -21,7 +21,8 @@ _i32, _i64 = ctypes.c_int32, ctypes.c_int64
 class ChunkStepArgs(ctypes.Structure):
     """struct oscar_chunk_step (include/oscar_amd.h)."""
     _fields_ = [("num_requests", _i32), ("num_tokens", _i32), ("num_heads", _i32), ("window", _i32),
-                ("table_cols", _i32), ("narrow", _i32), ("wide", _i32), ("joins", _i32), ("items_size", _i64),
+                ("table_cols", _i32), ("narrow", _i32), ("wide", _i32), ("joins", _i32), ("few_joins", _i32), ("reserved", _i32),
+                ("items_size", _i64),
                 ("workspace_size", _i64)]
 
 
@@ -77,7 +78,7 @@ class ChunkStep:
         self.tokens = args.num_tokens
         self.num_heads = num_heads
         self.workspace_size = args.workspace_size
-        self.geometry = (cache.num_kv_heads, cache.head_size, cache.block_size)
+        self.geometry = cache.geometry
         self.device = device
         self.block_tables = block_tables
         self.items_ptr, self.table_ptr, self.table_stride = (self.items.data_ptr(), block_tables.data_ptr(),
@@ -99,29 +100,35 @@ def chunk_attention(query: torch.Tensor, cache: PagedCache, step: ChunkStep, sca
     left as they were.  scale must be positive.  Keys on pages outside the cache
     are left out; a row that sees no key becomes zeros."""
     device = cache.device
-    if (cache.num_kv_heads, cache.head_size, cache.block_size) != step.geometry or device != step.device:
+    if cache.geometry != step.geometry or device != step.device:
         raise ValueError("the step was built for another cache geometry or device")
-    d = cache.head_size
+    d, dtype, tokens = cache.head_size, cache.dtype, step.tokens
     if not 0.0 < scale < 3.0e38:
         raise ValueError("scale must be positive and finite")
-    q = _rotary.heads(query, step.tokens, d, cache.dtype, device, "query")
-    if q.num_heads != step.num_heads:
+    q, hq = _rotary.heads(query, tokens, d, dtype, device, "query")
+    if hq != step.num_heads:
         raise ValueError(f"query must have the step's {step.num_heads} heads")
-    if (q.data | 2 * q.token_stride | 2 * q.head_stride) % 16:
+    if _misaligned(query):
         query = query.contiguous()
-        q = _rotary.heads(query, step.tokens, d, cache.dtype, device, "query")
+        q, _ = _rotary.heads(query, tokens, d, dtype, device, "query")
     if out is None:
-        out = torch.empty(query.shape, dtype=query.dtype, device=device)
-    o = _rotary.heads(out, step.tokens, d, cache.dtype, device, "out")
-    if o.num_heads != step.num_heads or (o.data | 2 * o.token_stride | 2 * o.head_stride) % 16:
-        raise ValueError("out must have the query's heads, rows at multiples of 16 bytes")
-    if step.tokens == 0:
+        out, o = _rotary.new_heads(query, query.shape[0], hq, d)
+    else:
+        o, count = _rotary.heads(out, tokens, d, dtype, device, "out")
+        if count != hq or _misaligned(out):
+            raise ValueError("out must have the query's heads, rows at multiples of 16 bytes")
+    if tokens == 0:
         return out
     if _lib.stream_handle(device) != step.stream:
         step._join(device)
     need = step.workspace_size
     ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
-    ref = ctypes.byref
     _lib.call_on(device, "oscar_chunk_attention", step.address, step.items_ptr, step.table_ptr, step.table_stride,
-                 cache.address, ref(q), ref(o), scale, _lib.ptr(ws), need)
+                 cache.address, q, o, scale, None if ws is None else ws.data_ptr(), need)
     return out
+
+
+def _misaligned(x: torch.Tensor) -> bool:
+    """Whether rows of x begin off multiples of 16 bytes (8 two-byte values)."""
+    token, head, _ = x.stride()
+    return ((x.data_ptr() >> 1) | token | head) & 7 != 0

@@ -11,6 +11,7 @@ in fp32 with one rounding; the rest pass through.  The map is orthogonal, so
 from __future__ import annotations
 
 import ctypes
+import struct
 
 import torch
 
@@ -89,34 +90,46 @@ class Rotary:
         self.address = ctypes.addressof(self.args)
 
 
-def heads(x: torch.Tensor, tokens: int, d: int, dtype, device, what: str) -> HeadsArgs:
-    """The first tokens of x [N, heads, d]."""
-    if x.ndim != 3 or x.shape[0] < tokens or x.shape[2] != d:
+# struct oscar_heads as bytes, which a call passes by their address: packing them
+# takes a fifth of what filling a ctypes structure does.
+pack_heads = struct.Struct("@Pqqii").pack
+
+
+def heads(x: torch.Tensor, tokens: int, d: int, dtype, device, what: str) -> tuple[bytes, int]:
+    """(struct oscar_heads, heads) of the first tokens of x [N, heads, d]."""
+    shape = x.shape
+    if len(shape) != 3 or shape[0] < tokens or shape[2] != d:
         raise ValueError(f"{what} must be [tokens, heads, {d}] with a row per token")
-    if x.dtype != dtype or x.device != device:
+    if x.dtype is not dtype or x.device != device:
         raise ValueError(f"{what} must be {dtype} on {device} as the other rows are")
     token, head, feature = x.stride()
     if feature != 1:
         raise ValueError(f"{what}: a head's features must be contiguous")
-    return HeadsArgs(x.data_ptr(), token, head, x.shape[1], 0)
+    return pack_heads(x.data_ptr(), token, head, shape[1], 0), shape[1]
+
+
+def new_heads(like: torch.Tensor, tokens: int, count: int, d: int) -> tuple[torch.Tensor, bytes]:
+    """A new tensor [tokens, count, d] of like's type and device, and its struct oscar_heads."""
+    x = like.new_empty((tokens, count, d))
+    return x, pack_heads(x.data_ptr(), count * d, d, count, 0)
 
 
 def positions_of(positions: torch.Tensor, rotary: Rotary, tokens: int, device) -> tuple[torch.Tensor, int]:
     """int64 positions [N], or [axes, N], and the stride between axes."""
-    if positions.dtype != torch.int64:
+    if positions.dtype is not torch.int64:
         if positions.dtype not in (torch.int32, torch.int16):
             raise ValueError(f"positions must be integers, got {positions.dtype}")
         positions = positions.to(torch.int64)
     if positions.device != device or rotary.device != device:
         raise ValueError("positions and rotary table must be on the rows' device")
-    if positions.ndim == 1:
-        positions = positions[None]
-    if positions.ndim != 2 or positions.shape[0] != rotary.axes or positions.shape[1] < tokens:
+    shape = positions.shape
+    if (len(shape) not in (1, 2) or shape[-1] < tokens or (len(shape) == 1 and rotary.axes != 1)
+            or (len(shape) == 2 and shape[0] != rotary.axes)):
         raise ValueError(f"positions must be [{rotary.axes}, tokens] with an entry per token"
                          + (" (or [tokens])" if rotary.axes == 1 else ""))
-    if positions.stride(1) != 1 and tokens > 1:
+    if positions.stride(-1) != 1 and tokens > 1:
         positions = positions.contiguous()
-    return positions, positions.stride(0)
+    return positions, positions.stride(0) if len(shape) == 2 else 0
 
 
 def rotate(query: torch.Tensor, key: torch.Tensor | None, positions: torch.Tensor, rotary: Rotary, query_out=None,
@@ -134,24 +147,26 @@ def rotate(query: torch.Tensor, key: torch.Tensor | None, positions: torch.Tenso
     n, _, d = query.shape
     if d < rotary.rotary_dim or d % 2 or d > 256:
         raise ValueError(f"head size {d} must be even, {rotary.rotary_dim} (rotary_dim) to 256")
-    q = heads(query, n, d, dtype, device, "query")
+    q, hq = heads(query, n, d, dtype, device, "query")
     if query_out is None:
-        query_out = torch.empty(query.shape, dtype=dtype, device=device)
-    qo = heads(query_out, n, d, dtype, device, "query_out")
+        query_out, qo = new_heads(query, n, hq, d)
+    else:
+        qo, count = heads(query_out, n, d, dtype, device, "query_out")
+        if count != hq:
+            raise ValueError("query_out must have the query's heads")
     k = ko = None
     if key is not None:
-        k = heads(key, n, d, dtype, device, "key")
+        k, hk = heads(key, n, d, dtype, device, "key")
         if key_out is None:
-            key_out = torch.empty((n, *key.shape[1:]), dtype=dtype, device=device)
-        ko = heads(key_out, n, d, dtype, device, "key_out")
-    if qo.num_heads != q.num_heads or (k is not None and ko.num_heads != k.num_heads):
-        raise ValueError("outputs must have their inputs' heads")
+            key_out, ko = new_heads(key, n, hk, d)
+        else:
+            ko, count = heads(key_out, n, d, dtype, device, "key_out")
+            if count != hk:
+                raise ValueError("key_out must have the key's heads")
     positions, axis_stride = positions_of(positions, rotary, n, device)
     if not query.is_cuda:
         raise ValueError("OSCAR kernels take device tensors")
     if n:
-        ref = ctypes.byref
-        _lib.call_on(device, "oscar_rotate_positions", rotary.address, positions.data_ptr(), axis_stride, n, ref(q),
-                     ref(qo), None if k is None else ref(k), None if ko is None else ref(ko), d, DTYPES[dtype],
-                     int(inverse))
+        _lib.call_on(device, "oscar_rotate_positions", rotary.address, positions.data_ptr(), axis_stride, n, q, qo, k,
+                     ko, d, DTYPES[dtype], int(inverse))
     return query_out, key_out if key is not None else None

@@ -8,7 +8,7 @@ import torch
 from oscar_amd.kernels import _lib, append, chunk, rotary
 
 PIECE, JOIN = struct.Struct("12i"), struct.Struct("8i")
-NARROW, WIDE, TILE = 32, 256, 32
+NARROW, WIDE, TILE = 32, 128, 32
 
 
 def plain_cache(pages=4, page=16, hk=2, d=128, dtype=torch.bfloat16):
@@ -84,8 +84,11 @@ def test_pieces_cover_every_row_and_key_once(reqs, window, group, d, hk):
                 _, _, _, _, slot0, step, count, _ = found[0]
                 assert [slot0 + step * k for k in range(count)] == want
     assert covered == {(i, head): n * group for i, (n, _) in enumerate(reqs) for head in range(hk) if n}
-    wide = pieces[args.narrow:]
-    assert all(a[7] - a[6] >= b[7] - b[6] for a, b in zip(wide, wide[1:]))
+    keys = [p[7] - p[6] for p in pieces[args.narrow:]]          # the longest first, the first 256 the other way round
+    first = min(256, len(keys))
+    keys[:first] = keys[:first][::-1]
+    assert keys == sorted(keys, reverse=True)
+    assert [j[6] <= 8 for j in joins] == [True] * args.few_joins + [False] * (args.joins - args.few_joins)
 
 
 def test_an_empty_step():
