@@ -8,11 +8,22 @@
 // bounds the kernel (three flops a value), and for a few tokens its latency.
 //
 // A workgroup takes a block of tokens.  It collects their cosines and sines in
-// LDS first (each table entry read once for all heads, each pair from its own
-// axis' row), while its first rows are already on their way; then every thread
-// takes pieces of rows: a rotating piece is kVec pairs, a copying one kVec
-// values (features past rotary_dim, and the values).
+// LDS (each table entry read once for all heads, each pair from its own axis'
+// row).  The rows' values go by in five jobs, one after the other: the turning
+// parts of queries and keys (a thread to kVec pairs), their parts past
+// rotary_dim and the values (a thread to kVec values).  A job's strides and
+// divisors are the same for all lanes, so they stay in scalar registers (with all
+// kinds of rows in one sequence of pieces each lane looked its own up: a write of
+// 65536 tokens 176 us instead of 119).  Every job's first round of loads goes out
+// before the cosines are collected.
+//
+// Measured: 30843 tokens of 32 + 8 heads of 128 (fp16, adjacent pairs) 121 us,
+// 5.4 TB/s; 9256 of 6 + 1 heads of 256 (64 features turn, three axes) 14.7 us, 4.7
+// TB/s; a write of 65536 tokens of that shape 119 us, 4.6 TB/s; a large copy moves
+// 5.05 TB/s.  One token takes 3 us.
 #include "plain_cache.h"
+
+#include <type_traits>
 
 namespace oscar {
 namespace {
@@ -21,32 +32,32 @@ constexpr int kRotThreads = 256;
 constexpr int kMaxTokens = 16;             // of a workgroup
 constexpr int kMaxRotary = 256;
 
-// Rows that a launch turns or copies: source, destination (or cache slots).
-struct RowSet {
+// What a launch does with one part of one kind of rows: `pieces` a head, from
+// feature `first` on.
+struct Job {
   const uint8_t* src;
-  uint8_t* dst;
-  int64_t src_token, src_head, dst_token, dst_head;    // bytes; in a cache dst_token is not used
-  int32_t heads;
-  int32_t pieces;          // of a head
-  int32_t turning;         // of them, the first ones
-  int32_t first;           // piece of a token at which the set starts
-  FastDiv by_pieces;
+  uint8_t* dst;            // rows of its own, or a cache
+  uint32_t src_token, src_head, dst_token, dst_head;   // bytes; in a cache dst_token is not used
+  int32_t a_token;         // pieces of a token: heads x pieces
+  int32_t pieces, first;
+  FastDiv by_token, by_head;
 };
+constexpr int kJobs = 5;                   // turned: queries, keys; copied: queries, keys, values
+constexpr bool turns(int job) { return job < 2; }
 
 struct RotArgs {
-  RowSet set[3];           // queries, keys, values
+  Job job[kJobs];
   const float* table;
   const int64_t* positions;
   int64_t axis_stride, table_rows, tokens;
   uint64_t pair_axis[4];
-  const int64_t* slots;    // null: sets have rows of their own
+  const int64_t* slots;    // null: keys have rows of their own
   int64_t num_slots, k_page, k_token, v_page, v_token;
   int32_t block_size, block_shift;         // shift: log2, or -1
-  int32_t axes, half;      // rotary_dim / 2
-  int32_t pieces;          // of a token
+  int32_t axes, half;      // half: rotary_dim / 2
   int32_t block_tokens;
   float sign;              // of the sines
-  FastDiv by_pieces, by_half;
+  FastDiv by_half;
 };
 
 template <typename T, int kVec>
@@ -56,14 +67,6 @@ struct Piece {
 template <typename T>
 struct Piece<T, 1> {
   typedef T Row;
-};
-
-// One thread's piece: where it lies, and its values.
-template <typename T, int kVec>
-struct Work {
-  typename Piece<T, kVec>::Row a, b;
-  const uint8_t* src;
-  int token, set, head, piece;             // set < 0: none
 };
 
 // kVec values to a load: 16 bytes where rows, strides and pairs allow, else one
@@ -77,40 +80,87 @@ __global__ __launch_bounds__(kRotThreads) void rotary_kernel(RotArgs a) {
   const int tid = (int)threadIdx.x;
   const int64_t tok0 = (int64_t)blockIdx.x * a.block_tokens;
   const int tokens = (int)min((int64_t)a.block_tokens, a.tokens - tok0);
-  const int count = tokens * a.pieces;
   constexpr int kPairs = kAdjacent && kVec > 1 ? kVec / 2 : kVec;     // of a turning piece
+  constexpr int kSpan = kAdjacent && kVec == 1 ? 2 : kVec;            // features from one turning piece to the next
   const int width = 2 * a.half;
 
-  auto locate = [&](int idx, Work<T, kVec>& w) {
-    w.set = -1;
-    if (idx >= count) return;
-    w.token = (int)fast_div((uint32_t)idx, a.by_pieces);
-    const int p = idx - w.token * a.pieces;
-    w.set = p >= a.set[2].first ? 2 : p >= a.set[1].first ? 1 : 0;
-    const RowSet& s = a.set[w.set];
-    w.head = (int)fast_div((uint32_t)(p - s.first), s.by_pieces);
-    w.piece = p - s.first - w.head * s.pieces;
-    w.src = s.src + (tok0 + w.token) * s.src_token + (int64_t)w.head * s.src_head;
+  struct Work {
+    Row a, b;
+    int token, head, feature, pair;
   };
-  // First feature of a piece, and of its partners (features j and j + half).
-  auto feature = [&](const Work<T, kVec>& w) {
-    const int turning = a.set[w.set].turning;
-    if (w.piece < turning) return w.piece * kVec * (kVec == 1 && kAdjacent ? 2 : 1);
-    return (w.set < 2 ? width : 0) + (w.piece - turning) * kVec;
-  };
-  auto fetch = [&](Work<T, kVec>& w) {
-    if (w.set < 0) return;
-    const T* x = reinterpret_cast<const T*>(w.src) + feature(w);
+  auto fetch = [&](auto tag, int idx, Work& w) {
+    constexpr int kJob = decltype(tag)::value;
+    const Job& j = a.job[kJob];
+    w.token = (int)fast_div((uint32_t)idx, j.by_token);
+    const int p = idx - w.token * j.a_token;
+    w.head = (int)fast_div((uint32_t)p, j.by_head);
+    const int piece = p - w.head * j.pieces;
+    w.feature = j.first + piece * (turns(kJob) ? kSpan : kVec);
+    w.pair = piece * kPairs;
+    const T* x = reinterpret_cast<const T*>(j.src + tok0 * j.src_token + (uint64_t)(uint32_t)w.token * j.src_token +
+                                            (uint64_t)(uint32_t)w.head * j.src_head) + w.feature;
     w.a = *reinterpret_cast<const Row*>(x);
-    if (w.piece < a.set[w.set].turning) {
-      if constexpr (!kAdjacent) w.b = *reinterpret_cast<const Row*>(x + a.half);
-      else if constexpr (kVec == 1) w.b = *reinterpret_cast<const Row*>(x + 1);
+    if constexpr (turns(kJob) && !kAdjacent) w.b = *reinterpret_cast<const Row*>(x + a.half);
+    else if constexpr (turns(kJob) && kVec == 1) w.b = *reinterpret_cast<const Row*>(x + 1);
+  };
+  auto finish = [&](auto tag, const Work& w) {
+    constexpr int kJob = decltype(tag)::value;
+    const Job& j = a.job[kJob];
+    if (live[w.token] == 0) return;
+    uint8_t* dst = j.dst + (uint64_t)(uint32_t)w.head * j.dst_head;
+    constexpr bool kValue = kJob == 4, kKey = kJob == 1 || kJob == 3;
+    if ((kKey && a.slots != nullptr) || kValue) {
+      const int64_t at = kKey ? at_k[w.token] : at_v[w.token];
+      if (at < 0) return;
+      dst += at;
+    } else {
+      dst += tok0 * j.dst_token + (uint64_t)(uint32_t)w.token * j.dst_token;
+    }
+    T* y = reinterpret_cast<T*>(dst) + w.feature;
+    if constexpr (!turns(kJob)) {
+      *reinterpret_cast<Row*>(y) = w.a;
+    } else {
+      const float* c = cs + w.token * width + w.pair;
+      const float* sn = c + a.half;
+      if constexpr (kVec == 1) {
+        const float x1 = (float)w.a, x2 = (float)w.b;
+        y[0] = (T)(x1 * c[0] - x2 * sn[0]);
+        y[kAdjacent ? 1 : a.half] = (T)(x2 * c[0] + x1 * sn[0]);
+      } else if constexpr (kAdjacent) {
+        Row o;
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i) {
+          const float x1 = (float)w.a[2 * i], x2 = (float)w.a[2 * i + 1];
+          o[2 * i] = (T)(x1 * c[i] - x2 * sn[i]);
+          o[2 * i + 1] = (T)(x2 * c[i] + x1 * sn[i]);
+        }
+        *reinterpret_cast<Row*>(y) = o;
+      } else {
+        Row o1, o2;
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) {
+          const float x1 = (float)w.a[i], x2 = (float)w.b[i];
+          o1[i] = (T)(x1 * c[i] - x2 * sn[i]);
+          o2[i] = (T)(x2 * c[i] + x1 * sn[i]);
+        }
+        *reinterpret_cast<Row*>(y) = o1;
+        *reinterpret_cast<Row*>(y + a.half) = o2;
+      }
     }
   };
+  auto each_job = [&](auto&& f) {
+    f(std::integral_constant<int, 0>{});
+    f(std::integral_constant<int, 1>{});
+    f(std::integral_constant<int, 2>{});
+    f(std::integral_constant<int, 3>{});
+    f(std::integral_constant<int, 4>{});
+  };
 
-  Work<T, kVec> next;
-  locate(tid, next);
-  fetch(next);
+  Work w0[kJobs];
+  each_job([&](auto tag) {
+    constexpr int kJob = decltype(tag)::value;
+    if (tid < tokens * a.job[kJob].a_token) fetch(tag, tid, w0[kJob]);
+  });
 
   // The tokens' cosines and sines, slots and whether their positions exist.
   for (int i = tid; i < tokens * a.half; i += kRotThreads) {
@@ -142,52 +192,19 @@ __global__ __launch_bounds__(kRotThreads) void rotary_kernel(RotArgs a) {
   }
   __syncthreads();
 
-  for (int idx = tid; idx < count; idx += kRotThreads) {
-    Work<T, kVec> w = next;
-    locate(idx + kRotThreads, next);
-    fetch(next);
-    if (live[w.token] == 0) continue;
-    const RowSet& s = a.set[w.set];
-    uint8_t* dst = s.dst + (int64_t)w.head * s.dst_head;
-    if (a.slots != nullptr && w.set > 0) {
-      const int64_t at = w.set == 1 ? at_k[w.token] : at_v[w.token];
-      if (at < 0) continue;
-      dst += at;
-    } else {
-      dst += (tok0 + w.token) * s.dst_token;
+  each_job([&](auto tag) {
+    constexpr int kJob = decltype(tag)::value;
+    const int count = tokens * a.job[kJob].a_token;
+    if (tid < count) finish(tag, w0[kJob]);
+    for (int idx = tid + kRotThreads; idx < count; idx += 2 * kRotThreads) {
+      Work u, v;
+      const bool two = idx + kRotThreads < count;
+      fetch(tag, idx, u);
+      if (two) fetch(tag, idx + kRotThreads, v);
+      finish(tag, u);
+      if (two) finish(tag, v);
     }
-    T* y = reinterpret_cast<T*>(dst) + feature(w);
-    if (w.piece < s.turning) {
-      const float* c = cs + w.token * width + w.piece * kPairs;
-      const float* sn = c + a.half;
-      if constexpr (kVec == 1) {
-        const float x1 = (float)w.a, x2 = (float)w.b;
-        y[0] = (T)(x1 * c[0] - x2 * sn[0]);
-        y[kAdjacent ? 1 : a.half] = (T)(x2 * c[0] + x1 * sn[0]);
-      } else if constexpr (kAdjacent) {
-        Row o;
-#pragma unroll
-        for (int i = 0; i < kPairs; ++i) {
-          const float x1 = (float)w.a[2 * i], x2 = (float)w.a[2 * i + 1];
-          o[2 * i] = (T)(x1 * c[i] - x2 * sn[i]);
-          o[2 * i + 1] = (T)(x2 * c[i] + x1 * sn[i]);
-        }
-        *reinterpret_cast<Row*>(y) = o;
-      } else {
-        Row o1, o2;
-#pragma unroll
-        for (int i = 0; i < kVec; ++i) {
-          const float x1 = (float)w.a[i], x2 = (float)w.b[i];
-          o1[i] = (T)(x1 * c[i] - x2 * sn[i]);
-          o2[i] = (T)(x2 * c[i] + x1 * sn[i]);
-        }
-        *reinterpret_cast<Row*>(y) = o1;
-        *reinterpret_cast<Row*>(y + a.half) = o2;
-      }
-    } else {
-      *reinterpret_cast<Row*>(y) = w.a;
-    }
-  }
+  });
 }
 
 template <typename T>
@@ -202,27 +219,36 @@ void launch_typed(const RotArgs& a, bool vec, bool adjacent, hipStream_t stream)
 
 int dtype_size(int32_t dtype) { return dtype == OSCAR_FP32 ? 4 : 2; }
 
+// One kind of rows: where they come from and go to (out null: a cache).
+struct Rows {
+  const uint8_t* src;
+  uint8_t* dst;
+  int64_t src_token, src_head, dst_token, dst_head;    // bytes
+  int32_t heads;
+};
+
 bool fits16(const void* p, int64_t token_bytes, int64_t head_bytes) {
   return ((uintptr_t)p | (uintptr_t)token_bytes | (uintptr_t)head_bytes) % 16 == 0;
 }
 
-// Source and destination of a set; out null: cache slots.
-bool make_set(RowSet& s, const oscar_heads* in, const oscar_heads* out, int size, bool& vec) {
-  if (in == nullptr || in->num_heads == 0) return true;
-  if (in->data == nullptr || in->num_heads < 0 || in->num_heads > (1 << 16)) return false;
+int make_rows(Rows& s, const oscar_heads* in, const oscar_heads* out, int size, bool& vec) {
+  if (in == nullptr || in->num_heads == 0) return kOk;
+  if (in->data == nullptr || in->num_heads < 0 || in->num_heads > (1 << 16)) return kErrInvalidArgument;
   s.src = static_cast<const uint8_t*>(in->data);
   s.src_token = in->token_stride * size;
   s.src_head = in->head_stride * size;
   s.heads = in->num_heads;
   vec = vec && fits16(s.src, s.src_token, s.src_head);
   if (out != nullptr) {
-    if (out->data == nullptr || out->num_heads != in->num_heads) return false;
+    if (out->data == nullptr || out->num_heads != in->num_heads) return kErrInvalidArgument;
     s.dst = static_cast<uint8_t*>(out->data);
     s.dst_token = out->token_stride * size;
     s.dst_head = out->head_stride * size;
     vec = vec && fits16(s.dst, s.dst_token, s.dst_head);
   }
-  return true;
+  for (const int64_t x : {s.src_token, s.src_head, s.dst_token, s.dst_head})
+    if (x < 0 || x > UINT32_MAX) return kErrUnsupportedGeometry;
+  return kOk;
 }
 
 int run(const oscar_rotary* r, const int64_t* positions, int64_t axis_stride, int64_t tokens, const oscar_heads* query,
@@ -240,14 +266,18 @@ int run(const oscar_rotary* r, const int64_t* positions, int64_t axis_stride, in
   const int size = dtype_size(dtype);
   RotArgs a{};
   bool vec = true;
-  if (!make_set(a.set[0], query, query_out, size, vec) || !make_set(a.set[1], key, key_out, size, vec) ||
-      !make_set(a.set[2], value, nullptr, size, vec))
-    return kErrInvalidArgument;
+  Rows rows[3] = {};
+  const oscar_heads* const in[3] = {query, key, value};
+  const oscar_heads* const out[3] = {query_out, key_out, nullptr};
+  for (int i = 0; i < 3; ++i) {
+    const int status = make_rows(rows[i], in[i], out[i], size, vec);
+    if (status != kOk) return status;
+  }
   if (cache != nullptr) {
-    a.set[1].dst = static_cast<uint8_t*>(cache->k);
-    a.set[1].dst_head = cache->k_stride_head;
-    a.set[2].dst = static_cast<uint8_t*>(cache->v);
-    a.set[2].dst_head = cache->v_stride_head;
+    rows[1].dst = static_cast<uint8_t*>(cache->k);
+    rows[1].dst_head = cache->k_stride_head;
+    rows[2].dst = static_cast<uint8_t*>(cache->v);
+    rows[2].dst_head = cache->v_stride_head;
     a.slots = slots;
     a.num_slots = cache->num_pages * cache->block_size;
     a.k_page = cache->k_stride_page;
@@ -264,17 +294,27 @@ int run(const oscar_rotary* r, const int64_t* positions, int64_t axis_stride, in
   const int wide = 16 / size;
   vec = vec && head_size % wide == 0 && (r->adjacent ? r->rotary_dim : r->rotary_dim / 2) % wide == 0;
   const int step = vec ? wide : 1;
-  for (int i = 0; i < 3; ++i) {
-    RowSet& s = a.set[i];
-    const bool in_place = i < 2 && s.src == s.dst && s.src_token == s.dst_token && s.src_head == s.dst_head &&
-                          !(cache != nullptr && i == 1);
-    s.turning = i == 2 ? 0 : (r->adjacent ? (vec ? r->rotary_dim / step : r->rotary_dim / 2) : r->rotary_dim / 2 / step);
-    s.pieces = i == 2 ? head_size / step : s.turning + (in_place ? 0 : (head_size - r->rotary_dim) / step);
-    s.first = i == 0 ? 0 : a.set[i - 1].first + a.set[i - 1].heads * a.set[i - 1].pieces;
-    s.by_pieces = make_fast_div((uint32_t)s.pieces);
-    a.pieces += s.heads * s.pieces;
+  int64_t work = 0;                         // pieces of a token
+  for (int i = 0; i < kJobs; ++i) {
+    const Rows& s = rows[turns(i) ? i : i - 2];
+    const bool in_place = s.src == s.dst && s.src_token == s.dst_token && s.src_head == s.dst_head;
+    Job& j = a.job[i];
+    j.src = s.src;
+    j.dst = s.dst;
+    j.src_token = (uint32_t)s.src_token;
+    j.src_head = (uint32_t)s.src_head;
+    j.dst_token = (uint32_t)s.dst_token;
+    j.dst_head = (uint32_t)s.dst_head;
+    if (turns(i)) j.pieces = r->adjacent && vec ? r->rotary_dim / step : r->rotary_dim / 2 / step;
+    else if (i == 4) j.pieces = head_size / step;
+    else j.pieces = in_place ? 0 : (head_size - r->rotary_dim) / step;
+    j.first = turns(i) || i == 4 ? 0 : r->rotary_dim;
+    j.a_token = s.heads * j.pieces;
+    j.by_token = make_fast_div((uint32_t)(j.a_token > 0 ? j.a_token : 1));
+    j.by_head = make_fast_div((uint32_t)(j.pieces > 0 ? j.pieces : 1));
+    work += j.a_token;
   }
-  if (a.pieces == 0) return kOk;
+  if (work == 0) return kOk;
   a.table = r->table;
   a.positions = positions;
   a.axis_stride = axis_stride;
@@ -284,12 +324,13 @@ int run(const oscar_rotary* r, const int64_t* positions, int64_t axis_stride, in
   a.axes = r->axes;
   a.half = r->rotary_dim / 2;
   a.sign = inverse ? -1.f : 1.f;
-  a.by_pieces = make_fast_div((uint32_t)a.pieces);
   a.by_half = make_fast_div((uint32_t)a.half);
-  // Tokens of a workgroup: eight pieces a thread, one token where they are few.
-  int block = (8 * kRotThreads + a.pieces - 1) / a.pieces;
-  block = block > kMaxTokens ? kMaxTokens : block;
-  while (block > 1 && (tokens + block - 1) / block < 1024) block /= 2;
+  // Tokens of a workgroup: a power of two, up to ten pieces a thread, fewer where
+  // that leaves less than 1024 workgroups (9256 tokens of 7 heads of 256: 8 tokens
+  // 14.7 us, 5 17.0; 30843 of 40 heads of 128: 4 tokens 121 us, 7 130; a write of
+  // 65536: 9 tokens 119 us, 5 120, 14 153).
+  int block = kMaxTokens;
+  while (block > 1 && (block * work > 10 * kRotThreads || (tokens + block - 1) / block < 1024)) block /= 2;
   a.block_tokens = block;
   if ((tokens + block - 1) / block > INT32_MAX) return kErrInvalidArgument;
   if (dtype == OSCAR_BF16) launch_typed<__bf16>(a, vec, r->adjacent != 0, stream);
