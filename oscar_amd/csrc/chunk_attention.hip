@@ -45,6 +45,7 @@ typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 typedef float floatx8 __attribute__((ext_vector_type(8)));
 typedef uint16_t ushortx2 __attribute__((ext_vector_type(2)));
+typedef uint16_t ushortx8 __attribute__((ext_vector_type(8)));
 typedef short shortx4 __attribute__((ext_vector_type(4)));
 typedef short shortx8 __attribute__((ext_vector_type(8)));
 typedef __attribute__((address_space(3))) void lds_void;
@@ -64,6 +65,7 @@ struct Num<__bf16> {
     return __builtin_bit_cast(V8, w);
   }
   static constexpr uint16_t kLazyBits = 0x4380;      // 2^kLazy
+  static constexpr uint16_t kInfBits = 0x7F80;
   static __device__ __forceinline__ floatx16 mfma(V8 a, V8 b, floatx16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
   }
@@ -87,6 +89,7 @@ struct Num<_Float16> {
     return __builtin_bit_cast(V8, w);
   }
   static constexpr uint16_t kLazyBits = 0x5C00;
+  static constexpr uint16_t kInfBits = 0x7C00;
   static __device__ __forceinline__ floatx16 mfma(V8 a, V8 b, floatx16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
   }
@@ -294,6 +297,65 @@ __device__ __forceinline__ typename Num<T>::V8 v_operand_at(const uint8_t* vt, i
   return __builtin_bit_cast(typename Num<T>::V8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
 }
 
+// Values that a row does not see must not reach it, and a weight of zero times an
+// infinity or NaN would.  Tiles that every row sees whole need no care; in the
+// others the values are looked over first (kBytes of V in LDS, by the wave), and
+// if some are not finite the product takes them as zeros; what they do to the
+// rows that do see them is added when the piece is done (add_special).
+template <typename T, int kBytes>
+__device__ __forceinline__ bool any_special(const uint8_t* vt, int lane) {
+  ushortx8 top{};
+#pragma unroll
+  for (int i = 0; i < kBytes / 1024; ++i) {
+    const ushortx8 u = *reinterpret_cast<const ushortx8*>(vt + i * 1024 + lane * 16);
+    top = __builtin_elementwise_max(top, u & (uint16_t)0x7FFF);
+  }
+  bool special = false;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) special = special || top[i] >= Num<T>::kInfBits;
+  return __ballot(special) != 0ull;
+}
+template <typename T>
+__device__ __forceinline__ typename Num<T>::V8 finite_values(typename Num<T>::V8 v) {
+  const ushortx8 u = __builtin_bit_cast(ushortx8, v);
+  const ushortx8 below = Num<T>::kInfBits - (u & Num<T>::kInfBits);        // 0: not finite
+  const ushortx8 keep = 0 - __builtin_elementwise_min(below, (ushortx8)(uint16_t)1);
+  return __builtin_bit_cast(typename Num<T>::V8, u & keep);
+}
+// The values of a tile that are not finite, added to the sums of the rows that
+// see them: what a positive weight makes of them.  Tiles that are whole and mapped
+// had them in the product.
+template <typename T, int D, int kKeys>
+__device__ __forceinline__ void add_special(const ChunkArgs& a, const Piece& p, int key0, bool whole, int lane,
+                                            RowState<T, D>& s) {
+  typedef T T4 __attribute__((ext_vector_type(4)));
+  auto page_of = [&](int key) {
+    const int page = a.table[(int64_t)p.table_row * a.table_stride + fast_div((uint32_t)key, a.block_div)];
+    return page >= 0 && page < a.num_pages ? page : -1;
+  };
+  const int end = min(key0 + kKeys, p.key1);
+  if (whole && page_of(key0) >= 0 && page_of(end - 1) >= 0) return;
+  for (int key = key0; key < end; ++key) {
+    const int page = page_of(key);
+    if (page < 0) continue;
+    const uint8_t* row = a.v + (int64_t)p.kv_head * a.v_head + (uint64_t)(uint32_t)page * a.v_page +
+                         (uint64_t)fast_mod((uint32_t)key, a.block_div) * (uint32_t)a.v_token + 8 * (lane >> 5);
+    const bool seen = key <= s.pos && (a.window == 0 || key > s.pos - a.window);
+#pragma unroll
+    for (int b = 0; b < D / 32; ++b)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const T4 x = *reinterpret_cast<const T4*>(row + 64 * b + 16 * j);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float v = (float)x[i];
+          s.acc[b][4 * j + i] += seen && !(fabsf(v) < __builtin_inff()) ? v : 0.f;
+        }
+        keep_order();                       // (few registers: this is rarely run)
+      }
+  }
+}
+
 // This lane's place in the reads of a K tile (key lane % 32, chunk 2 i + lane /
 // 32 of k-step i) and of a V tile (keys 4 g + (lane % 16) / 4, 16 features of
 // the lane's quarter).
@@ -353,6 +415,8 @@ __device__ __forceinline__ void narrow_piece(const ChunkArgs& a, const Piece p, 
   RowState<T, D> s;
   load_rows<T, D>(a, p, p.row0, lane, s);
   const int whole_from = a.window == 0 ? 0 : s.last - a.window + 1, whole_to = s.first - kKeys + 1;
+  auto whole = [&](int key0) { return key0 >= whole_from && key0 <= whole_to; };
+  bool special = false;                     // a tile that is not whole held values that are not finite
 
   const LanePlace k_place = lane_place<D, false>(a, lane), v_place = lane_place<D, true>(a, lane);
   auto page_of = [&](int t, int h) { return __builtin_amdgcn_readlane(pages, kHalves * t + h - page_base); };
@@ -386,7 +450,8 @@ __device__ __forceinline__ void narrow_piece(const ChunkArgs& a, const Piece p, 
     if (more) load_tile(t + 1, std::false_type{}, kt);
 
     const int key0 = t * kKeys;
-    if (!(key0 >= whole_from && key0 <= whole_to && unmapped == 0u)) mask_scores<8 * kHalves>(a, x, key0, unmapped, lane, s.pos);
+    const bool masked = !whole(key0) || unmapped != 0u;
+    if (masked) mask_scores<8 * kHalves>(a, x, key0, unmapped, lane, s.pos);
     float top = x[0];
 #pragma unroll
     for (int i = 1; i < 8 * kHalves; ++i) top = fmaxf(top, x[i]);
@@ -412,11 +477,16 @@ __device__ __forceinline__ void narrow_piece(const ChunkArgs& a, const Piece p, 
     if (more) wait_vmcnt<kLoads>();
     else wait_vmcnt<0>();
     asm volatile("" ::: "memory");
-#pragma unroll
-    for (int h = 0; h < kHalves; ++h)
-#pragma unroll
-      for (int b = 0; b < kBlocks; ++b)
-        s.acc[b] = Num<T>::mfma(v_operand_at<T, D>(vt, v_addr, h, b), w[h], s.acc[b]);
+    const bool clean = !masked || !any_special<T, kTileBytes>(vt, lane);
+    special = special || !clean;
+    keep_order();
+    each<kHalves * kBlocks>([&](auto step) {
+      constexpr int h = decltype(step)::value / kBlocks, b = decltype(step)::value % kBlocks;
+      V8 v = v_operand_at<T, D>(vt, v_addr, h, b);
+      if (__builtin_expect(!clean, 0)) v = finite_values<T>(v);
+      s.acc[b] = Num<T>::mfma(v, w[h], s.acc[b]);
+      if constexpr (b % 4 == 3 || b == kBlocks - 1) keep_order();
+    });
     asm volatile("" ::: "memory");
     if (more) load_tile(t + 1, std::true_type{}, vt);
   };
@@ -427,6 +497,8 @@ __device__ __forceinline__ void narrow_piece(const ChunkArgs& a, const Piece p, 
     load_tile(first, std::true_type{}, kt + kTileBytes);
   }
   for (int t = first; t < last; ++t) tile(t, kt, kt + kTileBytes);
+  if (__builtin_expect(special, 0))
+    for (int t = first; t < last; ++t) add_special<T, D, kKeys>(a, p, t * kKeys, whole(t * kKeys), lane, s);
 
   // Combine: the waves' sums through LDS, D / kRounds features at a time (16-byte
   // pieces, the row xor-ed in).
@@ -554,10 +626,8 @@ __device__ __forceinline__ void wide_piece(const ChunkArgs& a, const Piece p, ui
   };
   // Rows that do not see the whole of a tile lose what they do not see.
   const int whole_from = a.window == 0 ? 0 : s.last - a.window + 1, whole_to = s.first - kTileKeys + 1;
-  auto mask = [&](floatx16& x, int key0, uint32_t gone) {
-    if (__builtin_expect(key0 >= whole_from && key0 <= whole_to && gone == 0u, 1)) return;
-    mask_scores<16>(a, x, key0, gone, lane, s.pos);
-  };
+  auto whole = [&](int key0) { return key0 >= whole_from && key0 <= whole_to; };
+  bool special = false;                     // such a tile held values that are not finite
   auto weigh = [&](const floatx16& x, V8 (&w)[2]) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -572,8 +642,7 @@ __device__ __forceinline__ void wide_piece(const ChunkArgs& a, const Piece p, ui
   // their bits do, so this takes nine operations for a tile, where the maximum of
   // the scores takes one for each.
   auto beyond = [&](const V8 (&w)[2]) {
-    typedef uint16_t ushortx8 __attribute__((ext_vector_type(8)));
-    ushortx8 u = __builtin_elementwise_max(__builtin_bit_cast(ushortx8, w[0]), __builtin_bit_cast(ushortx8, w[1]));
+    const ushortx8 u = __builtin_elementwise_max(__builtin_bit_cast(ushortx8, w[0]), __builtin_bit_cast(ushortx8, w[1]));
     const ushortx2 top = __builtin_elementwise_max(
         __builtin_elementwise_max(__builtin_shufflevector(u, u, 0, 1), __builtin_shufflevector(u, u, 2, 3)),
         __builtin_elementwise_max(__builtin_shufflevector(u, u, 4, 5), __builtin_shufflevector(u, u, 6, 7)));
@@ -621,7 +690,12 @@ __device__ __forceinline__ void wide_piece(const ChunkArgs& a, const Piece p, ui
 #pragma unroll
     for (int i = 0; i < kAheadV; ++i) v[i] = v_operand(vt, i);
     __builtin_amdgcn_s_setprio(0);
-    mask(x, key0, gone);
+    bool clean = true;
+    if (__builtin_expect(!whole(key0) || gone != 0u, 0)) {
+      mask_scores<16>(a, x, key0, gone, lane, s.pos);
+      clean = !any_special<T, kTileBytes>(vt, lane);
+      special = special || !clean;
+    }
     V8 w[2];
     weigh(x, w);
     if (__ballot(beyond(w))) {
@@ -633,6 +707,7 @@ __device__ __forceinline__ void wide_piece(const ChunkArgs& a, const Piece p, ui
     // O^T += V^T P^T
     each<kPv>([&](auto step) {
       constexpr int i = decltype(step)::value, h = i / kBlocks, b = i % kBlocks;
+      if (__builtin_expect(!clean, 0)) v[i % kAheadV] = finite_values<T>(v[i % kAheadV]);
       s.acc[b] = Num<T>::mfma(v[i % kAheadV], w[h], s.acc[b]);
       pin(s.acc[b]);
       if constexpr (i + kAheadV < kPv) v[i % kAheadV] = v_operand(vt, i + kAheadV);
@@ -677,6 +752,9 @@ __device__ __forceinline__ void wide_piece(const ChunkArgs& a, const Piece p, ui
     run(smem + kStageBytes, smem);
   }
   arrive_all();                             // (loads to LDS that nobody waits for)
+  if (__builtin_expect(special, 0))
+    for (int key0 = p.key0; key0 < p.key1; key0 += kTileKeys)
+      add_special<T, D, kTileKeys>(a, p, key0, whole(key0), lane, s);
 
   const float l = sum_halves(s.l);
   const int at = kTileRows * wave + (lane & 31);

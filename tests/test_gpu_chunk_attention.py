@@ -152,6 +152,53 @@ def test_what_lies_in_unseen_slots_does_not_matter(device, d):
     check(want, q, caches, table, starts, seqs, 0, 0.1, 64)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("window", [0, 40])
+def test_what_a_row_does_not_see_does_not_reach_it(device, dtype, d, window):
+    """NaN and infinities in keys and values of single positions: rows that do not
+    see them are as without them, rows that do have the formula's NaN or infinity."""
+    g = torch.Generator(device=device).manual_seed(16)
+    for reqs in ([(16, 100), (3, 70)], [(200, 90)], [(260, 0), (2, 33)]):
+        q, caches, table, starts, seqs = make(g, reqs, 4, 2, d, 32, dtype)
+        table[0, 0] = -1 if reqs[0][1] == 90 else table[0, 0]     # (a tile that is whole, but half unmapped)
+        cache = append.PagedCache(*caches)
+        step = chunk.ChunkStep(starts, seqs, table, 4, cache, window)
+        clean = chunk.chunk_attention(q, cache, step, 0.1)
+        n, h = reqs[0]
+        at = {h + n // 2: (1, math.nan, 5), h + n - 2: (1, math.inf, 7), h + n - 5: (1, -math.inf, 7),
+              h + 3: (0, math.inf, 1), max(h - 20, 0) + 16: (1, math.inf, 2)}
+        for pos, (which, value, feature) in at.items():
+            caches[which][table[0, pos // 32].long(), pos % 32, 0, feature] = value
+        got = chunk.chunk_attention(q, cache, step, 0.1)
+        pos = h + torch.arange(n, device=device)
+        touched = torch.zeros(n, 2, d, dtype=torch.bool, device=device)      # (kv head 0: query heads 0 and 1)
+        without = torch.zeros(n, 2, 1, dtype=torch.bool, device=device)      # rows whose score of the infinite key is
+        for p, (which, value, feature) in at.items():                        # -inf: its weight is 0
+            sees = ((pos >= p) & ((pos < p + window) if window else True))[:, None, None]
+            if which == 0:
+                hidden = torch.arange(n + h, device=device) == p
+                touched |= sees & (q[:n, :2, 1:2] > 0)                       # +inf: no number in the whole row
+                without |= sees & (q[:n, :2, 1:2] < 0)
+            else:
+                touched[..., feature] |= sees[..., 0]
+        mine, were = got[:n, :2], clean[:n, :2]
+        assert torch.equal(got[:, 2:], clean[:, 2:]) and torch.equal(got[n:], clean[n:])
+        same = ~touched & ~without
+        assert torch.equal(mine[same], were[same])
+        assert not mine[touched].isfinite().any()
+        if reqs[0][1] != 90:
+            keys, values = gather(caches, table[0], n + h, 32)
+            values = torch.where(values.isfinite(), values, 0.0)
+            keys = torch.where(keys.isfinite(), keys, 0.0)
+            o, bound = expected(q[:n], keys, values, h, window, 0.1, hidden)
+            rest = (without & ~touched).expand_as(mine)
+            assert ((mine.double() - o[:, :2]).abs() <= bound[:, :2])[rest].all()
+        # a single infinity stays one
+        row = touched[..., 2] & ~touched[..., 1]
+        assert (mine[row][..., 2] == math.inf).all()
+
+
 def test_unmapped_pages_are_left_out(device):
     g = torch.Generator(device=device).manual_seed(7)
     reqs = [(2, 200), (40, 200), (1, 10), (3, 300)]
