@@ -299,28 +299,27 @@ __device__ __forceinline__ typename Num<T>::V8 v_operand_at(const uint8_t* vt, i
 
 // Values that a row does not see must not reach it, and a weight of zero times an
 // infinity or NaN would.  Tiles that every row sees whole need no care; in the
-// others the values are looked over first (kBytes of V in LDS, by the wave), and
-// if some are not finite the product takes them as zeros; what they do to the
-// rows that do see them is added when the piece is done (add_special).
+// others the wave looks over the values in LDS (kBytes) and, if some are not
+// finite, makes them zeros there; what they do to the rows that do see them is
+// added when the piece is done (add_special).  Waves that share a tile may do so
+// at the same time: they write the same, and one at least has seen them.
 template <typename T, int kBytes>
-__device__ __forceinline__ bool any_special(const uint8_t* vt, int lane) {
+__device__ __forceinline__ bool take_out_special(uint8_t* vt, int lane) {
+  ushortx8* const at = reinterpret_cast<ushortx8*>(vt) + lane;
   ushortx8 top{};
 #pragma unroll
-  for (int i = 0; i < kBytes / 1024; ++i) {
-    const ushortx8 u = *reinterpret_cast<const ushortx8*>(vt + i * 1024 + lane * 16);
-    top = __builtin_elementwise_max(top, u & (uint16_t)0x7FFF);
-  }
+  for (int i = 0; i < kBytes / 1024; ++i) top = __builtin_elementwise_max(top, at[64 * i] & (uint16_t)0x7FFF);
   bool special = false;
 #pragma unroll
   for (int i = 0; i < 8; ++i) special = special || top[i] >= Num<T>::kInfBits;
-  return __ballot(special) != 0ull;
-}
-template <typename T>
-__device__ __forceinline__ typename Num<T>::V8 finite_values(typename Num<T>::V8 v) {
-  const ushortx8 u = __builtin_bit_cast(ushortx8, v);
-  const ushortx8 below = Num<T>::kInfBits - (u & Num<T>::kInfBits);        // 0: not finite
-  const ushortx8 keep = 0 - __builtin_elementwise_min(below, (ushortx8)(uint16_t)1);
-  return __builtin_bit_cast(typename Num<T>::V8, u & keep);
+  if (__builtin_expect(__ballot(special) == 0ull, 1)) return false;
+#pragma unroll 1
+  for (int i = 0; i < kBytes / 1024; ++i) {
+    const ushortx8 u = at[64 * i];
+    const ushortx8 below = Num<T>::kInfBits - (u & Num<T>::kInfBits);      // 0: not finite
+    at[64 * i] = u & (0 - __builtin_elementwise_min(below, (ushortx8)(uint16_t)1));
+  }
+  return true;
 }
 // The values of a tile that are not finite, added to the sums of the rows that
 // see them: what a positive weight makes of them.  Tiles that are whole and mapped
@@ -477,14 +476,11 @@ __device__ __forceinline__ void narrow_piece(const ChunkArgs& a, const Piece p, 
     if (more) wait_vmcnt<kLoads>();
     else wait_vmcnt<0>();
     asm volatile("" ::: "memory");
-    const bool clean = !masked || !any_special<T, kTileBytes>(vt, lane);
-    special = special || !clean;
+    if (masked) special = take_out_special<T, kTileBytes>(vt, lane) || special;
     keep_order();
     each<kHalves * kBlocks>([&](auto step) {
       constexpr int h = decltype(step)::value / kBlocks, b = decltype(step)::value % kBlocks;
-      V8 v = v_operand_at<T, D>(vt, v_addr, h, b);
-      if (__builtin_expect(!clean, 0)) v = finite_values<T>(v);
-      s.acc[b] = Num<T>::mfma(v, w[h], s.acc[b]);
+      s.acc[b] = Num<T>::mfma(v_operand_at<T, D>(vt, v_addr, h, b), w[h], s.acc[b]);
       if constexpr (b % 4 == 3 || b == kBlocks - 1) keep_order();
     });
     asm volatile("" ::: "memory");
@@ -624,10 +620,13 @@ __device__ __forceinline__ void wide_piece(const ChunkArgs& a, const Piece p, ui
   auto v_operand = [&](const uint8_t* vt, int i) {
     return v_operand_at<T, D>(vt, kKeepAddresses ? v_addr : opaque(v_addr), i / kBlocks, i % kBlocks);
   };
-  // Rows that do not see the whole of a tile lose what they do not see.
-  const int whole_from = a.window == 0 ? 0 : s.last - a.window + 1, whole_to = s.first - kTileKeys + 1;
+  // Rows that do not see the whole of a tile lose what they do not see.  (Asked of
+  // the workgroup's rows together: its waves share the tiles.)
+  const int pos0 = p.pos0 + (int)fast_div((uint32_t)p.row0, a.group_div);
+  const int pos1 = p.pos0 + (int)fast_div((uint32_t)(p.row0 + p.rows - 1), a.group_div);
+  const int whole_from = a.window == 0 ? 0 : pos1 - a.window + 1, whole_to = pos0 - kTileKeys + 1;
   auto whole = [&](int key0) { return key0 >= whole_from && key0 <= whole_to; };
-  bool special = false;                     // such a tile held values that are not finite
+  bool special = false;                     // this wave found values that are not finite in such a tile
   auto weigh = [&](const floatx16& x, V8 (&w)[2]) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -664,7 +663,7 @@ __device__ __forceinline__ void wide_piece(const ChunkArgs& a, const Piece p, ui
   };
 
   // One tile; `requests(i)` goes out beside step i of its first product.
-  auto tile = [&](const uint8_t* __restrict__ kt, const uint8_t* __restrict__ vt, int key0, uint32_t gone,
+  auto tile = [&](const uint8_t* __restrict__ kt, uint8_t* __restrict__ vt, int key0, uint32_t gone,
                   auto&& requests) __attribute__((always_inline)) {
     if constexpr (!kKeepAddresses) {
       k_place = LanePlace{opaque(k_place.row), opaque(k_place.chunk)};
@@ -686,16 +685,14 @@ __device__ __forceinline__ void wide_piece(const ChunkArgs& a, const Piece p, ui
       requests(i);
       keep_order();
     });
+    __builtin_amdgcn_s_setprio(0);
+    if (__builtin_expect(!whole(key0) || gone != 0u, 0)) {
+      mask_scores<16>(a, x, key0, gone, lane, s.pos);
+      special = take_out_special<T, kTileBytes>(vt, lane) || special;
+    }
     V8 v[kAheadV];
 #pragma unroll
     for (int i = 0; i < kAheadV; ++i) v[i] = v_operand(vt, i);
-    __builtin_amdgcn_s_setprio(0);
-    bool clean = true;
-    if (__builtin_expect(!whole(key0) || gone != 0u, 0)) {
-      mask_scores<16>(a, x, key0, gone, lane, s.pos);
-      clean = !any_special<T, kTileBytes>(vt, lane);
-      special = special || !clean;
-    }
     V8 w[2];
     weigh(x, w);
     if (__ballot(beyond(w))) {
@@ -707,7 +704,6 @@ __device__ __forceinline__ void wide_piece(const ChunkArgs& a, const Piece p, ui
     // O^T += V^T P^T
     each<kPv>([&](auto step) {
       constexpr int i = decltype(step)::value, h = i / kBlocks, b = i % kBlocks;
-      if (__builtin_expect(!clean, 0)) v[i % kAheadV] = finite_values<T>(v[i % kAheadV]);
       s.acc[b] = Num<T>::mfma(v[i % kAheadV], w[h], s.acc[b]);
       pin(s.acc[b]);
       if constexpr (i + kAheadV < kPv) v[i % kAheadV] = v_operand(vt, i + kAheadV);
@@ -752,7 +748,10 @@ __device__ __forceinline__ void wide_piece(const ChunkArgs& a, const Piece p, ui
     run(smem + kStageBytes, smem);
   }
   arrive_all();                             // (loads to LDS that nobody waits for)
-  if (__builtin_expect(special, 0))
+  if (lane == 0) reinterpret_cast<int*>(smem)[wave] = special;
+  arrive_all();
+  const u32x4 found = *reinterpret_cast<const u32x4*>(smem);
+  if (__builtin_expect(__builtin_amdgcn_readfirstlane(found[0] | found[1] | found[2] | found[3]) != 0, 0))
     for (int key0 = p.key0; key0 < p.key1; key0 += kTileKeys)
       add_special<T, D, kTileKeys>(a, p, key0, whole(key0), lane, s);
 
