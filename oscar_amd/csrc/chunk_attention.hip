@@ -519,28 +519,47 @@ __device__ __forceinline__ void narrow_piece(const ChunkArgs& a, const Piece p, 
       ml[wave * 64 + (lane >> 5) * 32 + row] = lane < 32 ? s.m : s.l;
     }
     __syncthreads();
-    for (int i = tid; i < p.rows * (kPart / 4); i += kThreads) {
-      const int r = i / (kPart / 4), piece = i % (kPart / 4), feature = round * kPart + 4 * piece;
-      float m = ml[r];
+    // a thread to four features of some rows, kBatch of them at once
+    constexpr int kAcross = kThreads / (kPart / 4), kBatch = kAcross >= 16 ? 1 : 16 / kAcross;
+    const int piece = tid % (kPart / 4), feature = round * kPart + 4 * piece;
+    for (int r0 = tid / (kPart / 4); r0 < p.rows; r0 += kAcross * kBatch) {
+      float m[kBatch], l[kBatch];
+      floatx4 o[kBatch];
 #pragma unroll
-      for (int w = 1; w < kWaves; ++w) m = fmaxf(m, ml[w * 64 + r]);
-      floatx4 o{};
-      float l = 0.f;
+      for (int n = 0; n < kBatch; ++n) {
+        const int r = min(r0 + n * kAcross, p.rows - 1);
+        float wm[kWaves], wl[kWaves];
+        floatx4 x[kWaves];
 #pragma unroll
-      for (int w = 0; w < kWaves; ++w) {
-        const float f = __builtin_amdgcn_exp2f(ml[w * 64 + r] - m);
-        l += f * ml[w * 64 + 32 + r];
-        o += f * *reinterpret_cast<const floatx4*>(sums + (w * kTileRows + r) * kPart + 4 * (piece ^ (r & 15)));
+        for (int w = 0; w < kWaves; ++w) {
+          wm[w] = ml[w * 64 + r];
+          wl[w] = ml[w * 64 + 32 + r];
+          x[w] = *reinterpret_cast<const floatx4*>(sums + (w * kTileRows + r) * kPart + 4 * (piece ^ (r & 15)));
+        }
+        m[n] = fmaxf(fmaxf(wm[0], wm[1]), fmaxf(wm[2], wm[3]));
+        l[n] = 0.f;
+        o[n] = floatx4{};
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+          const float f = __builtin_amdgcn_exp2f(wm[w] - m[n]);
+          l[n] += f * wl[w];
+          o[n] += f * x[w];
+        }
       }
-      if (p.slot < 0) {
-        const float inv = l == 0.f ? 0.f : 1.f / l;
-        store4<T>(out_row(a, p.token0, p.kv_head, p.row0 + r) + 2 * feature, o * inv);
-      } else {
-        float* part = a.partials + (int64_t)p.slot * (kTileRows * (D + 2));
-        *reinterpret_cast<floatx4*>(part + r * D + feature) = o;
-        if (feature == 0) {
-          part[kTileRows * D + r] = m;
-          part[kTileRows * D + kTileRows + r] = l;
+#pragma unroll
+      for (int n = 0; n < kBatch; ++n) {
+        const int r = r0 + n * kAcross;
+        if (r >= p.rows) break;
+        if (p.slot < 0) {
+          const float inv = l[n] == 0.f ? 0.f : 1.f / l[n];
+          store4<T>(out_row(a, p.token0, p.kv_head, p.row0 + r) + 2 * feature, o[n] * inv);
+        } else {
+          float* part = a.partials + (int64_t)p.slot * (kTileRows * (D + 2));
+          *reinterpret_cast<floatx4*>(part + r * D + feature) = o[n];
+          if (feature == 0) {
+            part[kTileRows * D + r] = m[n];
+            part[kTileRows * D + kTileRows + r] = l[n];
+          }
         }
       }
     }
@@ -814,33 +833,32 @@ __global__ __launch_bounds__(kThreads, kWideWgs) void mixed_kernel(ChunkArgs a) 
 // 16 across the partials, whose sums meet in LDS.
 constexpr int kFewParts = 8;
 
-template <typename T, int D>
+template <typename T, int D, int kParts>
 __device__ __forceinline__ void join_few(const ChunkArgs& a, const Join j, int block) {
   const int i = block * 256 + (int)threadIdx.x, row = i / (D / 4), feature = 4 * (i % (D / 4));
   if (row >= j.rows) return;
   const float* const first = a.partials + (int64_t)j.slot0 * (kTileRows * (D + 2));
-  const int64_t step = (int64_t)j.step * (kTileRows * (D + 2));
-  float m[kFewParts], top = kNone;
-  floatx4 x[kFewParts];
+  float m[kParts], l[kParts], top = kNone;
+  floatx4 x[kParts];
 #pragma unroll
-  for (int s = 0; s < kFewParts; ++s) {
-    m[s] = kNone;
-    if (s < j.count) {
-      m[s] = first[s * step + kTileRows * D + row];
-      x[s] = *reinterpret_cast<const floatx4*>(first + s * step + row * D + feature);
-    }
-    top = fmaxf(top, m[s]);
+  for (int s = 0; s < kParts; ++s) {        // (the last one again for those that are not there: no load waits)
+    const float* at = first + (int64_t)(min(s, j.count - 1) * j.step) * (kTileRows * (D + 2));
+    m[s] = at[kTileRows * D + row];
+    l[s] = at[kTileRows * D + kTileRows + row];
+    x[s] = *reinterpret_cast<const floatx4*>(at + row * D + feature);
   }
-  floatx4 o{};
-  float l = 0.f;
 #pragma unroll
-  for (int s = 0; s < kFewParts; ++s)
+  for (int s = 0; s < kParts; ++s) top = fmaxf(top, m[s]);
+  floatx4 o{};
+  float sum = 0.f;
+#pragma unroll
+  for (int s = 0; s < kParts; ++s)
     if (s < j.count) {
       const float w = __builtin_amdgcn_exp2f(m[s] - top);
-      l += w * first[s * step + kTileRows * D + kTileRows + row];
+      sum += w * l[s];
       o += w * x[s];
     }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
   store4<T>(out_row(a, j.token0, j.kv_head, j.row0 + row) + 2 * feature, o * inv);
 }
 
@@ -888,7 +906,10 @@ __global__ __launch_bounds__(256) void join_kernel(ChunkArgs a) {
   constexpr int kFewBlocks = D / 32, kManyBlocks = kTileRows * D / 64;
   const int block = (int)blockIdx.x, few = a.few_joins * kFewBlocks;
   if (block < few) {
-    join_few<T, D>(a, a.joins[block / kFewBlocks], block % kFewBlocks);
+    const Join j = a.joins[block / kFewBlocks];
+    if (j.count <= 2) join_few<T, D, 2>(a, j, block % kFewBlocks);
+    else if (j.count <= 4) join_few<T, D, 4>(a, j, block % kFewBlocks);
+    else join_few<T, D, kFewParts>(a, j, block % kFewBlocks);
     return;
   }
   const int many = (block - few) / kManyBlocks, at = (block - few) % kManyBlocks;
@@ -954,7 +975,11 @@ void cut(const RowTile& x, const std::vector<int32_t>& cuts, Plan& plan, std::ve
 int32_t pieces_of(const RowTile& x, int64_t per) { return (int32_t)((x.tiles + per - 1) / per); }
 
 // Narrow tiles: the fewest key tiles a piece with which the pieces fit the
-// workgroups that are resident at once.
+// workgroups that are resident at once.  Where the longest row tile is short, all
+// stay whole, and there is no second launch: one token of one user over 256 keys,
+// D = 256, whole 7.9 us of GPU time, cut 8.3 (over 512: 10.9, 9.3); D = 128, 8 kv
+// heads, over 512 whole 7.2, cut 7.1 and 6.2 against 10.6 where the host launches
+// (over 1024: 11.1, 8.4).
 void plan_narrow(const std::vector<RowTile>& rows, int32_t head_size, bool alone, Plan& plan) {
   int64_t total = 0;
   int32_t most = 0;
@@ -962,6 +987,7 @@ void plan_narrow(const std::vector<RowTile>& rows, int32_t head_size, bool alone
     total += x.tiles;
     most = std::max(most, x.tiles);
   }
+  const int32_t uncut = head_size == 256 ? 8 : 16;
   const int64_t resident = (int64_t)kCus * (alone ? narrow_wgs(head_size) : 2);
   int64_t per = std::max<int64_t>(kWaves, (total + resident - 1) / resident);
   auto count = [&](int64_t t) {
@@ -969,7 +995,7 @@ void plan_narrow(const std::vector<RowTile>& rows, int32_t head_size, bool alone
     for (const RowTile& x : rows) c += pieces_of(x, t);
     return c;
   };
-  if ((int64_t)rows.size() >= resident) per = std::max<int64_t>(per, most);
+  if ((int64_t)rows.size() >= resident || most <= uncut) per = std::max<int64_t>(per, most);
   while (per < most && count(per) > resident) ++per;
   std::vector<int32_t> cuts;
   for (const RowTile& x : rows) {
