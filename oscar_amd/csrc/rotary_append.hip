@@ -17,9 +17,9 @@
 // 65536 tokens 176 us instead of 119).  Every job's first round of loads goes out
 // before the cosines are collected.
 //
-// Measured: 30843 tokens of 32 + 8 heads of 128 (fp16, adjacent pairs) 121 us,
-// 5.4 TB/s; 9256 of 6 + 1 heads of 256 (64 features turn, three axes) 14.7 us, 4.7
-// TB/s; a write of 65536 tokens of that shape 119 us, 4.6 TB/s; a large copy moves
+// Measured: 30843 tokens of 32 + 8 heads of 128 (fp16, adjacent pairs) 114 us,
+// 5.6 TB/s; 9256 of 6 + 1 heads of 256 (64 features turn, three axes) 13.3 us, 5.2
+// TB/s; a write of 65536 tokens of that shape 106 us, 5.1 TB/s; a large copy moves
 // 5.05 TB/s.  One token takes 3 us.
 #include "plain_cache.h"
 
@@ -31,6 +31,7 @@ namespace {
 constexpr int kRotThreads = 256;
 constexpr int kMaxTokens = 16;             // of a workgroup
 constexpr int kMaxRotary = 256;
+constexpr int64_t kLastCache = 256ll << 20;      // bytes
 
 // What a launch does with one part of one kind of rows: `pieces` a head, from
 // feature `first` on.
@@ -69,9 +70,21 @@ struct Piece<T, 1> {
   typedef T Row;
 };
 
+// Rows past the caches, where they would only push out what is read again.
+template <bool kOnce, typename Row>
+__device__ __forceinline__ Row load_row(const Row* x) {
+  if constexpr (kOnce) return __builtin_nontemporal_load(x);
+  else return *x;
+}
+template <bool kOnce, typename Row>
+__device__ __forceinline__ void store_row(Row* y, Row x) {
+  if constexpr (kOnce) __builtin_nontemporal_store(x, y);
+  else *y = x;
+}
+
 // kVec values to a load: 16 bytes where rows, strides and pairs allow, else one
 // value (a model's head size and projection decide, not the caller).
-template <typename T, int kVec, bool kAdjacent>
+template <typename T, int kVec, bool kAdjacent, bool kOnce>
 __global__ __launch_bounds__(kRotThreads) void rotary_kernel(RotArgs a) {
   typedef typename Piece<T, kVec>::Row Row;
   __shared__ __attribute__((aligned(16))) float cs[kMaxTokens * kMaxRotary];   // [token][cos | sin]
@@ -99,9 +112,9 @@ __global__ __launch_bounds__(kRotThreads) void rotary_kernel(RotArgs a) {
     w.pair = piece * kPairs;
     const T* x = reinterpret_cast<const T*>(j.src + tok0 * j.src_token + (uint64_t)(uint32_t)w.token * j.src_token +
                                             (uint64_t)(uint32_t)w.head * j.src_head) + w.feature;
-    w.a = *reinterpret_cast<const Row*>(x);
-    if constexpr (turns(kJob) && !kAdjacent) w.b = *reinterpret_cast<const Row*>(x + a.half);
-    else if constexpr (turns(kJob) && kVec == 1) w.b = *reinterpret_cast<const Row*>(x + 1);
+    w.a = load_row<kOnce>(reinterpret_cast<const Row*>(x));
+    if constexpr (turns(kJob) && !kAdjacent) w.b = load_row<kOnce>(reinterpret_cast<const Row*>(x + a.half));
+    else if constexpr (turns(kJob) && kVec == 1) w.b = load_row<kOnce>(reinterpret_cast<const Row*>(x + 1));
   };
   auto finish = [&](auto tag, const Work& w) {
     constexpr int kJob = decltype(tag)::value;
@@ -118,7 +131,7 @@ __global__ __launch_bounds__(kRotThreads) void rotary_kernel(RotArgs a) {
     }
     T* y = reinterpret_cast<T*>(dst) + w.feature;
     if constexpr (!turns(kJob)) {
-      *reinterpret_cast<Row*>(y) = w.a;
+      store_row<kOnce>(reinterpret_cast<Row*>(y), w.a);
     } else {
       const float* c = cs + w.token * width + w.pair;
       const float* sn = c + a.half;
@@ -134,7 +147,7 @@ __global__ __launch_bounds__(kRotThreads) void rotary_kernel(RotArgs a) {
           o[2 * i] = (T)(x1 * c[i] - x2 * sn[i]);
           o[2 * i + 1] = (T)(x2 * c[i] + x1 * sn[i]);
         }
-        *reinterpret_cast<Row*>(y) = o;
+        store_row<kOnce>(reinterpret_cast<Row*>(y), o);
       } else {
         Row o1, o2;
 #pragma unroll
@@ -143,8 +156,8 @@ __global__ __launch_bounds__(kRotThreads) void rotary_kernel(RotArgs a) {
           o1[i] = (T)(x1 * c[i] - x2 * sn[i]);
           o2[i] = (T)(x2 * c[i] + x1 * sn[i]);
         }
-        *reinterpret_cast<Row*>(y) = o1;
-        *reinterpret_cast<Row*>(y + a.half) = o2;
+        store_row<kOnce>(reinterpret_cast<Row*>(y), o1);
+        store_row<kOnce>(reinterpret_cast<Row*>(y + a.half), o2);
       }
     }
   };
@@ -207,14 +220,18 @@ __global__ __launch_bounds__(kRotThreads) void rotary_kernel(RotArgs a) {
   });
 }
 
-template <typename T>
-void launch_typed(const RotArgs& a, bool vec, bool adjacent, hipStream_t stream) {
-  constexpr int kVec = 16 / (int)sizeof(T);
+template <typename T, int kVec, bool kOnce>
+void launch_kernel(const RotArgs& a, bool adjacent, hipStream_t stream) {
   const dim3 grid((uint32_t)((a.tokens + a.block_tokens - 1) / a.block_tokens));
-  if (vec && adjacent) rotary_kernel<T, kVec, true><<<grid, kRotThreads, 0, stream>>>(a);
-  else if (vec) rotary_kernel<T, kVec, false><<<grid, kRotThreads, 0, stream>>>(a);
-  else if (adjacent) rotary_kernel<T, 1, true><<<grid, kRotThreads, 0, stream>>>(a);
-  else rotary_kernel<T, 1, false><<<grid, kRotThreads, 0, stream>>>(a);
+  if (adjacent) rotary_kernel<T, kVec, true, kOnce><<<grid, kRotThreads, 0, stream>>>(a);
+  else rotary_kernel<T, kVec, false, kOnce><<<grid, kRotThreads, 0, stream>>>(a);
+}
+template <typename T>
+void launch_typed(const RotArgs& a, bool vec, bool once, bool adjacent, hipStream_t stream) {
+  constexpr int kVec = 16 / (int)sizeof(T);
+  if (!vec) launch_kernel<T, 1, false>(a, adjacent, stream);
+  else if (once) launch_kernel<T, kVec, true>(a, adjacent, stream);
+  else launch_kernel<T, kVec, false>(a, adjacent, stream);
 }
 
 int dtype_size(int32_t dtype) { return dtype == OSCAR_FP32 ? 4 : 2; }
@@ -294,7 +311,7 @@ int run(const oscar_rotary* r, const int64_t* positions, int64_t axis_stride, in
   const int wide = 16 / size;
   vec = vec && head_size % wide == 0 && (r->adjacent ? r->rotary_dim : r->rotary_dim / 2) % wide == 0;
   const int step = vec ? wide : 1;
-  int64_t work = 0;                         // pieces of a token
+  int64_t work = 0, read = 0;               // pieces and bytes of a token
   for (int i = 0; i < kJobs; ++i) {
     const Rows& s = rows[turns(i) ? i : i - 2];
     const bool in_place = s.src == s.dst && s.src_token == s.dst_token && s.src_head == s.dst_head;
@@ -313,6 +330,7 @@ int run(const oscar_rotary* r, const int64_t* positions, int64_t axis_stride, in
     j.by_token = make_fast_div((uint32_t)(j.a_token > 0 ? j.a_token : 1));
     j.by_head = make_fast_div((uint32_t)(j.pieces > 0 ? j.pieces : 1));
     work += j.a_token;
+    read += (int64_t)j.a_token * step * size * (turns(i) && !(r->adjacent && vec) ? 2 : 1);
   }
   if (work == 0) return kOk;
   a.table = r->table;
@@ -333,9 +351,13 @@ int run(const oscar_rotary* r, const int64_t* positions, int64_t axis_stride, in
   while (block > 1 && (block * work > 10 * kRotThreads || (tokens + block - 1) / block < 1024)) block /= 2;
   a.block_tokens = block;
   if ((tokens + block - 1) / block > INT32_MAX) return kErrInvalidArgument;
-  if (dtype == OSCAR_BF16) launch_typed<__bf16>(a, vec, r->adjacent != 0, stream);
-  else if (dtype == OSCAR_FP16) launch_typed<_Float16>(a, vec, r->adjacent != 0, stream);
-  else launch_typed<float>(a, vec, r->adjacent != 0, stream);
+  // More than the last-level cache holds, read and written: rows go past the caches
+  // (7 heads of 256, 64 MB read: 32 us past them, 25 through; 128 MB 56.5 both; 192
+  // MB 81.5, 86.5; 1 GB 411, 428).
+  const bool once = 2 * tokens * read > kLastCache;
+  if (dtype == OSCAR_BF16) launch_typed<__bf16>(a, vec, once, r->adjacent != 0, stream);
+  else if (dtype == OSCAR_FP16) launch_typed<_Float16>(a, vec, once, r->adjacent != 0, stream);
+  else launch_typed<float>(a, vec, once, r->adjacent != 0, stream);
   return hipGetLastError() == hipSuccess ? kOk : kErrLaunch;
 }
 

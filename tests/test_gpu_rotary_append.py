@@ -213,6 +213,30 @@ def test_offsets_past_32_bits(device):
     assert torch.equal(joint[-1, 0, 15], x[1])          # position 0 turns nothing
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("adjacent", [False, True])
+def test_more_rows_than_the_caches_hold(device, dtype, adjacent):
+    """More than 128 MB of rows take another way to memory; some of them checked."""
+    g = torch.Generator(device=device).manual_seed(11)
+    turn = rotary.Rotary(rotary.rotary_table(3000, 32, device=device), adjacent)
+    n = (150 << 20) // (10 * 64 * dtype.itemsize)
+    q, k, v = rows(g, n, 6, 2, 64, dtype, True)
+    pos = torch.randint(0, 3000, (n,), generator=g, device=device)
+    some = torch.cat([torch.arange(40), torch.arange(n - 40, n), torch.randint(0, n, (200,))]).to(device)
+    got = rotary.rotate(q, k, pos, turn)
+    close(got[0][some], turned(q[some], pos[some], turn, adjacent, None))
+    close(got[1][some], turned(k[some], pos[some], turn, adjacent, None))
+    if dtype == torch.float32:
+        return                              # (a cache is bf16 or fp16)
+    caches = [torch.zeros(-(-n // 16) + 1, 16, 2, 64, device=device, dtype=dtype) for _ in range(2)]
+    slots = torch.randperm(16 * (caches[0].shape[0] - 1), generator=g, device=device)[:n]
+    out = append.append_rotated(q, k, v, pos, turn, append.PagedCache(*caches), slots)
+    assert torch.equal(out, got[0])
+    flat = [c.view(-1, 2, 64) for c in caches]
+    assert torch.equal(flat[0][slots], got[1]) and torch.equal(flat[1][slots], v)
+    assert all((c[-1] == 0).all() for c in caches)
+
+
 def test_streams_and_replays(device):
     g = torch.Generator(device=device).manual_seed(9)
     turn = rotary.Rotary(rotary.rotary_table(600, 64, device=device))
