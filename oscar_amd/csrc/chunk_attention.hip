@@ -809,6 +809,7 @@ __device__ __forceinline__ void wide_piece(const ChunkArgs& a, const Piece p, ui
 
 // ---------------------------------------------------------------- kernels
 constexpr int narrow_wgs(int d) { return 256 / d; }             // workgroups a CU
+constexpr int kFewNarrow = kCus;
 template <typename T, int D>
 __global__ __launch_bounds__(kThreads, narrow_wgs(D)) void narrow_kernel(ChunkArgs a) {
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
@@ -826,9 +827,10 @@ __global__ __launch_bounds__(kThreads, kWideWgs) void wide_kernel(ChunkArgs a) {
 template <typename T, int D>
 __global__ __launch_bounds__(kThreads, kWideWgs) void mixed_kernel(ChunkArgs a) {
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
-  const int i = (int)blockIdx.x;
-  if (i < a.wide) wide_piece<T, D>(a, a.pieces[a.narrow + i], smem);
-  else narrow_piece<T, D, beside_keys(D)>(a, a.pieces[i - a.wide], smem);
+  const int total = a.narrow + a.wide, lead = a.narrow <= kFewNarrow ? 0 : a.narrow;
+  const int at = (int)blockIdx.x + lead, i = at < total ? at : at - total;
+  if (i >= a.narrow) wide_piece<T, D>(a, a.pieces[i], smem);
+  else narrow_piece<T, D, beside_keys(D)>(a, a.pieces[i], smem);
 }
 
 // ---------------------------------------------------------------- join
@@ -985,7 +987,7 @@ int32_t pieces_of(const RowTile& x, int64_t per) { return (int32_t)((x.tiles + p
 // D = 256, whole 7.9 us of GPU time, cut 8.3 (over 512: 10.9, 9.3); D = 128, 8 kv
 // heads, over 512 whole 7.2, cut 7.1 and 6.2 against 10.6 where the host launches
 // (over 1024: 11.1, 8.4).
-void plan_narrow(const std::vector<RowTile>& rows, int32_t head_size, bool alone, Plan& plan) {
+void plan_narrow(const std::vector<RowTile>& rows, int32_t head_size, double beside, Plan& plan) {
   int64_t total = 0;
   int32_t most = 0;
   for (const RowTile& x : rows) {
@@ -993,7 +995,7 @@ void plan_narrow(const std::vector<RowTile>& rows, int32_t head_size, bool alone
     most = std::max(most, x.tiles);
   }
   const int32_t uncut = head_size == 256 ? 8 : 16;
-  const int64_t resident = (int64_t)kCus * (alone ? narrow_wgs(head_size) : 2);
+  const int64_t resident = beside == 0. ? kCus * narrow_wgs(head_size) : total > 160 * beside ? 2 * kCus : 2 * kCus / 3;
   int64_t per = std::max<int64_t>(kWaves, (total + resident - 1) / resident);
   auto count = [&](int64_t t) {
     int64_t c = 0;
@@ -1025,7 +1027,7 @@ void plan_narrow(const std::vector<RowTile>& rows, int32_t head_size, bool alone
 //   of 300 over 500 51 / 56;  D = 64, 16 heads: 8192 over 8192 427 / 461, 1024
 //   over 1024 37 / 27.
 constexpr int32_t kPieceCost = 4, kCutCost = 15, kLeastPiece = 8, kShares = kCus * kWideWgs;
-void plan_wide(const std::vector<RowTile>& rows, int32_t head_size, Plan& plan) {
+double plan_wide(const std::vector<RowTile>& rows, int32_t head_size, Plan& plan) {
   int64_t total = 0;
   int32_t most = 0;
   for (const RowTile& x : rows) {
@@ -1065,6 +1067,7 @@ void plan_wide(const std::vector<RowTile>& rows, int32_t head_size, Plan& plan) 
   // The first two rounds of workgroups share CUs in order: the longest pieces,
   // shortest first, meet the next ones, longest first.
   std::reverse(plan.wide.begin(), plan.wide.begin() + (std::ptrdiff_t)std::min<size_t>(kCus, plan.wide.size()));
+  return std::min(whole, parted);
 }
 
 void make_plan(const int32_t* qsl, const int32_t* seqs, int32_t num_requests, int32_t group, int32_t kv_heads,
@@ -1077,8 +1080,8 @@ void make_plan(const int32_t* qsl, const int32_t* seqs, int32_t num_requests, in
     else
       row_tiles(qsl[i], n, seqs[i], i, group, kv_heads, window, kWideRows, wide);
   }
-  if (!narrow.empty()) plan_narrow(narrow, head_size, wide.empty(), plan);
-  if (!wide.empty()) plan_wide(wide, head_size, plan);
+  const double beside = wide.empty() ? 0. : plan_wide(wide, head_size, plan);
+  if (!narrow.empty()) plan_narrow(narrow, head_size, beside, plan);
   std::stable_partition(plan.joins.begin(), plan.joins.end(), [](const Join& j) { return j.count <= kFewParts; });
 }
 
