@@ -630,12 +630,12 @@ __device__ __forceinline__ void wide_piece(const ChunkArgs& a, const Piece p, ui
       in_page += advance;
       in_page -= in_page >= a.block_size ? a.block_size : 0;
     }
-    load_keys<D, false, kLoads, kKept>(a, p, p.key0 + kTiles * kTileKeys * stage + kKeys * wave, kKeys * wave, page, in_page,
-                                to, k_place);
+    load_keys<D, false, kLoads, kKept>(a, p, p.key0 + kTiles * kTileKeys * stage + kKeys * wave, kKeys * wave, page,
+                                       in_page, to, k_place);
   };
   auto request_v = [&](int stage, uint8_t* to) __attribute__((always_inline)) {
-    load_keys<D, true, kLoads, kKept>(a, p, p.key0 + kTiles * kTileKeys * stage + kKeys * wave, kKeys * wave, page, in_page,
-                               to + kTiles * kTileBytes, v_place);
+    load_keys<D, true, kLoads, kKept>(a, p, p.key0 + kTiles * kTileKeys * stage + kKeys * wave, kKeys * wave, page,
+                                      in_page, to + kTiles * kTileBytes, v_place);
   };
   auto k_operand = [&](const uint8_t* kt, int i) {
     const int at = kKeepAddresses ? k_addr : opaque(k_addr);
@@ -809,7 +809,6 @@ __device__ __forceinline__ void wide_piece(const ChunkArgs& a, const Piece p, ui
 
 // ---------------------------------------------------------------- kernels
 constexpr int narrow_wgs(int d) { return 256 / d; }             // workgroups a CU
-constexpr int kFewNarrow = kCus;
 template <typename T, int D>
 __global__ __launch_bounds__(kThreads, narrow_wgs(D)) void narrow_kernel(ChunkArgs a) {
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
@@ -820,10 +819,12 @@ __global__ __launch_bounds__(kThreads, kWideWgs) void wide_kernel(ChunkArgs a) {
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
   wide_piece<T, D>(a, a.pieces[blockIdx.x], smem);
 }
-// A step with both: the wide pieces first, the narrow ones where they leave room
-// (1024 tokens beside seven users' 4, D = 128: 159 us; two launches 163, the narrow
-// ones first 161, eight of each in turn 193: reads at full rate leave the wide
-// pieces' next stage late).
+// A step with both.  Narrow pieces that fill the GPU come after the wide ones, where
+// those leave room: reads at full rate leave the wide pieces' next stage late.  A few
+// (plan_narrow) come first, and read for as long as the wide ones compute.  1024
+// tokens over 4096 beside seven users' 4, D = 128, 124 us: the wide ones alone take
+// 90, the narrow ones alone 38; D = 256 71 us (the wide ones first 83).
+constexpr int kFewNarrow = kCus;
 template <typename T, int D>
 __global__ __launch_bounds__(kThreads, kWideWgs) void mixed_kernel(ChunkArgs a) {
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
@@ -958,9 +959,8 @@ void row_tiles(int32_t token0, int32_t n, int32_t seq, int32_t table_row, int32_
   }
 }
 
-// A row tile in pieces between the key tiles `cuts` (from 0 to its last).
-void cut(const RowTile& x, const std::vector<int32_t>& cuts, Plan& plan, std::vector<Piece>& out) {
-  const int32_t n = (int32_t)cuts.size() - 1;
+// A row tile in n pieces of equal length, but for a key tile.
+void cut(const RowTile& x, int32_t n, Plan& plan, std::vector<Piece>& out) {
   if (n <= 1) {
     out.push_back(x.piece);
     return;
@@ -971,8 +971,8 @@ void cut(const RowTile& x, const std::vector<int32_t>& cuts, Plan& plan, std::ve
                               std::min(kTileRows, x.piece.rows - g * kTileRows), plan.slots + g, groups, n, 0});
   for (int32_t s = 0; s < n; ++s) {
     Piece p = x.piece;
-    p.key0 = x.piece.key0 + kTileKeys * cuts[s];
-    p.key1 = std::min<int32_t>(x.piece.key1, x.piece.key0 + kTileKeys * cuts[s + 1]);
+    p.key0 = x.piece.key0 + kTileKeys * (int32_t)((int64_t)x.tiles * s / n);
+    p.key1 = std::min<int32_t>(x.piece.key1, x.piece.key0 + kTileKeys * (int32_t)((int64_t)x.tiles * (s + 1) / n));
     p.slot = plan.slots;
     plan.slots += groups;
     out.push_back(p);
@@ -984,9 +984,15 @@ int32_t pieces_of(const RowTile& x, int64_t per) { return (int32_t)((x.tiles + p
 // Narrow tiles: the fewest key tiles a piece with which the pieces fit the
 // workgroups that are resident at once.  Where the longest row tile is short, all
 // stay whole, and there is no second launch: one token of one user over 256 keys,
-// D = 256, whole 7.9 us of GPU time, cut 8.3 (over 512: 10.9, 9.3); D = 128, 8 kv
+// D = 256, whole 7.9 us of GPU time, cut 8.3 (over 512: 10.9, 8.3); D = 128, 8 kv
 // heads, over 512 whole 7.2, cut 7.1 and 6.2 against 10.6 where the host launches
-// (over 1024: 11.1, 8.4).
+// (over 1024: 11.1, 7.0).
+// Beside wide tiles whose time (`beside`, in their units) is longer than the reading
+// takes, two narrow workgroups to three CUs (16 users over 8000 keys beside two
+// prompts, D = 256: 37 to 45 us, two a CU 43 to 55; 12 over 2000 beside 512 tokens,
+// D = 128: 30, 35); where the reading takes longer, two a CU (16 over 8000 beside two prompts, D =
+// 128: 107 us, two to three CUs 128).  A narrow tile reads 128 D bytes, at 5.2 TB/s
+// about 1/160 unit.
 void plan_narrow(const std::vector<RowTile>& rows, int32_t head_size, double beside, Plan& plan) {
   int64_t total = 0;
   int32_t most = 0;
@@ -995,7 +1001,7 @@ void plan_narrow(const std::vector<RowTile>& rows, int32_t head_size, double bes
     most = std::max(most, x.tiles);
   }
   const int32_t uncut = head_size == 256 ? 8 : 16;
-  const int64_t resident = beside == 0. ? kCus * narrow_wgs(head_size) : total > 160 * beside ? 2 * kCus : 2 * kCus / 3;
+  const int64_t resident = beside == 0. ? kCus * narrow_wgs(head_size) : total > 240 * beside ? 2 * kCus : 2 * kCus / 3;
   int64_t per = std::max<int64_t>(kWaves, (total + resident - 1) / resident);
   auto count = [&](int64_t t) {
     int64_t c = 0;
@@ -1004,70 +1010,70 @@ void plan_narrow(const std::vector<RowTile>& rows, int32_t head_size, double bes
   };
   if ((int64_t)rows.size() >= resident || most <= uncut) per = std::max<int64_t>(per, most);
   while (per < most && count(per) > resident) ++per;
-  std::vector<int32_t> cuts;
-  for (const RowTile& x : rows) {
-    const int32_t n = pieces_of(x, per);
-    cuts.clear();
-    for (int32_t i = 0; i <= n; ++i) cuts.push_back((int32_t)((int64_t)x.tiles * i / n));
-    cut(x, cuts, plan, plan.narrow);
-  }
+  for (const RowTile& x : rows) cut(x, pieces_of(x, per), plan, plan.narrow);
 }
 
-// Wide tiles.  Workgroups take pieces as they come free, two to a CU.  Tiles are
-// left whole, or the line of all tiles' keys is cut in equal shares, two a CU:
-// whichever is estimated to end first.  In units of a key tile's time on a busy
-// CU (D = 256 1.05 us, 128 0.47, 64 0.27): a piece costs 4 beside its tiles, one
-// of a cut row tile 15 (its partials are written and read again: the same at any
-// D, as both go with D); a workgroup alone on its CU takes 1.07, 1.45 or 1.5 units
-// a tile; the join is a launch of 5 us; shares end a tenth later than their mean,
-// as they are not dealt out as they were cut.  Measured, whole / cut, us:
-//   D = 256, 6 heads: 9256 tokens over 15360 1208 / 1242, 4096 over 28672 1165 /
-//   790, 3001 alone 109 / 60, 1024 alone 45 / 33;
-//   D = 128, 32 heads: 8192 alone 514 / 567, 1024 over 4096 119 / 103, 8 prompts
-//   of 300 over 500 51 / 56;  D = 64, 16 heads: 8192 over 8192 427 / 461, 1024
-//   over 1024 37 / 27.
-constexpr int32_t kPieceCost = 4, kCutCost = 15, kLeastPiece = 8, kShares = kCus * kWideWgs;
+// Wide tiles.  Workgroups take pieces as they come free, two to a CU.  Row tiles
+// are left whole or cut in pieces of at most so many key tiles, whichever is
+// estimated to end first.  In units of a key tile's time on a busy CU (D = 256 1.05
+// us, 128 0.47, 64 0.27): a piece costs 4 beside its tiles, one of a cut row tile 15
+// (its partials are written and read again: the same at any D, as both go with D);
+// a workgroup alone on its CU takes 1.07, 1.45 or 1.5 units a tile; the join is a
+// launch of 5 us; cut pieces end a tenth later than their sum, as they are not dealt
+// out as is assumed here.  Measured, whole / cut, us:
+//   D = 256, 6 heads: 9256 tokens over 15360 1208 / 1257, 4096 over 28672 1165 /
+//   815, 3001 alone 109 / 60, 1024 alone 45 / 29;
+//   D = 128, 32 heads: 8192 alone 508 / 567, 1024 over 4096 119 / 90, 8 prompts
+//   of 300 over 500 51 / 56;  D = 64, 16 heads: 8192 over 8192 422 / 461, 1024
+//   over 1024 37 / 23.
+// Returns the estimate.
+constexpr int32_t kPieceCost = 4, kCutCost = 15, kLeastPiece = 8, kMostPieces = 2048;
 double plan_wide(const std::vector<RowTile>& rows, int32_t head_size, Plan& plan) {
-  int64_t total = 0;
   int32_t most = 0;
-  for (const RowTile& x : rows) {
-    total += x.tiles;
-    most = std::max(most, x.tiles);
-  }
+  for (const RowTile& x : rows) most = std::max(most, x.tiles);
   const double alone = head_size == 256 ? 1.07 : head_size == 128 ? 1.45 : 1.5;
   const double join = head_size == 256 ? 5.0 : head_size == 128 ? 11.0 : 18.0;
-  // Whole tiles, dealt out to the CUs longest first, there and back.
-  std::vector<int32_t> length;
-  length.reserve(rows.size());
-  for (const RowTile& x : rows) length.push_back(x.tiles + kPieceCost);
-  std::sort(length.begin(), length.end(), std::greater<int32_t>());
-  std::vector<int64_t> load(kCus, 0);
-  for (size_t i = 0; i < length.size(); ++i) load[(i / kCus) % 2 ? kCus - 1 - i % kCus : i % kCus] += length[i];
-  const double whole = std::max((double)*std::max_element(load.begin(), load.end()), alone * most);
-  const double share = std::max((double)total / kShares, (double)kLeastPiece);
-  const double pieces = (double)rows.size() + std::min((double)kShares, total / share);
-  const double parted = std::max(1.1 * (total + kCutCost * pieces) / kCus, alone * share + kCutCost) + join;
-  const int64_t shares = parted < whole ? kShares : 0;
-  int64_t at = 0;                           // on the line
-  for (const RowTile& x : rows) {
-    std::vector<int32_t> cuts{0};
-    if (shares > 0) {
-      // the share's ends inside this tile, but for slivers
-      for (int64_t s = at * shares / total; s <= (at + x.tiles) * shares / total; ++s) {
-        const int64_t end = s * total / shares - at;
-        if (end >= cuts.back() + kLeastPiece && end <= x.tiles - kLeastPiece) cuts.push_back((int32_t)end);
-      }
+  // In pieces of at most `per` key tiles, dealt out to the CUs longest first, there
+  // and back.
+  std::vector<int32_t> count;               // of pieces, by cost
+  std::vector<int64_t> load(kCus);
+  auto parted = [&](int32_t per) {
+    count.assign(per + kCutCost + 1, 0);
+    bool cuts = false;
+    for (const RowTile& x : rows) {
+      const int32_t n = pieces_of(x, per);
+      cuts = cuts || n > 1;
+      count[(x.tiles + n - 1) / n + (n > 1 ? kCutCost : kPieceCost)] += n;
     }
-    cuts.push_back(x.tiles);
-    cut(x, cuts, plan, plan.wide);
-    at += x.tiles;
+    std::fill(load.begin(), load.end(), 0);
+    int64_t dealt = 0, longest = 0;
+    for (int32_t cost = (int32_t)count.size() - 1; cost > 0; --cost)
+      for (int32_t n = count[cost]; n > 0; --n, ++dealt) {
+        const int64_t at = dealt % kCus;
+        load[dealt / kCus % 2 ? kCus - 1 - at : at] += cost;
+        longest = std::max<int64_t>(longest, cost);
+      }
+    const double busiest = (double)*std::max_element(load.begin(), load.end());
+    return std::max(cuts ? 1.1 * busiest : busiest, alone * longest) + (cuts ? join : 0.);
+  };
+  int32_t per = most;
+  double best = parted(most);
+  for (int32_t parts = 2; (size_t)parts * rows.size() <= kMostPieces; parts += 1 + parts / 8) {
+    const int32_t at_most = (most + parts - 1) / parts;
+    if (at_most < kLeastPiece) break;
+    const double t = parted(at_most);
+    if (t < best) {
+      best = t;
+      per = at_most;
+    }
   }
+  for (const RowTile& x : rows) cut(x, pieces_of(x, per), plan, plan.wide);
   std::stable_sort(plan.wide.begin(), plan.wide.end(),
                    [](const Piece& x, const Piece& y) { return x.key1 - x.key0 > y.key1 - y.key0; });
   // The first two rounds of workgroups share CUs in order: the longest pieces,
   // shortest first, meet the next ones, longest first.
   std::reverse(plan.wide.begin(), plan.wide.begin() + (std::ptrdiff_t)std::min<size_t>(kCus, plan.wide.size()));
-  return std::min(whole, parted);
+  return best;
 }
 
 void make_plan(const int32_t* qsl, const int32_t* seqs, int32_t num_requests, int32_t group, int32_t kv_heads,
