@@ -543,7 +543,7 @@ typedef struct oscar_plain_cache {
  * axes: 1 for text, 3 for the time, height and width of images and video
  * (at most 4); pair_axis: two bits per pair, pair 0 lowest. */
 typedef struct oscar_rotary {
-  const float* table; /* [positions][rotary_dim] fp32, 16-byte aligned */
+  const float* table; /* [positions][rotary_dim] fp32 */
   int64_t positions;
   int32_t rotary_dim; /* even, 2 .. 256 */
   int32_t adjacent;
@@ -553,7 +553,8 @@ typedef struct oscar_rotary {
 } oscar_rotary;
 
 /* Heads of a batch of tokens: value f of head h of token t lies at element
- * t * token_stride + h * head_stride + f of `data`. */
+ * t * token_stride + h * head_stride + f of `data`; strides of rows that turn are
+ * not negative and below 4 GiB. */
 typedef struct oscar_heads {
   void* data;
   int64_t token_stride;
@@ -609,7 +610,9 @@ int oscar_append_rotated(const oscar_rotary* rotary, const int64_t* positions, i
  *   query, out: 16-byte aligned rows of the cache's type (strides multiples of 8)
  *     from token 0 of the step on; rows of no request are left as they were;
  *   workspace: workspace_size bytes, 16-byte aligned; scale: positive.
- * head_size 64, 128 or 256; block_size a multiple of 16.
+ * head_size 64, 128 or 256; block_size a multiple of 16; page strides below 4 GiB;
+ * seq_lens and a request's tokens x query heads of a kv head at most 2^30.  A cache
+ * of another geometry than the step's is refused.
  */
 typedef struct oscar_chunk_step {
   int32_t num_requests;
@@ -621,7 +624,9 @@ typedef struct oscar_chunk_step {
   int32_t wide;
   int32_t joins;
   int32_t few_joins;
-  int32_t reserved; /* 0 */
+  int32_t num_kv_heads; /* of the caches that it was cut for, like the next two */
+  int32_t head_size;
+  int32_t block_size;
   int64_t items_size;
   int64_t workspace_size;
 } oscar_chunk_step;

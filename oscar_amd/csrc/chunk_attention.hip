@@ -987,12 +987,12 @@ int32_t pieces_of(const RowTile& x, int64_t per) { return (int32_t)((x.tiles + p
 // D = 256, whole 7.9 us of GPU time, cut 8.3 (over 512: 10.9, 8.3); D = 128, 8 kv
 // heads, over 512 whole 7.2, cut 7.1 and 6.2 against 10.6 where the host launches
 // (over 1024: 11.1, 7.0).
-// Beside wide tiles whose time (`beside`, in their units) is longer than the reading
-// takes, two narrow workgroups to three CUs (16 users over 8000 keys beside two
-// prompts, D = 256: 37 to 45 us, two a CU 43 to 55; 12 over 2000 beside 512 tokens,
-// D = 128: 30, 35); where the reading takes longer, two a CU (16 over 8000 beside two prompts, D =
-// 128: 107 us, two to three CUs 128).  A narrow tile reads 128 D bytes, at 5.2 TB/s
-// about 1/160 unit.
+// Beside wide tiles that take at least two thirds of the reading's time (`beside`, in
+// their units, of which a narrow tile's 128 D bytes at 5.2 TB/s are 1/160), two narrow
+// workgroups to three CUs (16 users over 8000 keys beside two prompts, D = 256: 37 to
+// 45 us, two a CU 43 to 55; 12 over 2000 beside 512 tokens, D = 128: 30, 35); where the
+// reading takes longer, two a CU (16 over 8000 beside two prompts, D = 128: 107 us, two
+// to three CUs 128).
 void plan_narrow(const std::vector<RowTile>& rows, int32_t head_size, double beside, Plan& plan) {
   int64_t total = 0;
   int32_t most = 0;
@@ -1153,6 +1153,9 @@ extern "C" int oscar_chunk_plan(const int32_t* query_start_loc, const int32_t* s
     step->num_requests = num_requests;
     step->num_tokens = num_requests > 0 ? query_start_loc[num_requests] : 0;
     step->num_heads = num_heads;
+    step->num_kv_heads = cache->num_kv_heads;
+    step->head_size = cache->head_size;
+    step->block_size = cache->block_size;
     step->window = std::min(window, kMostKeys);
     step->table_cols = pages;
     step->narrow = (int32_t)plan.narrow.size();
@@ -1184,6 +1187,9 @@ extern "C" int oscar_chunk_attention(const oscar_chunk_step* step, const void* i
   if (step == nullptr || query == nullptr || out == nullptr || query->num_heads != step->num_heads ||
       out->num_heads != step->num_heads || step->num_heads < 1 || step->num_heads % cache->num_kv_heads ||
       !(scale > 0.f) || !(scale <= 3.0e38f))
+    return kErrInvalidArgument;
+  if (step->num_kv_heads != cache->num_kv_heads || step->head_size != cache->head_size ||
+      step->block_size != cache->block_size)
     return kErrInvalidArgument;
   if (step->narrow < 0 || step->wide < 0 || step->few_joins < 0 || step->joins < step->few_joins)
     return kErrInvalidArgument;

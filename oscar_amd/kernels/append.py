@@ -69,8 +69,8 @@ def append_rotated(query: torch.Tensor | None, key: torch.Tensor, value: torch.T
     """Write key (turned by its positions) and value [N, Hk, D] of the tokens of
     slot_mapping (int64 [N]) to their slots, and return query [N, Hq, D] turned
     (a new tensor, or query_out, which may be query itself; None without a
-    query).  Rows are of the cache's type, with any token and head strides;
-    rows past the slots' count are not read.  Slots < 0 or past the cache are
+    query).  Rows are of the cache's type, with any token and head strides
+    below 4 GiB; rows past the slots' count are not read.  Slots < 0 or past the cache are
     skipped, tokens with a position outside the table left out whole; slots of a
     call are distinct."""
     if slot_mapping.ndim != 1 or slot_mapping.device != cache.device:
@@ -88,9 +88,7 @@ def append_rotated(query: torch.Tensor | None, key: torch.Tensor, value: torch.T
         if query_out is None:
             query_out, qo = _rotary.new_heads(query, n, hq, d)
         else:
-            qo, count = _rotary.heads(query_out, n, d, dtype, device, "query_out")
-            if count != hq:
-                raise ValueError("query_out must have the query's heads")
+            qo = _rotary.out_heads(query_out, n, hq, d, dtype, device, "query_out")
     if slot_mapping.dtype is not torch.int64 or (n > 1 and slot_mapping.stride(0) != 1):
         if slot_mapping.dtype not in (torch.int64, torch.int32):
             raise ValueError(f"slot_mapping must be integers, got {slot_mapping.dtype}")

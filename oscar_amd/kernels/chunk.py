@@ -21,8 +21,8 @@ _i32, _i64 = ctypes.c_int32, ctypes.c_int64
 class ChunkStepArgs(ctypes.Structure):
     """struct oscar_chunk_step (include/oscar_amd.h)."""
     _fields_ = [("num_requests", _i32), ("num_tokens", _i32), ("num_heads", _i32), ("window", _i32),
-                ("table_cols", _i32), ("narrow", _i32), ("wide", _i32), ("joins", _i32), ("few_joins", _i32), ("reserved", _i32),
-                ("items_size", _i64),
+                ("table_cols", _i32), ("narrow", _i32), ("wide", _i32), ("joins", _i32), ("few_joins", _i32),
+                ("num_kv_heads", _i32), ("head_size", _i32), ("block_size", _i32), ("items_size", _i64),
                 ("workspace_size", _i64)]
 
 
@@ -35,8 +35,9 @@ class ChunkStep:
     qsl [requests + 1] and seqs [requests] are host lists (query starts from the
     step's token 0; keys after the step); block_tables int32 [requests, pages] on
     the cache's device.  A step is not built under graph capture; a captured call
-    keeps this step's lengths (its block table is read at every replay) and needs
-    the step to live as long as the graph."""
+    keeps this step's lengths and needs the step to live as long as the graph; the
+    block table is read at every call and replay where it is int32 with rows of
+    their own, and else copied here."""
 
     def __init__(self, qsl, seqs, block_tables: torch.Tensor, num_heads: int, cache: PagedCache, window: int = 0):
         layout = decode.request_layout(qsl, seqs)
@@ -62,8 +63,9 @@ class ChunkStep:
         device = cache.device
         if device.type != "cuda":
             raise ValueError("OSCAR kernels take device tensors")
-        if block_tables.dtype != torch.int32 or block_tables.stride(1) != 1:
-            block_tables = block_tables.to(torch.int32).contiguous()
+        if (block_tables.dtype != torch.int32 or block_tables.stride(1) != 1
+                or block_tables.stride(0) < block_tables.shape[1]):
+            block_tables = block_tables.to(torch.int32).clone(memory_format=torch.contiguous_format)
         if torch.cuda.is_current_stream_capturing():
             raise ValueError("a step is built before its calls are captured")
         with torch.cuda.device(device):
@@ -96,8 +98,8 @@ class ChunkStep:
 def chunk_attention(query: torch.Tensor, cache: PagedCache, step: ChunkStep, scale: float, out=None) -> torch.Tensor:
     """Causal attention of query [N, Hq, D] (the cache's type; token t of the
     step in row t) over the cache; returns [N, Hq, D] of that type, a new tensor
-    or `out`, whose rows past the step's tokens (and of tokens of no request) are
-    left as they were.  scale must be positive.  Keys on pages outside the cache
+    or `out` (which may be query itself), whose rows past the step's tokens and of
+    tokens of no request are not written.  scale must be positive.  Keys on pages outside the cache
     are left out; a row that sees no key becomes zeros."""
     device = cache.device
     if cache.geometry != step.geometry or device != step.device:
@@ -109,14 +111,14 @@ def chunk_attention(query: torch.Tensor, cache: PagedCache, step: ChunkStep, sca
     if hq != step.num_heads:
         raise ValueError(f"query must have the step's {step.num_heads} heads")
     if _misaligned(query):
-        query = query.contiguous()
+        query = query.clone(memory_format=torch.contiguous_format)
         q, _ = _rotary.heads(query, tokens, d, dtype, device, "query")
     if out is None:
         out, o = _rotary.new_heads(query, query.shape[0], hq, d)
     else:
-        o, count = _rotary.heads(out, tokens, d, dtype, device, "out")
-        if count != hq or _misaligned(out):
-            raise ValueError("out must have the query's heads, rows at multiples of 16 bytes")
+        o = _rotary.out_heads(out, tokens, hq, d, dtype, device, "out")
+        if _misaligned(out):
+            raise ValueError("out must have rows at multiples of 16 bytes")
     if tokens == 0:
         return out
     if _lib.stream_handle(device) != step.stream:

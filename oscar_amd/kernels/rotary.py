@@ -108,6 +108,19 @@ def heads(x: torch.Tensor, tokens: int, d: int, dtype, device, what: str) -> tup
     return pack_heads(x.data_ptr(), token, head, shape[1], 0), shape[1]
 
 
+def out_heads(x: torch.Tensor, tokens: int, count: int, d: int, dtype, device, what: str) -> bytes:
+    """heads() of an output of `count` heads, whose rows do not share memory."""
+    packed, given = heads(x, tokens, d, dtype, device, what)
+    if given != count:
+        raise ValueError(f"{what} must have the {'key' if what == 'key_out' else 'query'}'s heads")
+    token, head, _ = x.stride()
+    token, head = token if tokens > 1 else d, head if count > 1 else d      # (of one entry they mean nothing)
+    apart = head >= (tokens - 1) * token + d if token < head else token >= (count - 1) * head + d
+    if min(token, head) < d or (tokens > 1 and count > 1 and not apart):
+        raise ValueError(f"{what}: rows overlap")
+    return packed
+
+
 def new_heads(like: torch.Tensor, tokens: int, count: int, d: int) -> tuple[torch.Tensor, bytes]:
     """A new tensor [tokens, count, d] of like's type and device, and its struct oscar_heads."""
     x = like.new_empty((tokens, count, d))
@@ -136,7 +149,7 @@ def rotate(query: torch.Tensor, key: torch.Tensor | None, positions: torch.Tenso
            key_out=None, inverse: bool = False):
     """query [N, Hq, D] and key [N, Hk, D] (or None) turned by their positions
     (int64 [N], or [axes, N]), bf16, fp16 or fp32 alike, with any token and head
-    strides.  Returns (query_out, key_out): new tensors, or the ones given, which
+    strides below 4 GiB.  Returns (query_out, key_out): new tensors, or the ones given, which
     may be the inputs themselves.  A token with a position outside the table is
     left out: its output rows keep what they held."""
     dtype, device = query.dtype, query.device
@@ -151,18 +164,14 @@ def rotate(query: torch.Tensor, key: torch.Tensor | None, positions: torch.Tenso
     if query_out is None:
         query_out, qo = new_heads(query, n, hq, d)
     else:
-        qo, count = heads(query_out, n, d, dtype, device, "query_out")
-        if count != hq:
-            raise ValueError("query_out must have the query's heads")
+        qo = out_heads(query_out, n, hq, d, dtype, device, "query_out")
     k = ko = None
     if key is not None:
         k, hk = heads(key, n, d, dtype, device, "key")
         if key_out is None:
             key_out, ko = new_heads(key, n, hk, d)
         else:
-            ko, count = heads(key_out, n, d, dtype, device, "key_out")
-            if count != hk:
-                raise ValueError("key_out must have the key's heads")
+            ko = out_heads(key_out, n, hk, d, dtype, device, "key_out")
     positions, axis_stride = positions_of(positions, rotary, n, device)
     if not query.is_cuda:
         raise ValueError("OSCAR kernels take device tensors")

@@ -141,6 +141,10 @@ def test_attention_entry_refuses():
     heads = rotary.HeadsArgs
     assert status(step=None) == -1 and status(items=None) == -1 and status(table=None) == -1
     assert status(stride=args.table_cols - 1) == -1
+    for field, value in (("num_kv_heads", 4), ("head_size", 64), ("block_size", 32)):        # another cache's step
+        other = chunk.ChunkStepArgs.from_buffer_copy(args)
+        setattr(other, field, value)
+        assert status(step=other) == -1
     for scale in (0.0, -1.0, float("nan"), float("inf")):
         assert status(scale=scale) == -1
     assert status(q=heads(fake, 1024, 128, 4, 0)) == -1 and status(o=heads(fake, 1024, 128, 4, 0)) == -1

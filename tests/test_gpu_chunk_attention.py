@@ -199,6 +199,20 @@ def test_what_a_row_does_not_see_does_not_reach_it(device, dtype, d, window):
         assert (mine[row][..., 2] == math.inf).all()
 
 
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_many_decodes_beside_prompts(device, d):
+    """More short row tiles than CUs, and wide ones cut in many pieces."""
+    g = torch.Generator(device=device).manual_seed(30 + d)
+    reqs = [(1, 3000)] * 40 + [(40, 0), (50, 9000)]
+    q, caches, table, starts, seqs = make(g, reqs, 4, 4, d, 32, torch.bfloat16)
+    cache = append.PagedCache(*caches)
+    for window in (0, 700):
+        step = chunk.ChunkStep(starts, seqs, table, 4, cache, window)
+        assert step.args.wide > 0 and (window or step.args.narrow > 256)
+        got = chunk.chunk_attention(q, cache, step, 0.1)
+        check(got, q, caches, table, starts, seqs, window, 0.1, 32)
+
+
 def test_unmapped_pages_are_left_out(device):
     g = torch.Generator(device=device).manual_seed(7)
     reqs = [(2, 200), (40, 200), (1, 10), (3, 300)]
@@ -254,6 +268,53 @@ def test_strided_queries_and_outputs(device):
     assert torch.equal(chunk.chunk_attention(odd, cache, step, 0.125), want)
     with pytest.raises(ValueError, match="16 bytes"):
         chunk.chunk_attention(q, cache, step, 0.125, out=odd)
+    with pytest.raises(ValueError, match="overlap"):
+        chunk.chunk_attention(q, cache, step, 0.125, out=out[:, :1].expand(41, 6, 64))
+    early = torch.zeros(41 * 6 * 64 + 1, device=device, dtype=torch.float16)[1:].view(41, 6, 64)       # 2 bytes off
+    early.copy_(q)
+    assert torch.equal(chunk.chunk_attention(early, cache, step, 0.125), want)
+    mine = q.clone()
+    assert chunk.chunk_attention(mine, cache, step, 0.125, out=mine) is mine and torch.equal(mine, want)
+
+
+@pytest.mark.parametrize("kind", ["int64", "columns first", "one row for all"])
+def test_block_tables_of_other_layouts(device, kind):
+    g = torch.Generator(device=device).manual_seed(21)
+    q, caches, table, starts, seqs = make(g, [(40, 50), (40, 50)], 4, 2, 64, 16, torch.bfloat16)
+    cache = append.PagedCache(*caches)
+    if kind == "one row for all":
+        table[1] = table[0]
+    want = chunk.chunk_attention(q, cache, chunk.ChunkStep(starts, seqs, table, 4, cache), 0.125)
+    other = {"int64": table.long(), "columns first": table.t().contiguous().t(),
+             "one row for all": table[:1].expand(2, -1)}[kind]
+    assert torch.equal(chunk.chunk_attention(q, cache, chunk.ChunkStep(starts, seqs, other, 4, cache), 0.125), want)
+
+
+@pytest.mark.parametrize("new", [3, 300])
+def test_pages_past_32_bits(device, new):
+    """A cache of 6 GB (K and V pages in turn) whose last pages are used, at both tile sizes."""
+    base = torch.empty(3 << 30, dtype=torch.bfloat16, device=device)
+    joint = base.view(-1, 2, 16, 2, 128)
+    cache = append.PagedCache(joint[:, 0], joint[:, 1])
+    g = torch.Generator(device=device).manual_seed(new)
+    q, caches, table, starts, seqs = make(g, [(new, 350)], 4, 2, 128, 16, torch.bfloat16)
+    high = torch.where(table % 2 == 0, joint.shape[0] - 1 - table, table)
+    for c in range(2):
+        joint[high[0].long(), c] = caches[c][table[0].long()]
+    got = chunk.chunk_attention(q, cache, chunk.ChunkStep(starts, seqs, high, 4, cache), 0.1)
+    small = append.PagedCache(*caches)
+    assert torch.equal(got, chunk.chunk_attention(q, small, chunk.ChunkStep(starts, seqs, table, 4, small), 0.1))
+
+
+def test_a_long_row_of_tokens(device):
+    """One token of a request of 2^18 keys, and a window at its end."""
+    g = torch.Generator(device=device).manual_seed(8)
+    n = 1 << 18
+    q, caches, table, starts, seqs = make(g, [(1, n - 1)], 2, 1, 64, 64, torch.float16)
+    cache = append.PagedCache(*caches)
+    for window in (0, 5, n):
+        got = chunk.chunk_attention(q, cache, chunk.ChunkStep(starts, seqs, table, 2, cache, window), 0.125)
+        check(got, q, caches, table, starts, seqs, window, 0.125, 64)
 
 
 def test_streams_and_replays(device):

@@ -101,6 +101,10 @@ def _rotate_args(**over):
     ({"key": torch.zeros(5, 2, 64, dtype=torch.float16)}, "key"),
     ({"query_out": torch.zeros(5, 3, 64)}, "heads"), ({"query_out": torch.zeros(4, 4, 64)}, "query_out"),
     ({"key_out": torch.zeros(5, 1, 64)}, "heads"),
+    ({"query_out": torch.zeros(5, 1, 64).expand(5, 4, 64)}, "overlap"),
+    ({"query_out": torch.zeros(1, 4, 64).expand(5, 4, 64)}, "overlap"),
+    ({"key_out": torch.zeros(400).as_strided((5, 2, 64), (66, 64, 1))}, "overlap"),
+    ({"key_out": torch.zeros(600).as_strided((5, 2, 64), (64, 256, 1))}, "overlap"),
     ({"positions": torch.zeros(4, dtype=torch.int64)}, "positions"),
     ({"positions": torch.zeros(5)}, "integers"), ({"positions": torch.zeros(3, 5, dtype=torch.int64)}, "positions"),
     ({"positions": torch.zeros(5, dtype=torch.int64), "rotary": rotary.Rotary(rotary.rotary_table(8, 32),
@@ -131,6 +135,7 @@ def _append_args(**over):
     ({"value": torch.zeros(5, 3, 64, dtype=torch.bfloat16)}, "2 heads"),
     ({"query": torch.zeros(4, 4, 64, dtype=torch.bfloat16)}, "query"),
     ({"query_out": torch.zeros(5, 5, 64, dtype=torch.bfloat16)}, "query's heads"),
+    ({"query_out": torch.zeros(5, 1, 64, dtype=torch.bfloat16).expand(5, 4, 64)}, "overlap"),
     ({"positions": torch.zeros(4, dtype=torch.int64)}, "positions"),
     ({"rotary": rotary.Rotary(rotary.rotary_table(8, 128))}, "rotary_dim"),
     ({}, "device tensors"),
