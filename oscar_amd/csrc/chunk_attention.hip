@@ -155,6 +155,14 @@ __device__ __forceinline__ int opaque(int x) {
   return x;
 }
 
+// x ^ kBits, computed where it is written.
+template <int kBits>
+__device__ __forceinline__ int xor_here(int x) {
+  int y;
+  asm volatile("v_xor_b32 %0, %1, %2" : "=v"(y) : "i"(kBits), "v"(x));
+  return y;
+}
+
 // A product stays before what is written after it.
 __device__ __forceinline__ void pin(floatx16& x) { asm volatile("" : "+v"(x)); }
 // The instructions before this stay before those after it: a product's steps are
@@ -293,10 +301,11 @@ __device__ __forceinline__ void mask_scores(const ChunkArgs& a, floatx16& x, int
   }
 }
 
-// V^T operand of feature block b and keys 16 h + 8 (u / 4) + 4 g + u % 4.
+// V^T operand of feature block b (in `place`, v_read ^ 64 b) and keys 8 (u / 4) + 4 g
+// + u % 4 of the 16 that begin at vt.
 template <typename T, int D>
-__device__ __forceinline__ typename Num<T>::V8 v_operand_at(const uint8_t* vt, int v_addr, int h, int b) {
-  const uint8_t* at = vt + (v_addr ^ (64 * b)) + h * 32 * D;
+__device__ __forceinline__ typename Num<T>::V8 v_operand_at(const uint8_t* vt, int place) {
+  const uint8_t* at = vt + place;
   const shortx4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)at);
   const shortx4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(at + 16 * D));
   return __builtin_bit_cast(typename Num<T>::V8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
@@ -485,7 +494,7 @@ __device__ __forceinline__ void narrow_piece(const ChunkArgs& a, const Piece p, 
     keep_order();
     each<kHalves * kBlocks>([&](auto step) {
       constexpr int h = decltype(step)::value / kBlocks, b = decltype(step)::value % kBlocks;
-      s.acc[b] = Num<T>::mfma(v_operand_at<T, D>(vt, v_addr, h, b), w[h], s.acc[b]);
+      s.acc[b] = Num<T>::mfma(v_operand_at<T, D>(vt + h * 32 * D, v_addr ^ (64 * b)), w[h], s.acc[b]);
       if constexpr (b % 4 == 3 || b == kBlocks - 1) keep_order();
     });
     asm volatile("" ::: "memory");
@@ -581,8 +590,7 @@ constexpr int kWideRows = 32 * kWaves;
 constexpr int kWideWgs = 2;                                      // workgroups a CU
 constexpr int stage_tiles(int d) { return d == 256 ? 1 : 2; }    // 32-key tiles of a stage
 
-template <int D>
-constexpr int wide_lds() { return 2 * 2 * stage_tiles(D) * kTileKeys * 2 * D; }
+constexpr int wide_lds(int d) { return 2 * 2 * stage_tiles(d) * kTileKeys * 2 * d; }
 
 template <typename T, int D>
 __device__ __forceinline__ void wide_piece(const ChunkArgs& a, const Piece p, uint8_t* smem) {
@@ -637,12 +645,23 @@ __device__ __forceinline__ void wide_piece(const ChunkArgs& a, const Piece p, ui
     load_keys<D, true, kLoads, kKept>(a, p, p.key0 + kTiles * kTileKeys * stage + kKeys * wave, kKeys * wave, page,
                                       in_page, to + kTiles * kTileBytes, v_place);
   };
-  auto k_operand = [&](const uint8_t* kt, int i) {
-    const int at = kKeepAddresses ? k_addr : opaque(k_addr);
-    return *reinterpret_cast<const V8*>(kt + (at ^ (32 * i)));
+  // The operands' places: steps i and i + kSteps / 2 of the first product, and blocks
+  // b and b + kBlocks / 2 of the second, lie a constant apart at D = 256 (there the
+  // xor-ed bits are below it), so they are taken in turn and share a register.
+  int k_place_now, v_place_now;
+  auto k_step = [](int j) { return kKeepAddresses ? j : (j >> 1) + (j & 1) * (kSteps / 2); };
+  auto v_block = [](int j) { return kKeepAddresses ? j : (j >> 1) + (j & 1) * (kBlocks / 2); };
+  auto k_operand = [&](const uint8_t* kt, auto step) {
+    constexpr int j = decltype(step)::value;
+    if constexpr (kKeepAddresses) return *reinterpret_cast<const V8*>(kt + (k_addr ^ (32 * j)));
+    if constexpr (j % 2 == 0) k_place_now = xor_here<16 * j>(k_addr);
+    return *reinterpret_cast<const V8*>(kt + k_place_now + j % 2 * D);
   };
-  auto v_operand = [&](const uint8_t* vt, int i) {
-    return v_operand_at<T, D>(vt, kKeepAddresses ? v_addr : opaque(v_addr), i / kBlocks, i % kBlocks);
+  auto v_operand = [&](const uint8_t* vt, auto step) {
+    constexpr int h = decltype(step)::value / kBlocks, j = decltype(step)::value % kBlocks;
+    if constexpr (kKeepAddresses) return v_operand_at<T, D>(vt + h * 32 * D, v_addr ^ (64 * j));
+    if constexpr (j % 2 == 0) v_place_now = xor_here<32 * j>(v_addr);
+    return v_operand_at<T, D>(vt + h * 32 * D + j % 2 * D, v_place_now);
   };
   // Rows that do not see the whole of a tile lose what they do not see.  (Asked of
   // the workgroup's rows together: its waves share the tiles.)
@@ -695,16 +714,15 @@ __device__ __forceinline__ void wide_piece(const ChunkArgs& a, const Piece p, ui
     }
     // S^T = K Q^T
     V8 k[kAheadK];
-#pragma unroll
-    for (int i = 0; i < kAheadK; ++i) k[i] = k_operand(kt, i);
+    each<kAheadK>([&](auto step) { k[decltype(step)::value] = k_operand(kt, step); });
     keep_order();
     __builtin_amdgcn_s_setprio(1);
     floatx16 x;
     each<kSteps>([&](auto step) {
       constexpr int i = decltype(step)::value;
-      x = Num<T>::mfma(k[i % kAheadK], s.q[i], i == 0 ? floatx16{} : x);
+      x = Num<T>::mfma(k[i % kAheadK], s.q[k_step(i)], i == 0 ? floatx16{} : x);
       pin(x);
-      if constexpr (i + kAheadK < kSteps) k[i % kAheadK] = k_operand(kt, i + kAheadK);
+      if constexpr (i + kAheadK < kSteps) k[i % kAheadK] = k_operand(kt, std::integral_constant<int, i + kAheadK>{});
       keep_order();
       requests(i);
       keep_order();
@@ -715,8 +733,7 @@ __device__ __forceinline__ void wide_piece(const ChunkArgs& a, const Piece p, ui
       special = take_out_special<T, kTileBytes>(vt, lane) || special;
     }
     V8 v[kAheadV];
-#pragma unroll
-    for (int i = 0; i < kAheadV; ++i) v[i] = v_operand(vt, i);
+    each<kAheadV>([&](auto step) { v[decltype(step)::value] = v_operand(vt, step); });
     V8 w[2];
     weigh(x, w);
     if (__ballot(beyond(w))) {
@@ -727,10 +744,10 @@ __device__ __forceinline__ void wide_piece(const ChunkArgs& a, const Piece p, ui
     __builtin_amdgcn_s_setprio(1);
     // O^T += V^T P^T
     each<kPv>([&](auto step) {
-      constexpr int i = decltype(step)::value, h = i / kBlocks, b = i % kBlocks;
+      constexpr int i = decltype(step)::value, h = i / kBlocks, b = v_block(i % kBlocks);
       s.acc[b] = Num<T>::mfma(v[i % kAheadV], w[h], s.acc[b]);
       pin(s.acc[b]);
-      if constexpr (i + kAheadV < kPv) v[i % kAheadV] = v_operand(vt, i + kAheadV);
+      if constexpr (i + kAheadV < kPv) v[i % kAheadV] = v_operand(vt, std::integral_constant<int, i + kAheadV>{});
       if constexpr (b == 0) s.l = Num<T>::sum8(w[h], s.l);
       keep_order();
     });
@@ -808,15 +825,18 @@ __device__ __forceinline__ void wide_piece(const ChunkArgs& a, const Piece p, ui
 }
 
 // ---------------------------------------------------------------- kernels
+// (LDS of fixed size: its place is then known when addresses are computed, which in
+// the wide tiles' steps is one addition an operand less: D = 256, 9256 tokens over
+// 15360 1190 -> 1130 us.)
 constexpr int narrow_wgs(int d) { return 256 / d; }             // workgroups a CU
 template <typename T, int D>
 __global__ __launch_bounds__(kThreads, narrow_wgs(D)) void narrow_kernel(ChunkArgs a) {
-  extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[narrow_lds(D, kTileKeys)];
   narrow_piece<T, D, kTileKeys>(a, a.pieces[blockIdx.x], smem);
 }
 template <typename T, int D>
 __global__ __launch_bounds__(kThreads, kWideWgs) void wide_kernel(ChunkArgs a) {
-  extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[wide_lds(D)];
   wide_piece<T, D>(a, a.pieces[blockIdx.x], smem);
 }
 // A step with both.  Narrow pieces that fill the GPU come after the wide ones, where
@@ -825,9 +845,10 @@ __global__ __launch_bounds__(kThreads, kWideWgs) void wide_kernel(ChunkArgs a) {
 // tokens over 4096 beside seven users' 4, D = 128, 124 us: the wide ones alone take
 // 90, the narrow ones alone 38; D = 256 71 us (the wide ones first 83).
 constexpr int kFewNarrow = kCus;
+constexpr int mixed_lds(int d) { return std::max(narrow_lds(d, beside_keys(d)), wide_lds(d)); }
 template <typename T, int D>
 __global__ __launch_bounds__(kThreads, kWideWgs) void mixed_kernel(ChunkArgs a) {
-  extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[mixed_lds(D)];
   const int total = a.narrow + a.wide, lead = a.narrow <= kFewNarrow ? 0 : a.narrow;
   const int at = (int)blockIdx.x + lead, i = at < total ? at : at - total;
   if (i >= a.narrow) wide_piece<T, D>(a, a.pieces[i], smem);
@@ -1093,15 +1114,11 @@ void make_plan(const int32_t* qsl, const int32_t* seqs, int32_t num_requests, in
 
 template <typename T, int D>
 int launch(const ChunkArgs& a, const oscar_chunk_step& step, hipStream_t stream) {
-  static std::atomic<uint64_t> done[3];
-  constexpr int kLds[3] = {narrow_lds(D, kTileKeys), wide_lds<D>(),
-                           std::max(narrow_lds(D, beside_keys(D)), wide_lds<D>())};
-  static_assert(kLds[2] <= 80 * 1024, "two workgroups' LDS must fit the CU's 160 KiB");
+  static_assert(kWideWgs * mixed_lds(D) <= 160 * 1024 && narrow_wgs(D) * narrow_lds(D, kTileKeys) <= 160 * 1024,
+                "the workgroups of a CU must fit its 160 KiB of LDS");
   void (*const kernels[3])(ChunkArgs) = {&narrow_kernel<T, D>, &wide_kernel<T, D>, &mixed_kernel<T, D>};
   const int which = step.wide == 0 ? 0 : step.narrow == 0 ? 1 : 2;
-  const int st = set_dynamic_lds(reinterpret_cast<const void*>(kernels[which]), kLds[which], done[which]);
-  if (st != kOk) return st;
-  kernels[which]<<<step.narrow + step.wide, kThreads, kLds[which], stream>>>(a);
+  kernels[which]<<<step.narrow + step.wide, kThreads, 0, stream>>>(a);
   const int64_t blocks = (int64_t)step.few_joins * (D / 32) + (int64_t)(step.joins - step.few_joins) * (kTileRows * D / 64);
   if (blocks > INT32_MAX) return kErrInvalidArgument;
   if (blocks > 0) join_kernel<T, D><<<(uint32_t)blocks, 256, 0, stream>>>(a);
