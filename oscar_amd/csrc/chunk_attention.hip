@@ -404,8 +404,12 @@ __device__ __forceinline__ uint8_t* out_row(const ChunkArgs& a, int token0, int 
 // tile when its sums are, so that one or two tiles are always on their way.
 // Tiles are 32 keys, or, beside wide pieces at D = 256, 16 (the upper half of the
 // score tile is then the lower one's again and not used), so that two workgroups
-// fit a CU's LDS; alone they are slower (32 users' 4 tokens over 2K to 16K keys
-// 61.8 us with 32 keys, 64.7 with 16).
+// fit a CU's LDS; alone, few keys take longer with those (one token over 256 keys 8.7
+// us, 8.0 with 32; 32 users' 4 tokens over 2K to 16K 55 with either).
+// Measured: 8 users' token over 32K keys (D = 256) 48.5 us, 5.5 TB/s (a large copy
+// moves 5.05); 32 users' 4 tokens over 2K to 16K 55 us, 5.3 TB/s.  One user's over 1K
+// takes 7.4 us and 3.6 of join: three memory round trips (piece, page, keys) and one
+// for each of a wave's tiles.
 constexpr int beside_keys(int d) { return d == 256 ? 16 : 32; }
 constexpr int narrow_lds(int d, int keys) { return kWaves * 2 * keys * 2 * d + kWaves * 2 * kTileRows * 4; }
 
@@ -586,6 +590,15 @@ __device__ __forceinline__ void narrow_piece(const ChunkArgs& a, const Piece p, 
 // way.  A wave does a tile's products and softmax one after the other; the
 // matrix unit is kept busy by the waves of the other workgroups on the CU, which
 // no barrier ties to this one.
+// Two workgroups of four waves fill the registers at D = 256 (64 of queries, 128 of
+// sums a lane), so the order in which a tile's products and reads are issued is
+// written out: the compiler's own spills registers to memory.
+// What bounds it: the matrix unit together with the vector instructions of the
+// softmax (and, at D = 64, those alone: 16 exponentials a lane against 8 products),
+// at the clock the power limit leaves (1.75 GHz in the longest cases).  Measured:
+// D = 256, 6 heads on one, 9256 tokens over 15360 keys 1081 us, 1.05 PFLOP/s; D = 128,
+// 32 on 8, 8192 over 8192 1443 us, 1.14; D = 64, 16 on 4, 8192 over 8192 412 us, 1.0
+// (a large bf16 matrix product: 1.38).
 constexpr int kWideRows = 32 * kWaves;
 constexpr int kWideWgs = 2;                                      // workgroups a CU
 constexpr int stage_tiles(int d) { return d == 256 ? 1 : 2; }    // 32-key tiles of a stage
@@ -601,7 +614,7 @@ __device__ __forceinline__ void wide_piece(const ChunkArgs& a, const Piece p, ui
   constexpr int kLoads = kTiles * kTileBytes / 1024 / kWaves;    // of a stage's K, a wave
   constexpr int kKeys = kTiles * kTileKeys / kWaves;             // that it loads: inside a group of 16
   constexpr int kSteps = D / 16, kBlocks = D / 32, kPv = 2 * kBlocks;
-  constexpr int kAheadK = D == 128 ? 6 : 4, kAheadV = D == 256 ? 2 : D == 128 ? 6 : 4;     // operands read ahead
+  constexpr int kAheadK = D == 128 ? 6 : 4, kAheadV = D == 256 ? 3 : D == 128 ? 6 : 4;     // operands read ahead
   constexpr bool kKeepAddresses = D <= 128;      // of the operand reads in registers (D = 256 has none left)
   const int tid = (int)threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -859,7 +872,10 @@ __global__ __launch_bounds__(kThreads, kWideWgs) void mixed_kernel(ChunkArgs a) 
 // The partials of cut row tiles.  A 32-row group of few partials (kFewParts): a
 // thread to four features of a row, 256 to a workgroup, every partial in turn.  Of
 // more: a workgroup to 64 features of a row, 16 threads across the features and
-// 16 across the partials, whose sums meet in LDS.
+// 16 across the partials, whose sums meet in LDS.  (Few up to 8: 2048 tokens beside
+// 16 users' 4, D = 256, 180 us, up to 4 203, up to 16 183.)  The partials' bytes bound
+// it (512 wide pieces of D = 128: 43 MB, 9.8 us), or, where there is little, latency:
+// 2.3 to 5 us.
 constexpr int kFewParts = 8;
 
 template <typename T, int D, int kParts>
@@ -1036,17 +1052,17 @@ void plan_narrow(const std::vector<RowTile>& rows, int32_t head_size, double bes
 
 // Wide tiles.  Workgroups take pieces as they come free, two to a CU.  Row tiles
 // are left whole or cut in pieces of at most so many key tiles, whichever is
-// estimated to end first.  In units of a key tile's time on a busy CU (D = 256 1.05
+// estimated to end first.  In units of a key tile's time on a busy CU (D = 256 0.97
 // us, 128 0.47, 64 0.27): a piece costs 4 beside its tiles, one of a cut row tile 15
 // (its partials are written and read again: the same at any D, as both go with D);
 // a workgroup alone on its CU takes 1.07, 1.45 or 1.5 units a tile; the join is a
 // launch of 5 us; cut pieces end a tenth later than their sum, as they are not dealt
 // out as is assumed here.  Measured, whole / cut, us:
-//   D = 256, 6 heads: 9256 tokens over 15360 1208 / 1257, 4096 over 28672 1165 /
-//   815, 3001 alone 109 / 60, 1024 alone 45 / 29;
-//   D = 128, 32 heads: 8192 alone 508 / 567, 1024 over 4096 119 / 90, 8 prompts
-//   of 300 over 500 51 / 56;  D = 64, 16 heads: 8192 over 8192 422 / 461, 1024
-//   over 1024 37 / 23.
+//   D = 256, 6 heads: 9256 tokens over 15360 1081 / 1143, 4096 over 28672 1061 /
+//   711, 3001 alone 98 / 54, 1024 alone 40 / 28, 77 over 20011 578 / 33;
+//   D = 128, 32 heads: 1024 over 4096 111 / 88, 8 prompts of 300 over 500 50 / 70;
+//   D = 64, 16 heads: 8192 over 8192 412 / 425, 1024 over 1024 37 / 23, 6000 + 1501
+//   tokens in a window of 1024 45 / 59.
 // Returns the estimate.
 constexpr int32_t kPieceCost = 4, kCutCost = 15, kLeastPiece = 8, kMostPieces = 2048;
 double plan_wide(const std::vector<RowTile>& rows, int32_t head_size, Plan& plan) {
