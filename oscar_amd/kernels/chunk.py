@@ -14,6 +14,7 @@ from . import _lib, decode, rotary as _rotary
 from .append import PagedCache
 
 HEAD_SIZES = (64, 128, 256)
+_TOO_SMALL = -3                             # OSCAR_ERR_WORKSPACE_TOO_SMALL
 
 _i32, _i64 = ctypes.c_int32, ctypes.c_int64
 
@@ -53,9 +54,7 @@ class ChunkStep:
         if layout.qsl and layout.qsl[0] < 0:
             raise ValueError("query starts are counted from the step's token 0")
         args = ChunkStepArgs()
-        plan = [ctypes.addressof(layout.qstart), ctypes.addressof(layout.seq_t), requests, num_heads, window,
-                cache.address]
-        _lib.call("oscar_chunk_plan", *plan, None, 0, ctypes.byref(args))
+        items = _plan(layout, requests, num_heads, window, cache, args)
         if block_tables.ndim != 2 or block_tables.shape[0] < requests or block_tables.shape[1] < args.table_cols:
             raise ValueError(f"block table must be [requests, pages] with the {args.table_cols} pages of the longest")
         if block_tables.device != cache.device:
@@ -70,7 +69,7 @@ class ChunkStep:
             raise ValueError("a step is built before its calls are captured")
         with torch.cuda.device(device):
             host = torch.empty(max(args.items_size, 16), dtype=torch.uint8, pin_memory=True)
-            _lib.call("oscar_chunk_plan", *plan, host.data_ptr(), host.numel(), ctypes.byref(args))
+            host.copy_(items[:host.numel()])
             self.items = host.to(device, non_blocking=True)
             self.ready = torch.cuda.Event()
             self.ready.record()
@@ -128,6 +127,23 @@ def chunk_attention(query: torch.Tensor, cache: PagedCache, step: ChunkStep, sca
     _lib.call_on(device, "oscar_chunk_attention", step.address, step.items_ptr, step.table_ptr, step.table_stride,
                  cache.address, q, o, scale, None if ws is None else ws.data_ptr(), need)
     return out
+
+
+def _plan(layout, requests: int, num_heads: int, window: int, cache: PagedCache, args: ChunkStepArgs) -> torch.Tensor:
+    """The step's items (host bytes), its sizes in args.  Planned straight into
+    128 KB, which most steps' items fit; a step that needs more is planned again."""
+    size = 1 << 17
+    while True:
+        items = torch.empty(size, dtype=torch.uint8)
+        status = _lib.load().oscar_chunk_plan(
+            ctypes.addressof(layout.qstart), ctypes.addressof(layout.seq_t), requests, num_heads, window,
+            cache.address, items.data_ptr(), size, ctypes.byref(args))
+        if status != _TOO_SMALL:
+            break
+        size = args.items_size
+    if status != 0:
+        raise _lib.OscarKernelError(f"oscar_chunk_plan failed: {_lib.STATUS.get(status, status)}")
+    return items
 
 
 def _misaligned(x: torch.Tensor) -> bool:

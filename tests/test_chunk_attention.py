@@ -5,7 +5,7 @@ import struct
 import pytest
 import torch
 
-from oscar_amd.kernels import _lib, append, chunk, rotary
+from oscar_amd.kernels import _lib, append, chunk, decode, rotary
 
 PIECE, JOIN = struct.Struct("12i"), struct.Struct("8i")
 NARROW, WIDE, TILE = 32, 128, 32
@@ -96,6 +96,17 @@ def test_an_empty_step():
     assert not pieces and not joins and args.items_size == 0 and args.num_tokens == 0
     args, pieces, joins = plan([0, 0, 0], [5, 0], 8, 0, plain_cache())
     assert not pieces and args.workspace_size == 0
+
+
+@pytest.mark.parametrize("requests", [1, 3000])
+def test_a_step_plans_its_items(requests):
+    """Items that fit the first buffer, and those (144 KB) that need another."""
+    cache, starts, seqs = plain_cache(hk=1), list(range(requests + 1)), [9] * requests
+    args, pieces, _ = plan(starts, seqs, 4, 0, cache)
+    own = chunk.ChunkStepArgs()
+    items = chunk._plan(decode.request_layout(starts, seqs), requests, 4, 0, cache, own)
+    assert own.items_size == args.items_size == PIECE.size * requests and (own.items_size > 1 << 17) == (requests > 1)
+    assert [PIECE.unpack_from(items.numpy().tobytes(), PIECE.size * i) for i in range(requests)] == pieces
 
 
 def _plan_status(starts=(0, 4), seqs=(9,), heads=8, window=0, cache=None, requests=None):
