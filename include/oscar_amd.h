@@ -607,7 +607,7 @@ int oscar_append_rotated(const oscar_rotary* rotary, const int64_t* positions, i
  *     [block_table_stride] int32, of whose rows the first table_cols entries at
  *     most are read: keys on pages outside [0, num_pages) are left out, like
  *     keys that a row does not see, and a row that sees none becomes zeros;
- *   query, out: 16-byte aligned rows of the cache's type (strides multiples of 8)
+ *   query, out: 16-byte aligned rows of the cache's type (strides multiples of 8, >= 0)
  *     from token 0 of the step on; rows of no request are left as they were;
  *   workspace: workspace_size bytes, 16-byte aligned; scale: positive.
  * head_size 64, 128 or 256; block_size a multiple of 16; page strides below 4 GiB;

@@ -1233,7 +1233,8 @@ extern "C" int oscar_chunk_attention(const oscar_chunk_step* step, const void* i
   if ((int64_t)workspace_size < step->workspace_size || (step->workspace_size > 0 && workspace == nullptr))
     return kErrWorkspaceTooSmall;
   if (((uintptr_t)query->data | (uintptr_t)out->data | (uintptr_t)workspace | (uintptr_t)items) % 16 ||
-      (query->token_stride | query->head_stride | out->token_stride | out->head_stride) % 8)
+      (query->token_stride | query->head_stride | out->token_stride | out->head_stride) % 8 ||
+      std::min({query->token_stride, query->head_stride, out->token_stride, out->head_stride}) < 0)
     return kErrUnsupportedGeometry;
   ChunkArgs a{};
   a.q = static_cast<const uint8_t*>(query->data);

@@ -162,6 +162,7 @@ def test_attention_entry_refuses():
     assert status(q=heads(None, 1024, 128, 8, 0)) == -1 and status(o=heads(None, 1024, 128, 8, 0)) == -1
     assert status(ws=None) == -3 and status(size=args.workspace_size - 1) == -3
     assert status(q=heads(fake + 8, 1024, 128, 8, 0)) == -5 and status(o=heads(fake, 1028, 128, 8, 0)) == -5
+    assert status(q=heads(fake, -1024, 128, 8, 0)) == -5 and status(o=heads(fake, 1024, -128, 8, 0)) == -5
     assert status(ws=fake + 8) == -5 and status(items=fake + 4) == -5
     empty, _, _ = plan([0, 0], [9], 8, 0, cache)
     assert status(step=empty, size=0, ws=None) == 0

@@ -213,6 +213,17 @@ def test_many_decodes_beside_prompts(device, d):
         check(got, q, caches, table, starts, seqs, window, 0.1, 32)
 
 
+@pytest.mark.parametrize("hq, hk, page", [(64, 1, 1024), (40, 1, 16), (33, 1, 240), (66, 2, 128), (1, 1, 4096)])
+def test_large_groups_and_pages(device, hq, hk, page):
+    """Groups of more heads than a narrow tile's rows; pages of many tiles, or of 15 groups of 16 keys."""
+    g = torch.Generator(device=device).manual_seed(hq + page)
+    q, caches, table, starts, seqs = make(g, [(1, 1500), (3, 40), (0, 7), (9, 5000)], hq, hk, 128, page, torch.float16)
+    cache = append.PagedCache(*caches)
+    for window in (0, 333):
+        got = chunk.chunk_attention(q, cache, chunk.ChunkStep(starts, seqs, table, hq, cache, window), 0.09)
+        check(got, q, caches, table, starts, seqs, window, 0.09, page)
+
+
 def test_unmapped_pages_are_left_out(device):
     g = torch.Generator(device=device).manual_seed(7)
     reqs = [(2, 200), (40, 200), (1, 10), (3, 300)]
