@@ -39,7 +39,8 @@ constexpr int kThreads = 64 * kWaves;
 constexpr int kCus = 256;
 constexpr int32_t kMostKeys = 1 << 30;     // of a request, and rows: positions and windows add without overflow
 constexpr float kNone = -3.0e38f;          // running maximum before any key
-constexpr float kLazy = 8.f;               // a maximum is raised when a score exceeds it by 2^8
+constexpr float kLazy = 8.f;               // a maximum is raised when a score exceeds it by this
+constexpr float kMostWeight = 256.f;       // 2^kLazy
 
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 half2v __attribute__((ext_vector_type(2)));
@@ -693,7 +694,14 @@ __device__ __forceinline__ void wide_piece(const ChunkArgs& a, const Piece p, ui
       __builtin_amdgcn_sched_barrier(0);    // (eight at a time: registers)
     }
   };
-  // Some weight is above 2^kLazy (or no number).  Positive numbers compare as
+  // Whether some weight is above 2^kLazy (or no number) shows in the tile's sum of
+  // weights at D = 128; at the other sizes the sums are added up beside the second
+  // product and the weights asked (from the sum / from the weights: 8 prompts of 300
+  // over 500, D = 128, 45.7 / 50.8 us; 6000 + 1501 tokens in a window, D = 64, 49 /
+  // 45.5; 9256 over 15360, D = 256, 1127 / 1104).
+  constexpr bool kSumFirst = D == 128;
+  auto sum = [](const V8 (&w)[2]) { return Num<T>::sum8(w[0], 0.f) + Num<T>::sum8(w[1], 0.f); };
+  // Positive numbers compare as
   // their bits do, so this takes nine operations for a tile, where the maximum of
   // the scores takes one for each.
   auto beyond = [&](const V8 (&w)[2]) {
@@ -749,10 +757,13 @@ __device__ __forceinline__ void wide_piece(const ChunkArgs& a, const Piece p, ui
     each<kAheadV>([&](auto step) { v[decltype(step)::value] = v_operand(vt, step); });
     V8 w[2];
     weigh(x, w);
-    if (__ballot(beyond(w))) {
+    float l = kSumFirst ? sum(w) : 0.f;
+    if (__ballot(kSumFirst ? !(l <= kMostWeight) : beyond(w))) {
       raise(x);
       weigh(x, w);
+      if constexpr (kSumFirst) l = sum(w);
     }
+    if constexpr (kSumFirst) s.l += l;
     keep_order();
     __builtin_amdgcn_s_setprio(1);
     // O^T += V^T P^T
@@ -761,7 +772,7 @@ __device__ __forceinline__ void wide_piece(const ChunkArgs& a, const Piece p, ui
       s.acc[b] = Num<T>::mfma(v[i % kAheadV], w[h], s.acc[b]);
       pin(s.acc[b]);
       if constexpr (i + kAheadV < kPv) v[i % kAheadV] = v_operand(vt, std::integral_constant<int, i + kAheadV>{});
-      if constexpr (b == 0) s.l = Num<T>::sum8(w[h], s.l);
+      if constexpr (b == 0 && !kSumFirst) s.l = Num<T>::sum8(w[h], s.l);
       keep_order();
     });
     __builtin_amdgcn_s_setprio(0);

@@ -361,6 +361,54 @@ def test_streams_and_replays(device):
         out.zero_()
 
 
+def test_a_captured_step_reads_its_inputs_anew(device):
+    """Write and attention of a mixed step in one graph: rows, positions, slots and
+    block table change between replays; two streams run the step at once."""
+    g = torch.Generator(device=device).manual_seed(12)
+    hq, hk, d, page, dtype = 6, 2, 128, 32, torch.float16
+    turn = rotary.Rotary(rotary.rotary_table(900, d, device=device))
+    lengths, history = (4, 90), (500, 300)
+    starts, seqs, n = [0, 4, 94], [504, 390], 94
+    caches = [torch.randn(60, page, hk, d, generator=g, device=device).to(dtype) for _ in range(2)]
+    cache = append.PagedCache(*caches)
+    x = torch.zeros(n, hq + 2 * hk, d, device=device, dtype=dtype)
+    q, k, v = x.split((hq, hk, hk), 1)
+    pos, slots = torch.zeros(n, dtype=torch.int64, device=device), torch.zeros(n, dtype=torch.int64, device=device)
+    table = torch.zeros(2, 16, dtype=torch.int32, device=device)
+    step = chunk.ChunkStep(starts, seqs, table, hq, cache)
+
+    def run(cache):
+        return chunk.chunk_attention(append.append_rotated(q, k, v, pos, turn, cache, slots), cache, step, 0.1)
+
+    def change():
+        x.copy_(torch.randn(x.shape, generator=g, device=device))
+        pos.copy_(torch.randint(0, 900, (n,), generator=g, device=device))
+        table.copy_(torch.randperm(60, generator=g, device=device)[:32].view(2, 16))
+        slots.copy_(torch.cat([table[i].long()[(h + torch.arange(m, device=device)) // page] * page
+                               + (h + torch.arange(m, device=device)) % page
+                               for i, (m, h) in enumerate(zip(lengths, history))]))
+
+    change()
+    run(cache)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run(cache)
+    side = torch.cuda.Stream()
+    for _ in range(3):
+        change()
+        copies = [c.clone() for c in caches]
+        other = append.PagedCache(*copies)
+        side.wait_stream(torch.cuda.current_stream())
+        graph.replay()
+        with torch.cuda.stream(side):
+            want = run(other)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and all(torch.equal(a, b) for a, b in zip(caches, copies))
+        keys, values = gather(caches, table[1], seqs[1], page)
+        o, bound = expected(rotary.rotate(q, None, pos, turn)[0][4:], keys, values, history[1], 0, 0.1)
+        assert ((out[4:].double() - o).abs() <= bound).all()
+
+
 def test_append_then_attend(device):
     """A prompt, its follow-up chunk and MTP steps of two requests, rotated on
     image positions, written and read; against the formula over all tokens."""
