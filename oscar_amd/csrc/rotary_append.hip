@@ -17,10 +17,11 @@
 // 65536 tokens 176 us instead of 119).  Every job's first round of loads goes out
 // before the cosines are collected.
 //
-// Measured: 30843 tokens of 32 + 8 heads of 128 (fp16, adjacent pairs) 114 us,
-// 5.6 TB/s; 9256 of 6 + 1 heads of 256 (64 features turn, three axes) 13.3 us, 5.2
-// TB/s; a write of 65536 tokens of that shape 106 us, 5.1 TB/s; a large copy moves
-// 5.05 TB/s.  One token takes 3 us.
+// Measured: 30843 tokens of 32 + 8 heads of 128 (fp16, adjacent pairs) 112 us,
+// 5.8 TB/s; 9256 of 6 + 1 heads of 256 (64 features turn, three axes) 13.3 us, 5.2
+// TB/s; a write of 65536 tokens of that shape 105 us, 5.2 TB/s; a large copy moves
+// 5.05 TB/s.  One token takes 5 us: positions, table and rows, a memory round trip
+// each.
 #include "plain_cache.h"
 
 #include <type_traits>
@@ -343,12 +344,13 @@ int run(const oscar_rotary* r, const int64_t* positions, int64_t axis_stride, in
   a.half = r->rotary_dim / 2;
   a.sign = inverse ? -1.f : 1.f;
   a.by_half = make_fast_div((uint32_t)a.half);
-  // Tokens of a workgroup: a power of two, up to ten pieces a thread, fewer where
-  // that leaves less than 1024 workgroups (9256 tokens of 7 heads of 256: 8 tokens
-  // 14.7 us, 5 17.0; 30843 of 40 heads of 128: 4 tokens 121 us, 7 130; a write of
-  // 65536: 9 tokens 119 us, 5 120, 14 153).
+  // Tokens of a workgroup: a power of two, up to ten pieces a thread (30843 tokens of
+  // 40 heads of 128: up to 5 112 us, 10 114, 20 123; a write of 65536 of 8 heads of 256:
+  // 124, 106, 115), fewer where that leaves less than 512 workgroups (a write of 32 MB:
+  // 14.1 us, with 1024 16.3; 24 MB of 8 heads of 256: 11.7, 14.1; of 40 heads of 128:
+  // 12.0, 10.7).
   int block = kMaxTokens;
-  while (block > 1 && (block * work > 10 * kRotThreads || (tokens + block - 1) / block < 1024)) block /= 2;
+  while (block > 1 && (block * work > 10 * kRotThreads || (tokens + block - 1) / block < 512)) block /= 2;
   a.block_tokens = block;
   if ((tokens + block - 1) / block > INT32_MAX) return kErrInvalidArgument;
   // More than the last-level cache holds, read and written: rows go past the caches
