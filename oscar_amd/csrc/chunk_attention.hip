@@ -712,14 +712,17 @@ __device__ __forceinline__ void wide_piece(const ChunkArgs& a, const Piece p, ui
     const ushortx2 most{Num<T>::kLazyBits, Num<T>::kLazyBits};
     return __builtin_bit_cast(uint32_t, __builtin_elementwise_sub_sat(top, most)) != 0u;
   };
-  // Raises the running maximum to that of the tile's scores where a weight was
-  // too large (always so for the first keys of a row), and rescales the sums.
-  auto raise = [&](const floatx16& x) __attribute__((always_inline)) {
+  // Raises the running maximum to that of the tile's scores where a weight, or their
+  // sum, was too large (always so for the first keys of a row; other rows stay as
+  // they are, so a row's result does not depend on its neighbours), and rescales the
+  // sums.
+  auto raise = [&](const floatx16& x, float l) __attribute__((always_inline)) {
     float top = x[0];
 #pragma unroll
     for (int i = 1; i < 16; ++i) top = fmaxf(top, x[i]);
     top = max_halves(top) * a.scale_log2;
-    const float m = top > s.m + kLazy ? top : s.m, f = __builtin_amdgcn_exp2f(s.m - m);
+    const bool over = kSumFirst ? !(max_halves(l) <= kMostWeight) && top > s.m : top > s.m + kLazy;
+    const float m = over ? top : s.m, f = __builtin_amdgcn_exp2f(s.m - m);
 #pragma unroll
     for (int b = 0; b < kBlocks; ++b) s.acc[b] *= f;
     s.l *= f;
@@ -759,7 +762,7 @@ __device__ __forceinline__ void wide_piece(const ChunkArgs& a, const Piece p, ui
     weigh(x, w);
     float l = kSumFirst ? sum(w) : 0.f;
     if (__ballot(kSumFirst ? !(l <= kMostWeight) : beyond(w))) {
-      raise(x);
+      raise(x, l);
       weigh(x, w);
       if constexpr (kSumFirst) l = sum(w);
     }

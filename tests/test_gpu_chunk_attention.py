@@ -134,6 +134,26 @@ def test_scores_of_any_size(device):
 
 
 @pytest.mark.parametrize("d", [64, 128, 256])
+def test_rows_do_not_depend_on_their_neighbours(device, d):
+    """Scores that grow along the keys at another pace for every row: a row's result is
+    the same among the others and among copies of itself."""
+    g = torch.Generator(device=device).manual_seed(14)
+    n, h = 64, 700
+    q, caches, table, starts, seqs = make(g, [(n, h)], 2, 1, d, 16, torch.bfloat16)
+    caches[0].mul_(0.125)
+    keys = torch.arange(n + h, device=device)
+    caches[0][table[0][keys // 16].long(), keys % 16, 0, 0] = (keys / 16).bfloat16()
+    q[..., 0] = torch.arange(2 * n, device=device).view(n, 2).flip(0) / 64       # (a score rises by 2 along the keys, or 80)
+    cache = append.PagedCache(*caches)
+    step = chunk.ChunkStep(starts, seqs, table, 2, cache)
+    got = chunk.chunk_attention(q, cache, step, 1.0)
+    check(got, q, caches, table, starts, seqs, 0, 1.0, 16)
+    for row in (0, 17, 40, 63):
+        alone = chunk.chunk_attention(q[row:row + 1].expand(n, 2, d), cache, step, 1.0)
+        assert torch.equal(alone[row], got[row])
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
 def test_what_lies_in_unseen_slots_does_not_matter(device, d):
     """Slots past a request's keys, other requests' pages: NaN and infinities."""
     g = torch.Generator(device=device).manual_seed(6)
