@@ -1032,12 +1032,14 @@ void cut(const RowTile& x, int32_t n, Plan& plan, std::vector<Piece>& out) {
 
 int32_t pieces_of(const RowTile& x, int64_t per) { return (int32_t)((x.tiles + per - 1) / per); }
 
-// Narrow tiles: the fewest key tiles a piece with which the pieces fit the
-// workgroups that are resident at once.  Where the longest row tile is short, all
-// stay whole, and there is no second launch: one token of one user over 256 keys,
-// D = 256, whole 7.9 us of GPU time, cut 8.3 (over 512: 10.9, 8.3); D = 128, 8 kv
-// heads, over 512 whole 7.2, cut 7.1 and 6.2 against 10.6 where the host launches
-// (over 1024: 11.1, 7.0).
+// Narrow tiles: the fewest key tiles a piece with which there is a piece a CU, or,
+// where that leaves the longest piece a seventh above the mean, as many pieces as
+// reside at once (D = 128: 8 users' 4 tokens over 4000 keys, 8 kv heads, a piece a CU
+// 27.3 us, two 28.7, 4 users' over 2048 10.4, 12.8; 24 users' over 100 to 16200 a piece
+// a CU 166 us, two 140).  Where the longest row tile is short, all stay whole, and
+// there is no second launch: one token of one user over 256 keys, D = 256, whole 7.9 us
+// of GPU time, cut 8.3 (over 512: 10.9, 8.3); D = 128, 8 kv heads, over 512 whole 7.2,
+// cut 7.1 and 6.2 against 10.6 where the host launches (over 1024: 11.1, 7.0).
 // Beside wide tiles that take at least two thirds of the reading's time (`beside`, in
 // their units, of which a narrow tile's 128 D bytes at 5.2 TB/s are 1/160), two narrow
 // workgroups to three CUs (16 users over 8000 keys beside two prompts, D = 256: 37 to
@@ -1052,15 +1054,20 @@ void plan_narrow(const std::vector<RowTile>& rows, int32_t head_size, double bes
     most = std::max(most, x.tiles);
   }
   const int32_t uncut = head_size == 256 ? 8 : 16;
-  const int64_t resident = beside == 0. ? kCus * narrow_wgs(head_size) : total > 240 * beside ? 2 * kCus : 2 * kCus / 3;
-  int64_t per = std::max<int64_t>(kWaves, (total + resident - 1) / resident);
-  auto count = [&](int64_t t) {
-    int64_t c = 0;
-    for (const RowTile& x : rows) c += pieces_of(x, t);
-    return c;
+  auto fit = [&](int64_t resident) {
+    int64_t per = std::max<int64_t>(kWaves, (total + resident - 1) / resident);
+    auto count = [&](int64_t t) {
+      int64_t c = 0;
+      for (const RowTile& x : rows) c += pieces_of(x, t);
+      return c;
+    };
+    if ((int64_t)rows.size() >= resident || most <= uncut) per = std::max<int64_t>(per, most);
+    while (per < most && count(per) > resident) ++per;
+    return per;
   };
-  if ((int64_t)rows.size() >= resident || most <= uncut) per = std::max<int64_t>(per, most);
-  while (per < most && count(per) > resident) ++per;
+  int64_t per = fit(beside == 0. ? kCus : total > 240 * beside ? 2 * kCus : 2 * kCus / 3);
+  if (beside == 0. && (rows.size() >= kCus || 100 * per * kCus > 115 * total))
+    per = fit((int64_t)kCus * narrow_wgs(head_size));
   for (const RowTile& x : rows) cut(x, pieces_of(x, per), plan, plan.narrow);
 }
 
