@@ -869,7 +869,7 @@ __global__ __launch_bounds__(kThreads, kWideWgs) void wide_kernel(ChunkArgs a) {
 // A step with both.  Narrow pieces that fill the GPU come after the wide ones, where
 // those leave room: reads at full rate leave the wide pieces' next stage late.  A few
 // (plan_narrow) come first, and read for as long as the wide ones compute.  1024
-// tokens over 4096 beside seven users' 4, D = 128, 124 us: the wide ones alone take
+// tokens over 4096 beside seven users' 4, D = 128, 119 us: the wide ones alone take
 // 90, the narrow ones alone 38; D = 256 71 us (the wide ones first 83).
 constexpr int kFewNarrow = kCus;
 constexpr int mixed_lds(int d) { return std::max(narrow_lds(d, beside_keys(d)), wide_lds(d)); }
@@ -884,7 +884,7 @@ __global__ __launch_bounds__(kThreads, kWideWgs) void mixed_kernel(ChunkArgs a) 
 
 // ---------------------------------------------------------------- join
 // The partials of cut row tiles.  A 32-row group of few partials (kFewParts): a
-// thread to four features of a row, 256 to a workgroup, every partial in turn.  Of
+// thread to four features of a row, 256 to a workgroup, all partials at once.  Of
 // more: a workgroup to 64 features of a row, 16 threads across the features and
 // 16 across the partials, whose sums meet in LDS.  (Few up to 8: 2048 tokens beside
 // 16 users' 4, D = 256, 180 us, up to 4 203, up to 16 183.)  The partials' bytes bound
