@@ -38,9 +38,15 @@ constexpr int kWaves = 4;
 constexpr int kThreads = 64 * kWaves;
 constexpr int kCus = 256;
 constexpr int32_t kMostKeys = 1 << 30;     // of a request, and rows: positions and windows add without overflow
-constexpr float kNone = -3.0e38f;          // running maximum before any key
-constexpr float kLazy = 8.f;               // a maximum is raised when a score exceeds it by this
-constexpr float kMostWeight = 256.f;       // 2^kLazy
+constexpr float kNone = -3.0e38f;          // m before any key
+// A row's m is its running maximum less Num<T>::kLift (both in units of a factor of
+// 2), so that the largest weights lie between 2^kLift and 2^(kLift + kLazy): m is
+// raised when a score exceeds it by kLift + kLazy.  bf16 has fp32's range, any place
+// in it will do.  fp16 rounds weights below 2^-14 by steps of 2^-24; lifted by 2^7,
+// up to half of its largest value, those are keys of less than 2^-21 of the heaviest
+// one's weight, each off by 2^-32 of it at most.  (Without the lift 24000 keys of
+// 2^-24.6 each counted half as much again.)
+constexpr float kLazy = 8.f;
 
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 half2v __attribute__((ext_vector_type(2)));
@@ -65,7 +71,9 @@ struct Num<__bf16> {
     asm volatile("" : "+v"(w));
     return __builtin_bit_cast(V8, w);
   }
-  static constexpr uint16_t kLazyBits = 0x4380;      // 2^kLazy
+  static constexpr float kLift = 0.f;
+  static constexpr float kMostWeight = 256.f;        // 2^(kLift + kLazy)
+  static constexpr uint16_t kMostBits = 0x4380;      // its bits
   static constexpr uint16_t kInfBits = 0x7F80;
   static __device__ __forceinline__ floatx16 mfma(V8 a, V8 b, floatx16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
@@ -89,7 +97,9 @@ struct Num<_Float16> {
     asm volatile("" : "+v"(w));
     return __builtin_bit_cast(V8, w);
   }
-  static constexpr uint16_t kLazyBits = 0x5C00;
+  static constexpr float kLift = 7.f;
+  static constexpr float kMostWeight = 32768.f;
+  static constexpr uint16_t kMostBits = 0x7800;
   static constexpr uint16_t kInfBits = 0x7C00;
   static __device__ __forceinline__ floatx16 mfma(V8 a, V8 b, floatx16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
@@ -474,9 +484,9 @@ __device__ __forceinline__ void narrow_piece(const ChunkArgs& a, const Piece p, 
 #pragma unroll
     for (int i = 1; i < 8 * kHalves; ++i) top = fmaxf(top, x[i]);
     top = max_halves(top) * a.scale_log2;
-    const bool raise = top > s.m + kLazy;
+    const bool raise = top > s.m + (kLazy + Num<T>::kLift);
     if (__ballot(raise)) {
-      const float m = raise ? top : s.m, f = __builtin_amdgcn_exp2f(s.m - m);
+      const float m = raise ? top - Num<T>::kLift : s.m, f = __builtin_amdgcn_exp2f(s.m - m);
 #pragma unroll
       for (int b = 0; b < kBlocks; ++b) s.acc[b] *= f;
       s.l *= f;
@@ -694,7 +704,7 @@ __device__ __forceinline__ void wide_piece(const ChunkArgs& a, const Piece p, ui
       __builtin_amdgcn_sched_barrier(0);    // (eight at a time: registers)
     }
   };
-  // Whether some weight is above 2^kLazy (or no number) shows in the tile's sum of
+  // Whether some weight is above the most (or no number) shows in the tile's sum of
   // weights at D = 128; at the other sizes the sums are added up beside the second
   // product and the weights asked (from the sum / from the weights: 8 prompts of 300
   // over 500, D = 128, 45.7 / 50.8 us; 6000 + 1501 tokens in a window, D = 64, 49 /
@@ -709,7 +719,7 @@ __device__ __forceinline__ void wide_piece(const ChunkArgs& a, const Piece p, ui
     const ushortx2 top = __builtin_elementwise_max(
         __builtin_elementwise_max(__builtin_shufflevector(u, u, 0, 1), __builtin_shufflevector(u, u, 2, 3)),
         __builtin_elementwise_max(__builtin_shufflevector(u, u, 4, 5), __builtin_shufflevector(u, u, 6, 7)));
-    const ushortx2 most{Num<T>::kLazyBits, Num<T>::kLazyBits};
+    const ushortx2 most{Num<T>::kMostBits, Num<T>::kMostBits};
     return __builtin_bit_cast(uint32_t, __builtin_elementwise_sub_sat(top, most)) != 0u;
   };
   // Raises the running maximum to that of the tile's scores where a weight, or their
@@ -721,8 +731,9 @@ __device__ __forceinline__ void wide_piece(const ChunkArgs& a, const Piece p, ui
 #pragma unroll
     for (int i = 1; i < 16; ++i) top = fmaxf(top, x[i]);
     top = max_halves(top) * a.scale_log2;
-    const bool over = kSumFirst ? !(max_halves(l) <= kMostWeight) && top > s.m : top > s.m + kLazy;
-    const float m = over ? top : s.m, f = __builtin_amdgcn_exp2f(s.m - m);
+    const bool over = kSumFirst ? !(max_halves(l) <= Num<T>::kMostWeight) && top - Num<T>::kLift > s.m
+                                : top > s.m + (kLazy + Num<T>::kLift);
+    const float m = over ? top - Num<T>::kLift : s.m, f = __builtin_amdgcn_exp2f(s.m - m);
 #pragma unroll
     for (int b = 0; b < kBlocks; ++b) s.acc[b] *= f;
     s.l *= f;
@@ -761,7 +772,7 @@ __device__ __forceinline__ void wide_piece(const ChunkArgs& a, const Piece p, ui
     V8 w[2];
     weigh(x, w);
     float l = kSumFirst ? sum(w) : 0.f;
-    if (__ballot(kSumFirst ? !(l <= kMostWeight) : beyond(w))) {
+    if (__ballot(kSumFirst ? !(l <= Num<T>::kMostWeight) : beyond(w))) {
       raise(x, l);
       weigh(x, w);
       if constexpr (kSumFirst) l = sum(w);

@@ -462,3 +462,39 @@ def test_append_then_attend(device):
                                 total[i], 0, d ** -0.5)
             assert ((got[a:b].double() - o).abs() <= bound).all()
             total[i] += m
+
+
+@pytest.mark.parametrize("d, reqs, hq, hk", [(256, [(1, 32767)] * 300, 2, 1), (128, [(1, 32767)] * 600, 2, 1),
+                                             (64, [(1, 32767)] * 1100, 2, 1), (64, [(2048, 32768)], 32, 4),
+                                             (128, [(2048, 32768)], 32, 4), (256, [(1024, 24576)], 32, 4)])
+@pytest.mark.parametrize("below", [24.59375, 22.40625])
+def test_many_faint_keys_beside_one_keep_their_share(device, d, reqs, hq, hk, below):
+    """fp16: the first key outweighs each of the others by 2^below, and those together
+    are half a percent of a row and more.  (All requests read the same pages.)  The
+    weights are rounded in fp16 relative to 2^7 of the largest's, so one below 2^-14 is
+    off by 2^-25, which is 2^-32 of the row's sum; else the bounds above, with B = |o|."""
+    n, h = reqs[0]
+    seq, page = n + h, 128
+    pages = -(-seq // page)
+    keys = torch.zeros(pages, page, hk, d, device=device, dtype=torch.float16)
+    keys[..., 0] = -below
+    keys[0, 0, :, 0] = 0
+    feature = 1 + torch.arange(d, device=device) / d                     # (exact in fp16)
+    values = feature.half().expand(pages, page, hk, d).clone()
+    values[0, 0] = 0
+    cache = append.PagedCache(keys, values)
+    starts = [n * i for i in range(len(reqs) + 1)]
+    table = torch.arange(pages, device=device, dtype=torch.int32).expand(len(reqs), pages)
+    q = torch.zeros(starts[-1], hq, d, device=device, dtype=torch.float16)
+    q[..., 0] = 1
+    scale = math.log(2)
+    step = chunk.ChunkStep(starts, [seq] * len(reqs), table, hq, cache)
+    got = chunk.chunk_attention(q, cache, step, scale).double()
+    others = (seq - n + torch.arange(n, device=device, dtype=torch.float64)).repeat(len(reqs))[:, None, None]
+    weight = math.exp(-below * scale)
+    o = others * weight / (1 + others * weight) * feature.double()
+    eps = 2.0 ** -10
+    bound = eps / 2 * 2 * o + eps / 2 * o * (1 + eps) + (2 * below * scale * (d + 2) * 2.0 ** -24 + 2.0 ** -20) * o
+    bound += others * 2.0 ** -32 * 2 + torch.finfo(torch.float16).smallest_normal * eps / 2
+    off = (got - o).abs() - bound
+    assert off.max().item() <= 0, f"off by {off.max().item():.3e} more than the bound"
