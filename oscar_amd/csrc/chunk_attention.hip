@@ -694,12 +694,13 @@ __device__ __forceinline__ void wide_piece(const ChunkArgs& a, const Piece p, ui
   const int whole_from = a.window == 0 ? 0 : pos1 - a.window + 1, whole_to = pos0 - kTileKeys + 1;
   auto whole = [&](int key0) { return key0 >= whole_from && key0 <= whole_to; };
   bool special = false;                     // this wave found values that are not finite in such a tile
+  auto weight = [&](float x) { return __builtin_amdgcn_exp2f(__builtin_fmaf(x, a.scale_log2, -s.m)); };
   auto weigh = [&](const floatx16& x, V8 (&w)[2]) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       float f[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] = __builtin_amdgcn_exp2f(x[8 * h + i] * a.scale_log2 - s.m);
+      for (int i = 0; i < 8; ++i) f[i] = weight(x[8 * h + i]);
       w[h] = Num<T>::round8(f);
       __builtin_amdgcn_sched_barrier(0);    // (eight at a time: registers)
     }
@@ -723,16 +724,20 @@ __device__ __forceinline__ void wide_piece(const ChunkArgs& a, const Piece p, ui
     return __builtin_bit_cast(uint32_t, __builtin_elementwise_sub_sat(top, most)) != 0u;
   };
   // Raises the running maximum to that of the tile's scores where a weight, or their
-  // sum, was too large (always so for the first keys of a row; other rows stay as
-  // they are, so a row's result does not depend on its neighbours), and rescales the
-  // sums.
+  // sum, was too large (always so for the first keys of a row), and rescales the sums.
+  // A row is asked for its heaviest weight just as it was rounded: other rows stay as
+  // they are, so what becomes of a row does not depend on its neighbours.  (Asked for
+  // its score, one whose weight rounds to the most would be raised beside a heavier
+  // neighbour, but not by itself.)
   auto raise = [&](const floatx16& x, float l) __attribute__((always_inline)) {
     float top = x[0];
 #pragma unroll
     for (int i = 1; i < 16; ++i) top = fmaxf(top, x[i]);
-    top = max_halves(top) * a.scale_log2;
+    top = max_halves(top);
+    const float heaviest = (float)(T)weight(top);
+    top *= a.scale_log2;
     const bool over = kSumFirst ? !(max_halves(l) <= Num<T>::kMostWeight) && top - Num<T>::kLift > s.m
-                                : top > s.m + (kLazy + Num<T>::kLift);
+                                : heaviest > Num<T>::kMostWeight;
     const float m = over ? top - Num<T>::kLift : s.m, f = __builtin_amdgcn_exp2f(s.m - m);
 #pragma unroll
     for (int b = 0; b < kBlocks; ++b) s.acc[b] *= f;

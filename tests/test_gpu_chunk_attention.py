@@ -498,3 +498,25 @@ def test_many_faint_keys_beside_one_keep_their_share(device, d, reqs, hq, hk, be
     bound += others * 2.0 ** -32 * 2 + torch.finfo(torch.float16).smallest_normal * eps / 2
     off = (got - o).abs() - bound
     assert off.max().item() <= 0, f"off by {off.max().item():.3e} more than the bound"
+
+
+@pytest.mark.parametrize("dtype, above", [(torch.bfloat16, 2.0 ** -8), (torch.float16, 2.0 ** -11)], ids=str)
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_rows_at_the_edge_of_a_raise_do_not_depend_on_their_neighbours(device, dtype, above, d):
+    """A score so little above the limit for raising the maximum (2^8 of it) that its
+    weight rounds to the limit, beside rows whose scores go far beyond: the row is the
+    same among copies of itself."""
+    n, h, page = 32, 64, 32
+    keys, values = (torch.zeros(3, page, 1, d, device=device, dtype=dtype) for _ in range(2))
+    keys[1, :4, 0, 0], keys[1, :4, 0, 1] = 8, above                      # the second tile, the third is not seen:
+    keys[2, :, 0, 0] = -60
+    values[0, :, 0] = (1 + torch.arange(d, device=device) / d).to(dtype)
+    cache = append.PagedCache(keys, values)
+    table = torch.arange(3, device=device, dtype=torch.int32)[None]
+    q = torch.ones(n, 2, d, device=device, dtype=dtype)
+    q[1::2, :, 0] = 10
+    step = chunk.ChunkStep([0, n], [n + h], table, 2, cache)
+    assert step.args.wide == 1
+    got = chunk.chunk_attention(q, cache, step, math.log(2))
+    alone = chunk.chunk_attention(q[:1].expand(n, 2, d), cache, step, math.log(2))
+    assert torch.equal(got[0], alone[0]) and torch.equal(got[::2], alone[::2])
