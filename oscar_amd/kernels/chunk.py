@@ -14,6 +14,8 @@ from . import _lib, decode, rotary as _rotary
 from .append import PagedCache
 
 HEAD_SIZES = (64, 128, 256)
+MAX_HEADS = 1 << 16
+MAX_KEYS = 1 << 30                          # of a request
 _TOO_SMALL = -3                             # OSCAR_ERR_WORKSPACE_TOO_SMALL
 
 _i32, _i64 = ctypes.c_int32, ctypes.c_int64
@@ -45,8 +47,11 @@ class ChunkStep:
         requests = len(layout.lengths)
         if num_heads < 1 or num_heads % cache.num_kv_heads:
             raise ValueError(f"{num_heads} query heads do not share {cache.num_kv_heads} kv heads")
+        if num_heads > MAX_HEADS:
+            raise ValueError(f"chunk attention takes at most {MAX_HEADS} query heads, got {num_heads}")
         if window < 0:
             raise ValueError("the window must be positive, or 0 for none")
+        window = min(window, MAX_KEYS)      # (no request is longer; a larger integer would be taken modulo 2^32)
         if cache.head_size not in HEAD_SIZES:
             raise ValueError(f"chunk attention takes head sizes {HEAD_SIZES}, got {cache.head_size}")
         if cache.block_size % 16:

@@ -21,6 +21,7 @@ from ..format import check_d
 from . import _lib, staging
 from .quant import cache_geometry
 
+_INT32_MAX = 2 ** 31 - 1
 MAX_QUERY_LEN = 16          # rows per request <= 16 tokens x group (backend.py:277)
 
 def workspace(device: torch.device, nbytes: int) -> torch.Tensor:
@@ -50,6 +51,10 @@ class RequestLayout:
         self.qsl = tuple(int(x) for x in qsl)
         self.seqs = tuple(int(x) for x in seqs)
         self.lengths = validate_layout(self.qsl, self.seqs)
+        # (ctypes would take what does not fit modulo 2^32; starts do not decrease)
+        if max(self.seqs, default=0) > _INT32_MAX or (self.qsl and not -_INT32_MAX <= self.qsl[0] <= self.qsl[-1]
+                                                      <= _INT32_MAX):
+            raise ValueError("OSCAR query starts and sequence lengths are 32-bit")
         self.max_q = max(self.lengths, default=0)
         self.max_hist = max((s - m for s, m in zip(self.seqs, self.lengths)), default=0)
         self.qstart = (ctypes.c_int32 * max(len(self.qsl), 1))(*self.qsl)

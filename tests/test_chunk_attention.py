@@ -202,3 +202,45 @@ def test_step_struct_matches_the_header(tmp_path):
     got = subprocess.run([str(tmp_path / "layout")], check=True, capture_output=True, text=True).stdout.split()
     assert [int(x) for x in got] == [ctypes.sizeof(chunk.ChunkStepArgs)] + [getattr(chunk.ChunkStepArgs, f).offset
                                                                             for f in fields]
+
+
+@pytest.mark.parametrize("window, planned", [
+    (5, 5), (1 << 30, 1 << 30), ((1 << 30) + 1, 1 << 30), ((1 << 31) - 1, 1 << 30), (1 << 31, 1 << 30),
+    ((1 << 32) + 5, 1 << 30), (1 << 64, 1 << 30)])
+def test_windows_of_any_size(monkeypatch, window, planned):
+    """A window past the longest request is that of all keys, past 32 bits too."""
+    seen = []
+    plan_step = chunk._plan
+
+    def keep(*args):
+        items = plan_step(*args)
+        seen.append(args[-1])
+        return items
+
+    monkeypatch.setattr(chunk, "_plan", keep)
+    with pytest.raises(ValueError, match="device tensors"):       # (planned, then refused without a GPU)
+        chunk.ChunkStep([0, 4], [9], torch.zeros(1, 1, dtype=torch.int32), 8, plain_cache(), window)
+    assert seen[0].window == planned
+
+
+@pytest.mark.parametrize("window", [(1 << 30) + 1, (1 << 31) - 1])
+def test_plan_clamps_the_window(window):
+    reqs = ([0, 4, 300], [9000, 300], 8)
+    none, pieces, joins = plan(*reqs, 0, plain_cache())
+    args, same_pieces, same_joins = plan(*reqs, window, plain_cache())
+    assert args.window == 1 << 30 and none.window == 0 and (same_pieces, same_joins) == (pieces, joins)
+
+
+@pytest.mark.parametrize("qsl, seqs", [([0, 4], [(1 << 32) + 9]), ([0, 4], [1 << 31]), ([1 << 32, (1 << 32) + 4], [9]),
+                                       ([0, 1 << 31], [1 << 31]), ([-(1 << 32), 4 - (1 << 32)], [9])])
+def test_lengths_past_32_bits_are_refused(qsl, seqs):
+    with pytest.raises(ValueError, match="32-bit"):
+        decode.RequestLayout(qsl, seqs)
+    with pytest.raises(ValueError, match="32-bit"):
+        chunk.ChunkStep(qsl, seqs, torch.zeros(1, 1, dtype=torch.int32), 8, plain_cache())
+
+
+@pytest.mark.parametrize("heads, match", [((1 << 32) + 8, "at most"), ((1 << 16) + 2, "at most"), (1 << 16, "device")])
+def test_more_heads_than_the_plan_takes_are_refused(heads, match):
+    with pytest.raises(ValueError, match=match):
+        chunk.ChunkStep([0, 4], [9], torch.zeros(1, 1, dtype=torch.int32), heads, plain_cache())
