@@ -1078,7 +1078,13 @@ void plan_narrow(const std::vector<RowTile>& rows, int32_t head_size, double bes
       return c;
     };
     if ((int64_t)rows.size() >= resident || most <= uncut) per = std::max<int64_t>(per, most);
-    while (per < most && count(per) > resident) ++per;
+    // (The count falls as pieces get longer.  Step by step the search took 5 ms for 250
+    // short rows beside 2^20 keys, and 17 s beside 2^30.)
+    for (int64_t high = std::max<int64_t>(per, most); per < high;) {
+      const int64_t mid = (per + high) / 2;
+      if (count(mid) > resident) per = mid + 1;
+      else high = mid;
+    }
     return per;
   };
   int64_t per = fit(beside == 0. ? kCus : total > 240 * beside ? 2 * kCus : 2 * kCus / 3);

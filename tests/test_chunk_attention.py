@@ -1,6 +1,7 @@
 """The chunk attention's plan, and what is refused, without a GPU."""
 import ctypes
 import struct
+import time
 
 import pytest
 import torch
@@ -244,3 +245,18 @@ def test_lengths_past_32_bits_are_refused(qsl, seqs):
 def test_more_heads_than_the_plan_takes_are_refused(heads, match):
     with pytest.raises(ValueError, match=match):
         chunk.ChunkStep([0, 4], [9], torch.zeros(1, 1, dtype=torch.int32), heads, plain_cache())
+
+
+@pytest.mark.parametrize("short, long, pieces", [(254, 1 << 30, 2), (250, 1 << 20, 6), (255, 1 << 20, 1), (100, 1 << 25, 156)])
+def test_one_long_row_among_short_ones_is_planned_at_once(short, long, pieces):
+    """The fewest key tiles a piece with which there are at most 256 pieces (one wide
+    cache head of 256 features), found in time that does not go by the keys: 50 us each
+    (a second here, for a machine with other work)."""
+    cache = plain_cache(d=256, hk=1)
+    began = time.perf_counter()
+    args, items, joins = plan(list(range(short + 2)), [11] * short + [long], 6, 0, cache)
+    assert time.perf_counter() - began < 1.0
+    parts = sorted((p[6], p[7]) for p in items if p[2] == short)
+    assert len(items) == short + pieces and len(parts) == pieces and len(joins) == (pieces > 1)
+    tiles = [-(-(b - a) // TILE) for a, b in parts]
+    assert parts[0][0] == 0 and parts[-1][1] == long and max(tiles) - min(tiles) <= 1
