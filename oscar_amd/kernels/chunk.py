@@ -16,6 +16,7 @@ from .append import PagedCache
 HEAD_SIZES = (64, 128, 256)
 MAX_HEADS = 1 << 16
 MAX_KEYS = 1 << 30                          # of a request
+MAX_INT32 = (1 << 31) - 1
 _TOO_SMALL = -3                             # OSCAR_ERR_WORKSPACE_TOO_SMALL
 
 _i32, _i64 = ctypes.c_int32, ctypes.c_int64
@@ -36,8 +37,8 @@ class ChunkStep:
     table.
 
     qsl [requests + 1] and seqs [requests] are host lists (query starts from the
-    step's token 0; keys after the step); block_tables int32 [requests, pages] on
-    the cache's device.  A step is not built under graph capture; a captured call
+    step's token 0; keys after the step); block_tables of integers
+    [requests, pages] on the cache's device.  A step is not built under graph capture; a captured call
     keeps this step's lengths and needs the step to live as long as the graph; the
     block table is read at every call and replay where it is int32 with rows of
     their own, and else copied here."""
@@ -62,6 +63,8 @@ class ChunkStep:
         items = _plan(layout, requests, num_heads, window, cache, args)
         if block_tables.ndim != 2 or block_tables.shape[0] < requests or block_tables.shape[1] < args.table_cols:
             raise ValueError(f"block table must be [requests, pages] with the {args.table_cols} pages of the longest")
+        if block_tables.dtype not in (torch.int32, torch.int64, torch.int16, torch.int8, torch.uint8):
+            raise ValueError(f"block tables hold integers, got {block_tables.dtype}")
         if block_tables.device != cache.device:
             raise ValueError("the block table must be on the cache's device")
         device = cache.device
@@ -69,6 +72,8 @@ class ChunkStep:
             raise ValueError("OSCAR kernels take device tensors")
         if (block_tables.dtype != torch.int32 or block_tables.stride(1) != 1
                 or block_tables.stride(0) < block_tables.shape[1]):
+            if block_tables.dtype == torch.int64:       # (what does not fit stays outside every cache)
+                block_tables = block_tables.clamp(-1, MAX_INT32)
             block_tables = block_tables.to(torch.int32).clone(memory_format=torch.contiguous_format)
         if torch.cuda.is_current_stream_capturing():
             raise ValueError("a step is built before its calls are captured")

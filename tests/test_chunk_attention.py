@@ -260,3 +260,9 @@ def test_one_long_row_among_short_ones_is_planned_at_once(short, long, pieces):
     assert len(items) == short + pieces and len(parts) == pieces and len(joins) == (pieces > 1)
     tiles = [-(-(b - a) // TILE) for a, b in parts]
     assert parts[0][0] == 0 and parts[-1][1] == long and max(tiles) - min(tiles) <= 1
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.bool], ids=str)
+def test_block_tables_of_other_types_are_refused(dtype):
+    with pytest.raises(ValueError, match="integers"):
+        chunk.ChunkStep([0, 4], [9], torch.zeros(1, 1, dtype=dtype), 8, plain_cache())

@@ -520,3 +520,22 @@ def test_rows_at_the_edge_of_a_raise_do_not_depend_on_their_neighbours(device, d
     got = chunk.chunk_attention(q, cache, step, math.log(2))
     alone = chunk.chunk_attention(q[:1].expand(n, 2, d), cache, step, math.log(2))
     assert torch.equal(got[0], alone[0]) and torch.equal(got[::2], alone[::2])
+
+
+def test_pages_past_32_bits_of_an_int64_table_are_left_out(device):
+    """Entries that name pages of the cache modulo 2^32, and those at the ends of both types."""
+    g = torch.Generator(device=device).manual_seed(23)
+    q, caches, table, starts, seqs = make(g, [(3, 230)], 4, 2, 64, 32, torch.bfloat16)
+    cache = append.PagedCache(*caches)
+    for far in ((1 << 32) + 1, -(1 << 32), (1 << 31) + 2, (1 << 63) - 1, -(1 << 63), -1):
+        bad = table.clone()
+        bad[0, 2] = -1
+        wide = table.long()
+        wide[0, 2] = far
+        want = chunk.chunk_attention(q, cache, chunk.ChunkStep(starts, seqs, bad, 4, cache), 0.1)
+        got = chunk.chunk_attention(q, cache, chunk.ChunkStep(starts, seqs, wide, 4, cache), 0.1)
+        assert torch.equal(got, want)
+    want = chunk.chunk_attention(q, cache, chunk.ChunkStep(starts, seqs, table, 4, cache), 0.1)
+    for dtype in (torch.uint8, torch.int16):
+        step = chunk.ChunkStep(starts, seqs, table.to(dtype), 4, cache)
+        assert torch.equal(chunk.chunk_attention(q, cache, step, 0.1), want)
