@@ -554,7 +554,8 @@ typedef struct oscar_rotary {
 
 /* Heads of a batch of tokens: value f of head h of token t lies at element
  * t * token_stride + h * head_stride + f of `data`; strides of rows that turn are
- * not negative and below 4 GiB. */
+ * not negative and below 4 GiB.  A stride between tokens or heads of which a call
+ * has one is not looked at. */
 typedef struct oscar_heads {
   void* data;
   int64_t token_stride;

@@ -1279,17 +1279,21 @@ extern "C" int oscar_chunk_attention(const oscar_chunk_step* step, const void* i
     return kErrInvalidArgument;
   if ((int64_t)workspace_size < step->workspace_size || (step->workspace_size > 0 && workspace == nullptr))
     return kErrWorkspaceTooSmall;
-  if (((uintptr_t)query->data | (uintptr_t)out->data | (uintptr_t)workspace | (uintptr_t)items) % 16 ||
-      (query->token_stride | query->head_stride | out->token_stride | out->head_stride) % 8 ||
-      std::min({query->token_stride, query->head_stride, out->token_stride, out->head_stride}) < 0)
-    return kErrUnsupportedGeometry;
   ChunkArgs a{};
   a.q = static_cast<const uint8_t*>(query->data);
   a.out = static_cast<uint8_t*>(out->data);
-  a.q_token = 2 * query->token_stride;
-  a.q_head = 2 * query->head_stride;
-  a.out_token = 2 * out->token_stride;
-  a.out_head = 2 * out->head_stride;
+  if (step->num_tokens > 1) {               // (a stride between rows of which there is one means nothing)
+    a.q_token = 2 * query->token_stride;
+    a.out_token = 2 * out->token_stride;
+  }
+  if (step->num_heads > 1) {
+    a.q_head = 2 * query->head_stride;
+    a.out_head = 2 * out->head_stride;
+  }
+  if (((uintptr_t)query->data | (uintptr_t)out->data | (uintptr_t)workspace | (uintptr_t)items) % 16 ||
+      (a.q_token | a.q_head | a.out_token | a.out_head) % 16 ||
+      std::min({a.q_token, a.q_head, a.out_token, a.out_head}) < 0)
+    return kErrUnsupportedGeometry;
   a.k = static_cast<const uint8_t*>(cache->k);
   a.v = static_cast<const uint8_t*>(cache->v);
   a.k_page = (uint32_t)cache->k_stride_page;

@@ -249,19 +249,20 @@ bool fits16(const void* p, int64_t token_bytes, int64_t head_bytes) {
   return ((uintptr_t)p | (uintptr_t)token_bytes | (uintptr_t)head_bytes) % 16 == 0;
 }
 
-int make_rows(Rows& s, const oscar_heads* in, const oscar_heads* out, int size, bool& vec) {
+// (Strides between rows of which there is one mean nothing.)
+int make_rows(Rows& s, const oscar_heads* in, const oscar_heads* out, int64_t tokens, int size, bool& vec) {
   if (in == nullptr || in->num_heads == 0) return kOk;
   if (in->data == nullptr || in->num_heads < 0 || in->num_heads > (1 << 16)) return kErrInvalidArgument;
   s.src = static_cast<const uint8_t*>(in->data);
-  s.src_token = in->token_stride * size;
-  s.src_head = in->head_stride * size;
+  s.src_token = tokens > 1 ? in->token_stride * size : 0;
+  s.src_head = in->num_heads > 1 ? in->head_stride * size : 0;
   s.heads = in->num_heads;
   vec = vec && fits16(s.src, s.src_token, s.src_head);
   if (out != nullptr) {
     if (out->data == nullptr || out->num_heads != in->num_heads) return kErrInvalidArgument;
     s.dst = static_cast<uint8_t*>(out->data);
-    s.dst_token = out->token_stride * size;
-    s.dst_head = out->head_stride * size;
+    s.dst_token = tokens > 1 ? out->token_stride * size : 0;
+    s.dst_head = out->num_heads > 1 ? out->head_stride * size : 0;
     vec = vec && fits16(s.dst, s.dst_token, s.dst_head);
   }
   for (const int64_t x : {s.src_token, s.src_head, s.dst_token, s.dst_head})
@@ -288,7 +289,7 @@ int run(const oscar_rotary* r, const int64_t* positions, int64_t axis_stride, in
   const oscar_heads* const in[3] = {query, key, value};
   const oscar_heads* const out[3] = {query_out, key_out, nullptr};
   for (int i = 0; i < 3; ++i) {
-    const int status = make_rows(rows[i], in[i], out[i], size, vec);
+    const int status = make_rows(rows[i], in[i], out[i], tokens, size, vec);
     if (status != kOk) return status;
   }
   if (cache != nullptr) {

@@ -119,14 +119,14 @@ def chunk_attention(query: torch.Tensor, cache: PagedCache, step: ChunkStep, sca
     q, hq = _rotary.heads(query, tokens, d, dtype, device, "query")
     if hq != step.num_heads:
         raise ValueError(f"query must have the step's {step.num_heads} heads")
-    if _misaligned(query):
+    if _misaligned(query, tokens):
         query = query.clone(memory_format=torch.contiguous_format)
         q, _ = _rotary.heads(query, tokens, d, dtype, device, "query")
     if out is None:
         out, o = _rotary.new_heads(query, query.shape[0], hq, d)
     else:
         o = _rotary.out_heads(out, tokens, hq, d, dtype, device, "out")
-        if _misaligned(out):
+        if _misaligned(out, tokens):
             raise ValueError("out must have rows at multiples of 16 bytes")
     if tokens == 0:
         return out
@@ -156,7 +156,13 @@ def _plan(layout, requests: int, num_heads: int, window: int, cache: PagedCache,
     return items
 
 
-def _misaligned(x: torch.Tensor) -> bool:
-    """Whether rows of x begin off multiples of 16 bytes (8 two-byte values)."""
+def _misaligned(x: torch.Tensor, tokens: int) -> bool:
+    """Whether the first `tokens` rows of x begin off multiples of 16 bytes (8
+    two-byte values).  Strides of axes of one entry mean nothing."""
     token, head, _ = x.stride()
-    return ((x.data_ptr() >> 1) | token | head) & 7 != 0
+    at = x.data_ptr() >> 1
+    if tokens > 1:
+        at |= token
+    if x.shape[1] > 1:
+        at |= head
+    return at & 7 != 0

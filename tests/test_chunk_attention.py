@@ -266,3 +266,23 @@ def test_one_long_row_among_short_ones_is_planned_at_once(short, long, pieces):
 def test_block_tables_of_other_types_are_refused(dtype):
     with pytest.raises(ValueError, match="integers"):
         chunk.ChunkStep([0, 4], [9], torch.zeros(1, 1, dtype=dtype), 8, plain_cache())
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="the addresses are no device memory")
+def test_strides_of_single_rows_are_not_looked_at():
+    """Without a GPU what passes the checks ends at the launch (-4)."""
+    fake, heads = 1 << 20, rotary.HeadsArgs
+
+    def status(tokens, hq, q, o):
+        cache = plain_cache(hk=1)
+        args, _, _ = plan([0, tokens], [40], hq, 0, cache)
+        return _lib.load().oscar_chunk_attention(ctypes.byref(args), fake, fake, 10, cache.address,
+                                                 ctypes.byref(heads(fake, *q, hq, 0)),
+                                                 ctypes.byref(heads(fake, *o, hq, 0)), 0.1, fake, args.workspace_size,
+                                                 None)
+
+    good, odd = (512, 128), (513, 128)
+    assert status(1, 4, good, odd) == status(1, 4, odd, good) == status(1, 4, good, (-1, 128)) == -4
+    assert status(2, 4, good, odd) == status(2, 4, odd, good) == -5
+    assert status(2, 1, good, (128, 129)) == status(2, 1, (128, -5), good) == -4
+    assert status(2, 2, good, (512, 129)) == -5

@@ -539,3 +539,18 @@ def test_pages_past_32_bits_of_an_int64_table_are_left_out(device):
     for dtype in (torch.uint8, torch.int16):
         step = chunk.ChunkStep(starts, seqs, table.to(dtype), 4, cache)
         assert torch.equal(chunk.chunk_attention(q, cache, step, 0.1), want)
+
+
+def test_strides_of_single_tokens_and_heads_mean_nothing(device):
+    """One token's query and output of any token stride, one head's of any head stride."""
+    g = torch.Generator(device=device).manual_seed(24)
+    for (n, hq, hk), token, head in (((1, 6, 2), 6 * 64 + 1, 64), ((5, 1, 1), 64, 67), ((1, 1, 1), 3, 5)):
+        q, caches, table, starts, seqs = make(g, [(n, 50)], hq, hk, 64, 16, torch.bfloat16)
+        cache = append.PagedCache(*caches)
+        step = chunk.ChunkStep(starts, seqs, table, hq, cache)
+        want = chunk.chunk_attention(q, cache, step, 0.125)
+        store = torch.zeros(2, 4000, device=device, dtype=torch.bfloat16)
+        mine, out = (x.as_strided((n, hq, 64), (token, head, 1)) for x in store)
+        mine.copy_(q)
+        assert chunk.chunk_attention(mine, cache, step, 0.125, out=out) is out and torch.equal(out, want)
+        assert torch.equal(chunk.chunk_attention(mine, cache, step, 0.125), want)

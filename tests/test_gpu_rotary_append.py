@@ -263,3 +263,21 @@ def test_streams_and_replays(device):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, want) and all(torch.equal(a, b) for a, b in zip(caches, want_caches))
+
+
+def test_strides_of_single_tokens_and_heads_mean_nothing(device):
+    """One token whose stride is past 4 GiB, one head of an odd stride."""
+    g = torch.Generator(device=device).manual_seed(25)
+    turn = rotary.Rotary(rotary.rotary_table(30, 32, device=device))
+    for (n, h), token, head in (((1, 4), 1 << 33, 64), ((5, 1), 64, (1 << 33) + 1), ((1, 1), 1 << 34, 1 << 34)):
+        x = torch.randn(n, h, 64, generator=g, device=device).half()
+        pos = torch.arange(n, device=device) + 3
+        want, _ = rotary.rotate(x, None, pos, turn)
+        mine, out = (torch.zeros(4000, device=device).half().as_strided((n, h, 64), (token, head, 1)) for _ in range(2))
+        mine.copy_(x)
+        got, _ = rotary.rotate(mine, None, pos, turn, query_out=out)
+        assert got is out and torch.equal(out, want)
+        if h == 1:
+            cache = append.PagedCache(*(torch.zeros(2, 16, 1, 64, device=device).half() for _ in range(2)))
+            append.append_rotated(None, mine, mine, pos, turn, cache, torch.arange(n, device=device))
+            assert torch.equal(cache.k_cache[0, :n], want) and torch.equal(cache.v_cache[0, :n], x)

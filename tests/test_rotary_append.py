@@ -254,3 +254,16 @@ def test_argument_structs_match_the_header(tmp_path):
                     str(tmp_path / "layout")], check=True)
     got = subprocess.run([str(tmp_path / "layout")], check=True, capture_output=True, text=True).stdout.split()
     assert [int(x) for x in got] == want
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="the addresses are no device memory")
+def test_strides_of_single_rows_are_not_looked_at():
+    """Without a GPU what passes the checks ends at the launch (-4)."""
+    r, far = _c_rotary(), 1 << 40
+
+    def status(tokens, token, heads, head):
+        x = rotary.HeadsArgs(FAKE, token, head, heads, 0)
+        return _status("oscar_rotate_positions", r, FAKE, 0, tokens, x, x, None, None, 64, 0, 0, None)
+
+    assert status(1, far, 2, 64) == status(1, -1, 2, 64) == status(5, 64, 1, far) == status(5, 64, 1, -1) == -4
+    assert status(2, far, 2, 64) == status(2, -64, 2, 64) == status(5, 64, 2, far) == GEOMETRY
