@@ -33,6 +33,7 @@ enum oscar_status {
   OSCAR_ERR_WORKSPACE_TOO_SMALL = -3,
   OSCAR_ERR_LAUNCH = -4,
   OSCAR_ERR_UNSUPPORTED_GEOMETRY = -5,
+  OSCAR_ERR_OVERLAP = -6, /* an output shares memory with other rows of the call */
 };
 
 /* ---------------------------------------------------------------- rotation
@@ -566,7 +567,7 @@ typedef struct oscar_heads {
 
 /* Queries and keys turned by their positions (inverse = 1: turned back, which
  * is also the gradient), in fp32, rounded once to their type.  An output may be
- * its input (same address and strides); otherwise the two do not overlap.
+ * its input (same address and strides); otherwise it overlaps no rows of the call.
  *   positions: int64, axis a of token t at a * position_axis_stride + t.
  * A token with a position outside [0, rotary->positions) on any axis is left
  * out: its output rows keep what they held.  dtype: of all rows; head_size any
@@ -578,8 +579,8 @@ int oscar_rotate_positions(const oscar_rotary* rotary, const int64_t* positions,
                            int32_t inverse, oscar_stream_t stream);
 
 /* The write of a step's keys and values to a plain cache, one launch: queries
- * turned into query_out, keys turned on the way to their slots, values written
- * as they are.  The cache's type (bf16 or fp16), head size and kv heads are the
+ * turned into query_out (as above), keys turned on the way to their slots, values
+ * written as they are.  The cache's type (bf16 or fp16), head size and kv heads are the
  * rows'.
  *   slot_mapping: [num_tokens] int64; slots < 0 or at or beyond num_pages *
  *     block_size are skipped (the token's query is still turned).  Slots of a
@@ -609,7 +610,8 @@ int oscar_append_rotated(const oscar_rotary* rotary, const int64_t* positions, i
  *     most are read: keys on pages outside [0, num_pages) are left out, like
  *     keys that a row does not see, and a row that sees none becomes zeros;
  *   query, out: 16-byte aligned rows of the cache's type (strides multiples of 8, >= 0)
- *     from token 0 of the step on; rows of no request are left as they were;
+ *     from token 0 of the step on, the same rows or apart; rows of no request are
+ *     left as they were;
  *   workspace: workspace_size bytes, 16-byte aligned; scale: positive.
  * head_size 64, 128 or 256; block_size a multiple of 16; page strides below 4 GiB;
  * seq_lens and a request's tokens x query heads of a kv head at most 2^30.  A cache

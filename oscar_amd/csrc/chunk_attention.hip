@@ -20,6 +20,7 @@
 // head, or a wide one, over a range of keys) that fill the GPU; a row tile in
 // several pieces leaves fp32 partials that a second launch joins.
 #include "plain_cache.h"
+#include "row_span.h"
 
 #include <algorithm>
 #include <cstddef>
@@ -1294,6 +1295,11 @@ extern "C" int oscar_chunk_attention(const oscar_chunk_step* step, const void* i
       (a.q_token | a.q_head | a.out_token | a.out_head) % 16 ||
       std::min({a.q_token, a.q_head, a.out_token, a.out_head}) < 0)
     return kErrUnsupportedGeometry;
+  // (a row is read by the workgroup that writes it, or by a launch before the one that does)
+  const RowSpan from{(uint64_t)(uintptr_t)a.q, a.q_token, a.q_head, step->num_tokens, step->num_heads, 2 * cache->head_size};
+  const RowSpan to{(uint64_t)(uintptr_t)a.out, a.out_token, a.out_head, step->num_tokens, step->num_heads,
+                   2 * cache->head_size};
+  if (!same_rows(from, to) && !rows_apart(from, to)) return kErrOverlap;
   a.k = static_cast<const uint8_t*>(cache->k);
   a.v = static_cast<const uint8_t*>(cache->v);
   a.k_page = (uint32_t)cache->k_stride_page;

@@ -36,6 +36,7 @@ enum Status : int {
   kErrWorkspaceTooSmall = -3,
   kErrLaunch = -4,
   kErrUnsupportedGeometry = -5,
+  kErrOverlap = -6,
 };
 
 // hipFuncSetAttribute(MaxDynamicSharedMemorySize) once per (kernel, device):

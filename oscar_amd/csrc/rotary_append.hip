@@ -23,6 +23,7 @@
 // 5.05 TB/s.  One token takes 5 us: positions, table and rows, a memory round trip
 // each.
 #include "plain_cache.h"
+#include "row_span.h"
 
 #include <type_traits>
 
@@ -245,6 +246,13 @@ struct Rows {
   int32_t heads;
 };
 
+RowSpan source(const Rows& s, int64_t tokens, int64_t row) {
+  return RowSpan{(uint64_t)(uintptr_t)s.src, s.src_token, s.src_head, tokens, s.heads, row};
+}
+RowSpan target(const Rows& s, int64_t tokens, int64_t row) {
+  return RowSpan{(uint64_t)(uintptr_t)s.dst, s.dst_token, s.dst_head, tokens, s.heads, row};
+}
+
 bool fits16(const void* p, int64_t token_bytes, int64_t head_bytes) {
   return ((uintptr_t)p | (uintptr_t)token_bytes | (uintptr_t)head_bytes) % 16 == 0;
 }
@@ -291,6 +299,18 @@ int run(const oscar_rotary* r, const int64_t* positions, int64_t axis_stride, in
   for (int i = 0; i < 3; ++i) {
     const int status = make_rows(rows[i], in[i], out[i], tokens, size, vec);
     if (status != kOk) return status;
+  }
+  // An output that is its input is read and written row by row by one thread; of any
+  // other rows that it shares memory with, some would be read after they are written.
+  const int64_t row = (int64_t)head_size * size;
+  for (int i = 0; i < 2; ++i) {
+    if (out[i] == nullptr) continue;
+    const RowSpan to = target(rows[i], tokens, row);
+    for (int j = 0; j < 3; ++j) {
+      const RowSpan from = source(rows[j], tokens, row);
+      if (!(i == j && same_rows(to, from)) && !rows_apart(to, from)) return kErrOverlap;
+    }
+    if (i == 0 && out[1] != nullptr && !rows_apart(to, target(rows[1], tokens, row))) return kErrOverlap;
   }
   if (cache != nullptr) {
     rows[1].dst = static_cast<uint8_t*>(cache->k);

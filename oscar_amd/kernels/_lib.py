@@ -96,6 +96,7 @@ STATUS = {
     -3: "workspace too small",
     -4: "kernel launch failed",
     -5: "unsupported cache geometry (slot widths, strides or alignment)",
+    -6: "an output overlaps other rows of the call (it must be its input as it stands, or apart)",
 }
 
 _lib = None

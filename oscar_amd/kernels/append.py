@@ -68,8 +68,8 @@ def append_rotated(query: torch.Tensor | None, key: torch.Tensor, value: torch.T
                    rotary: _rotary.Rotary, cache: PagedCache, slot_mapping: torch.Tensor, query_out=None):
     """Write key (turned by its positions) and value [N, Hk, D] of the tokens of
     slot_mapping (int64 [N]) to their slots, and return query [N, Hq, D] turned
-    (a new tensor, or query_out, which may be query itself; None without a
-    query).  Rows are of the cache's type, with any token and head strides
+    (a new tensor, or query_out: query itself or apart from the call's rows; None
+    without a query).  Rows are of the cache's type, with any token and head strides
     below 4 GiB; rows past the slots' count are not read.  Slots < 0 or past the cache are
     skipped, tokens with a position outside the table left out whole; slots of a
     call are distinct."""

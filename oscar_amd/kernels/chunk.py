@@ -107,7 +107,7 @@ class ChunkStep:
 def chunk_attention(query: torch.Tensor, cache: PagedCache, step: ChunkStep, scale: float, out=None) -> torch.Tensor:
     """Causal attention of query [N, Hq, D] (the cache's type; token t of the
     step in row t) over the cache; returns [N, Hq, D] of that type, a new tensor
-    or `out` (which may be query itself), whose rows past the step's tokens and of
+    or `out` (query itself or apart from it), whose rows past the step's tokens and of
     tokens of no request are not written.  scale must be positive.  Keys on pages outside the cache
     are left out; a row that sees no key becomes zeros."""
     device = cache.device

@@ -149,8 +149,8 @@ def rotate(query: torch.Tensor, key: torch.Tensor | None, positions: torch.Tenso
            key_out=None, inverse: bool = False):
     """query [N, Hq, D] and key [N, Hk, D] (or None) turned by their positions
     (int64 [N], or [axes, N]), bf16, fp16 or fp32 alike, with any token and head
-    strides below 4 GiB.  Returns (query_out, key_out): new tensors, or the ones given, which
-    may be the inputs themselves; no autograd graph is recorded (the gradient is
+    strides below 4 GiB.  Returns (query_out, key_out): new tensors, or the ones given, each its
+    own input as it stands or apart from all rows of the call; no autograd graph is recorded (the gradient is
     the inverse of the outputs' gradients).  A token with a position outside the table is
     left out: its output rows keep what they held."""
     dtype, device = query.dtype, query.device

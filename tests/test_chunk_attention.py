@@ -284,5 +284,5 @@ def test_strides_of_single_rows_are_not_looked_at():
     good, odd = (512, 128), (513, 128)
     assert status(1, 4, good, odd) == status(1, 4, odd, good) == status(1, 4, good, (-1, 128)) == -4
     assert status(2, 4, good, odd) == status(2, 4, odd, good) == -5
-    assert status(2, 1, good, (128, 129)) == status(2, 1, (128, -5), good) == -4
+    assert status(2, 1, (128, 128), (128, 129)) == status(2, 1, (128, -5), (128, 128)) == -4
     assert status(2, 2, good, (512, 129)) == -5

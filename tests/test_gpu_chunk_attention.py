@@ -16,7 +16,7 @@ import math
 import pytest
 import torch
 
-from oscar_amd.kernels import append, chunk, rotary
+from oscar_amd.kernels import _lib, append, chunk, rotary
 
 pytestmark = pytest.mark.gpu
 
@@ -554,3 +554,19 @@ def test_strides_of_single_tokens_and_heads_mean_nothing(device):
         mine.copy_(q)
         assert chunk.chunk_attention(mine, cache, step, 0.125, out=out) is out and torch.equal(out, want)
         assert torch.equal(chunk.chunk_attention(mine, cache, step, 0.125), want)
+
+
+def test_outputs_that_overlap_the_queries_are_refused(device):
+    g = torch.Generator(device=device).manual_seed(26)
+    q, caches, table, starts, seqs = make(g, [(40, 50)], 4, 2, 64, 16, torch.bfloat16)
+    cache = append.PagedCache(*caches)
+    step = chunk.ChunkStep(starts, seqs, table, 4, cache)
+    want = chunk.chunk_attention(q, cache, step, 0.125)
+    x = torch.zeros(41, 8, 64, device=device, dtype=torch.bfloat16)
+    x[:40, :4] = q
+    for out in (x[1:, :4], x[:40, 2:6], x[:40, 1:5]):
+        with pytest.raises(_lib.OscarKernelError, match="overlaps"):
+            chunk.chunk_attention(x[:40, :4], cache, step, 0.125, out=out)
+    assert torch.equal(x[:40, :4], q)
+    assert torch.equal(chunk.chunk_attention(x[:40, :4], cache, step, 0.125, out=x[:40, 4:]), want)
+    assert torch.equal(chunk.chunk_attention(x[:40, :4], cache, step, 0.125, out=x[:40, :4]), want)

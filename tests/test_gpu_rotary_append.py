@@ -9,7 +9,7 @@ bit for bit."""
 import pytest
 import torch
 
-from oscar_amd.kernels import append, rotary
+from oscar_amd.kernels import _lib, append, rotary
 
 pytestmark = pytest.mark.gpu
 TYPES = [torch.bfloat16, torch.float16, torch.float32]
@@ -281,3 +281,24 @@ def test_strides_of_single_tokens_and_heads_mean_nothing(device):
             cache = append.PagedCache(*(torch.zeros(2, 16, 1, 64, device=device).half() for _ in range(2)))
             append.append_rotated(None, mine, mine, pos, turn, cache, torch.arange(n, device=device))
             assert torch.equal(cache.k_cache[0, :n], want) and torch.equal(cache.v_cache[0, :n], x)
+
+
+def test_outputs_among_the_calls_rows(device):
+    """In place in slices of one projection; an exchange is refused."""
+    g = torch.Generator(device=device).manual_seed(27)
+    turn = rotary.Rotary(rotary.rotary_table(30, 32, device=device))
+    x = torch.randn(9, 3, 64, generator=g, device=device).half()
+    pos = torch.arange(9, device=device)
+    before = x.clone()
+    want = rotary.rotate(x[:, :1], x[:, 1:2], pos, turn)
+    for call in (lambda: rotary.rotate(x[:, :1], x[:, 1:2], pos, turn, query_out=x[:, 1:2], key_out=x[:, :1]),
+                 lambda: rotary.rotate(x[:8], None, pos[:8], turn, query_out=x[1:]),
+                 lambda: append.append_rotated(
+                     x[:, :1], x[:, 1:2], x[:, 2:], pos, turn,
+                     append.PagedCache(*(torch.zeros(1, 16, 1, 64, device=device).half() for _ in range(2))), pos,
+                     query_out=x[:, 2:])):
+        with pytest.raises(_lib.OscarKernelError, match="overlaps"):
+            call()
+    assert torch.equal(x, before)
+    rotary.rotate(x[:, :1], x[:, 1:2], pos, turn, query_out=x[:, :1], key_out=x[:, 1:2])
+    assert torch.equal(x[:, :1], want[0]) and torch.equal(x[:, 1:2], want[1]) and torch.equal(x[:, 2], before[:, 2])

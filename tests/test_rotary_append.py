@@ -267,3 +267,76 @@ def test_strides_of_single_rows_are_not_looked_at():
 
     assert status(1, far, 2, 64) == status(1, -1, 2, 64) == status(5, 64, 1, far) == status(5, 64, 1, -1) == -4
     assert status(2, far, 2, 64) == status(2, -64, 2, 64) == status(5, 64, 2, far) == GEOMETRY
+
+
+# ------------------------------------------------------------------ outputs and the rows they may lie among
+OVERLAP, LAUNCHED = -6, -4          # (without a GPU what passes the checks ends at the launch)
+no_gpu = pytest.mark.skipif(torch.cuda.is_available(), reason="the addresses are host memory")
+
+
+def _view(x):
+    token, head, _ = x.stride()
+    return rotary.HeadsArgs(x.data_ptr(), token, head, x.shape[1], 0)
+
+
+def _rotate_views(q, qo, k=None, ko=None):
+    views = [None if x is None else _view(x) for x in (q, qo, k, ko)]
+    return _status("oscar_rotate_positions", _c_rotary(rotary_dim=2), FAKE, 0, len(q), *views, q.shape[2], 2, 0, None)
+
+
+def _memory(x):
+    token, head, _ = x.stride()
+    return {x.storage_offset() + t * token + h * head + f for t in range(x.shape[0]) for h in range(x.shape[1])
+            for f in range(x.shape[2])}
+
+
+@no_gpu
+def test_rows_that_share_memory_never_count_as_apart():
+    """Random views of one store as output and input: refused whenever they share a
+    value, and, all but the tangled ones, only then."""
+    import random
+
+    rng, store, passed, apart = random.Random(1), torch.zeros(4096), 0, 0
+    for _ in range(4000):
+        tokens, d = rng.choice((1, 2, 3, 5)), rng.choice((2, 4, 8))
+        strides = [rng.choice((0, 2, 4, 8, 12, 16, 24, 40)) for _ in range(4)]
+        if rng.random() < 0.5:
+            strides[2:] = strides[:2]
+        heads = rng.choice((1, 2, 4))
+        x, y = (store.as_strided((tokens, heads, d), (*strides[2 * i:2 * i + 2], 1), rng.randint(0, 60))
+                for i in range(2))
+        same = all(a == b for a, b, n in zip((x.data_ptr(), *x.stride()), (y.data_ptr(), *y.stride()), (9, tokens, heads))
+                   if n > 1)
+        truth, status = not _memory(x) & _memory(y), _rotate_views(x, y)
+        assert status in (OVERLAP, LAUNCHED) and (status == OVERLAP or truth or same)
+        passed, apart = passed + (status == LAUNCHED and not same), apart + truth
+    assert passed > 0.9 * apart > 1000
+
+
+@no_gpu
+@pytest.mark.parametrize("views, status", [
+    (lambda x: (x[:, :2], x[:, 2:4], x[:, 2:4], x[:, :2]), OVERLAP),                     # exchanged
+    (lambda x: (x[:, :4], x[:, 2:6], None, None), OVERLAP),                              # two heads further on
+    (lambda x: (x[:4], x[1:5], None, None), OVERLAP),                                    # a token further on
+    (lambda x: (x[:4], x[:8:2], None, None), OVERLAP),                                   # another stride
+    (lambda x: (x[:, :4], x[:, 6:10], x[:, 10:], x[:, 2:4]), OVERLAP),                   # keys onto queries
+    (lambda x: (x[:, :4], x[:, 9:11].repeat(1, 2, 1), x[:, 4:6], x[:, 3:5]), OVERLAP),
+    (lambda x: (x[:, :2], x[:, 4:6], x[:, 6:8], x[:, 4:6]), OVERLAP),                    # both to one place
+    (lambda x: (x[:, :2], x[:, 4:6], x[:, 4:6], x[:, 6:8]), OVERLAP),                    # queries onto keys
+    (lambda x: (x[:, :4], x[:, :4], x[:, 4:6], x[:, 4:6]), LAUNCHED),                    # in place
+    (lambda x: (x[:, :4], x[:, 6:10], x[:, 4:6], x[:, 10:]), LAUNCHED),                  # slices of one projection
+    (lambda x: (x[:4, :4], x[4:, :4], x[:4, 4:6], x[4:, 4:6]), LAUNCHED),                # tokens of one tensor
+    (lambda x: (x[:1, :4], x[:1, :4].as_strided((1, 4, 64), (1, 64, 1)), None, None), LAUNCHED),
+    (lambda x: (x[:, ::3], x[:, ::3], x[:, 1::3], x[:, 1::3]), LAUNCHED),                # heads in turn
+    (lambda x: (x[:, ::3], x[:, 2::3], x[:, 1::3], None), INVALID),
+    (lambda x: (x.transpose(0, 1)[:, :3], x.transpose(0, 1)[:, 3:6], None, None), LAUNCHED)])     # heads first
+def test_outputs_among_the_calls_rows(views, status):
+    assert _rotate_views(*views(torch.zeros(8, 12, 64))) == status
+
+
+@no_gpu
+@pytest.mark.parametrize("first, status", [(0, LAUNCHED), (8, LAUNCHED), (1, OVERLAP), (4, OVERLAP), (6, OVERLAP)])
+def test_append_refuses_outputs_among_its_rows(first, status):
+    x = torch.zeros(5, 12, 64, dtype=torch.bfloat16)       # queries, 2 heads of keys, 2 of values, 4 more
+    q, k, v, out = (_view(x[:, a:b]) for a, b in ((0, 4), (4, 6), (6, 8), (first, first + 4)))
+    assert _status("oscar_append_rotated", _c_rotary(), FAKE, 0, 5, q, out, k, v, _c_cache(), FAKE, None) == status
