@@ -72,7 +72,7 @@ def append_rotated(query: torch.Tensor | None, key: torch.Tensor, value: torch.T
     without a query).  Rows are of the cache's type, with any token and head strides
     below 4 GiB; rows past the slots' count are not read.  Slots < 0 or past the cache are
     skipped, tokens with a position outside the table left out whole; slots of a
-    call are distinct."""
+    call are distinct.  For serving: no autograd graph is recorded."""
     if slot_mapping.ndim != 1 or slot_mapping.device != cache.device:
         raise ValueError("slot_mapping must be [tokens], on the cache's device")
     n, d, dtype, device = slot_mapping.shape[0], cache.head_size, cache.dtype, cache.device

@@ -109,7 +109,8 @@ def chunk_attention(query: torch.Tensor, cache: PagedCache, step: ChunkStep, sca
     step in row t) over the cache; returns [N, Hq, D] of that type, a new tensor
     or `out` (query itself or apart from it), whose rows past the step's tokens and of
     tokens of no request are not written.  scale must be positive.  Keys on pages outside the cache
-    are left out; a row that sees no key becomes zeros."""
+    are left out; a row that sees no key becomes zeros.  For serving: no autograd
+    graph is recorded."""
     device = cache.device
     if cache.geometry != step.geometry or device != step.device:
         raise ValueError("the step was built for another cache geometry or device")

@@ -6,7 +6,8 @@ text or on several (time, height, width) for image and video prompts.  The
 heads' first ``rotary_dim`` features turn in pairs by the cosines and sines of
 a table (one row per position, cosines first: the layout serving engines keep),
 in fp32 with one rounding; the rest pass through.  The map is orthogonal, so
-``inverse=True`` both takes positions off and gives the gradient.
+``inverse=True`` both takes positions off and gives the gradient, which autograd
+takes too.
 """
 from __future__ import annotations
 
@@ -149,10 +150,45 @@ def rotate(query: torch.Tensor, key: torch.Tensor | None, positions: torch.Tenso
            key_out=None, inverse: bool = False):
     """query [N, Hq, D] and key [N, Hk, D] (or None) turned by their positions
     (int64 [N], or [axes, N]), bf16, fp16 or fp32 alike, with any token and head
-    strides below 4 GiB.  Returns (query_out, key_out): new tensors, or the ones given, each its
-    own input as it stands or apart from all rows of the call; no autograd graph is recorded (the gradient is
-    the inverse of the outputs' gradients).  A token with a position outside the table is
-    left out: its output rows keep what they held."""
+    strides below 4 GiB.  Returns (query_out, key_out): new tensors, or the ones
+    given, each its own input as it stands or apart from all rows of the call.
+    New tensors carry a gradient to rows that require one (theirs, turned the
+    other way); a call with a given output records no autograd graph.  A token
+    with a position outside the table is left out: its output rows keep what they
+    held, and its inputs' gradient is zero."""
+    if ((query.requires_grad or (key is not None and key.requires_grad)) and torch.is_grad_enabled()
+            and query_out is None and key_out is None):
+        if key is not None and key.shape[0] > query.shape[0]:
+            key = key[:query.shape[0]]
+        return _Turned.apply(query, key, positions, rotary, inverse, False)
+    return _rotate(query, key, positions, rotary, query_out, key_out, inverse)
+
+
+class _Turned(torch.autograd.Function):
+    """rotate() into new tensors, zeros where a token is left out if `blank`.  Its
+    gradient is such a rotation the other way, itself with a gradient."""
+
+    @staticmethod
+    def forward(ctx, query, key, positions, rotary, inverse, blank):
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(positions)
+        ctx.back = (rotary, not inverse, True)
+        outs = [torch.zeros_like(x, memory_format=torch.contiguous_format) if blank and x is not None else None
+                for x in (query, key)]
+        return _rotate(query, key, positions, rotary, *outs, inverse)
+
+    @staticmethod
+    def backward(ctx, *grads):
+        positions, = ctx.saved_tensors
+        # (a sum's gradient is one number, expanded)
+        rows = [g if g.stride(-1) == 1 else g.contiguous()
+                for g, needed in zip(grads, ctx.needs_input_grad) if needed and g is not None]
+        turned = iter(_Turned.apply(*rows, *(None,) * (2 - len(rows)), positions, *ctx.back) if rows else ())
+        return (*(next(turned) if needed and g is not None else None
+                  for g, needed in zip(grads, ctx.needs_input_grad)), None, None, None, None)
+
+
+def _rotate(query, key, positions, rotary, query_out, key_out, inverse):
     dtype, device = query.dtype, query.device
     if dtype not in DTYPES:
         raise ValueError(f"rotate takes bf16, fp16 or fp32 rows, got {dtype}")

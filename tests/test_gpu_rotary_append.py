@@ -302,3 +302,87 @@ def test_outputs_among_the_calls_rows(device):
     assert torch.equal(x, before)
     rotary.rotate(x[:, :1], x[:, 1:2], pos, turn, query_out=x[:, :1], key_out=x[:, 1:2])
     assert torch.equal(x[:, :1], want[0]) and torch.equal(x[:, 1:2], want[1]) and torch.equal(x[:, 2], before[:, 2])
+
+
+@pytest.mark.parametrize("inverse", [False, True])
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_gradients_flow_through_rotate(device, dtype, inverse):
+    """Slices of a projection that requires a gradient: the formula's, turned the other
+    way and rounded once; none for tokens that are left out, nor for the values."""
+    g = torch.Generator(device=device).manual_seed(28)
+    axes = rotary.section_axes((6, 5, 5))
+    turn = rotary.Rotary(rotary.rotary_table(100, 32, device=device), axes=axes)
+    pos = torch.randint(0, 100, (3, 9), generator=g, device=device)
+    x = torch.randn(9, 5, 48, generator=g, device=device).to(dtype).requires_grad_()
+    w = torch.randn(9, 4, 48, generator=g, device=device).to(dtype)
+    q, k, _ = x.split((3, 1, 1), 1)
+    got = rotary.rotate(q, k, pos, turn, inverse=inverse)
+    plain = rotary.rotate(q.detach(), k.detach(), pos, turn, inverse=inverse)
+    assert all(torch.equal(a, b) and a.requires_grad and not b.requires_grad for a, b in zip(got, plain))
+    torch.autograd.backward(got, w.split((3, 1), 1))
+    close(x.grad[:, :4], turned(w, pos, turn, False, axes, inverse=not inverse))
+    assert (x.grad[:, 4] == 0).all()
+
+    pos[1, 2] = 100                                                     # left out: its rows give and get nothing
+    leaf = x.detach()[:, :4].clone().requires_grad_()
+    out = rotary.rotate(leaf, None, pos, turn, inverse=inverse)[0]
+    kept = torch.tensor([0, 1, 3, 4, 5, 6, 7, 8], device=device)
+    grad, = torch.autograd.grad(out, leaf, w)
+    y, bound = turned(w[kept], pos[:, kept], turn, False, axes, inverse=not inverse)
+    close(grad[kept], (y, bound))
+    assert (grad[2] == 0).all()
+
+
+def test_gradients_of_what_requires_them(device):
+    """Queries or keys alone, broadcast gradients, differences, second derivatives, none without grad mode or
+    into given tensors."""
+    g = torch.Generator(device=device).manual_seed(29)
+    turn = rotary.Rotary(rotary.rotary_table(100, 32, device=device), adjacent=True)
+    pos = torch.randint(0, 100, (7,), generator=g, device=device)
+    q, k = (torch.randn(7, h, 48, generator=g, device=device) for h in (2, 1))
+    ones = turned(torch.ones_like(q), pos, turn, True, None, inverse=True)
+    a = q.clone().requires_grad_()
+    out_q, out_k = rotary.rotate(a, k, pos, turn)
+    assert out_q.requires_grad
+    (out_q.sum() + out_k.sum()).backward()                               # (an expanded gradient)
+    close(a.grad, ones)
+    b = k.clone().requires_grad_()
+    rotary.rotate(q, b, pos, turn)[1].sum().backward()
+    close(b.grad, tuple(x[:, :1] for x in ones))
+    c, d = q.clone().requires_grad_(), k.clone().requires_grad_()
+    rotary.rotate(c, d, pos, turn)[0].sum().backward()                   # (the keys' output is not used)
+    close(c.grad, ones)
+    assert d.grad is None
+    e = torch.randn(9, 1, 48, generator=g, device=device).requires_grad_()      # (more key rows than queries)
+    rotary.rotate(q, e, pos, turn)[1].sum().backward()
+    close(e.grad[:7], tuple(x[:, :1] for x in ones))
+    assert (e.grad[7:] == 0).all()
+
+    # sum(rotate(x)^4) by differences of step h, in 64 bits; |x| <= 3, so |y| <= 4.3, and
+    # two outputs depend on an x.  Their third derivatives are 24 |y| <= 104 each: off by
+    # h^2 / 6 * 208.  Each y is off by 2^-23 * 6 + 2^-24 * 4.3 <= 2^-20, its fourth power by
+    # 4 |y|^3 2^-20 <= 2^-11.6, and four of them over 2 h by 2^-10.6 / h; the gradient, 8
+    # roundings of 4 |y|^3 twice, by 2^-24 * 8 * 640 = 2^-11.6
+    x = q.clamp(-3, 3).requires_grad_()
+    grad, = torch.autograd.grad((rotary.rotate(x, None, pos, turn)[0] ** 4).sum(), x, create_graph=True)
+    h = 2.0 ** -5
+    for at in ((0, 0, 0), (3, 1, 17), (6, 0, 31), (2, 1, 40)):
+        sums = []
+        for sign in (1, -1):
+            z = x.detach().clone()
+            z[at] += sign * h
+            sums.append((rotary.rotate(z, None, pos, turn)[0].double() ** 4).sum().item())
+        assert (sums[0] - sums[1]) / (2 * h) == pytest.approx(grad[at].item(), abs=h * h / 6 * 208 + 2.0 ** -10.6 / h + 2.0 ** -11)
+    # d/dx of sum(w grad): 12 rotate back(y^2 rotate(w)); u is off by 8 roundings, 2^-21 of
+    # the largest, and two of them make a value
+    w = torch.randn(q.shape, generator=g, device=device)
+    second, = torch.autograd.grad((grad * w).sum(), x)
+    y = rotary.rotate(x.detach(), None, pos, turn)[0].double()
+    u = (12 * y ** 2 * rotary.rotate(w, None, pos, turn)[0].double()).float()
+    want, bound = turned(u, pos, turn, True, None, inverse=True)
+    close(second, (want, bound + 2.0 ** -20 * u.abs().amax().item()))
+
+    with torch.no_grad():
+        assert not rotary.rotate(a, b, pos, turn)[0].requires_grad
+    into = torch.empty_like(q)
+    assert not rotary.rotate(a, None, pos, turn, query_out=into)[0].requires_grad
