@@ -38,10 +38,15 @@ class ChunkStep:
 
     qsl [requests + 1] and seqs [requests] are host lists (query starts from the
     step's token 0; keys after the step); block_tables of integers
-    [requests, pages] on the cache's device.  A step is not built under graph capture; a captured call
-    keeps this step's lengths and needs the step to live as long as the graph; the
-    block table is read at every call and replay where it is int32 with rows of
-    their own, and else copied here."""
+    [requests, pages] on the cache's device.  The block table is read at every call
+    and replay where it is int32 with rows of their own, and else copied here.
+
+    Building copies the step's arrays to the device on the current stream; calls
+    on other streams wait for that by themselves.  A step is not built under graph
+    capture.  A captured call keeps this step's lengths and needs the step to live
+    as long as the graph, and its replays to come after that copy: torch.cuda.graph
+    sees to it (it waits for the device before it captures), and a capture begun in
+    another way has to, by a wait of its stream for the one the step was built on."""
 
     def __init__(self, qsl, seqs, block_tables: torch.Tensor, num_heads: int, cache: PagedCache, window: int = 0):
         layout = decode.request_layout(qsl, seqs)
@@ -98,7 +103,7 @@ class ChunkStep:
     def _join(self, device) -> None:
         """Order this step's arrays before the current stream, which is not the one it was built on."""
         stream = torch.cuda.current_stream(device)
-        if not torch.cuda.is_current_stream_capturing():        # (a capture begins with the device idle)
+        if not torch.cuda.is_current_stream_capturing():        # (a captured stream cannot wait for another's event)
             stream.wait_event(self.ready)
         self.items.record_stream(stream)
         self.block_tables.record_stream(stream)

@@ -570,3 +570,33 @@ def test_outputs_that_overlap_the_queries_are_refused(device):
     assert torch.equal(x[:40, :4], q)
     assert torch.equal(chunk.chunk_attention(x[:40, :4], cache, step, 0.125, out=x[:40, 4:]), want)
     assert torch.equal(chunk.chunk_attention(x[:40, :4], cache, step, 0.125, out=x[:40, :4]), want)
+
+
+@pytest.mark.parametrize("kind", ["int32", "int64"])
+def test_a_capture_that_waits_for_the_step(device, kind):
+    """A step built on one stream just before another one, which waits for it, begins
+    to capture a call by hand; replays there and on the first stream."""
+    g = torch.Generator(device=device).manual_seed(31)
+    q, caches, table, starts, seqs = make(g, [(4, 5000), (100, 900)], 6, 1, 128, 128, torch.bfloat16)
+    table = table.to(getattr(torch, kind))
+    cache = append.PagedCache(*caches)
+    want = chunk.chunk_attention(q, cache, chunk.ChunkStep(starts, seqs, table, 6, cache), 0.1)
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    big = torch.ones(1 << 28, device=device)
+    for _ in range(10):
+        big.mul_(1.0)                       # (a millisecond and more of other work ahead of the copy)
+    step = chunk.ChunkStep(starts, seqs, table, 6, cache)
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        graph.capture_begin()
+        out = chunk.chunk_attention(q, cache, step, 0.1)
+        graph.capture_end()
+        graph.replay()
+    side.synchronize()
+    assert torch.equal(out, want)
+    for _ in range(2):
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
