@@ -19,6 +19,15 @@
 // The work is cut on the host into pieces (a 32-row tile of a request and kv
 // head, or a wide one, over a range of keys) that fill the GPU; a row tile in
 // several pieces leaves fp32 partials that a second launch joins.
+//
+// The matrix unit takes both operands in one type, so the weights are rounded to the
+// cache's (off by 2^-8 of each at most in bf16, 2^-11 in fp16, as the output is by its
+// own rounding) and summed as rounded: what remains is a mean with weights off by so
+// much.  Scores, maxima, sums and partials are fp32.
+//
+// Times under "Measured" are of these kernels, with their spread between cards.
+// Where two ways are set against each other, both were timed in turn on one card,
+// with the rest of the kernels as it then was.
 #include "plain_cache.h"
 #include "row_span.h"
 
@@ -418,10 +427,10 @@ __device__ __forceinline__ uint8_t* out_row(const ChunkArgs& a, int token0, int 
 // score tile is then the lower one's again and not used), so that two workgroups
 // fit a CU's LDS; alone, few keys take longer with those (one token over 256 keys 8.7
 // us, 8.0 with 32; 32 users' 4 tokens over 2K to 16K 55 with either).
-// Measured: 8 users' token over 32K keys (D = 256) 48.5 us, 5.5 TB/s (a large copy
-// moves 5.05); 32 users' 4 tokens over 2K to 16K 55 us, 5.3 TB/s.  One user's over 1K
-// takes 7.4 us and 3.6 of join: three memory round trips (piece, page, keys) and one
-// for each of a wave's tiles.
+// Measured: 8 users' token over 32K keys (D = 256) 48 us, 5.6 TB/s (a large copy
+// moves 5.1, reading alone reaches 6.2 to 6.5); 32 users' 4 tokens over 2K to 16K 55
+// us, 5.3 TB/s.  One user's over 1K takes 7.3 us and 3 of join: three memory round
+// trips (piece, page, keys) and one for each of a wave's tiles.
 constexpr int beside_keys(int d) { return d == 256 ? 16 : 32; }
 constexpr int narrow_lds(int d, int keys) { return kWaves * 2 * keys * 2 * d + kWaves * 2 * kTileRows * 4; }
 
@@ -607,10 +616,11 @@ __device__ __forceinline__ void narrow_piece(const ChunkArgs& a, const Piece p, 
 // written out: the compiler's own spills registers to memory.
 // What bounds it: the matrix unit together with the vector instructions of the
 // softmax (and, at D = 64, those alone: 16 exponentials a lane against 8 products),
-// at the clock the power limit leaves (1.75 GHz in the longest cases).  Measured:
-// D = 256, 6 heads on one, 9256 tokens over 15360 keys 1081 us, 1.05 PFLOP/s; D = 128,
-// 32 on 8, 8192 over 8192 1443 us, 1.14; D = 64, 16 on 4, 8192 over 8192 412 us, 1.0
-// (a large bf16 matrix product: 1.38).
+// at the clock the power limit leaves (1.6 GHz in the longest cases).  Measured:
+// D = 256, 6 heads on one, 9256 tokens over 15360 keys 960 to 1120 us, 1.0 to 1.19
+// PFLOP/s; D = 128, 32 on 8, 8192 over 8192 1440 to 1550 us, 1.06 to 1.14; D = 64, 16
+// on 4, 8192 over 8192 410 to 435 us, 0.95 to 1.0 (a large bf16 matrix product: 1.34
+// to 1.38).
 constexpr int kWideRows = 32 * kWaves;
 constexpr int kWideWgs = 2;                                      // workgroups a CU
 constexpr int stage_tiles(int d) { return d == 256 ? 1 : 2; }    // 32-key tiles of a stage
@@ -713,9 +723,8 @@ __device__ __forceinline__ void wide_piece(const ChunkArgs& a, const Piece p, ui
   // 45.5; 9256 over 15360, D = 256, 1127 / 1104).
   constexpr bool kSumFirst = D == 128;
   auto sum = [](const V8 (&w)[2]) { return Num<T>::sum8(w[0], 0.f) + Num<T>::sum8(w[1], 0.f); };
-  // Positive numbers compare as
-  // their bits do, so this takes nine operations for a tile, where the maximum of
-  // the scores takes one for each.
+  // Positive numbers compare as their bits do, so this takes nine operations for a
+  // tile, where the maximum of the scores takes one for each.
   auto beyond = [&](const V8 (&w)[2]) {
     const ushortx8 u = __builtin_elementwise_max(__builtin_bit_cast(ushortx8, w[0]), __builtin_bit_cast(ushortx8, w[1]));
     const ushortx2 top = __builtin_elementwise_max(
@@ -886,8 +895,9 @@ __global__ __launch_bounds__(kThreads, kWideWgs) void wide_kernel(ChunkArgs a) {
 // A step with both.  Narrow pieces that fill the GPU come after the wide ones, where
 // those leave room: reads at full rate leave the wide pieces' next stage late.  A few
 // (plan_narrow) come first, and read for as long as the wide ones compute.  1024
-// tokens over 4096 beside seven users' 4, D = 128, 119 us: the wide ones alone take
-// 90, the narrow ones alone 38; D = 256 71 us (the wide ones first 83).
+// tokens over 4096 beside seven users' 4, D = 256: 71 us, the wide ones first 83.
+// Measured: D = 128 119 to 133 us; the wide ones alone take 90 to 102, the narrow ones
+// alone 38.
 constexpr int kFewNarrow = kCus;
 constexpr int mixed_lds(int d) { return std::max(narrow_lds(d, beside_keys(d)), wide_lds(d)); }
 template <typename T, int D>
@@ -905,7 +915,7 @@ __global__ __launch_bounds__(kThreads, kWideWgs) void mixed_kernel(ChunkArgs a) 
 // more: a workgroup to 64 features of a row, 16 threads across the features and
 // 16 across the partials, whose sums meet in LDS.  (Few up to 8: 2048 tokens beside
 // 16 users' 4, D = 256, 180 us, up to 4 203, up to 16 183.)  The partials' bytes bound
-// it (512 wide pieces of D = 128: 43 MB, 9.8 us), or, where there is little, latency:
+// it (512 wide pieces of D = 128: 43 MB, 9.7 us), or, where there is little, latency:
 // 2.3 to 5 us.
 constexpr int kFewParts = 8;
 
@@ -1049,20 +1059,27 @@ void cut(const RowTile& x, int32_t n, Plan& plan, std::vector<Piece>& out) {
 
 int32_t pieces_of(const RowTile& x, int64_t per) { return (int32_t)((x.tiles + per - 1) / per); }
 
-// Narrow tiles: the fewest key tiles a piece with which there is a piece a CU, or,
-// where that leaves the longest piece a seventh above the mean, as many pieces as
-// reside at once (D = 128: 8 users' 4 tokens over 4000 keys, 8 kv heads, a piece a CU
-// 27.3 us, two 28.7, 4 users' over 2048 10.4, 12.8; 24 users' over 100 to 16200 a piece
-// a CU 166 us, two 140).  Where the longest row tile is short, all stay whole, and
-// there is no second launch: one token of one user over 256 keys, D = 256, whole 7.9 us
-// of GPU time, cut 8.3 (over 512: 10.9, 8.3); D = 128, 8 kv heads, over 512 whole 7.2,
-// cut 7.1 and 6.2 against 10.6 where the host launches (over 1024: 11.1, 7.0).
+// Narrow tiles: the fewest key tiles a piece, one number for all row tiles, with which
+// there is a piece a CU at most, or, where that leaves the longest piece a seventh
+// above the mean, as many pieces as reside at once (D = 128: 8 users' 4 tokens over
+// 4000 keys, 8 kv heads, a piece a CU 27.3 us, two 28.7, 4 users' over 2048 10.4, 12.8;
+// 24 users' over 100 to 16200 a piece a CU 166 us, two 140).  Where the longest row
+// tile is short, all stay whole, and there is no second launch: one token of one user
+// over 256 keys, D = 256, whole 7.9 us of GPU time, cut 8.3 (over 512: 10.9, 8.3); D =
+// 128, 8 kv heads, over 512 whole 7.2, cut 7.1 and 6.2 against 10.6 where the host
+// launches (over 1024: 11.1, 7.0).
 // Beside wide tiles that take at least two thirds of the reading's time (`beside`, in
 // their units, of which a narrow tile's 128 D bytes at 5.2 TB/s are 1/160), two narrow
 // workgroups to three CUs (16 users over 8000 keys beside two prompts, D = 256: 37 to
 // 45 us, two a CU 43 to 55; 12 over 2000 beside 512 tokens, D = 128: 30, 35); where the
 // reading takes longer, two a CU (16 over 8000 beside two prompts, D = 128: 107 us, two
 // to three CUs 128).
+// So row tiles are cut only as far as there are fewer of them than that many pieces:
+// where there are as many or more, all stay whole, in the order of the requests.  That
+// is right for even lengths, and for ragged ones (256 users of 100 to 8000 keys, D =
+// 256, 190 us, 5.2 TB/s), but one request that is far longer than the others is then
+// read by one workgroup (300 users of 1000 keys and one of 131072 2.2 ms, where the
+// bytes take 0.09), and by a few where there are just fewer (250 and one: 0.39 ms).
 void plan_narrow(const std::vector<RowTile>& rows, int32_t head_size, double beside, Plan& plan) {
   int64_t total = 0;
   int32_t most = 0;
@@ -1107,6 +1124,10 @@ void plan_narrow(const std::vector<RowTile>& rows, int32_t head_size, double bes
 //   D = 128, 32 heads: 1024 over 4096 111 / 88, 8 prompts of 300 over 500 50 / 70;
 //   D = 64, 16 heads: 8192 over 8192 412 / 425, 1024 over 1024 37 / 23, 6000 + 1501
 //   tokens in a window of 1024 45 / 59.
+// Cuts are tried while their number times all row tiles stays within kMostPieces, also
+// where only some row tiles are long enough to be cut: beside many short prompts a
+// chunk over a long cache stays whole (8 prompts of 512 beside 64 tokens over 32768,
+// D = 128, 640 us, where the keys take 43).
 // Returns the estimate.
 constexpr int32_t kPieceCost = 4, kCutCost = 15, kLeastPiece = 8, kMostPieces = 2048;
 double plan_wide(const std::vector<RowTile>& rows, int32_t head_size, Plan& plan) {
@@ -1296,7 +1317,8 @@ extern "C" int oscar_chunk_attention(const oscar_chunk_step* step, const void* i
       std::min({a.q_token, a.q_head, a.out_token, a.out_head}) < 0)
     return kErrUnsupportedGeometry;
   // (a row is read by the workgroup that writes it, or by a launch before the one that does)
-  const RowSpan from{(uint64_t)(uintptr_t)a.q, a.q_token, a.q_head, step->num_tokens, step->num_heads, 2 * cache->head_size};
+  const RowSpan from{(uint64_t)(uintptr_t)a.q, a.q_token, a.q_head, step->num_tokens, step->num_heads,
+                     2 * cache->head_size};
   const RowSpan to{(uint64_t)(uintptr_t)a.out, a.out_token, a.out_head, step->num_tokens, step->num_heads,
                    2 * cache->head_size};
   if (!same_rows(from, to) && !rows_apart(from, to)) return kErrOverlap;
