@@ -247,7 +247,8 @@ def test_more_heads_than_the_plan_takes_are_refused(heads, match):
         chunk.ChunkStep([0, 4], [9], torch.zeros(1, 1, dtype=torch.int32), heads, plain_cache())
 
 
-@pytest.mark.parametrize("short, long, pieces", [(254, 1 << 30, 2), (250, 1 << 20, 6), (255, 1 << 20, 1), (100, 1 << 25, 156)])
+@pytest.mark.parametrize("short, long, pieces", [(254, 1 << 30, 2), (250, 1 << 20, 6), (255, 1 << 20, 1),
+                                                 (100, 1 << 25, 156)])
 def test_one_long_row_among_short_ones_is_planned_at_once(short, long, pieces):
     """The fewest key tiles a piece with which there are at most 256 pieces (one wide
     cache head of 256 features), found in time that does not go by the keys: 50 us each

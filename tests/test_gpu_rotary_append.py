@@ -334,8 +334,8 @@ def test_gradients_flow_through_rotate(device, dtype, inverse):
 
 
 def test_gradients_of_what_requires_them(device):
-    """Queries or keys alone, broadcast gradients, differences, second derivatives, none without grad mode or
-    into given tensors."""
+    """Queries or keys alone, broadcast gradients, differences, second derivatives;
+    none without grad mode or into given tensors."""
     g = torch.Generator(device=device).manual_seed(29)
     turn = rotary.Rotary(rotary.rotary_table(100, 32, device=device), adjacent=True)
     pos = torch.randint(0, 100, (7,), generator=g, device=device)
@@ -372,7 +372,8 @@ def test_gradients_of_what_requires_them(device):
             z = x.detach().clone()
             z[at] += sign * h
             sums.append((rotary.rotate(z, None, pos, turn)[0].double() ** 4).sum().item())
-        assert (sums[0] - sums[1]) / (2 * h) == pytest.approx(grad[at].item(), abs=h * h / 6 * 208 + 2.0 ** -10.6 / h + 2.0 ** -11)
+        off = h * h / 6 * 208 + 2.0 ** -10.6 / h + 2.0 ** -11
+        assert (sums[0] - sums[1]) / (2 * h) == pytest.approx(grad[at].item(), abs=off)
     # d/dx of sum(w grad): 12 rotate back(y^2 rotate(w)); u is off by 8 roundings, 2^-21 of
     # the largest, and two of them make a value
     w = torch.randn(q.shape, generator=g, device=device)
@@ -386,3 +387,29 @@ def test_gradients_of_what_requires_them(device):
         assert not rotary.rotate(a, b, pos, turn)[0].requires_grad
     into = torch.empty_like(q)
     assert not rotary.rotate(a, None, pos, turn, query_out=into)[0].requires_grad
+
+
+def test_a_captured_gradient(device):
+    """Rotation and gradient in one graph; rows, gradient and positions change between replays."""
+    g = torch.Generator(device=device).manual_seed(32)
+    turn = rotary.Rotary(rotary.rotary_table(100, 64, device=device))
+    x = torch.randn(33, 4, 64, generator=g, device=device).bfloat16().requires_grad_()
+    w = torch.randn(33, 4, 64, generator=g, device=device).bfloat16()
+    pos = torch.arange(33, device=device)
+    rotary.rotate(w, None, pos, turn)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = rotary.rotate(x, None, pos, turn)[0]
+        grad, = torch.autograd.grad(out, x, w)
+    for last in (32, 99, 100):                                          # (100: left out, no gradient)
+        with torch.no_grad():
+            x.copy_(torch.randn(x.shape, generator=g, device=device))
+            w.copy_(torch.randn(x.shape, generator=g, device=device))
+            pos[32] = last
+        graph.replay()
+        torch.cuda.synchronize()
+        want = torch.zeros_like(w)
+        rotary.rotate(w, None, pos, turn, query_out=want, inverse=True)
+        assert torch.equal(grad, want)
+        assert torch.equal(out[:32], rotary.rotate(x.detach(), None, pos, turn)[0][:32])
+        assert (grad[32] == 0).all() == (last == 100)

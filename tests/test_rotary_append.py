@@ -305,8 +305,8 @@ def test_rows_that_share_memory_never_count_as_apart():
         heads = rng.choice((1, 2, 4))
         x, y = (store.as_strided((tokens, heads, d), (*strides[2 * i:2 * i + 2], 1), rng.randint(0, 60))
                 for i in range(2))
-        same = all(a == b for a, b, n in zip((x.data_ptr(), *x.stride()), (y.data_ptr(), *y.stride()), (9, tokens, heads))
-                   if n > 1)
+        same = all(a == b for a, b, n in zip((x.data_ptr(), *x.stride()), (y.data_ptr(), *y.stride()),
+                                             (9, tokens, heads)) if n > 1)
         truth, status = not _memory(x) & _memory(y), _rotate_views(x, y)
         assert status in (OVERLAP, LAUNCHED) and (status == OVERLAP or truth or same)
         passed, apart = passed + (status == LAUNCHED and not same), apart + truth
