@@ -455,7 +455,7 @@ def _quantise(x, kind):
     e = torch.where(mantissa > 0.875, exponent - 8, exponent - 9)           # 448 = 0.875 * 2^9
     e = torch.where(mantissa == 0, low, e).clamp(low, high)
     scaled = x * _power(-e)
-    most = torch.where(e == high, 240.0, 448.0)                             # (the next code would pass the type's largest)
+    most = torch.where(e == high, 240.0, 448.0)     # (the next code would pass the type's largest)
     return torch.minimum(torch.maximum(scaled, -most), most).to(torch.float8_e4m3fn), (e[..., 0] + 127).to(torch.uint8)
 
 
@@ -490,8 +490,8 @@ def _plain_attention(state):
         at = torch.arange(low, seq, device=q.device)
         pages = state["table"][i, at // page].long()
         if case["bits"] == 8:
-            keys, values = (_plain_values(x.view(torch.uint8)[pages, at % page], state["cache"][2][pages, :, at % page, n])
-                            for n, x in enumerate(state["cache"][:2]))
+            keys, values = (_plain_values(state["cache"][n].view(torch.uint8)[pages, at % page],
+                                          state["cache"][2][pages, :, at % page, n]) for n in range(2))
         else:
             keys, values = (x[pages, at % page].float() for x in state["cache"])
         keys, values = keys.permute(1, 2, 0).contiguous(), values.transpose(0, 1).contiguous()
