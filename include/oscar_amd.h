@@ -592,6 +592,88 @@ int oscar_append_rotated(const oscar_rotary* rotary, const int64_t* positions, i
                          const oscar_heads* key, const oscar_heads* value, const oscar_plain_cache* cache,
                          const int64_t* slot_mapping, oscar_stream_t stream);
 
+/* ---------------------------------------------------------------- normed heads
+ * Norms of query and key heads before their positions:
+ *   y = R(p) [x / sqrt(sum x^2 / head_size + eps) * (weight + offset)],
+ * in fp32, rounded once to the rows' type.  Weights: [head_size] of weight_dtype
+ * (any oscar_dtype), one for all query heads and one for all key heads; null: that
+ * kind is turned without a norm. */
+typedef struct oscar_head_norm {
+  const void* query_weight;
+  const void* key_weight;
+  int32_t weight_dtype; /* oscar_dtype, of both */
+  float eps;            /* not negative */
+  float offset;         /* 0, or 1 for weights that are kept around zero */
+  int32_t reserved;     /* 0 */
+} oscar_head_norm;
+
+/* oscar_rotate_positions with norms before it: the same rows, positions, outputs
+ * and refusals. */
+int oscar_norm_rotate(const oscar_rotary* rotary, const oscar_head_norm* norm, const int64_t* positions,
+                      int64_t position_axis_stride, int64_t num_tokens, const oscar_heads* query,
+                      const oscar_heads* query_out, const oscar_heads* key, const oscar_heads* key_out,
+                      int32_t head_size, int32_t dtype, oscar_stream_t stream);
+
+/* Its gradient: query_grad and key_grad (null: not asked for) from the inputs and the
+ * outputs' gradients, and the weights' (of weight_dtype, null: not asked for).
+ * Gradients written are apart from all other rows.  A token that the forward leaves
+ * out has a gradient of zero.  workspace, for the weights' alone: 4-byte aligned, >=
+ * oscar_norm_rotate_backward_workspace_bytes(...) bytes.  Sums are of fixed order. */
+size_t oscar_norm_rotate_backward_workspace_bytes(int64_t num_tokens, int32_t head_size);
+int oscar_norm_rotate_backward(const oscar_rotary* rotary, const oscar_head_norm* norm, const int64_t* positions,
+                               int64_t position_axis_stride, int64_t num_tokens, const oscar_heads* query,
+                               const oscar_heads* query_out_grad, const oscar_heads* query_grad,
+                               const oscar_heads* key, const oscar_heads* key_out_grad, const oscar_heads* key_grad,
+                               void* query_weight_grad, void* key_weight_grad, int32_t head_size, int32_t dtype,
+                               void* workspace, size_t workspace_size, oscar_stream_t stream);
+
+/* oscar_append_rotated with norms before the rotation. */
+int oscar_append_normed(const oscar_rotary* rotary, const oscar_head_norm* norm, const int64_t* positions,
+                        int64_t position_axis_stride, int64_t num_tokens, const oscar_heads* query,
+                        const oscar_heads* query_out, const oscar_heads* key, const oscar_heads* value,
+                        const oscar_plain_cache* cache, const int64_t* slot_mapping, oscar_stream_t stream);
+
+/* ---------------------------------------------------------------- 8-bit paged caches
+ * K and V pages of one byte a value: code f of head h of token t of page p lies at
+ * byte p * stride_page + t * stride_token + h * stride_head + f, an e4m3 number, and
+ * stands for code * 2^(b - 127), b the byte at exponents[((p * num_kv_heads + h) *
+ * block_size + t) * 2], of V the byte after it.  Base addresses and strides are
+ * multiples of 16 bytes and tokens and heads do not overlap; head_size is a multiple
+ * of 16, at most 256.  dtype: of the rows that are written and read (bf16 or fp16). */
+typedef struct oscar_quant_cache {
+  void* k;
+  void* v;
+  uint8_t* exponents;
+  int64_t num_pages;
+  int64_t k_stride_page;
+  int64_t k_stride_token;
+  int64_t k_stride_head;
+  int64_t v_stride_page;
+  int64_t v_stride_token;
+  int64_t v_stride_head;
+  int32_t block_size;
+  int32_t num_kv_heads;
+  int32_t head_size;
+  int32_t dtype; /* oscar_dtype */
+} oscar_quant_cache;
+
+/* The write of a step's keys and values to such a cache: oscar_append_normed's
+ * arguments, keys and values rounded to codes (to nearest, ties to even).  A row's
+ * power of two is the smallest, of 2^-80 .. 2^100 (bf16) or 2^-15 .. 2^8 (fp16), with
+ * which its largest finite magnitude is at most 448 times it; smaller values than the
+ * least power reaches round to zero, larger ones than the greatest reaches become 240
+ * times it; infinities and NaN become NaN. */
+int oscar_append_quantized(const oscar_rotary* rotary, const oscar_head_norm* norm, const int64_t* positions,
+                           int64_t position_axis_stride, int64_t num_tokens, const oscar_heads* query,
+                           const oscar_heads* query_out, const oscar_heads* key, const oscar_heads* value,
+                           const oscar_quant_cache* cache, const int64_t* slot_mapping, oscar_stream_t stream);
+
+/* Rows of given slots as the values they stand for, exactly, in the cache's type or
+ * fp32.  slots: [num_tokens] int64; those < 0 or past the cache give zeros.
+ * key_out, value_out: 16-byte aligned rows, strides not negative, apart. */
+int oscar_read_back(const oscar_quant_cache* cache, const int64_t* slots, int64_t num_tokens,
+                    const oscar_heads* key_out, const oscar_heads* value_out, int32_t dtype, oscar_stream_t stream);
+
 /* ---------------------------------------------------------------- chunk attention over a plain cache
  * Causal attention of a step's new tokens over a plain paged cache that holds
  * their keys and values already (oscar_append_rotated's).  Token j of request

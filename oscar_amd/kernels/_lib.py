@@ -85,6 +85,13 @@ SIGNATURES = {
     "oscar_rotate_positions": (_c_i32, [_c_p, _c_p, _c_i64, _c_i64, _c_p, _c_p, _c_p, _c_p, _c_i32, _c_i32, _c_i32,
                                         _c_p]),
     "oscar_append_rotated": (_c_i32, [_c_p, _c_p, _c_i64, _c_i64, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p]),
+    "oscar_norm_rotate": (_c_i32, [_c_p, _c_p, _c_p, _c_i64, _c_i64, _c_p, _c_p, _c_p, _c_p, _c_i32, _c_i32, _c_p]),
+    "oscar_norm_rotate_backward_workspace_bytes": (_c_sz, [_c_i64, _c_i32]),
+    "oscar_norm_rotate_backward": (_c_i32, [_c_p, _c_p, _c_p, _c_i64, _c_i64, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p,
+                                            _c_p, _c_i32, _c_i32, _c_p, _c_sz, _c_p]),
+    "oscar_append_normed": (_c_i32, [_c_p, _c_p, _c_p, _c_i64, _c_i64, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p]),
+    "oscar_append_quantized": (_c_i32, [_c_p, _c_p, _c_p, _c_i64, _c_i64, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p]),
+    "oscar_read_back": (_c_i32, [_c_p, _c_p, _c_i64, _c_p, _c_p, _c_i32, _c_p]),
     "oscar_chunk_plan": (_c_i32, [_c_p, _c_p, _c_i32, _c_i32, _c_i32, _c_p, _c_p, _c_sz, _c_p]),
     "oscar_chunk_attention": (_c_i32, [_c_p, _c_p, _c_p, _c_i64, _c_p, _c_p, _c_p, _c_f32, _c_p, _c_sz, _c_p]),
 }

@@ -1,4 +1,5 @@
-"""Position rotation of query and key heads (oscar_rotate_positions).
+"""Position rotation of query and key heads (oscar_rotate_positions), and their
+norms with it (oscar_norm_rotate).
 
 The INT2 write and the attention impl take queries and keys that already carry
 their positions; this is the rotation that puts them there, on one axis for
@@ -7,7 +8,8 @@ heads' first ``rotary_dim`` features turn in pairs by the cosines and sines of
 a table (one row per position, cosines first: the layout serving engines keep),
 in fp32 with one rounding; the rest pass through.  The map is orthogonal, so
 ``inverse=True`` both takes positions off and gives the gradient, which autograd
-takes too.
+takes too.  Models that norm each head before its position have both in one pass
+(``norm_rotate``), the gradients of heads and weights too.
 """
 from __future__ import annotations
 
@@ -215,4 +217,126 @@ def _rotate(query, key, positions, rotary, query_out, key_out, inverse):
     if n:
         _lib.call_on(device, "oscar_rotate_positions", rotary.address, positions.data_ptr(), axis_stride, n, q, qo, k,
                      ko, d, DTYPES[dtype], int(inverse))
+    return query_out, key_out if key is not None else None
+
+
+# struct oscar_head_norm
+_pack_norm = struct.Struct("@PPiffi").pack
+MAX_FLOAT = 3.0e38
+
+
+def pack_norm(query_weight, key_weight, eps: float, offset: float, d: int, device) -> bytes:
+    """struct oscar_head_norm of weights [d] (None: that kind has no norm)."""
+    if not 0.0 <= eps < MAX_FLOAT or not -MAX_FLOAT < offset < MAX_FLOAT:
+        raise ValueError("eps must be finite and not negative, the offset finite")
+    dtype, at = None, [0, 0]
+    for i, (w, what) in enumerate(((query_weight, "query_weight"), (key_weight, "key_weight"))):
+        if w is None:
+            continue
+        if w.shape != (d,) or w.dtype not in DTYPES or w.device != device or (d > 1 and w.stride(0) != 1):
+            raise ValueError(f"{what} must be a contiguous bf16, fp16 or fp32 [{d}] tensor on the rows' device")
+        if dtype is not None and w.dtype is not dtype:
+            raise ValueError("query_weight and key_weight must be of one type")
+        dtype, at[i] = w.dtype, w.data_ptr()
+    return _pack_norm(*at, DTYPES[dtype] if dtype is not None else 0, eps, offset, 0)
+
+
+def norm_rotate(query: torch.Tensor, key: torch.Tensor | None, query_weight: torch.Tensor,
+                key_weight: torch.Tensor | None, positions: torch.Tensor, rotary: Rotary, eps: float = 1e-6,
+                offset: float = 0.0, query_out=None, key_out=None):
+    """query [N, Hq, D] and key [N, Hk, D] (or None), each head normed and then turned
+    by its token's position:
+      x / sqrt(mean x^2 + eps) * (weight + offset), through ``rotate``,
+    in fp32 with one rounding.  Weights are [D] of one type (bf16, fp16 or fp32), one
+    for all query heads and one for all key heads; offset 1 is for models that keep
+    them around zero.  Rows, positions and outputs are as ``rotate`` takes them.  New
+    tensors carry a gradient to rows and weights that require one (a single time); a
+    call with a given output records no autograd graph.  A token with a position
+    outside the table is left out: its output rows keep what they held, and it adds
+    nothing to a gradient."""
+    if query_weight is None or (key is not None and key_weight is None):
+        raise ValueError("norm_rotate takes a weight for queries, and for keys where they are given")
+    if key is None:
+        key_weight = None
+    leaves = [x for x in (query, key, query_weight, key_weight) if x is not None]
+    if (torch.is_grad_enabled() and any(x.requires_grad for x in leaves) and query_out is None and key_out is None):
+        if key is not None and key.shape[0] > query.shape[0]:
+            key = key[:query.shape[0]]
+        return _Normed.apply(query, key, query_weight, key_weight, positions, rotary, eps, offset)
+    return _norm_rotate(query, key, query_weight, key_weight, positions, rotary, eps, offset, query_out, key_out)
+
+
+class _Normed(torch.autograd.Function):
+    """norm_rotate() into new tensors."""
+
+    @staticmethod
+    def forward(ctx, query, key, query_weight, key_weight, positions, rotary, eps, offset):
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(query, key, query_weight, key_weight, positions)
+        ctx.settings = rotary, eps, offset
+        return _norm_rotate(query, key, query_weight, key_weight, positions, rotary, eps, offset, None, None)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, *grads):
+        query, key, query_weight, key_weight, positions = ctx.saved_tensors
+        rotary, eps, offset = ctx.settings
+        n, _, d = query.shape
+        device = query.device
+        if n == 0:
+            leaves = (query, key, query_weight, key_weight)
+            return (*(torch.zeros_like(x) if needed else None for x, needed in zip(leaves, ctx.needs_input_grad)),
+                    None, None, None, None)
+        rows, back, weights, held = [], [None, None], [None, None], []
+        for i, (x, w, g) in enumerate(((query, query_weight, grads[0]), (key, key_weight, grads[1]))):
+            if g is None or not (ctx.needs_input_grad[i] or ctx.needs_input_grad[2 + i]):
+                rows += [None, None, None]
+                continue
+            if g.stride(-1) != 1:           # (a sum's gradient is one number, expanded)
+                g = g.contiguous()
+            held.append(g)                  # (until the call: rows are addresses)
+            rows += [heads(x, n, d, x.dtype, device, "rows")[0], heads(g, n, d, x.dtype, device, "gradient")[0], None]
+            if ctx.needs_input_grad[i]:
+                back[i], rows[-1] = new_heads(x, n, x.shape[1], d)
+            if ctx.needs_input_grad[2 + i]:
+                weights[i] = torch.empty_like(w)
+        if any(x is not None for x in rows):
+            positions, axis_stride = positions_of(positions, rotary, n, device)
+            need = (_lib.load().oscar_norm_rotate_backward_workspace_bytes(n, d)
+                    if any(w is not None for w in weights) else 0)
+            ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+            _lib.call_on(device, "oscar_norm_rotate_backward", rotary.address,
+                         pack_norm(query_weight, key_weight, eps, offset, d, device), positions.data_ptr(), axis_stride,
+                         n, *rows, *(_lib.ptr(w) for w in weights), d, DTYPES[query.dtype], _lib.ptr(ws), need)
+        return (*back, *weights, None, None, None, None)
+
+
+def _norm_rotate(query, key, query_weight, key_weight, positions, rotary, eps, offset, query_out, key_out):
+    dtype, device = query.dtype, query.device
+    if dtype not in DTYPES:
+        raise ValueError(f"norm_rotate takes bf16, fp16 or fp32 rows, got {dtype}")
+    if query.ndim != 3:
+        raise ValueError("query must be [tokens, heads, head size]")
+    n, _, d = query.shape
+    if d < rotary.rotary_dim or d % 2 or d > 256:
+        raise ValueError(f"head size {d} must be even, {rotary.rotary_dim} (rotary_dim) to 256")
+    norm = pack_norm(query_weight, key_weight, eps, offset, d, device)
+    q, hq = heads(query, n, d, dtype, device, "query")
+    if query_out is None:
+        query_out, qo = new_heads(query, n, hq, d)
+    else:
+        qo = out_heads(query_out, n, hq, d, dtype, device, "query_out")
+    k = ko = None
+    if key is not None:
+        k, hk = heads(key, n, d, dtype, device, "key")
+        if key_out is None:
+            key_out, ko = new_heads(key, n, hk, d)
+        else:
+            ko = out_heads(key_out, n, hk, d, dtype, device, "key_out")
+    positions, axis_stride = positions_of(positions, rotary, n, device)
+    if not query.is_cuda:
+        raise ValueError("OSCAR kernels take device tensors")
+    if n:
+        _lib.call_on(device, "oscar_norm_rotate", rotary.address, norm, positions.data_ptr(), axis_stride, n, q, qo, k,
+                     ko, d, DTYPES[dtype])
     return query_out, key_out if key is not None else None
