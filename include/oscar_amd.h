@@ -714,11 +714,27 @@ typedef struct oscar_chunk_step {
   int32_t block_size;
   int64_t items_size;
   int64_t workspace_size;
+  int32_t parts; /* joins of rows that share a prefix */
+  int32_t reserved;
 } oscar_chunk_step;
+
+/* Keys [0, keys) that requests first .. first + requests - 1 of a step begin with, on
+ * pages that hold the same: they are computed once for the rows of all, from the block
+ * table row of the first of them that has tokens. */
+typedef struct oscar_prefix {
+  int32_t first;
+  int32_t requests;
+  int32_t keys; /* at most each one's keys before the step's own */
+} oscar_prefix;
 
 int oscar_chunk_plan(const int32_t* query_start_loc, const int32_t* seq_lens, int32_t num_requests,
                      int32_t num_heads, int32_t window, const oscar_plain_cache* cache, void* items,
                      size_t items_size, oscar_chunk_step* step);
+/* oscar_chunk_plan of a step whose requests share prefixes: in the order of their
+ * requests, none in two; without a window. */
+int oscar_chunk_plan_shared(const int32_t* query_start_loc, const int32_t* seq_lens, int32_t num_requests,
+                            int32_t num_heads, int32_t window, const oscar_prefix* prefixes, int32_t num_prefixes,
+                            const oscar_plain_cache* cache, void* items, size_t items_size, oscar_chunk_step* step);
 int oscar_chunk_attention(const oscar_chunk_step* step, const void* items, const int32_t* block_table,
                           int64_t block_table_stride, const oscar_plain_cache* cache, const oscar_heads* query,
                           const oscar_heads* out, float scale, void* workspace, size_t workspace_size,

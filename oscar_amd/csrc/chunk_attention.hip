@@ -4,8 +4,6 @@
 #include "chunk_plan.h"
 #include "row_span.h"
 
-#include <cstring>
-
 namespace oscar {
 namespace {
 
@@ -49,7 +47,8 @@ int launch(const ChunkArgs& a, const oscar_chunk_step& step, hipStream_t stream)
   kernels[which]<<<step.narrow + step.wide, kThreads, 0, stream>>>(a);
   const int64_t blocks = (int64_t)step.few_joins * (D / 32) + (int64_t)(step.joins - step.few_joins) * (kTileRows * D / 64);
   if (blocks > INT32_MAX) return kErrInvalidArgument;
-  if (blocks > 0) join_kernel<T, D><<<(uint32_t)blocks, 256, 0, stream>>>(a);
+  if (blocks > 0 && step.parts == 0) join_kernel<T, D, false><<<(uint32_t)blocks, 256, 0, stream>>>(a);
+  else if (blocks > 0) join_kernel<T, D, true><<<(uint32_t)blocks, 256, 0, stream>>>(a);
   return hipGetLastError() == hipSuccess ? kOk : kErrLaunch;
 }
 
@@ -71,30 +70,25 @@ int check_chunk_cache(const oscar_plain_cache* c) {
 }  // namespace
 }  // namespace oscar
 
-extern "C" int oscar_chunk_plan(const int32_t* query_start_loc, const int32_t* seq_lens, int32_t num_requests,
-                                int32_t num_heads, int32_t window, const oscar_plain_cache* cache, void* items,
-                                size_t items_size, oscar_chunk_step* step) {
+extern "C" int oscar_chunk_plan_shared(const int32_t* query_start_loc, const int32_t* seq_lens, int32_t num_requests,
+                                       int32_t num_heads, int32_t window, const oscar_prefix* prefixes,
+                                       int32_t num_prefixes, const oscar_plain_cache* cache, void* items,
+                                       size_t items_size, oscar_chunk_step* step) {
   using namespace oscar;
-  const int status = check_chunk_cache(cache);
+  int status = check_chunk_cache(cache);
   if (status != kOk) return status;
-  if (step == nullptr || num_requests < 0 || (num_requests > 0 && (query_start_loc == nullptr || seq_lens == nullptr)) ||
-      num_heads < 1 || num_heads % cache->num_kv_heads || num_heads > (1 << 16) || window < 0)
-    return kErrInvalidArgument;
-  const int32_t group = num_heads / cache->num_kv_heads;
+  if (step == nullptr) return kErrInvalidArgument;
   int32_t pages = 0;
-  for (int32_t i = 0; i < num_requests; ++i) {
-    const int64_t n = (int64_t)query_start_loc[i + 1] - query_start_loc[i];
-    if (query_start_loc[i] < 0 || n < 0 || seq_lens[i] < n || n * group > kMostKeys ||
-        seq_lens[i] > kMostKeys)
-      return kErrInvalidArgument;
-    if (n > 0) pages = std::max(pages, (seq_lens[i] - 1) / cache->block_size + 1);
-  }
+  status = check_step(query_start_loc, seq_lens, num_requests, num_heads, cache->num_kv_heads, window, cache->block_size,
+                      &pages);
+  if (status != kOk) return status;
+  const int32_t group = num_heads / cache->num_kv_heads;
   try {
+    std::vector<Prefix> shared;
+    status = check_prefixes(prefixes, num_prefixes, query_start_loc, seq_lens, num_requests, group, window, shared);
+    if (status != kOk) return status;
     Plan plan;
-    make_plan(query_start_loc, seq_lens, num_requests, group, cache->num_kv_heads, cache->head_size, window, plan);
-    const size_t narrow = plan.narrow.size() * sizeof(Piece), wide = plan.wide.size() * sizeof(Piece);
-    const size_t joins = plan.joins.size() * sizeof(Join);
-    if (plan.narrow.size() + plan.wide.size() > INT32_MAX || plan.joins.size() > INT32_MAX) return kErrInvalidArgument;
+    make_plan(query_start_loc, seq_lens, num_requests, group, cache->num_kv_heads, cache->head_size, window, shared, plan);
     step->num_requests = num_requests;
     step->num_tokens = num_requests > 0 ? query_start_loc[num_requests] : 0;
     step->num_heads = num_heads;
@@ -103,23 +97,17 @@ extern "C" int oscar_chunk_plan(const int32_t* query_start_loc, const int32_t* s
     step->block_size = cache->block_size;
     step->window = std::min(window, kMostKeys);
     step->table_cols = pages;
-    step->narrow = (int32_t)plan.narrow.size();
-    step->wide = (int32_t)plan.wide.size();
-    step->joins = (int32_t)plan.joins.size();
-    step->few_joins = (int32_t)std::count_if(plan.joins.begin(), plan.joins.end(),
-                                             [](const Join& j) { return j.count <= kFewParts; });
-    step->items_size = (int64_t)(narrow + wide + joins);
-    step->workspace_size = (int64_t)plan.slots * kTileRows * (cache->head_size + 2) * 4;
-    if (items == nullptr) return kOk;
-    if (items_size < narrow + wide + joins) return kErrWorkspaceTooSmall;
-    uint8_t* to = static_cast<uint8_t*>(items);
-    if (narrow > 0) std::memcpy(to, plan.narrow.data(), narrow);
-    if (wide > 0) std::memcpy(to + narrow, plan.wide.data(), wide);
-    if (joins > 0) std::memcpy(to + narrow + wide, plan.joins.data(), joins);
+    return pack_plan(plan, cache->head_size, items, items_size, step);
   } catch (...) {
     return kErrInvalidArgument;
   }
-  return kOk;
+}
+
+extern "C" int oscar_chunk_plan(const int32_t* query_start_loc, const int32_t* seq_lens, int32_t num_requests,
+                                int32_t num_heads, int32_t window, const oscar_plain_cache* cache, void* items,
+                                size_t items_size, oscar_chunk_step* step) {
+  return oscar_chunk_plan_shared(query_start_loc, seq_lens, num_requests, num_heads, window, nullptr, 0, cache, items,
+                                 items_size, step);
 }
 
 extern "C" int oscar_chunk_attention(const oscar_chunk_step* step, const void* items, const int32_t* block_table,
@@ -136,7 +124,7 @@ extern "C" int oscar_chunk_attention(const oscar_chunk_step* step, const void* i
   if (step->num_kv_heads != cache->num_kv_heads || step->head_size != cache->head_size ||
       step->block_size != cache->block_size)
     return kErrInvalidArgument;
-  if (step->narrow < 0 || step->wide < 0 || step->few_joins < 0 || step->joins < step->few_joins)
+  if (step->narrow < 0 || step->wide < 0 || step->few_joins < 0 || step->joins < step->few_joins || step->parts < 0)
     return kErrInvalidArgument;
   if (step->narrow + step->wide == 0) return kOk;
   if (items == nullptr || block_table == nullptr || query->data == nullptr || out->data == nullptr ||
@@ -181,6 +169,7 @@ extern "C" int oscar_chunk_attention(const oscar_chunk_step* step, const void* i
   a.wide = step->wide;
   a.few_joins = step->few_joins;
   a.joins = reinterpret_cast<const Join*>(a.pieces + step->narrow + step->wide);
+  a.parts = reinterpret_cast<const SharedPart*>(a.joins + step->joins);
   a.partials = static_cast<float*>(workspace);
   a.scale_log2 = scale * 1.4426950408889634f;
   a.group = step->num_heads / cache->num_kv_heads;

@@ -131,11 +131,17 @@ struct Piece {
   int32_t slot;            // first partial of 32 rows, -1: rows are finished here
   int32_t pad[3];
 };
-// 32 rows whose partials are slots slot0, slot0 + step, ...
+// 32 rows whose partials are slots slot0, slot0 + step, ... and, if `shared` > 0, those
+// of a prefix that their request shares: parts[shared - 1].
 struct Join {
-  int32_t token0, kv_head, row0, rows, slot0, step, count, pad;
+  int32_t token0, kv_head, row0, rows, slot0, step, count, shared;
 };
-static_assert(sizeof(Piece) == 48 && sizeof(Join) == 32, "item sizes");
+// Row r of the join is row `row` + r of the prefix' rows, 32 to a slot, whose partials
+// begin at slots slot0, slot0 + step, ...
+struct SharedPart {
+  int32_t slot0, step, count, row;
+};
+static_assert(sizeof(Piece) == 48 && sizeof(Join) == 32 && sizeof(SharedPart) == 16, "item sizes");
 
 struct ChunkArgs {
   const uint8_t* q;
@@ -156,6 +162,7 @@ struct ChunkArgs {
   int32_t narrow, wide;    // pieces, narrow ones first
   int32_t few_joins;       // joins of few partials come first
   FastDiv group_div, block_div;
+  const SharedPart* parts; // after the joins
 };
 
 // f(0), f(1), .. f(N - 1) with constants.
@@ -885,19 +892,37 @@ __device__ __forceinline__ void wide_piece(const ChunkArgs& a, const Piece p, ui
 // 2.3 to 5 us.
 constexpr int kFewParts = 8;
 
-template <typename T, int D, int kParts>
-__device__ __forceinline__ void join_few(const ChunkArgs& a, const Join j, int block) {
+// A partial of one row: its slot, and the row's place there.
+struct RowPart {
+  const float* slot;
+  int row;
+};
+// Partial i of a join's row: its own, then (kShared) those of the prefix.
+template <int D, bool kShared>
+__device__ __forceinline__ RowPart part_of(const ChunkArgs& a, const Join& j, const SharedPart& p, int row, int i) {
+  if constexpr (kShared) {
+    if (i >= j.count) {
+      const int at = p.row + row;
+      return RowPart{a.partials + (int64_t)(p.slot0 + (i - j.count) * p.step + at / kTileRows) * (kTileRows * (D + 2)),
+                     at % kTileRows};
+    }
+  }
+  return RowPart{a.partials + (int64_t)(j.slot0 + i * j.step) * (kTileRows * (D + 2)), row};
+}
+
+template <typename T, int D, int kParts, bool kShared>
+__device__ __forceinline__ void join_few(const ChunkArgs& a, const Join j, const SharedPart p, int block) {
   const int i = block * 256 + (int)threadIdx.x, row = i / (D / 4), feature = 4 * (i % (D / 4));
   if (row >= j.rows) return;
-  const float* const first = a.partials + (int64_t)j.slot0 * (kTileRows * (D + 2));
+  const int count = kShared ? j.count + p.count : j.count;
   float m[kParts], l[kParts], top = kNone;
   floatx4 x[kParts];
 #pragma unroll
   for (int s = 0; s < kParts; ++s) {        // (the last one again for those that are not there: no load waits)
-    const float* at = first + (int64_t)(min(s, j.count - 1) * j.step) * (kTileRows * (D + 2));
-    m[s] = at[kTileRows * D + row];
-    l[s] = at[kTileRows * D + kTileRows + row];
-    x[s] = *reinterpret_cast<const floatx4*>(at + row * D + feature);
+    const RowPart at = part_of<D, kShared>(a, j, p, row, min(s, count - 1));
+    m[s] = at.slot[kTileRows * D + at.row];
+    l[s] = at.slot[kTileRows * D + kTileRows + at.row];
+    x[s] = *reinterpret_cast<const floatx4*>(at.slot + at.row * D + feature);
   }
 #pragma unroll
   for (int s = 0; s < kParts; ++s) top = fmaxf(top, m[s]);
@@ -905,7 +930,7 @@ __device__ __forceinline__ void join_few(const ChunkArgs& a, const Join j, int b
   float sum = 0.f;
 #pragma unroll
   for (int s = 0; s < kParts; ++s)
-    if (s < j.count) {
+    if (s < count) {
       const float w = __builtin_amdgcn_exp2f(m[s] - top);
       sum += w * l[s];
       o += w * x[s];
@@ -914,21 +939,24 @@ __device__ __forceinline__ void join_few(const ChunkArgs& a, const Join j, int b
   store4<T>(out_row(a, j.token0, j.kv_head, j.row0 + row) + 2 * feature, o * inv);
 }
 
-template <typename T, int D>
-__device__ __forceinline__ void join_many(const ChunkArgs& a, const Join j, int row, int part64) {
+template <typename T, int D, bool kShared>
+__device__ __forceinline__ void join_many(const ChunkArgs& a, const Join j, const SharedPart p, int row, int part64) {
   const int tid = (int)threadIdx.x, feature = 64 * part64 + 4 * (tid & 15), part = tid >> 4;
   __shared__ float red[16][64 + 4];
   __shared__ float red_m[16], red_l[16];
-  auto slot = [&](int i) { return a.partials + (int64_t)(j.slot0 + i * j.step) * (kTileRows * (D + 2)); };
+  const int count = kShared ? j.count + p.count : j.count;
   float m = kNone;
-  for (int i = part; i < j.count; i += 16) m = fmaxf(m, slot(i)[kTileRows * D + row]);
+  for (int i = part; i < count; i += 16) {
+    const RowPart at = part_of<D, kShared>(a, j, p, row, i);
+    m = fmaxf(m, at.slot[kTileRows * D + at.row]);
+  }
   floatx4 o{};
   float l = 0.f;
-  for (int i = part; i < j.count; i += 16) {
-    const float* s = slot(i);
-    const float w = __builtin_amdgcn_exp2f(s[kTileRows * D + row] - m);
-    l += w * s[kTileRows * D + kTileRows + row];
-    o += w * *reinterpret_cast<const floatx4*>(s + row * D + feature);
+  for (int i = part; i < count; i += 16) {
+    const RowPart at = part_of<D, kShared>(a, j, p, row, i);
+    const float w = __builtin_amdgcn_exp2f(at.slot[kTileRows * D + at.row] - m);
+    l += w * at.slot[kTileRows * D + kTileRows + at.row];
+    o += w * *reinterpret_cast<const floatx4*>(at.slot + at.row * D + feature);
   }
   *reinterpret_cast<floatx4*>(&red[part][4 * (tid & 15)]) = o;
   if ((tid & 15) == 0) {
@@ -953,20 +981,23 @@ __device__ __forceinline__ void join_many(const ChunkArgs& a, const Join j, int 
 }
 
 // Groups of few partials first, D / 32 workgroups each; then 32 x D / 64 a group.
-template <typename T, int D>
+template <typename T, int D, bool kShared>
 __global__ __launch_bounds__(256) void join_kernel(ChunkArgs a) {
   constexpr int kFewBlocks = D / 32, kManyBlocks = kTileRows * D / 64;
   const int block = (int)blockIdx.x, few = a.few_joins * kFewBlocks;
+  const int many = (block - few) / kManyBlocks, at = (block - few) % kManyBlocks;
+  const Join j = a.joins[block < few ? block / kFewBlocks : a.few_joins + many];
+  SharedPart p{};
+  if constexpr (kShared)
+    if (j.shared > 0) p = a.parts[j.shared - 1];
   if (block < few) {
-    const Join j = a.joins[block / kFewBlocks];
-    if (j.count <= 2) join_few<T, D, 2>(a, j, block % kFewBlocks);
-    else if (j.count <= 4) join_few<T, D, 4>(a, j, block % kFewBlocks);
-    else join_few<T, D, kFewParts>(a, j, block % kFewBlocks);
+    const int count = j.count + p.count;
+    if (count <= 2) join_few<T, D, 2, kShared>(a, j, p, block % kFewBlocks);
+    else if (count <= 4) join_few<T, D, 4, kShared>(a, j, p, block % kFewBlocks);
+    else join_few<T, D, kFewParts, kShared>(a, j, p, block % kFewBlocks);
     return;
   }
-  const int many = (block - few) / kManyBlocks, at = (block - few) % kManyBlocks;
-  const Join j = a.joins[a.few_joins + many];
-  if (at / (D / 64) < j.rows) join_many<T, D>(a, j, at / (D / 64), at % (D / 64));
+  if (at / (D / 64) < j.rows) join_many<T, D, kShared>(a, j, p, at / (D / 64), at % (D / 64));
 }
 
 }  // namespace

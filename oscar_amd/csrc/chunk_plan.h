@@ -5,6 +5,7 @@
 
 #include <algorithm>
 #include <cstddef>
+#include <cstring>
 #include <vector>
 
 namespace oscar {
@@ -13,17 +14,32 @@ namespace {
 struct Plan {
   std::vector<Piece> narrow, wide;
   std::vector<Join> joins;
+  std::vector<SharedPart> parts;
   int32_t slots = 0;
+};
+
+// Keys [0, keys) that requests first .. first + count - 1 begin with, computed for all
+// their rows as if they were one request's.
+struct Prefix {
+  int32_t first, count, keys;
+};
+// The rows of a prefix and kv head, 32 to a slot, in pieces that all have the same keys.
+struct PrefixRows {
+  int32_t slot0 = -1, groups = 0, pieces = 0;
 };
 
 struct RowTile {
   Piece piece;
   int32_t tiles;           // of 32 keys
+  int32_t of_prefix = -1;  // PrefixRows that it is some of
+  int32_t with_prefix = -1, prefix_row = 0;      // PrefixRows that its rows go on from, and where they begin there
 };
 
-// The row tiles of a request, `rows` rows each, with the keys that they see.
+// The row tiles of a request, `rows` rows each, with the keys that they see from `from`
+// (a multiple of 32) on.  with_prefix: PrefixRows of its first kv head, or -1.
 void row_tiles(int32_t token0, int32_t n, int32_t seq, int32_t table_row, int32_t group, int32_t kv_heads,
-               int32_t window, int32_t rows, std::vector<RowTile>& out) {
+               int32_t window, int32_t rows, std::vector<RowTile>& out, int32_t from = 0, int32_t with_prefix = -1,
+               int32_t prefix_row = 0) {
   const int32_t all = n * group;
   for (int32_t r = 0; r < all; r += rows) {
     Piece p{};
@@ -33,32 +49,68 @@ void row_tiles(int32_t token0, int32_t n, int32_t seq, int32_t table_row, int32_
     p.row0 = r;
     p.rows = std::min(rows, all - r);
     p.slot = -1;
-    const int32_t lo = window > 0 ? std::max(0, p.pos0 + r / group - window + 1) : 0;
+    const int32_t lo = window > 0 ? std::max(0, p.pos0 + r / group - window + 1) : from;
     p.key0 = lo / kTileKeys * kTileKeys;
     p.key1 = p.pos0 + (r + p.rows - 1) / group + 1;
     for (int32_t h = 0; h < kv_heads; ++h) {
       p.kv_head = h;
-      out.push_back(RowTile{p, (p.key1 - p.key0 + kTileKeys - 1) / kTileKeys});
+      RowTile x{p, (p.key1 - p.key0 + kTileKeys - 1) / kTileKeys};
+      if (with_prefix >= 0) {
+        x.with_prefix = with_prefix + h;
+        x.prefix_row = prefix_row + r;
+      }
+      out.push_back(x);
     }
   }
 }
 
+// The row tiles of a prefix: all rows of `tokens` tokens from token0 on, which see all
+// of its keys.
+void prefix_tiles(int32_t token0, int32_t tokens, int32_t keys, int32_t table_row, int32_t group, int32_t kv_heads,
+                  int32_t rows, int32_t of_prefix, std::vector<RowTile>& out) {
+  const int32_t all = tokens * group;
+  for (int32_t r = 0; r < all; r += rows)
+    for (int32_t h = 0; h < kv_heads; ++h) {
+      RowTile x{Piece{token0, keys, table_row, h, r, std::min(rows, all - r), 0, keys, -1, {}}, keys / kTileKeys};
+      x.of_prefix = of_prefix + h;
+      out.push_back(x);
+    }
+}
+
+// Whether a row tile in n pieces leaves partials.
+bool leaves_partials(const RowTile& x, int32_t n) { return n > 1 || x.of_prefix >= 0 || x.with_prefix >= 0; }
+
 // A row tile in n pieces of equal length, but for a key tile.
-void cut(const RowTile& x, int32_t n, Plan& plan, std::vector<Piece>& out) {
-  if (n <= 1) {
+void cut(const RowTile& x, int32_t n, Plan& plan, std::vector<PrefixRows>& prefixes, std::vector<Piece>& out) {
+  if (!leaves_partials(x, n)) {
     out.push_back(x.piece);
     return;
   }
   const int32_t groups = (x.piece.rows + kTileRows - 1) / kTileRows;
-  for (int32_t g = 0; g < groups; ++g)
-    plan.joins.push_back(Join{x.piece.token0, x.piece.kv_head, x.piece.row0 + g * kTileRows,
-                              std::min(kTileRows, x.piece.rows - g * kTileRows), plan.slots + g, groups, n, 0});
+  int32_t slot = plan.slots, step = groups;
+  if (x.of_prefix >= 0) {                   // (the join's rows are the requests')
+    PrefixRows& rows = prefixes[x.of_prefix];
+    if (rows.slot0 < 0) {
+      rows.slot0 = plan.slots;
+      rows.pieces = n;
+      plan.slots += n * rows.groups;
+    }
+    slot = rows.slot0 + x.piece.row0 / kTileRows;
+    step = rows.groups;
+  } else {
+    plan.slots += n * groups;
+    for (int32_t g = 0; g < groups; ++g) {
+      if (x.with_prefix >= 0) plan.parts.push_back(SharedPart{x.with_prefix, 0, 0, x.prefix_row + g * kTileRows});
+      plan.joins.push_back(Join{x.piece.token0, x.piece.kv_head, x.piece.row0 + g * kTileRows,
+                                std::min(kTileRows, x.piece.rows - g * kTileRows), slot + g, step, n,
+                                x.with_prefix >= 0 ? (int32_t)plan.parts.size() : 0});
+    }
+  }
   for (int32_t s = 0; s < n; ++s) {
     Piece p = x.piece;
     p.key0 = x.piece.key0 + kTileKeys * (int32_t)((int64_t)x.tiles * s / n);
     p.key1 = std::min<int32_t>(x.piece.key1, x.piece.key0 + kTileKeys * (int32_t)((int64_t)x.tiles * (s + 1) / n));
-    p.slot = plan.slots;
-    plan.slots += groups;
+    p.slot = slot + s * step;
     out.push_back(p);
   }
 }
@@ -86,7 +138,8 @@ int32_t pieces_of(const RowTile& x, int64_t per) { return (int32_t)((x.tiles + p
 // 256, 190 us, 5.2 TB/s), but one request that is far longer than the others is then
 // read by one workgroup (300 users of 1000 keys and one of 131072 2.2 ms, where the
 // bytes take 0.09), and by a few where there are just fewer (250 and one: 0.39 ms).
-void plan_narrow(const std::vector<RowTile>& rows, int32_t head_size, double beside, Plan& plan) {
+void plan_narrow(const std::vector<RowTile>& rows, int32_t head_size, double beside, Plan& plan,
+                 std::vector<PrefixRows>& prefixes) {
   int64_t total = 0;
   int32_t most = 0;
   for (const RowTile& x : rows) {
@@ -114,7 +167,7 @@ void plan_narrow(const std::vector<RowTile>& rows, int32_t head_size, double bes
   int64_t per = fit(beside == 0. ? kCus : total > 240 * beside ? 2 * kCus : 2 * kCus / 3);
   if (beside == 0. && (rows.size() >= kCus || 100 * per * kCus > 115 * total))
     per = fit((int64_t)kCus * narrow_wgs(head_size));
-  for (const RowTile& x : rows) cut(x, pieces_of(x, per), plan, plan.narrow);
+  for (const RowTile& x : rows) cut(x, pieces_of(x, per), plan, prefixes, plan.narrow);
 }
 
 // Wide tiles.  Workgroups take pieces as they come free, two to a CU.  Row tiles
@@ -136,7 +189,7 @@ void plan_narrow(const std::vector<RowTile>& rows, int32_t head_size, double bes
 // D = 128, 640 us, where the keys take 43).
 // Returns the estimate.
 constexpr int32_t kPieceCost = 4, kCutCost = 15, kLeastPiece = 8, kMostPieces = 2048;
-double plan_wide(const std::vector<RowTile>& rows, int32_t head_size, Plan& plan) {
+double plan_wide(const std::vector<RowTile>& rows, int32_t head_size, Plan& plan, std::vector<PrefixRows>& prefixes) {
   int32_t most = 0;
   for (const RowTile& x : rows) most = std::max(most, x.tiles);
   const double alone = head_size == 256 ? 1.07 : head_size == 128 ? 1.45 : 1.5;
@@ -150,8 +203,8 @@ double plan_wide(const std::vector<RowTile>& rows, int32_t head_size, Plan& plan
     bool cuts = false;
     for (const RowTile& x : rows) {
       const int32_t n = pieces_of(x, per);
-      cuts = cuts || n > 1;
-      count[(x.tiles + n - 1) / n + (n > 1 ? kCutCost : kPieceCost)] += n;
+      cuts = cuts || leaves_partials(x, n);
+      count[(x.tiles + n - 1) / n + (leaves_partials(x, n) ? kCutCost : kPieceCost)] += n;
     }
     std::fill(load.begin(), load.end(), 0);
     int64_t dealt = 0, longest = 0;
@@ -175,7 +228,7 @@ double plan_wide(const std::vector<RowTile>& rows, int32_t head_size, Plan& plan
       per = at_most;
     }
   }
-  for (const RowTile& x : rows) cut(x, pieces_of(x, per), plan, plan.wide);
+  for (const RowTile& x : rows) cut(x, pieces_of(x, per), plan, prefixes, plan.wide);
   std::stable_sort(plan.wide.begin(), plan.wide.end(),
                    [](const Piece& x, const Piece& y) { return x.key1 - x.key0 > y.key1 - y.key0; });
   // The first two rounds of workgroups share CUs in order: the longest pieces,
@@ -185,22 +238,116 @@ double plan_wide(const std::vector<RowTile>& rows, int32_t head_size, Plan& plan
 }
 
 void make_plan(const int32_t* qsl, const int32_t* seqs, int32_t num_requests, int32_t group, int32_t kv_heads,
-               int32_t head_size, int32_t window, Plan& plan) {
+               int32_t head_size, int32_t window, const std::vector<Prefix>& shared, Plan& plan) {
   // Up to 32 rows a request is narrow (28 rows of 16 users over 1000 keys, D = 128: 20.4
   // us, as wide tiles 24.2; 30 of 8 users over 16000, D = 256, 31.1, 30.1), from 33 on
   // wide, where narrow tiles would read its keys twice (48 rows, the same: 24.7 us, as
-  // narrow 23.2; 32.2, 36.1; 32 users over 4000 32.5, 49.6).
+  // narrow 23.2; 32.2, 36.1; 32 users over 4000 32.5, 49.6).  So are the rows of a prefix.
   std::vector<RowTile> narrow, wide;
+  std::vector<PrefixRows> prefixes;
+  auto prefix = shared.begin();
+  int32_t keys = 0, until = 0, first_token = 0;        // of the prefix that request i begins with
   for (int32_t i = 0; i < num_requests; ++i) {
     const int32_t n = qsl[i + 1] - qsl[i];
+    if (i >= until) keys = 0;
+    if (prefix != shared.end() && i == prefix->first) {
+      keys = prefix->keys;
+      until = i + prefix->count;
+      first_token = qsl[i];
+      const int32_t tokens = qsl[until] - qsl[i], at = (int32_t)prefixes.size();
+      int32_t table_row = i;                           // a request's that has tokens
+      while (qsl[table_row + 1] == qsl[table_row]) ++table_row;
+      PrefixRows rows;
+      rows.groups = (tokens * group + kTileRows - 1) / kTileRows;
+      prefixes.insert(prefixes.end(), kv_heads, rows);
+      if (tokens * (int64_t)group <= kTileRows)
+        prefix_tiles(qsl[i], tokens, keys, table_row, group, kv_heads, kTileRows, at, narrow);
+      else
+        prefix_tiles(qsl[i], tokens, keys, table_row, group, kv_heads, kWideRows, at, wide);
+      ++prefix;
+    }
+    const int32_t with = keys > 0 ? (int32_t)prefixes.size() - kv_heads : -1;
+    const int32_t row = keys > 0 ? (qsl[i] - first_token) * group : 0;
     if (n * (int64_t)group <= kTileRows)
-      row_tiles(qsl[i], n, seqs[i], i, group, kv_heads, window, kTileRows, narrow);
+      row_tiles(qsl[i], n, seqs[i], i, group, kv_heads, window, kTileRows, narrow, keys, with, row);
     else
-      row_tiles(qsl[i], n, seqs[i], i, group, kv_heads, window, kWideRows, wide);
+      row_tiles(qsl[i], n, seqs[i], i, group, kv_heads, window, kWideRows, wide, keys, with, row);
   }
-  const double beside = wide.empty() ? 0. : plan_wide(wide, head_size, plan);
-  if (!narrow.empty()) plan_narrow(narrow, head_size, beside, plan);
-  std::stable_partition(plan.joins.begin(), plan.joins.end(), [](const Join& j) { return j.count <= kFewParts; });
+  const double beside = wide.empty() ? 0. : plan_wide(wide, head_size, plan, prefixes);
+  if (!narrow.empty()) plan_narrow(narrow, head_size, beside, plan, prefixes);
+  for (SharedPart& p : plan.parts) {
+    const PrefixRows& rows = prefixes[p.slot0];
+    p = SharedPart{rows.slot0, rows.groups, rows.pieces, p.row};
+  }
+  std::stable_partition(plan.joins.begin(), plan.joins.end(), [&](const Join& j) {
+    return j.count + (j.shared > 0 ? plan.parts[j.shared - 1].count : 0) <= kFewParts;
+  });
+}
+
+// ---------------------------------------------------------------- the step
+// A step's arguments.  *pages: of the block table, in pages of block_size.
+int check_step(const int32_t* qsl, const int32_t* seqs, int32_t num_requests, int32_t num_heads, int32_t num_kv_heads,
+               int32_t window, int32_t block_size, int32_t* pages) {
+  if (num_requests < 0 || (num_requests > 0 && (qsl == nullptr || seqs == nullptr)) || num_heads < 1 ||
+      num_heads % num_kv_heads || num_heads > (1 << 16) || window < 0)
+    return kErrInvalidArgument;
+  const int32_t group = num_heads / num_kv_heads;
+  *pages = 0;
+  for (int32_t i = 0; i < num_requests; ++i) {
+    const int64_t n = (int64_t)qsl[i + 1] - qsl[i];
+    if (qsl[i] < 0 || n < 0 || seqs[i] < n || n * group > kMostKeys || seqs[i] > kMostKeys) return kErrInvalidArgument;
+    if (n > 0) *pages = std::max(*pages, (seqs[i] - 1) / block_size + 1);
+  }
+  return kOk;
+}
+
+// Prefixes in the order of their requests, whole key tiles of them (what is left a request
+// reads with its own keys), without those of less than two requests with tokens.
+int check_prefixes(const oscar_prefix* prefixes, int32_t count, const int32_t* qsl, const int32_t* seqs,
+                   int32_t num_requests, int32_t group, int32_t window, std::vector<Prefix>& out) {
+  if (count < 0 || (count > 0 && (prefixes == nullptr || window > 0))) return kErrInvalidArgument;
+  int32_t until = 0;
+  for (int32_t i = 0; i < count; ++i) {
+    const oscar_prefix& p = prefixes[i];
+    if (p.first < until || p.requests < 0 || p.keys < 0 || p.requests > num_requests - p.first) return kErrInvalidArgument;
+    until = p.first + p.requests;
+    int32_t with_tokens = 0;
+    for (int32_t r = p.first; r < until; ++r) {
+      const int32_t n = qsl[r + 1] - qsl[r];
+      if (n == 0) continue;
+      ++with_tokens;
+      if (p.keys > seqs[r] - n) return kErrInvalidArgument;
+    }
+    const int64_t rows = ((int64_t)qsl[until] - qsl[p.first]) * group;
+    if (rows > kMostKeys) return kErrInvalidArgument;
+    if (with_tokens > 1 && p.keys >= kTileKeys) out.push_back(Prefix{p.first, p.requests, p.keys / kTileKeys * kTileKeys});
+  }
+  return kOk;
+}
+
+// Sizes of a plan, and its items: pieces, joins, prefix parts.
+int pack_plan(const Plan& plan, int32_t head_size, void* items, size_t items_size, oscar_chunk_step* step) {
+  if (plan.narrow.size() + plan.wide.size() > INT32_MAX || plan.joins.size() > INT32_MAX) return kErrInvalidArgument;
+  step->narrow = (int32_t)plan.narrow.size();
+  step->wide = (int32_t)plan.wide.size();
+  step->joins = (int32_t)plan.joins.size();
+  step->parts = (int32_t)plan.parts.size();
+  step->few_joins = (int32_t)std::count_if(plan.joins.begin(), plan.joins.end(), [&](const Join& j) {
+    return j.count + (j.shared > 0 ? plan.parts[j.shared - 1].count : 0) <= kFewParts;
+  });
+  const void* const from[4] = {plan.narrow.data(), plan.wide.data(), plan.joins.data(), plan.parts.data()};
+  const size_t size[4] = {plan.narrow.size() * sizeof(Piece), plan.wide.size() * sizeof(Piece),
+                          plan.joins.size() * sizeof(Join), plan.parts.size() * sizeof(SharedPart)};
+  step->items_size = (int64_t)(size[0] + size[1] + size[2] + size[3]);
+  step->workspace_size = (int64_t)plan.slots * kTileRows * (head_size + 2) * 4;
+  if (items == nullptr) return kOk;
+  if ((int64_t)items_size < step->items_size) return kErrWorkspaceTooSmall;
+  uint8_t* to = static_cast<uint8_t*>(items);
+  for (int i = 0; i < 4; ++i) {
+    if (size[i] > 0) std::memcpy(to, from[i], size[i]);
+    to += size[i];
+  }
+  return kOk;
 }
 
 }  // namespace

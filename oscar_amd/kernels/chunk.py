@@ -27,7 +27,7 @@ class ChunkStepArgs(ctypes.Structure):
     _fields_ = [("num_requests", _i32), ("num_tokens", _i32), ("num_heads", _i32), ("window", _i32),
                 ("table_cols", _i32), ("narrow", _i32), ("wide", _i32), ("joins", _i32), ("few_joins", _i32),
                 ("num_kv_heads", _i32), ("head_size", _i32), ("block_size", _i32), ("items_size", _i64),
-                ("workspace_size", _i64)]
+                ("workspace_size", _i64), ("parts", _i32), ("reserved", _i32)]
 
 
 class ChunkStep:
@@ -41,6 +41,12 @@ class ChunkStep:
     [requests, pages] on the cache's device.  The block table is read at every call
     and replay where it is int32 with rows of their own, and else copied here.
 
+    prefixes: (first, requests, keys) of groups of requests, one after the other in the
+    step, whose first `keys` keys are the same and come before each one's own tokens (a
+    system prompt, samples of one prompt).  They are computed once for all the group's
+    rows, from the pages of its first request that has tokens, which keeps its results
+    within rounding of a step without them.  They do not go with a window.
+
     Building copies the step's arrays to the device on the current stream; calls
     on other streams wait for that by themselves.  A step is not built under graph
     capture.  A captured call keeps this step's lengths and needs the step to live
@@ -48,7 +54,8 @@ class ChunkStep:
     sees to it (it waits for the device before it captures), and a capture begun in
     another way has to, by a wait of its stream for the one the step was built on."""
 
-    def __init__(self, qsl, seqs, block_tables: torch.Tensor, num_heads: int, cache: PagedCache, window: int = 0):
+    def __init__(self, qsl, seqs, block_tables: torch.Tensor, num_heads: int, cache: PagedCache, window: int = 0,
+                 prefixes=()):
         layout = decode.request_layout(qsl, seqs)
         requests = len(layout.lengths)
         if num_heads < 1 or num_heads % cache.num_kv_heads:
@@ -64,8 +71,10 @@ class ChunkStep:
             raise ValueError("chunk attention needs a cache block size that is a multiple of 16")
         if layout.qsl and layout.qsl[0] < 0:
             raise ValueError("query starts are counted from the step's token 0")
+        prefixes = _check_prefixes(prefixes, layout, window)
         args = ChunkStepArgs()
-        items = _plan(layout, requests, num_heads, window, cache, args)
+        items = (_plan(layout, requests, num_heads, window, cache, args) if prefixes is None else
+                 _plan(layout, requests, num_heads, window, cache, args, prefixes))
         if block_tables.ndim != 2 or block_tables.shape[0] < requests or block_tables.shape[1] < args.table_cols:
             raise ValueError(f"block table must be [requests, pages] with the {args.table_cols} pages of the longest")
         if block_tables.dtype not in (torch.int32, torch.int64, torch.int16, torch.int8, torch.uint8):
@@ -145,14 +154,35 @@ def chunk_attention(query: torch.Tensor, cache: PagedCache, step: ChunkStep, sca
     return out
 
 
-def _plan(layout, requests: int, num_heads: int, window: int, cache: PagedCache, args: ChunkStepArgs) -> torch.Tensor:
+def _check_prefixes(prefixes, layout, window: int):
+    """The prefixes' struct oscar_prefix array as int32, in the order of their requests; None without any."""
+    if not len(prefixes):
+        return None
+    if window:
+        raise ValueError("requests of a step with a window share no prefix")
+    until, flat = 0, []
+    for first, requests, keys in sorted(tuple(int(x) for x in p) for p in prefixes):
+        if first < until or requests < 0 or first + requests > len(layout.lengths) or keys < 0:
+            raise ValueError("prefixes are (first request, requests, keys) of the step, no request in two")
+        until = first + requests
+        for i in range(first, until):
+            new = layout.qsl[i + 1] - layout.qsl[i]
+            if new > 0 and keys > layout.seqs[i] - new:
+                raise ValueError(f"request {i} has fewer keys before its own than the prefix")
+        flat += [first, requests, min(keys, MAX_KEYS)]
+    return (_i32 * len(flat))(*flat)
+
+
+def _plan(layout, requests: int, num_heads: int, window: int, cache: PagedCache, args: ChunkStepArgs,
+          prefixes=None) -> torch.Tensor:
     """The step's items (host bytes), its sizes in args.  Planned straight into
     128 KB, which most steps' items fit; a step that needs more is planned again."""
     size = 1 << 17
     while True:
         items = torch.empty(size, dtype=torch.uint8)
-        status = _lib.load().oscar_chunk_plan(
+        status = _lib.load().oscar_chunk_plan_shared(
             ctypes.addressof(layout.qstart), ctypes.addressof(layout.seq_t), requests, num_heads, window,
+            None if prefixes is None else ctypes.addressof(prefixes), 0 if prefixes is None else len(prefixes) // 3,
             cache.address, items.data_ptr(), size, ctypes.byref(args))
         if status != _TOO_SMALL:
             break
