@@ -740,6 +740,26 @@ int oscar_chunk_attention(const oscar_chunk_step* step, const void* items, const
                           const oscar_heads* out, float scale, void* workspace, size_t workspace_size,
                           oscar_stream_t stream);
 
+/* ---------------------------------------------------------------- chunk attention over an 8-bit cache
+ * The same attention over oscar_append_quantized's cache: the arguments of
+ * oscar_chunk_plan_shared and oscar_chunk_attention, with this cache and step.
+ * query, out: rows of the cache's dtype.  Requests of many rows have their keys
+ * converted in the workspace, 4 bytes a value of K and V together. */
+typedef struct oscar_quant_step {
+  oscar_chunk_step chunk;
+  int64_t partials_size;
+  int32_t sources; /* ranges of keys that are converted */
+  int32_t pages;   /* of 16 keys each */
+} oscar_quant_step;
+
+int oscar_quant_plan(const int32_t* query_start_loc, const int32_t* seq_lens, int32_t num_requests, int32_t num_heads,
+                     int32_t window, const oscar_prefix* prefixes, int32_t num_prefixes,
+                     const oscar_quant_cache* cache, void* items, size_t items_size, oscar_quant_step* step);
+int oscar_quant_attention(const oscar_quant_step* step, const void* items, const int32_t* block_table,
+                          int64_t block_table_stride, const oscar_quant_cache* cache, const oscar_heads* query,
+                          const oscar_heads* out, float scale, void* workspace, size_t workspace_size,
+                          oscar_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -35,6 +35,7 @@ PER_FILE = {
     # reads them (by default kernels of more than 256 registers get them in
     # accumulation registers and a move per score).
     "chunk_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+    "quant_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
 }
 
 

@@ -2,7 +2,6 @@
 // cache that already holds their keys and values (oscar_chunk_attention).
 #include "chunk_pieces.h"
 #include "chunk_plan.h"
-#include "row_span.h"
 
 namespace oscar {
 namespace {
@@ -45,11 +44,7 @@ int launch(const ChunkArgs& a, const oscar_chunk_step& step, hipStream_t stream)
   void (*const kernels[3])(ChunkArgs) = {&narrow_kernel<T, D>, &wide_kernel<T, D>, &mixed_kernel<T, D>};
   const int which = step.wide == 0 ? 0 : step.narrow == 0 ? 1 : 2;
   kernels[which]<<<step.narrow + step.wide, kThreads, 0, stream>>>(a);
-  const int64_t blocks = (int64_t)step.few_joins * (D / 32) + (int64_t)(step.joins - step.few_joins) * (kTileRows * D / 64);
-  if (blocks > INT32_MAX) return kErrInvalidArgument;
-  if (blocks > 0 && step.parts == 0) join_kernel<T, D, false><<<(uint32_t)blocks, 256, 0, stream>>>(a);
-  else if (blocks > 0) join_kernel<T, D, true><<<(uint32_t)blocks, 256, 0, stream>>>(a);
-  return hipGetLastError() == hipSuccess ? kOk : kErrLaunch;
+  return launch_joins<T, D>(a, step, stream);
 }
 
 template <typename T>
@@ -88,7 +83,8 @@ extern "C" int oscar_chunk_plan_shared(const int32_t* query_start_loc, const int
     status = check_prefixes(prefixes, num_prefixes, query_start_loc, seq_lens, num_requests, group, window, shared);
     if (status != kOk) return status;
     Plan plan;
-    make_plan(query_start_loc, seq_lens, num_requests, group, cache->num_kv_heads, cache->head_size, window, shared, plan);
+    make_plan(query_start_loc, seq_lens, num_requests, group, cache->num_kv_heads, plain_rule(cache->head_size), window,
+              shared, plan);
     step->num_requests = num_requests;
     step->num_tokens = num_requests > 0 ? query_start_loc[num_requests] : 0;
     step->num_heads = num_heads;
@@ -127,32 +123,10 @@ extern "C" int oscar_chunk_attention(const oscar_chunk_step* step, const void* i
   if (step->narrow < 0 || step->wide < 0 || step->few_joins < 0 || step->joins < step->few_joins || step->parts < 0)
     return kErrInvalidArgument;
   if (step->narrow + step->wide == 0) return kOk;
-  if (items == nullptr || block_table == nullptr || query->data == nullptr || out->data == nullptr ||
-      block_table_stride < step->table_cols)
-    return kErrInvalidArgument;
-  if ((int64_t)workspace_size < step->workspace_size || (step->workspace_size > 0 && workspace == nullptr))
-    return kErrWorkspaceTooSmall;
   ChunkArgs a{};
-  a.q = static_cast<const uint8_t*>(query->data);
-  a.out = static_cast<uint8_t*>(out->data);
-  if (step->num_tokens > 1) {               // (a stride between rows of which there is one means nothing)
-    a.q_token = 2 * query->token_stride;
-    a.out_token = 2 * out->token_stride;
-  }
-  if (step->num_heads > 1) {
-    a.q_head = 2 * query->head_stride;
-    a.out_head = 2 * out->head_stride;
-  }
-  if (((uintptr_t)query->data | (uintptr_t)out->data | (uintptr_t)workspace | (uintptr_t)items) % 16 ||
-      (a.q_token | a.q_head | a.out_token | a.out_head) % 16 ||
-      std::min({a.q_token, a.q_head, a.out_token, a.out_head}) < 0)
-    return kErrUnsupportedGeometry;
-  // (a row is read by the workgroup that writes it, or by a launch before the one that does)
-  const RowSpan from{(uint64_t)(uintptr_t)a.q, a.q_token, a.q_head, step->num_tokens, step->num_heads,
-                     2 * cache->head_size};
-  const RowSpan to{(uint64_t)(uintptr_t)a.out, a.out_token, a.out_head, step->num_tokens, step->num_heads,
-                   2 * cache->head_size};
-  if (!same_rows(from, to) && !rows_apart(from, to)) return kErrOverlap;
+  const int bad = step_args(step, items, block_table, block_table_stride, query, out, scale, workspace, workspace_size,
+                            step->workspace_size, a);
+  if (bad != kOk) return bad;
   a.k = static_cast<const uint8_t*>(cache->k);
   a.v = static_cast<const uint8_t*>(cache->v);
   a.k_page = (uint32_t)cache->k_stride_page;
@@ -162,21 +136,6 @@ extern "C" int oscar_chunk_attention(const oscar_chunk_step* step, const void* i
   a.v_token = (int32_t)cache->v_stride_token;
   a.k_head = (int32_t)cache->k_stride_head;
   a.v_head = (int32_t)cache->v_stride_head;
-  a.table = block_table;
-  a.table_stride = block_table_stride;
-  a.pieces = static_cast<const Piece*>(items);
-  a.narrow = step->narrow;
-  a.wide = step->wide;
-  a.few_joins = step->few_joins;
-  a.joins = reinterpret_cast<const Join*>(a.pieces + step->narrow + step->wide);
-  a.parts = reinterpret_cast<const SharedPart*>(a.joins + step->joins);
-  a.partials = static_cast<float*>(workspace);
-  a.scale_log2 = scale * 1.4426950408889634f;
-  a.group = step->num_heads / cache->num_kv_heads;
-  a.block_size = cache->block_size;
-  a.window = step->window;
-  a.group_div = make_fast_div((uint32_t)a.group);
-  a.block_div = make_fast_div((uint32_t)a.block_size);
   return cache->dtype == OSCAR_BF16 ? launch_sized<__bf16>(cache->head_size, a, *step, stream)
                                     : launch_sized<_Float16>(cache->head_size, a, *step, stream);
 }

@@ -421,6 +421,79 @@ __device__ __forceinline__ uint8_t* out_row(const ChunkArgs& a, int token0, int 
   return a.out + (int64_t)(token0 + tok) * a.out_token + (int64_t)head * a.out_head;
 }
 
+// The waves' sums of a narrow piece through LDS, D / kRounds features at a time (16-byte
+// pieces, the row xor-ed in): the rows' outputs, or a partial.
+template <typename T, int D, int kRounds>
+__device__ __forceinline__ void combine_waves(const ChunkArgs& a, const Piece& p, RowState<T, D>& s, uint8_t* smem,
+                                              int tid, int lane, int wave) {
+  constexpr int kPart = D / kRounds, kTurn = kPart >= 64 ? 15 : kPart / 4 - 1;
+  float* const sums = reinterpret_cast<float*>(smem);
+  float* const ml = sums + kWaves * kTileRows * kPart;          // [wave][m | l][32]
+  s.l = sum_halves(s.l);
+  const int row = lane & 31;
+#pragma unroll
+  for (int round = 0; round < kRounds; ++round) {
+    arrive_all();
+    if (row < p.rows) {
+#pragma unroll
+      for (int b = 0; b < kPart / 32; ++b)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int piece = 8 * b + 2 * i + (lane >> 5);
+          const floatx16& acc = s.acc[round * kPart / 32 + b];
+          *reinterpret_cast<floatx4*>(sums + (wave * kTileRows + row) * kPart + 4 * (piece ^ (row & kTurn))) =
+              floatx4{acc[4 * i], acc[4 * i + 1], acc[4 * i + 2], acc[4 * i + 3]};
+        }
+      ml[wave * 64 + (lane >> 5) * 32 + row] = lane < 32 ? s.m : s.l;
+    }
+    __syncthreads();
+    // a thread to four features of some rows, kBatch of them at once
+    constexpr int kAcross = kThreads / (kPart / 4), kBatch = kAcross >= 16 ? 1 : 16 / kAcross;
+    const int piece = tid % (kPart / 4), feature = round * kPart + 4 * piece;
+    for (int r0 = tid / (kPart / 4); r0 < p.rows; r0 += kAcross * kBatch) {
+      float m[kBatch], l[kBatch];
+      floatx4 o[kBatch];
+#pragma unroll
+      for (int n = 0; n < kBatch; ++n) {
+        const int r = min(r0 + n * kAcross, p.rows - 1);
+        float wm[kWaves], wl[kWaves];
+        floatx4 x[kWaves];
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+          wm[w] = ml[w * 64 + r];
+          wl[w] = ml[w * 64 + 32 + r];
+          x[w] = *reinterpret_cast<const floatx4*>(sums + (w * kTileRows + r) * kPart + 4 * (piece ^ (r & kTurn)));
+        }
+        m[n] = fmaxf(fmaxf(wm[0], wm[1]), fmaxf(wm[2], wm[3]));
+        l[n] = 0.f;
+        o[n] = floatx4{};
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+          const float f = __builtin_amdgcn_exp2f(wm[w] - m[n]);
+          l[n] += f * wl[w];
+          o[n] += f * x[w];
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < kBatch; ++n) {
+        const int r = r0 + n * kAcross;
+        if (r >= p.rows) break;
+        if (p.slot < 0) {
+          const float inv = l[n] == 0.f ? 0.f : 1.f / l[n];
+          store4<T>(out_row(a, p.token0, p.kv_head, p.row0 + r) + 2 * feature, o[n] * inv);
+        } else {
+          float* part = a.partials + (int64_t)p.slot * (kTileRows * (D + 2));
+          *reinterpret_cast<floatx4*>(part + r * D + feature) = o[n];
+          if (feature == 0) {
+            part[kTileRows * D + r] = m[n];
+            part[kTileRows * D + kTileRows + r] = l[n];
+          }
+        }
+      }
+    }
+  }
+}
+
 // ---------------------------------------------------------------- 32 rows
 // One row tile, its keys shared out to four waves that walk their tiles on
 // their own (no barrier until they combine): few rows, so memory bounds it, and
@@ -540,74 +613,7 @@ __device__ __forceinline__ void narrow_piece(const ChunkArgs& a, const Piece p, 
   if (__builtin_expect(special, 0))
     for (int t = first; t < last; ++t) add_special<T, D, kKeys>(a, p, t * kKeys, whole(t * kKeys), lane, s);
 
-  // Combine: the waves' sums through LDS, D / kRounds features at a time (16-byte
-  // pieces, the row xor-ed in).
-  constexpr int kRounds = 32 / kKeys, kPart = D / kRounds;
-  float* const sums = reinterpret_cast<float*>(smem);
-  float* const ml = sums + kWaves * kTileRows * kPart;          // [wave][m | l][32]
-  s.l = sum_halves(s.l);
-  const int row = lane & 31;
-#pragma unroll
-  for (int round = 0; round < kRounds; ++round) {
-    arrive_all();
-    if (row < p.rows) {
-#pragma unroll
-      for (int b = 0; b < kPart / 32; ++b)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int piece = 8 * b + 2 * i + (lane >> 5);
-          const floatx16& acc = s.acc[round * kPart / 32 + b];
-          *reinterpret_cast<floatx4*>(sums + (wave * kTileRows + row) * kPart + 4 * (piece ^ (row & 15))) =
-              floatx4{acc[4 * i], acc[4 * i + 1], acc[4 * i + 2], acc[4 * i + 3]};
-        }
-      ml[wave * 64 + (lane >> 5) * 32 + row] = lane < 32 ? s.m : s.l;
-    }
-    __syncthreads();
-    // a thread to four features of some rows, kBatch of them at once
-    constexpr int kAcross = kThreads / (kPart / 4), kBatch = kAcross >= 16 ? 1 : 16 / kAcross;
-    const int piece = tid % (kPart / 4), feature = round * kPart + 4 * piece;
-    for (int r0 = tid / (kPart / 4); r0 < p.rows; r0 += kAcross * kBatch) {
-      float m[kBatch], l[kBatch];
-      floatx4 o[kBatch];
-#pragma unroll
-      for (int n = 0; n < kBatch; ++n) {
-        const int r = min(r0 + n * kAcross, p.rows - 1);
-        float wm[kWaves], wl[kWaves];
-        floatx4 x[kWaves];
-#pragma unroll
-        for (int w = 0; w < kWaves; ++w) {
-          wm[w] = ml[w * 64 + r];
-          wl[w] = ml[w * 64 + 32 + r];
-          x[w] = *reinterpret_cast<const floatx4*>(sums + (w * kTileRows + r) * kPart + 4 * (piece ^ (r & 15)));
-        }
-        m[n] = fmaxf(fmaxf(wm[0], wm[1]), fmaxf(wm[2], wm[3]));
-        l[n] = 0.f;
-        o[n] = floatx4{};
-#pragma unroll
-        for (int w = 0; w < kWaves; ++w) {
-          const float f = __builtin_amdgcn_exp2f(wm[w] - m[n]);
-          l[n] += f * wl[w];
-          o[n] += f * x[w];
-        }
-      }
-#pragma unroll
-      for (int n = 0; n < kBatch; ++n) {
-        const int r = r0 + n * kAcross;
-        if (r >= p.rows) break;
-        if (p.slot < 0) {
-          const float inv = l[n] == 0.f ? 0.f : 1.f / l[n];
-          store4<T>(out_row(a, p.token0, p.kv_head, p.row0 + r) + 2 * feature, o[n] * inv);
-        } else {
-          float* part = a.partials + (int64_t)p.slot * (kTileRows * (D + 2));
-          *reinterpret_cast<floatx4*>(part + r * D + feature) = o[n];
-          if (feature == 0) {
-            part[kTileRows * D + r] = m[n];
-            part[kTileRows * D + kTileRows + r] = l[n];
-          }
-        }
-      }
-    }
-  }
+  combine_waves<T, D, 32 / kKeys>(a, p, s, smem, tid, lane, wave);
 }
 
 // ---------------------------------------------------------------- 128 rows

@@ -2,6 +2,7 @@
 #pragma once
 
 #include "chunk_pieces.h"
+#include "row_span.h"
 
 #include <algorithm>
 #include <cstddef>
@@ -27,6 +28,21 @@ struct Prefix {
 struct PrefixRows {
   int32_t slot0 = -1, groups = 0, pieces = 0;
 };
+
+// What a cache asks of the plan.
+struct PlanRule {
+  int32_t head_size;
+  int32_t narrow_rows;     // of a request and kv head, at most
+  int32_t resident[2];     // narrow pieces that read at full rate, and that fit the GPU at once
+  double key_bytes;        // of a key's features, read
+};
+inline PlanRule plain_rule(int32_t head_size) {
+  // Up to 32 rows a request is narrow (28 rows of 16 users over 1000 keys, D = 128: 20.4
+  // us, as wide tiles 24.2; 30 of 8 users over 16000, D = 256, 31.1, 30.1), from 33 on
+  // wide, where narrow tiles would read its keys twice (48 rows, the same: 24.7 us, as
+  // narrow 23.2; 32.2, 36.1; 32 users over 4000 32.5, 49.6).
+  return PlanRule{head_size, kTileRows, {kCus, kCus * narrow_wgs(head_size)}, 2.};
+}
 
 struct RowTile {
   Piece piece;
@@ -138,7 +154,7 @@ int32_t pieces_of(const RowTile& x, int64_t per) { return (int32_t)((x.tiles + p
 // 256, 190 us, 5.2 TB/s), but one request that is far longer than the others is then
 // read by one workgroup (300 users of 1000 keys and one of 131072 2.2 ms, where the
 // bytes take 0.09), and by a few where there are just fewer (250 and one: 0.39 ms).
-void plan_narrow(const std::vector<RowTile>& rows, int32_t head_size, double beside, Plan& plan,
+void plan_narrow(const std::vector<RowTile>& rows, const PlanRule& rule, double beside, Plan& plan,
                  std::vector<PrefixRows>& prefixes) {
   int64_t total = 0;
   int32_t most = 0;
@@ -146,7 +162,7 @@ void plan_narrow(const std::vector<RowTile>& rows, int32_t head_size, double bes
     total += x.tiles;
     most = std::max(most, x.tiles);
   }
-  const int32_t uncut = head_size == 256 ? 8 : 16;
+  const int32_t uncut = rule.head_size == 256 ? 8 : 16;
   auto fit = [&](int64_t resident) {
     int64_t per = std::max<int64_t>(kWaves, (total + resident - 1) / resident);
     auto count = [&](int64_t t) {
@@ -164,9 +180,10 @@ void plan_narrow(const std::vector<RowTile>& rows, int32_t head_size, double bes
     }
     return per;
   };
-  int64_t per = fit(beside == 0. ? kCus : total > 240 * beside ? 2 * kCus : 2 * kCus / 3);
-  if (beside == 0. && (rows.size() >= kCus || 100 * per * kCus > 115 * total))
-    per = fit((int64_t)kCus * narrow_wgs(head_size));
+  const bool reading = total * rule.key_bytes > 2 * 240 * beside;
+  int64_t per = fit(beside == 0. ? rule.resident[0] : reading ? 2 * kCus : 2 * kCus / 3);
+  if (beside == 0. && ((int64_t)rows.size() >= rule.resident[0] || 100 * per * rule.resident[0] > 115 * total))
+    per = fit(rule.resident[1]);
   for (const RowTile& x : rows) cut(x, pieces_of(x, per), plan, prefixes, plan.narrow);
 }
 
@@ -238,11 +255,7 @@ double plan_wide(const std::vector<RowTile>& rows, int32_t head_size, Plan& plan
 }
 
 void make_plan(const int32_t* qsl, const int32_t* seqs, int32_t num_requests, int32_t group, int32_t kv_heads,
-               int32_t head_size, int32_t window, const std::vector<Prefix>& shared, Plan& plan) {
-  // Up to 32 rows a request is narrow (28 rows of 16 users over 1000 keys, D = 128: 20.4
-  // us, as wide tiles 24.2; 30 of 8 users over 16000, D = 256, 31.1, 30.1), from 33 on
-  // wide, where narrow tiles would read its keys twice (48 rows, the same: 24.7 us, as
-  // narrow 23.2; 32.2, 36.1; 32 users over 4000 32.5, 49.6).  So are the rows of a prefix.
+               const PlanRule& rule, int32_t window, const std::vector<Prefix>& shared, Plan& plan) {
   std::vector<RowTile> narrow, wide;
   std::vector<PrefixRows> prefixes;
   auto prefix = shared.begin();
@@ -260,7 +273,7 @@ void make_plan(const int32_t* qsl, const int32_t* seqs, int32_t num_requests, in
       PrefixRows rows;
       rows.groups = (tokens * group + kTileRows - 1) / kTileRows;
       prefixes.insert(prefixes.end(), kv_heads, rows);
-      if (tokens * (int64_t)group <= kTileRows)
+      if (tokens * (int64_t)group <= rule.narrow_rows)
         prefix_tiles(qsl[i], tokens, keys, table_row, group, kv_heads, kTileRows, at, narrow);
       else
         prefix_tiles(qsl[i], tokens, keys, table_row, group, kv_heads, kWideRows, at, wide);
@@ -268,13 +281,13 @@ void make_plan(const int32_t* qsl, const int32_t* seqs, int32_t num_requests, in
     }
     const int32_t with = keys > 0 ? (int32_t)prefixes.size() - kv_heads : -1;
     const int32_t row = keys > 0 ? (qsl[i] - first_token) * group : 0;
-    if (n * (int64_t)group <= kTileRows)
+    if (n * (int64_t)group <= rule.narrow_rows)
       row_tiles(qsl[i], n, seqs[i], i, group, kv_heads, window, kTileRows, narrow, keys, with, row);
     else
       row_tiles(qsl[i], n, seqs[i], i, group, kv_heads, window, kWideRows, wide, keys, with, row);
   }
-  const double beside = wide.empty() ? 0. : plan_wide(wide, head_size, plan, prefixes);
-  if (!narrow.empty()) plan_narrow(narrow, head_size, beside, plan, prefixes);
+  const double beside = wide.empty() ? 0. : plan_wide(wide, rule.head_size, plan, prefixes);
+  if (!narrow.empty()) plan_narrow(narrow, rule, beside, plan, prefixes);
   for (SharedPart& p : plan.parts) {
     const PrefixRows& rows = prefixes[p.slot0];
     p = SharedPart{rows.slot0, rows.groups, rows.pieces, p.row};
@@ -348,6 +361,62 @@ int pack_plan(const Plan& plan, int32_t head_size, void* items, size_t items_siz
     to += size[i];
   }
   return kOk;
+}
+
+// A plan's arguments that go by the step, the rows and the items; what a cache adds is
+// left to the caller.
+int step_args(const oscar_chunk_step* step, const void* items, const int32_t* block_table, int64_t block_table_stride,
+              const oscar_heads* query, const oscar_heads* out, float scale, void* workspace, size_t workspace_size,
+              int64_t need, ChunkArgs& a) {
+  if (items == nullptr || block_table == nullptr || query->data == nullptr || out->data == nullptr ||
+      block_table_stride < step->table_cols)
+    return kErrInvalidArgument;
+  if ((int64_t)workspace_size < need || (need > 0 && workspace == nullptr)) return kErrWorkspaceTooSmall;
+  a.q = static_cast<const uint8_t*>(query->data);
+  a.out = static_cast<uint8_t*>(out->data);
+  if (step->num_tokens > 1) {               // (a stride between rows of which there is one means nothing)
+    a.q_token = 2 * query->token_stride;
+    a.out_token = 2 * out->token_stride;
+  }
+  if (step->num_heads > 1) {
+    a.q_head = 2 * query->head_stride;
+    a.out_head = 2 * out->head_stride;
+  }
+  if (((uintptr_t)query->data | (uintptr_t)out->data | (uintptr_t)workspace | (uintptr_t)items) % 16 ||
+      (a.q_token | a.q_head | a.out_token | a.out_head) % 16 ||
+      std::min({a.q_token, a.q_head, a.out_token, a.out_head}) < 0)
+    return kErrUnsupportedGeometry;
+  // (a row is read by the workgroup that writes it, or by a launch before the one that does)
+  const RowSpan from{(uint64_t)(uintptr_t)a.q, a.q_token, a.q_head, step->num_tokens, step->num_heads,
+                     2 * step->head_size};
+  const RowSpan to{(uint64_t)(uintptr_t)a.out, a.out_token, a.out_head, step->num_tokens, step->num_heads,
+                   2 * step->head_size};
+  if (!same_rows(from, to) && !rows_apart(from, to)) return kErrOverlap;
+  a.table = block_table;
+  a.table_stride = block_table_stride;
+  a.pieces = static_cast<const Piece*>(items);
+  a.narrow = step->narrow;
+  a.wide = step->wide;
+  a.few_joins = step->few_joins;
+  a.joins = reinterpret_cast<const Join*>(a.pieces + step->narrow + step->wide);
+  a.parts = reinterpret_cast<const SharedPart*>(a.joins + step->joins);
+  a.partials = static_cast<float*>(workspace);
+  a.scale_log2 = scale * 1.4426950408889634f;
+  a.group = step->num_heads / step->num_kv_heads;
+  a.block_size = step->block_size;
+  a.window = step->window;
+  a.group_div = make_fast_div((uint32_t)a.group);
+  a.block_div = make_fast_div((uint32_t)a.block_size);
+  return kOk;
+}
+
+template <typename T, int D>
+int launch_joins(const ChunkArgs& a, const oscar_chunk_step& step, hipStream_t stream) {
+  const int64_t blocks = (int64_t)step.few_joins * (D / 32) + (int64_t)(step.joins - step.few_joins) * (kTileRows * D / 64);
+  if (blocks > INT32_MAX) return kErrInvalidArgument;
+  if (blocks > 0 && step.parts == 0) join_kernel<T, D, false><<<(uint32_t)blocks, 256, 0, stream>>>(a);
+  else if (blocks > 0) join_kernel<T, D, true><<<(uint32_t)blocks, 256, 0, stream>>>(a);
+  return hipGetLastError() == hipSuccess ? kOk : kErrLaunch;
 }
 
 }  // namespace

@@ -95,6 +95,8 @@ SIGNATURES = {
     "oscar_chunk_plan": (_c_i32, [_c_p, _c_p, _c_i32, _c_i32, _c_i32, _c_p, _c_p, _c_sz, _c_p]),
     "oscar_chunk_plan_shared": (_c_i32, [_c_p, _c_p, _c_i32, _c_i32, _c_i32, _c_p, _c_i32, _c_p, _c_p, _c_sz, _c_p]),
     "oscar_chunk_attention": (_c_i32, [_c_p, _c_p, _c_p, _c_i64, _c_p, _c_p, _c_p, _c_f32, _c_p, _c_sz, _c_p]),
+    "oscar_quant_plan": (_c_i32, [_c_p, _c_p, _c_i32, _c_i32, _c_i32, _c_p, _c_i32, _c_p, _c_p, _c_sz, _c_p]),
+    "oscar_quant_attention": (_c_i32, [_c_p, _c_p, _c_p, _c_i64, _c_p, _c_p, _c_p, _c_f32, _c_p, _c_sz, _c_p]),
 }
 
 STATUS = {

@@ -106,7 +106,7 @@ class QuantCache:
         self.args = QuantCacheArgs(k_codes.data_ptr(), v_codes.data_ptr(), exponents.data_ptr(), pages, *strides, bs, hk,
                                    d, _rotary.DTYPES[dtype])
         self.address = ctypes.addressof(self.args)
-        self.geometry = (hk, d, bs)
+        self.geometry = (hk, d, bs, 8)     # (never a plain cache's)
 
 
 def _code_strides(x: torch.Tensor) -> tuple[int, int, int]:

@@ -11,7 +11,7 @@ import ctypes
 import torch
 
 from . import _lib, decode, rotary as _rotary
-from .append import PagedCache
+from .append import PagedCache, QuantCache
 
 HEAD_SIZES = (64, 128, 256)
 MAX_HEADS = 1 << 16
@@ -28,6 +28,11 @@ class ChunkStepArgs(ctypes.Structure):
                 ("table_cols", _i32), ("narrow", _i32), ("wide", _i32), ("joins", _i32), ("few_joins", _i32),
                 ("num_kv_heads", _i32), ("head_size", _i32), ("block_size", _i32), ("items_size", _i64),
                 ("workspace_size", _i64), ("parts", _i32), ("reserved", _i32)]
+
+
+class QuantStepArgs(ctypes.Structure):
+    """struct oscar_quant_step (include/oscar_amd.h)."""
+    _fields_ = [("chunk", ChunkStepArgs), ("partials_size", _i64), ("sources", _i32), ("pages", _i32)]
 
 
 class ChunkStep:
@@ -72,11 +77,12 @@ class ChunkStep:
         if layout.qsl and layout.qsl[0] < 0:
             raise ValueError("query starts are counted from the step's token 0")
         prefixes = _check_prefixes(prefixes, layout, window)
-        args = ChunkStepArgs()
+        args = QuantStepArgs() if isinstance(cache, QuantCache) else ChunkStepArgs()
         items = (_plan(layout, requests, num_heads, window, cache, args) if prefixes is None else
                  _plan(layout, requests, num_heads, window, cache, args, prefixes))
-        if block_tables.ndim != 2 or block_tables.shape[0] < requests or block_tables.shape[1] < args.table_cols:
-            raise ValueError(f"block table must be [requests, pages] with the {args.table_cols} pages of the longest")
+        sizes = args.chunk if isinstance(args, QuantStepArgs) else args
+        if block_tables.ndim != 2 or block_tables.shape[0] < requests or block_tables.shape[1] < sizes.table_cols:
+            raise ValueError(f"block table must be [requests, pages] with the {sizes.table_cols} pages of the longest")
         if block_tables.dtype not in (torch.int32, torch.int64, torch.int16, torch.int8, torch.uint8):
             raise ValueError(f"block tables hold integers, got {block_tables.dtype}")
         if block_tables.device != cache.device:
@@ -92,7 +98,7 @@ class ChunkStep:
         if torch.cuda.is_current_stream_capturing():
             raise ValueError("a step is built before its calls are captured")
         with torch.cuda.device(device):
-            host = torch.empty(max(args.items_size, 16), dtype=torch.uint8, pin_memory=True)
+            host = torch.empty(max(sizes.items_size, 16), dtype=torch.uint8, pin_memory=True)
             host.copy_(items[:host.numel()])
             self.items = host.to(device, non_blocking=True)
             self.ready = torch.cuda.Event()
@@ -100,9 +106,9 @@ class ChunkStep:
             self.stream = _lib.stream_handle(device)
         self.args = args
         self.address = ctypes.addressof(args)
-        self.tokens = args.num_tokens
+        self.tokens = sizes.num_tokens
         self.num_heads = num_heads
-        self.workspace_size = args.workspace_size
+        self.workspace_size = sizes.workspace_size
         self.geometry = cache.geometry
         self.device = device
         self.block_tables = block_tables
@@ -149,7 +155,8 @@ def chunk_attention(query: torch.Tensor, cache: PagedCache, step: ChunkStep, sca
         step._join(device)
     need = step.workspace_size
     ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
-    _lib.call_on(device, "oscar_chunk_attention", step.address, step.items_ptr, step.table_ptr, step.table_stride,
+    entry = "oscar_quant_attention" if isinstance(cache, QuantCache) else "oscar_chunk_attention"
+    _lib.call_on(device, entry, step.address, step.items_ptr, step.table_ptr, step.table_stride,
                  cache.address, q, o, scale, None if ws is None else ws.data_ptr(), need)
     return out
 
@@ -173,22 +180,24 @@ def _check_prefixes(prefixes, layout, window: int):
     return (_i32 * len(flat))(*flat)
 
 
-def _plan(layout, requests: int, num_heads: int, window: int, cache: PagedCache, args: ChunkStepArgs,
-          prefixes=None) -> torch.Tensor:
+def _plan(layout, requests: int, num_heads: int, window: int, cache: PagedCache | QuantCache,
+          args: ChunkStepArgs | QuantStepArgs, prefixes=None) -> torch.Tensor:
     """The step's items (host bytes), its sizes in args.  Planned straight into
     128 KB, which most steps' items fit; a step that needs more is planned again."""
+    entry, sizes = (("oscar_quant_plan", args.chunk) if isinstance(cache, QuantCache) else
+                    ("oscar_chunk_plan_shared", args))
     size = 1 << 17
     while True:
         items = torch.empty(size, dtype=torch.uint8)
-        status = _lib.load().oscar_chunk_plan_shared(
+        status = getattr(_lib.load(), entry)(
             ctypes.addressof(layout.qstart), ctypes.addressof(layout.seq_t), requests, num_heads, window,
             None if prefixes is None else ctypes.addressof(prefixes), 0 if prefixes is None else len(prefixes) // 3,
             cache.address, items.data_ptr(), size, ctypes.byref(args))
         if status != _TOO_SMALL:
             break
-        size = args.items_size
+        size = sizes.items_size
     if status != 0:
-        raise _lib.OscarKernelError(f"oscar_chunk_plan failed: {_lib.STATUS.get(status, status)}")
+        raise _lib.OscarKernelError(f"{entry} failed: {_lib.STATUS.get(status, status)}")
     return items
 
 
