@@ -28,18 +28,19 @@ constexpr int kNormThreads = 256;
 constexpr int kMaxTokens = 16;             // of a workgroup at a time
 constexpr int kMaxRotary = 256;
 constexpr int64_t kLastCache = 256ll << 20;      // bytes
-constexpr int kBackBlocks = 2048;          // workgroups of the gradient, at most
+constexpr int kBackBlocks = 1024;          // workgroups of the gradient, at most
 
 enum Target { kRows, kPlain, kQuant };
 
-// What a launch does with one kind of rows.
+// What a launch does with one kind of rows: workgroups of its own, block_tokens tokens each.
 struct NormJob {
   const uint8_t* src;
   uint8_t* dst;            // rows of their own, or a cache
   const uint8_t* grad;     // of the gradient: the outputs'
   const void* weight;      // null: no norm
   uint32_t src_token, src_head, dst_token, dst_head, grad_token, grad_head;   // bytes; in a cache dst_token is not used
-  int32_t heads;
+  int32_t heads, half;     // half: rotary_dim / 2, or 0 for rows that do not turn
+  int32_t block_tokens, first_block;
   FastDiv by_heads;
 };
 enum { kQuery, kKey, kValue, kJobs };
@@ -55,12 +56,12 @@ struct NormArgs {
   uint8_t* exponents;      // [page][head][token][K | V]
   int32_t block_size, block_shift;         // shift: log2, or -1
   int32_t low, high;       // exponents
-  int32_t axes, half, adjacent;            // half: rotary_dim / 2
-  int32_t block_tokens;
-  int32_t d, lanes;        // lanes of a head
+  int32_t axes, half;      // half: rotary_dim / 2
+  int32_t adjacent;
+  int32_t d, lanes, lane_shift;            // lanes of a head
   int32_t weight_type;
   float eps, offset, per_d;
-  float* partials;         // of the weights' gradients: [workgroup][query | key][D]
+  float* partials;         // of the weights' gradients: [workgroup][D], queries' first
   FastDiv by_half;
 };
 
@@ -88,9 +89,11 @@ __device__ __forceinline__ float group_max(float x, int lanes) {
   return over_group(x, lanes, [](float a, float b) { return fmaxf(a, b); });
 }
 
-// A lane's part of a head: kSlots places, each two pieces of kVec features whose
-// values pair up: x[0][i] with x[1][i].  kVec is 8 where rows, strides and pairs are
-// multiples of 16 bytes, else 1 (a model's head size and projection decide).
+// A lane's part of a head: kSlots places, each two pieces of kVec features in the order
+// of memory.  kVec is 8 where rows, strides and pairs are multiples of 16 bytes, else 1
+// (a model's head size and projection decide).  Pairs that turn together are both of one
+// lane: the pieces' features of one index, or, where pairs are adjacent and kVec is 8,
+// neighbours in a piece.
 template <int kVec>
 struct Part {
   static constexpr int kSlots = kVec == 8 ? 1 : 2, kPairs = kSlots * kVec;
@@ -116,8 +119,7 @@ __device__ __forceinline__ Place place_of(const NormArgs& a, int half, int u) {
 template <typename T, int kVec, bool kOnce>
 struct Piece8 {
   typedef T Row __attribute__((ext_vector_type(8)));
-  typedef u32x4 Chunk[sizeof(T) / 2];
-  Chunk c;
+  u32x4 c[sizeof(T) / 2];
   __device__ __forceinline__ void load(const T* at) {
     const u32x4* p = reinterpret_cast<const u32x4*>(at);
 #pragma unroll
@@ -165,110 +167,121 @@ struct RawPart {
         p[s][1].load(row + at[s].second);
       }
   }
-};
-
-// Adjacent pairs (x0, x1), (x2, x3) .. of two pieces of 8 as first and second
-// partners, and back.
-template <int kVec>
-__device__ __forceinline__ void part_pairs(Part<kVec>& f) {
-  if constexpr (kVec == 8) {
-    float y[2][8];
+  // Its values (zeros where the lane has none).
+  __device__ __forceinline__ void get(const Place (&at)[Part<kVec>::kSlots], Part<kVec>& f) const {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      y[0][i] = f.x[i >> 2][2 * (i & 3)];
-      y[1][i] = f.x[i >> 2][2 * (i & 3) + 1];
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) f.x[0][i] = y[0][i], f.x[1][i] = y[1][i];
-  }
-}
-template <int kVec>
-__device__ __forceinline__ void join_pairs(Part<kVec>& f) {
-  if constexpr (kVec == 8) {
-    float y[2][8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      y[i >> 2][2 * (i & 3)] = f.x[0][i];
-      y[i >> 2][2 * (i & 3) + 1] = f.x[1][i];
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) f.x[0][i] = y[0][i], f.x[1][i] = y[1][i];
-  }
-}
-
-// The values of a raw part, partners in x[0] and x[1] (zeros where the lane has none).
-template <typename T, int kVec, bool kOnce>
-__device__ __forceinline__ void values_of(const RawPart<T, kVec, kOnce>& raw, const Place (&at)[Part<kVec>::kSlots],
-                                          bool paired, Part<kVec>& f) {
-#pragma unroll
-  for (int s = 0; s < Part<kVec>::kSlots; ++s)
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
+    for (int s = 0; s < Part<kVec>::kSlots; ++s) {
       if (at[s].there) {
-        raw.p[s][e].get(&f.x[e][kVec * s]);
+        p[s][0].get(&f.x[0][kVec * s]);
+        p[s][1].get(&f.x[1][kVec * s]);
       } else {
 #pragma unroll
-        for (int i = 0; i < kVec; ++i) f.x[e][kVec * s + i] = 0.f;
+        for (int i = 0; i < kVec; ++i) f.x[0][kVec * s + i] = f.x[1][kVec * s + i] = 0.f;
       }
     }
-  if (paired) part_pairs<kVec>(f);
-}
-
-// weight + offset of the lane's features (1 where there is no norm).
-template <int kVec>
-__device__ __forceinline__ void load_weights(const NormArgs& a, const void* weight,
-                                             const Place (&at)[Part<kVec>::kSlots], bool paired, Part<kVec>& w) {
+  }
+};
+template <typename T, int kVec, bool kOnce>
+__device__ __forceinline__ void store_part(T* row, const Place (&at)[Part<kVec>::kSlots], const Part<kVec>& f) {
 #pragma unroll
   for (int s = 0; s < Part<kVec>::kSlots; ++s)
+    if (at[s].there) {
+      Piece8<T, kVec, kOnce> p, q;
+      p.put(&f.x[0][kVec * s]);
+      q.put(&f.x[1][kVec * s]);
+      p.store(row + at[s].first);
+      q.store(row + at[s].second);
+    }
+}
+
+// Eight (or one) consecutive floats of LDS.
+template <int kVec>
+__device__ __forceinline__ void read_floats(const float* from, float* to) {
+  if constexpr (kVec == 8) {
+    const floatx4 lo = *reinterpret_cast<const floatx4*>(from), hi = *reinterpret_cast<const floatx4*>(from + 4);
 #pragma unroll
-    for (int e = 0; e < 2; ++e)
+    for (int i = 0; i < 4; ++i) to[i] = lo[i], to[4 + i] = hi[i];
+  } else {
+    *to = *from;
+  }
+}
+
+// R(p) x of a part, with the cosines and sines [cos | sin] of its token at `cs`; kBack:
+// R(p)^T x.
+template <int kVec, bool kAdjacent, bool kBack>
+__device__ __forceinline__ void turn_part(const float* cs, int half, const Place (&at)[Part<kVec>::kSlots], int u0,
+                                          int lanes, Part<kVec>& f) {
 #pragma unroll
-      for (int i = 0; i < kVec; ++i) {
-        float v = 1.f;
-        if (weight != nullptr && at[s].there) {
-          const int f = (e == 0 ? at[s].first : at[s].second) + i;
-          v = a.weight_type == OSCAR_FP32   ? static_cast<const float*>(weight)[f]
-              : a.weight_type == OSCAR_BF16 ? (float)static_cast<const __bf16*>(weight)[f]
-                                            : (float)static_cast<const _Float16*>(weight)[f];
-          v += a.offset;
+  for (int s = 0; s < Part<kVec>::kSlots; ++s)
+    if (at[s].turns) {
+      float c[kVec], sn[kVec];
+      read_floats<kVec>(cs + kVec * (u0 + s * lanes), c);
+      read_floats<kVec>(cs + half + kVec * (u0 + s * lanes), sn);
+      auto turn = [&](float& x1, float& x2, int i) __attribute__((always_inline)) {
+        const float a = x1, b = x2, t = kBack ? -sn[i] : sn[i];
+        x1 = a * c[i] - b * t;
+        x2 = b * c[i] + a * t;
+      };
+      if constexpr (kVec == 8 && kAdjacent) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          turn(f.x[0][2 * i], f.x[0][2 * i + 1], i);
+          turn(f.x[1][2 * i], f.x[1][2 * i + 1], 4 + i);
         }
-        w.x[e][kVec * s + i] = v;
+      } else {
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) turn(f.x[0][kVec * s + i], f.x[1][kVec * s + i], i);
       }
-  if (paired) part_pairs<kVec>(w);
-}
-
-// Cosines and sines (or 1 and 0) of the lane's pairs of a token.
-template <int kVec>
-__device__ __forceinline__ void load_turn(const float* cs, int half, const Place (&at)[Part<kVec>::kSlots], int u0,
-                                          int lanes, Part<kVec>& t) {
-#pragma unroll
-  for (int s = 0; s < Part<kVec>::kSlots; ++s)
-#pragma unroll
-    for (int i = 0; i < kVec; ++i) {
-      const int pair = kVec * (u0 + s * lanes) + i;
-      t.x[0][kVec * s + i] = at[s].turns ? cs[pair] : 1.f;
-      t.x[1][kVec * s + i] = at[s].turns ? cs[half + pair] : 0.f;
     }
 }
 
 struct TokenState {
   float cs[kMaxTokens * kMaxRotary];       // [token][cos | sin]
-  int64_t at_k[kMaxTokens], at_v[kMaxTokens], at_e[kMaxTokens];   // byte offset of the slot, -1: none
+  float weight[256];                       // weight + offset
+  int64_t at[kMaxTokens], at_e[kMaxTokens];        // byte offsets of the slot and of its power
   int live[kMaxTokens];
 };
 
-// The tokens' cosines and sines, whether their positions exist, and their slots.
-template <int kTarget>
-__device__ __forceinline__ void collect_tokens(const NormArgs& a, int64_t tok0, int tokens, TokenState& st) {
+// weight + offset of a kind (1 where there is no norm).
+__device__ __forceinline__ void collect_weights(const NormArgs& a, const void* weight, TokenState& st) {
+  const int f = (int)threadIdx.x;
+  if (f >= a.d) return;
+  float v = 1.f;
+  if (weight != nullptr) {
+    if (a.weight_type == OSCAR_FP32) v = static_cast<const float*>(weight)[f];
+    else if (a.weight_type == OSCAR_BF16) v = (float)static_cast<const __bf16*>(weight)[f];
+    else v = (float)static_cast<const _Float16*>(weight)[f];
+    v += a.offset;
+  }
+  st.weight[f] = v;
+}
+template <int kVec>
+__device__ __forceinline__ void load_weights(const float* from, const Place (&at)[Part<kVec>::kSlots], Part<kVec>& w) {
+#pragma unroll
+  for (int s = 0; s < Part<kVec>::kSlots; ++s) {
+    if (at[s].there) {
+      read_floats<kVec>(from + at[s].first, &w.x[0][kVec * s]);
+      read_floats<kVec>(from + at[s].second, &w.x[1][kVec * s]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kVec; ++i) w.x[0][kVec * s + i] = w.x[1][kVec * s + i] = 0.f;
+    }
+  }
+}
+
+// The tokens' cosines and sines (of rows that turn), whether their positions exist, and,
+// in a cache, their slots.
+__device__ __forceinline__ void collect_tokens(const NormArgs& a, const NormJob& j, bool cached, bool value,
+                                               int64_t tok0, int tokens, TokenState& st) {
   const int tid = (int)threadIdx.x, width = 2 * a.half;
-  for (int i = tid; i < tokens * a.half; i += kNormThreads) {
+  for (int i = tid; i < tokens * j.half; i += kNormThreads) {
     const int t = (int)fast_div((uint32_t)i, a.by_half);
-    const int j = i - t * a.half;
-    const int axis = (int)(a.pair_axis[j >> 5] >> (2 * (j & 31))) & 3;
+    const int p = i - t * a.half;
+    const int axis = (int)(a.pair_axis[p >> 5] >> (2 * (p & 31))) & 3;
     const int64_t pos = a.positions[axis * a.axis_stride + tok0 + t];
     const float* row = a.table + (pos >= 0 && pos < a.table_rows ? pos : 0) * width;
-    st.cs[t * width + j] = row[j];
-    st.cs[t * width + a.half + j] = row[a.half + j];
+    st.cs[t * width + p] = row[p];
+    st.cs[t * width + a.half + p] = row[a.half + p];
   }
   if (tid < tokens) {
     bool in = true;
@@ -276,18 +289,24 @@ __device__ __forceinline__ void collect_tokens(const NormArgs& a, int64_t tok0, 
       const int64_t pos = a.positions[x * a.axis_stride + tok0 + tid];
       in = in && pos >= 0 && pos < a.table_rows;
     }
-    st.live[tid] = in;
-    if constexpr (kTarget != kRows) {
+    if (cached) {
       const int64_t slot = a.slots[tok0 + tid];
       const bool write = slot >= 0 && slot < a.num_slots;
       const int64_t s = write ? slot : 0;
       const int64_t page = a.block_shift >= 0 ? s >> a.block_shift : s / a.block_size;
       const int64_t in_page = s - page * a.block_size;
-      st.at_k[tid] = write ? page * a.k_page + in_page * a.k_token : -1;
-      st.at_v[tid] = write ? page * a.v_page + in_page * a.v_token : -1;
-      st.at_e[tid] = 2 * (page * a.job[kKey].heads * a.block_size + in_page);
+      st.at[tid] = value ? page * a.v_page + in_page * a.v_token : page * a.k_page + in_page * a.k_token;
+      st.at_e[tid] = 2 * (page * j.heads * a.block_size + in_page) + (value ? 1 : 0);
+      in = in && write;
     }
+    st.live[tid] = in;
   }
+}
+
+// 1 / sqrt(x); the instruction takes no subnormal numbers.
+__device__ __forceinline__ float inverse_root(float x) {
+  const bool tiny = x < 1.2e-29f;          // 2^-96
+  return __builtin_amdgcn_rsqf(tiny ? x * 0x1p64f : x) * (tiny ? 0x1p32f : 1.f);
 }
 
 // One row of 8 bits: the power of two, its byte, and the codes.
@@ -319,272 +338,198 @@ __device__ __forceinline__ void store_codes(const NormArgs& a, const Part<kVec>&
   }
 }
 
-// Rows of a kind: job kJob's (token, head) rows of the workgroup's tokens, `lanes` lanes
-// each.  Every job's first rows are requested before the cosines are collected.
-template <typename T, int kVec, int kTarget, bool kOnce>
-__global__ __launch_bounds__(kNormThreads) void norm_kernel(NormArgs a) {
-  constexpr int kSlots = Part<kVec>::kSlots;
-  __shared__ __attribute__((aligned(16))) TokenState st;
-  const int tid = (int)threadIdx.x;
-  const int group = tid / a.lanes, u0 = tid - group * a.lanes, groups = kNormThreads / a.lanes;
-  const int64_t tok0 = (int64_t)blockIdx.x * a.block_tokens;
-  const int tokens = (int)min((int64_t)a.block_tokens, a.tokens - tok0);
-
-  struct Work {
-    RawPart<T, kVec, kOnce> raw;
-    int token, head;
-  };
-  Place turning[kSlots], still[kSlots];
-#pragma unroll
-  for (int s = 0; s < kSlots; ++s) {
-    turning[s] = place_of<kVec>(a, a.half, u0 + s * a.lanes);
-    still[s] = place_of<kVec>(a, 0, u0 + s * a.lanes);
-  }
-  auto places = [&](auto tag) -> const Place(&)[kSlots] {
-    if constexpr (decltype(tag)::value == kValue) return still;
-    else return turning;
-  };
-  auto fetch = [&](auto tag, int idx, Work& w) {
-    const NormJob& j = a.job[decltype(tag)::value];
-    w.token = (int)fast_div((uint32_t)idx, j.by_heads);
-    w.head = idx - w.token * j.heads;
-    w.raw.load(reinterpret_cast<const T*>(j.src + tok0 * j.src_token + (uint64_t)(uint32_t)w.token * j.src_token +
-                                          (uint64_t)(uint32_t)w.head * j.src_head), places(tag));
-  };
-  auto finish = [&](auto tag, const Work& w, const Part<kVec>& weight) {
-    constexpr int kJob = decltype(tag)::value;
-    constexpr bool kCache = kTarget != kRows && kJob != kQuery;
-    const NormJob& j = a.job[kJob];
-    const Place(&at)[kSlots] = places(tag);
-    if (st.live[w.token] == 0) return;
-    if constexpr (kCache)
-      if (st.at_k[w.token] < 0) return;
-    const bool paired = kJob != kValue && a.adjacent != 0 && kVec == 8 && at[0].turns;
-    Part<kVec> f;
-    values_of<T, kVec, kOnce>(w.raw, at, paired, f);
-    if constexpr (kJob != kValue) {
-      if (j.weight != nullptr) {
-        float sum = 0.f;
-#pragma unroll
-        for (int i = 0; i < Part<kVec>::kPairs; ++i) sum += f.x[0][i] * f.x[0][i] + f.x[1][i] * f.x[1][i];
-        const float r = 1.f / sqrtf(group_sum(sum, a.lanes) * a.per_d + a.eps);
-#pragma unroll
-        for (int i = 0; i < Part<kVec>::kPairs; ++i) {
-          f.x[0][i] = f.x[0][i] * r * weight.x[0][i];
-          f.x[1][i] = f.x[1][i] * r * weight.x[1][i];
-        }
-      }
-      Part<kVec> t;
-      load_turn<kVec>(st.cs + w.token * 2 * a.half, a.half, at, u0, a.lanes, t);
-#pragma unroll
-      for (int i = 0; i < Part<kVec>::kPairs; ++i) {
-        if (at[i / kVec].turns) {
-          const float x1 = f.x[0][i], x2 = f.x[1][i];
-          f.x[0][i] = x1 * t.x[0][i] - x2 * t.x[1][i];
-          f.x[1][i] = x2 * t.x[0][i] + x1 * t.x[1][i];
-        }
-      }
-      if (paired) join_pairs<kVec>(f);
-    }
-    uint8_t* dst = j.dst + (uint64_t)(uint32_t)w.head * j.dst_head;
-    if constexpr (kCache) dst += kJob == kKey ? st.at_k[w.token] : st.at_v[w.token];
-    else dst += tok0 * j.dst_token + (uint64_t)(uint32_t)w.token * j.dst_token;
-    if constexpr (kCache && kTarget == kQuant) {
-      store_codes<kVec>(a, f, at, u0 == 0, dst,
-                        a.exponents + st.at_e[w.token] + 2 * (int64_t)w.head * a.block_size + (kJob == kValue ? 1 : 0));
-    } else {
-      T* row = reinterpret_cast<T*>(dst);
-#pragma unroll
-      for (int s = 0; s < kSlots; ++s)
-        if (at[s].there) {
-          Piece8<T, kVec, kOnce> p;
-          p.put(&f.x[0][kVec * s]);
-          p.store(row + at[s].first);
-          p.put(&f.x[1][kVec * s]);
-          p.store(row + at[s].second);
-        }
-    }
-  };
-  auto each_job = [&](auto&& f) {
-    f(std::integral_constant<int, kQuery>{});
-    f(std::integral_constant<int, kKey>{});
-    if constexpr (kTarget != kRows) f(std::integral_constant<int, kValue>{});
-  };
-
-  Work first[kJobs];
-  each_job([&](auto tag) {
-    constexpr int kJob = decltype(tag)::value;
-    if (group < tokens * a.job[kJob].heads) fetch(tag, group, first[kJob]);
-  });
-  collect_tokens<kTarget>(a, tok0, tokens, st);
-  __syncthreads();
-  each_job([&](auto tag) {
-    constexpr int kJob = decltype(tag)::value;
-    const int count = tokens * a.job[kJob].heads;
-    if (group >= count) return;
-    Part<kVec> weight;
-    load_weights<kVec>(a, a.job[kJob].weight, places(tag), a.adjacent != 0 && kVec == 8 && turning[0].turns, weight);
-    finish(tag, first[kJob], weight);
-    for (int idx = group + groups; idx < count; idx += 2 * groups) {
-      Work u, v;
-      const bool two = idx + groups < count;
-      fetch(tag, idx, u);
-      if (two) fetch(tag, idx + groups, v);
-      finish(tag, u, weight);
-      if (two) finish(tag, v, weight);
-    }
-  });
+// A row of a workgroup's job: `lanes` lanes each, the next one's loads on their way while
+// one is computed.
+template <typename T, int kVec, bool kOnce>
+struct RowWork {
+  RawPart<T, kVec, kOnce> x;
+  int token, head;
+};
+template <typename T, int kVec, bool kOnce>
+__device__ __forceinline__ void fetch_row(const NormJob& j, int64_t tok0, int idx,
+                                          const Place (&at)[Part<kVec>::kSlots], RowWork<T, kVec, kOnce>& w) {
+  w.token = (int)fast_div((uint32_t)idx, j.by_heads);
+  w.head = idx - w.token * j.heads;
+  w.x.load(reinterpret_cast<const T*>(j.src + tok0 * j.src_token + (uint64_t)(uint32_t)w.token * j.src_token +
+                                      (uint64_t)(uint32_t)w.head * j.src_head), at);
 }
 
-// The gradient.  A workgroup goes from block of tokens to block of tokens, a lane's sums
-// for its weights in registers; at the end they meet in LDS and leave one partial a
+template <typename T, int kVec, bool kAdjacent, int kTarget, bool kOnce>
+__global__ __launch_bounds__(kNormThreads) void norm_kernel(NormArgs a) {
+  constexpr int kSlots = Part<kVec>::kSlots, kPairs = Part<kVec>::kPairs;
+  __shared__ __attribute__((aligned(16))) TokenState st;
+  const int kind = (int)blockIdx.x >= a.job[kValue].first_block ? kValue : (int)blockIdx.x >= a.job[kKey].first_block ? kKey : kQuery;
+  const NormJob& j = a.job[kind];
+  const int tid = (int)threadIdx.x;
+  const int group = tid >> a.lane_shift, u0 = tid & (a.lanes - 1), groups = kNormThreads >> a.lane_shift;
+  const int64_t tok0 = (int64_t)((int)blockIdx.x - j.first_block) * j.block_tokens;
+  const int tokens = (int)min((int64_t)j.block_tokens, a.tokens - tok0), count = tokens * j.heads;
+  const bool cached = kTarget != kRows && kind != kQuery;
+  Place at[kSlots];
+#pragma unroll
+  for (int s = 0; s < kSlots; ++s) at[s] = place_of<kVec>(a, j.half, u0 + s * a.lanes);
+
+  typedef RowWork<T, kVec, kOnce> Work;
+  auto finish = [&](const Work& w, const Part<kVec>& weight) {
+    if (st.live[w.token] == 0) return;
+    Part<kVec> f;
+    w.x.get(at, f);
+    if (j.weight != nullptr) {
+      float sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < kPairs; ++i) sum += f.x[0][i] * f.x[0][i] + f.x[1][i] * f.x[1][i];
+      const float r = inverse_root(group_sum(sum, a.lanes) * a.per_d + a.eps);
+#pragma unroll
+      for (int i = 0; i < kPairs; ++i) {
+        f.x[0][i] = f.x[0][i] * r * weight.x[0][i];
+        f.x[1][i] = f.x[1][i] * r * weight.x[1][i];
+      }
+    }
+    turn_part<kVec, kAdjacent, false>(st.cs + w.token * 2 * a.half, a.half, at, u0, a.lanes, f);
+    uint8_t* dst = j.dst + (uint64_t)(uint32_t)w.head * j.dst_head;
+    dst += cached ? st.at[w.token] : tok0 * j.dst_token + (uint64_t)(uint32_t)w.token * j.dst_token;
+    if (kTarget == kQuant && cached)
+      store_codes<kVec>(a, f, at, u0 == 0, dst, a.exponents + st.at_e[w.token] + 2 * (int64_t)w.head * a.block_size);
+    else
+      store_part<T, kVec, kOnce>(reinterpret_cast<T*>(dst), at, f);
+  };
+  Work now;
+  if (group < count) fetch_row(j, tok0, group, at, now);
+  collect_weights(a, j.weight, st);
+  collect_tokens(a, j, cached, kind == kValue, tok0, tokens, st);
+  __syncthreads();
+  Part<kVec> weight;
+  load_weights<kVec>(st.weight, at, weight);
+  for (int idx = group; idx < count; idx += groups) {
+    Work next;
+    if (idx + groups < count) fetch_row(j, tok0, idx + groups, at, next);
+    finish(now, weight);
+    now = next;
+  }
+}
+
+// The gradient.  A workgroup goes from block to block of a kind's tokens, a lane's sums for
+// its weights in registers; at the end they meet in LDS and leave one partial a
 // workgroup, which weight_kernel adds up in order.
-template <typename T, int kVec, bool kOnce>
+template <typename T, int kVec, bool kAdjacent, bool kOnce>
 __global__ __launch_bounds__(kNormThreads) void backward_kernel(NormArgs a) {
   constexpr int kSlots = Part<kVec>::kSlots, kPairs = Part<kVec>::kPairs;
   __shared__ __attribute__((aligned(16))) TokenState st;
+  const int kind = (int)blockIdx.x >= a.job[kKey].first_block ? kKey : kQuery;
+  const NormJob& j = a.job[kind];
+  const int stride = (kind == kKey ? (int)gridDim.x : a.job[kKey].first_block) - j.first_block;
   const int tid = (int)threadIdx.x;
-  const int group = tid / a.lanes, u0 = tid - group * a.lanes, groups = kNormThreads / a.lanes;
+  const int group = tid >> a.lane_shift, u0 = tid & (a.lanes - 1), groups = kNormThreads >> a.lane_shift;
   Place at[kSlots];
 #pragma unroll
-  for (int s = 0; s < kSlots; ++s) at[s] = place_of<kVec>(a, a.half, u0 + s * a.lanes);
-  const bool paired = a.adjacent != 0 && kVec == 8 && at[0].turns;
+  for (int s = 0; s < kSlots; ++s) at[s] = place_of<kVec>(a, j.half, u0 + s * a.lanes);
   struct Work {
-    RawPart<T, kVec, kOnce> x, g;
-    int token, head;
+    RowWork<T, kVec, kOnce> row;
+    RawPart<T, kVec, kOnce> g;
   };
-  Part<kVec> sums[2], weight[2];
+  Part<kVec> sums, weight;
 #pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    load_weights<kVec>(a, a.job[k].weight, at, paired, weight[k]);
-#pragma unroll
-    for (int i = 0; i < kPairs; ++i) sums[k].x[0][i] = sums[k].x[1][i] = 0.f;
-  }
-  auto each_job = [&](auto&& f) {
-    f(std::integral_constant<int, kQuery>{});
-    f(std::integral_constant<int, kKey>{});
-  };
-  for (int64_t block = blockIdx.x; block * a.block_tokens < a.tokens; block += gridDim.x) {
-    const int64_t tok0 = block * a.block_tokens;
-    const int tokens = (int)min((int64_t)a.block_tokens, a.tokens - tok0);
-    auto fetch = [&](auto tag, int idx, Work& w) {
-      const NormJob& j = a.job[decltype(tag)::value];
-      w.token = (int)fast_div((uint32_t)idx, j.by_heads);
-      w.head = idx - w.token * j.heads;
-      w.x.load(reinterpret_cast<const T*>(j.src + tok0 * j.src_token + (uint64_t)(uint32_t)w.token * j.src_token +
-                                          (uint64_t)(uint32_t)w.head * j.src_head), at);
-      w.g.load(reinterpret_cast<const T*>(j.grad + tok0 * j.grad_token + (uint64_t)(uint32_t)w.token * j.grad_token +
-                                          (uint64_t)(uint32_t)w.head * j.grad_head), at);
+  for (int i = 0; i < kPairs; ++i) sums.x[0][i] = sums.x[1][i] = 0.f;
+  collect_weights(a, j.weight, st);
+  __syncthreads();
+  load_weights<kVec>(st.weight, at, weight);
+  for (int64_t block = (int)blockIdx.x - j.first_block; block * j.block_tokens < a.tokens; block += stride) {
+    const int64_t tok0 = block * j.block_tokens;
+    const int tokens = (int)min((int64_t)j.block_tokens, a.tokens - tok0), count = tokens * j.heads;
+    auto fetch = [&](int idx, Work& w) {
+      fetch_row(j, tok0, idx, at, w.row);
+      w.g.load(reinterpret_cast<const T*>(j.grad + tok0 * j.grad_token + (uint64_t)(uint32_t)w.row.token * j.grad_token +
+                                          (uint64_t)(uint32_t)w.row.head * j.grad_head), at);
     };
-    auto finish = [&](auto tag, const Work& w) {
-      constexpr int kJob = decltype(tag)::value;
-      const NormJob& j = a.job[kJob];
+    auto finish = [&](const Work& w) {
       Part<kVec> x, u;
-      values_of<T, kVec, kOnce>(w.x, at, paired, x);
-      values_of<T, kVec, kOnce>(w.g, at, paired, u);
-      const bool live = st.live[w.token] != 0;
-      Part<kVec> t;
-      load_turn<kVec>(st.cs + w.token * 2 * a.half, a.half, at, u0, a.lanes, t);
+      w.row.x.get(at, x);
+      w.g.get(at, u);
+      const bool live = st.live[w.row.token] != 0;
+      turn_part<kVec, kAdjacent, true>(st.cs + w.row.token * 2 * a.half, a.half, at, u0, a.lanes, u);
       float xx = 0.f, ux = 0.f;
 #pragma unroll
-      for (int i = 0; i < kPairs; ++i) {
-        if (at[i / kVec].turns) {
-          const float g1 = u.x[0][i], g2 = u.x[1][i];
-          u.x[0][i] = g1 * t.x[0][i] + g2 * t.x[1][i];
-          u.x[1][i] = g2 * t.x[0][i] - g1 * t.x[1][i];
-        }
+      for (int i = 0; i < kPairs; ++i)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           xx += x.x[e][i] * x.x[e][i];
-          ux += x.x[e][i] * u.x[e][i] * weight[kJob].x[e][i];
+          ux += x.x[e][i] * u.x[e][i] * weight.x[e][i];
         }
-      }
-      const float r = 1.f / sqrtf(group_sum(xx, a.lanes) * a.per_d + a.eps);
+      const float r = inverse_root(group_sum(xx, a.lanes) * a.per_d + a.eps);
       const float inner = group_sum(ux, a.lanes) * a.per_d * r;
 #pragma unroll
       for (int i = 0; i < kPairs; ++i)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const float unit = x.x[e][i] * r, h = u.x[e][i];
-          sums[kJob].x[e][i] += live ? h * unit : 0.f;
-          u.x[e][i] = live ? r * (h * weight[kJob].x[e][i] - unit * inner) : 0.f;
+          sums.x[e][i] += live ? h * unit : 0.f;
+          u.x[e][i] = live ? r * (h * weight.x[e][i] - unit * inner) : 0.f;
         }
-      if (j.dst == nullptr) return;
-      if (paired) join_pairs<kVec>(u);
-      T* row = reinterpret_cast<T*>(j.dst + tok0 * j.dst_token + (uint64_t)(uint32_t)w.token * j.dst_token +
-                                    (uint64_t)(uint32_t)w.head * j.dst_head);
-#pragma unroll
-      for (int s = 0; s < kSlots; ++s)
-        if (at[s].there) {
-          Piece8<T, kVec, kOnce> p;
-          p.put(&u.x[0][kVec * s]);
-          p.store(row + at[s].first);
-          p.put(&u.x[1][kVec * s]);
-          p.store(row + at[s].second);
-        }
+      if (j.dst != nullptr)
+        store_part<T, kVec, kOnce>(
+            reinterpret_cast<T*>(j.dst + tok0 * j.dst_token + (uint64_t)(uint32_t)w.row.token * j.dst_token +
+                                 (uint64_t)(uint32_t)w.row.head * j.dst_head), at, u);
     };
-    Work first[2];
-    each_job([&](auto tag) {
-      constexpr int kJob = decltype(tag)::value;
-      if (group < tokens * a.job[kJob].heads) fetch(tag, group, first[kJob]);
-    });
+    Work now;
+    if (group < count) fetch(group, now);
     __syncthreads();                        // (the block before this one is done with the cosines)
-    collect_tokens<kRows>(a, tok0, tokens, st);
+    collect_tokens(a, j, false, false, tok0, tokens, st);
     __syncthreads();
-    each_job([&](auto tag) {
-      constexpr int kJob = decltype(tag)::value;
-      const int count = tokens * a.job[kJob].heads;
-      if (group >= count) return;
-      finish(tag, first[kJob]);
-      for (int idx = group + groups; idx < count; idx += groups) {
-        Work w;
-        fetch(tag, idx, w);
-        finish(tag, w);
-      }
-    });
+    for (int idx = group; idx < count; idx += groups) {
+      Work next;
+      if (idx + groups < count) fetch(idx + groups, next);
+      finish(now);
+      now = next;
+    }
   }
   if (a.partials == nullptr) return;
-  // The groups' sums, one kind after the other: a thread to a feature.
+  // The groups' sums: a thread to a feature.
   float* const all = st.cs;                 // [group][D]: at most 4096 values
   static_assert(kNormThreads * 2 * Part<8>::kPairs <= kMaxTokens * kMaxRotary &&
                 kNormThreads * 2 * Part<1>::kPairs <= kMaxTokens * kMaxRotary, "the sums fit");
+  __syncthreads();
 #pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    __syncthreads();
-    if (paired) join_pairs<kVec>(sums[k]);
+  for (int s = 0; s < kSlots; ++s)
+    if (at[s].there)
 #pragma unroll
-    for (int s = 0; s < kSlots; ++s)
-      if (at[s].there)
-#pragma unroll
-        for (int i = 0; i < kVec; ++i) {
-          all[group * a.d + at[s].first + i] = sums[k].x[0][kVec * s + i];
-          all[group * a.d + at[s].second + i] = sums[k].x[1][kVec * s + i];
-        }
-    __syncthreads();
-    if (tid < a.d) {
-      float sum = 0.f;
-      for (int g = 0; g < groups; ++g) sum += all[g * a.d + tid];
-      a.partials[((int64_t)blockIdx.x * 2 + k) * a.d + tid] = sum;
-    }
+      for (int i = 0; i < kVec; ++i) {
+        all[group * a.d + at[s].first + i] = sums.x[0][kVec * s + i];
+        all[group * a.d + at[s].second + i] = sums.x[1][kVec * s + i];
+      }
+  __syncthreads();
+  if (tid < a.d) {
+    float sum = 0.f;
+    for (int g = 0; g < groups; ++g) sum += all[g * a.d + tid];
+    a.partials[(int64_t)blockIdx.x * a.d + tid] = sum;
   }
 }
 
-// The weights' gradients: the workgroups' partials of 16 features, 16 threads to each.
-__global__ __launch_bounds__(256) void weight_kernel(const float* partials, int blocks, int d, void* query, void* key,
-                                                     int weight_type) {
-  __shared__ float red[16][17];
+// The weights' gradients: the workgroups' partials of 16 features, 64 threads to each,
+// eight loads at once.
+constexpr int kWeightParts = 64;
+__global__ __launch_bounds__(16 * kWeightParts) void weight_kernel(const float* partials, int queries, int keys, int d,
+                                                                   void* query, void* key, int weight_type) {
+  __shared__ float red[kWeightParts][17];
   const int f = 16 * (int)blockIdx.x + ((int)threadIdx.x & 15), part = (int)threadIdx.x >> 4, k = (int)blockIdx.y;
   void* const out = k == 0 ? query : key;
   if (out == nullptr) return;
-  float sum = 0.f;
+  const int blocks = k == 0 ? queries : keys;
+  const float* const from = partials + (k == 0 ? 0 : (int64_t)queries * d);
+  float sum[8] = {};
   if (f < d)
-    for (int b = part; b < blocks; b += 16) sum += partials[((int64_t)b * 2 + k) * d + f];
-  red[part][threadIdx.x & 15] = sum;
+    for (int b = part; b < blocks; b += 8 * kWeightParts)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int at = b + i * kWeightParts;
+        const float x = from[(int64_t)min(at, blocks - 1) * d + f];
+        sum[i] += at < blocks ? x : 0.f;
+      }
+  red[part][threadIdx.x & 15] = ((sum[0] + sum[1]) + (sum[2] + sum[3])) + ((sum[4] + sum[5]) + (sum[6] + sum[7]));
   __syncthreads();
   if (part != 0 || f >= d) return;
   float total = 0.f;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) total += red[i][threadIdx.x];
+  for (int i = 0; i < kWeightParts; ++i) total += red[i][threadIdx.x];
   if (weight_type == OSCAR_FP32) static_cast<float*>(out)[f] = total;
   else if (weight_type == OSCAR_BF16) static_cast<__bf16*>(out)[f] = (__bf16)total;
   else static_cast<_Float16*>(out)[f] = (_Float16)total;
@@ -646,6 +591,7 @@ void fill_args(NormArgs& a, const oscar_rotary* r, const oscar_head_norm* n, con
   a.lanes = 64;
   if (vec)
     for (a.lanes = 1; a.lanes < head_size / 16;) a.lanes *= 2;
+  for (a.lane_shift = 0; 1 << a.lane_shift < a.lanes;) ++a.lane_shift;
   a.weight_type = n->weight_dtype;
   a.eps = n->eps;
   a.offset = n->offset;
@@ -653,25 +599,33 @@ void fill_args(NormArgs& a, const oscar_rotary* r, const oscar_head_norm* n, con
   a.by_half = make_fast_div((uint32_t)a.half);
   a.job[kQuery].weight = n->query_weight;
   a.job[kKey].weight = n->key_weight;
-  for (NormJob& j : a.job) j.by_heads = make_fast_div((uint32_t)(j.heads > 0 ? j.heads : 1));
+  for (int i = 0; i < kJobs; ++i) {
+    a.job[i].by_heads = make_fast_div((uint32_t)(a.job[i].heads > 0 ? a.job[i].heads : 1));
+    a.job[i].half = i == kValue ? 0 : a.half;
+  }
 }
 
 bool pieces_of_16(const oscar_rotary* r, int32_t head_size) { return head_size % 16 == 0 && r->rotary_dim % 16 == 0; }
 
-// Tokens of a workgroup: a power of two, up to `rounds` heads a group of lanes, fewer
-// where that leaves less than 512 workgroups.
-int tokens_a_block(int64_t tokens, int64_t heads, int lanes, int rounds) {
+// Tokens of a workgroup of a kind: a power of two, up to kRounds heads a group of lanes,
+// fewer where that leaves less than kLeastBlocks workgroups.
+constexpr int kRounds = 8, kLeastBlocks = 512;
+int tokens_a_block(int64_t tokens, int64_t heads, int lanes) {
   int block = kMaxTokens;
-  while (block > 1 && (block * heads * lanes > rounds * kNormThreads || (tokens + block - 1) / block < 512)) block /= 2;
+  while (block > 1 && (block * heads * lanes > kRounds * kNormThreads || (tokens + block - 1) / block < kLeastBlocks))
+    block /= 2;
   return block;
 }
+int64_t blocks_of(const NormJob& j, int64_t tokens) { return j.heads == 0 ? 0 : (tokens + j.block_tokens - 1) / j.block_tokens; }
 
 template <typename T, int kTarget>
-void launch_norm(const NormArgs& a, bool vec, bool once, hipStream_t stream) {
-  const dim3 grid((uint32_t)((a.tokens + a.block_tokens - 1) / a.block_tokens));
-  if (!vec) norm_kernel<T, 1, kTarget, false><<<grid, kNormThreads, 0, stream>>>(a);
-  else if (once) norm_kernel<T, 8, kTarget, true><<<grid, kNormThreads, 0, stream>>>(a);
-  else norm_kernel<T, 8, kTarget, false><<<grid, kNormThreads, 0, stream>>>(a);
+void launch_norm(const NormArgs& a, uint32_t blocks, bool vec, bool once, hipStream_t stream) {
+  // (single values of adjacent pairs and of halves differ in their places alone)
+  const auto kernel = !vec            ? &norm_kernel<T, 1, false, kTarget, false>
+                      : a.adjacent    ? once ? &norm_kernel<T, 8, true, kTarget, true> : &norm_kernel<T, 8, true, kTarget, false>
+                      : once          ? &norm_kernel<T, 8, false, kTarget, true>
+                                      : &norm_kernel<T, 8, false, kTarget, false>;
+  kernel<<<blocks, kNormThreads, 0, stream>>>(a);
 }
 
 // kTarget's cache: plain or quant.
@@ -751,21 +705,29 @@ int run_norm(const oscar_rotary* r, const oscar_head_norm* n, const int64_t* pos
       if (a.block_size == (1 << s)) a.block_shift = s;
   }
   fill_args(a, r, n, positions, axis_stride, tokens, head_size, vec);
-  a.block_tokens = tokens_a_block(tokens, heads, a.lanes, 10);
-  if ((tokens + a.block_tokens - 1) / a.block_tokens > INT32_MAX) return kErrInvalidArgument;
+  int64_t blocks = 0;
+  for (int i = 0; i < kJobs; ++i) {
+    NormJob& j = a.job[i];
+    j.block_tokens = tokens_a_block(tokens, j.heads, a.lanes);
+    j.first_block = (int32_t)blocks;
+    blocks += blocks_of(j, tokens);
+    if (blocks > INT32_MAX) return kErrInvalidArgument;
+  }
   // More than the last-level cache holds, read and written: rows go past the caches.
   const bool once = 2 * tokens * heads * row > kLastCache;
-  if (dtype == OSCAR_BF16) launch_norm<__bf16, kTarget>(a, vec, once, stream);
-  else if (dtype == OSCAR_FP16) launch_norm<_Float16, kTarget>(a, vec, once, stream);
-  else if constexpr (kTarget == kRows) launch_norm<float, kTarget>(a, vec, once, stream);
+  if (dtype == OSCAR_BF16) launch_norm<__bf16, kTarget>(a, (uint32_t)blocks, vec, once, stream);
+  else if (dtype == OSCAR_FP16) launch_norm<_Float16, kTarget>(a, (uint32_t)blocks, vec, once, stream);
+  else if constexpr (kTarget == kRows) launch_norm<float, kTarget>(a, (uint32_t)blocks, vec, once, stream);
   return hipGetLastError() == hipSuccess ? kOk : kErrLaunch;
 }
 
 template <typename T>
 void launch_backward(const NormArgs& a, uint32_t blocks, bool vec, bool once, hipStream_t stream) {
-  if (!vec) backward_kernel<T, 1, false><<<blocks, kNormThreads, 0, stream>>>(a);
-  else if (once) backward_kernel<T, 8, true><<<blocks, kNormThreads, 0, stream>>>(a);
-  else backward_kernel<T, 8, false><<<blocks, kNormThreads, 0, stream>>>(a);
+  const auto kernel = !vec         ? &backward_kernel<T, 1, false, false>
+                      : a.adjacent ? once ? &backward_kernel<T, 8, true, true> : &backward_kernel<T, 8, true, false>
+                      : once       ? &backward_kernel<T, 8, false, true>
+                                   : &backward_kernel<T, 8, false, false>;
+  kernel<<<blocks, kNormThreads, 0, stream>>>(a);
 }
 
 }  // namespace
@@ -874,17 +836,24 @@ extern "C" int oscar_norm_rotate_backward(const oscar_rotary* rotary, const osca
     j.heads = rows[i][0].heads;
   }
   fill_args(a, rotary, norm, positions, position_axis_stride, num_tokens, head_size, vec);
-  a.block_tokens = tokens_a_block(num_tokens, heads, a.lanes, 10);
   a.partials = weights ? static_cast<float*>(workspace) : nullptr;
-  const int64_t blocks = std::min<int64_t>((num_tokens + a.block_tokens - 1) / a.block_tokens, kBackBlocks);
-  if (blocks > 0 && heads > 0) {
+  // Workgroups of the two kinds as their heads are, each at least one where there are rows.
+  int64_t blocks[2] = {};
+  for (int i = 0; i < 2; ++i) {
+    NormJob& j = a.job[i];
+    j.block_tokens = tokens_a_block(num_tokens, j.heads, a.lanes);
+    blocks[i] = std::min<int64_t>(blocks_of(j, num_tokens), std::max<int64_t>(1, kBackBlocks * j.heads / std::max<int64_t>(1, heads)));
+  }
+  a.job[kKey].first_block = (int32_t)blocks[0];
+  if (blocks[0] + blocks[1] > 0) {
     const bool once = 3 * num_tokens * heads * row > kLastCache;
-    if (dtype == OSCAR_BF16) launch_backward<__bf16>(a, (uint32_t)blocks, vec, once, stream);
-    else if (dtype == OSCAR_FP16) launch_backward<_Float16>(a, (uint32_t)blocks, vec, once, stream);
-    else launch_backward<float>(a, (uint32_t)blocks, vec, once, stream);
+    const uint32_t grid = (uint32_t)(blocks[0] + blocks[1]);
+    if (dtype == OSCAR_BF16) launch_backward<__bf16>(a, grid, vec, once, stream);
+    else if (dtype == OSCAR_FP16) launch_backward<_Float16>(a, grid, vec, once, stream);
+    else launch_backward<float>(a, grid, vec, once, stream);
   }
   if (weights)
-    weight_kernel<<<dim3((uint32_t)(head_size + 15) / 16, 2), 256, 0, stream>>>(
-        a.partials, heads > 0 ? (int)blocks : 0, head_size, query_weight_grad, key_weight_grad, norm->weight_dtype);
+    weight_kernel<<<dim3((uint32_t)(head_size + 15) / 16, 2), 16 * kWeightParts, 0, stream>>>(
+        a.partials, (int)blocks[0], (int)blocks[1], head_size, query_weight_grad, key_weight_grad, norm->weight_dtype);
   return hipGetLastError() == hipSuccess ? kOk : kErrLaunch;
 }
