@@ -28,7 +28,7 @@ constexpr int kNormThreads = 256;
 constexpr int kMaxTokens = 16;             // of a workgroup at a time
 constexpr int kMaxRotary = 256;
 constexpr int64_t kLastCache = 256ll << 20;      // bytes
-constexpr int kBackBlocks = 1024;          // workgroups of the gradient, at most
+constexpr int kBackBlocks = 4096;          // workgroups of the gradient, at most (1024: 30843 tokens' step 357 us for 297)
 
 enum Target { kRows, kPlain, kQuant };
 
@@ -414,7 +414,10 @@ __global__ __launch_bounds__(kNormThreads) void norm_kernel(NormArgs a) {
 template <typename T, int kVec, bool kAdjacent, bool kOnce>
 __global__ __launch_bounds__(kNormThreads) void backward_kernel(NormArgs a) {
   constexpr int kSlots = Part<kVec>::kSlots, kPairs = Part<kVec>::kPairs;
-  __shared__ __attribute__((aligned(16))) TokenState st;
+  constexpr size_t kSums = kNormThreads * 2 * kPairs * 4;      // [group][D]
+  __shared__ __attribute__((aligned(16))) uint8_t smem[kSums > sizeof(TokenState) ? kSums : sizeof(TokenState)];
+  TokenState& st = *reinterpret_cast<TokenState*>(smem);
+  float* const all = reinterpret_cast<float*>(smem);
   const int kind = (int)blockIdx.x >= a.job[kKey].first_block ? kKey : kQuery;
   const NormJob& j = a.job[kind];
   const int stride = (kind == kKey ? (int)gridDim.x : a.job[kKey].first_block) - j.first_block;
@@ -484,9 +487,6 @@ __global__ __launch_bounds__(kNormThreads) void backward_kernel(NormArgs a) {
   }
   if (a.partials == nullptr) return;
   // The groups' sums: a thread to a feature.
-  float* const all = st.cs;                 // [group][D]: at most 4096 values
-  static_assert(kNormThreads * 2 * Part<8>::kPairs <= kMaxTokens * kMaxRotary &&
-                kNormThreads * 2 * Part<1>::kPairs <= kMaxTokens * kMaxRotary, "the sums fit");
   __syncthreads();
 #pragma unroll
   for (int s = 0; s < kSlots; ++s)
@@ -607,12 +607,16 @@ void fill_args(NormArgs& a, const oscar_rotary* r, const oscar_head_norm* n, con
 
 bool pieces_of_16(const oscar_rotary* r, int32_t head_size) { return head_size % 16 == 0 && r->rotary_dim % 16 == 0; }
 
-// Tokens of a workgroup of a kind: a power of two, up to kRounds heads a group of lanes,
-// fewer where that leaves less than kLeastBlocks workgroups.
-constexpr int kRounds = 8, kLeastBlocks = 512;
+// Tokens of a workgroup of a kind: a power of two, up to kRounds heads a group of lanes (8:
+// 30843 tokens' gradient step 357 us for 303), fewer where that leaves less than 256
+// workgroups (512: 2000 tokens of 7 heads 7.7 us for 6.4), 16 only where there are 2048 of
+// them (where less do: 9256 tokens 17.5 us for 16.1; where none do: a write of 65536 tokens
+// 144 us for 137).
+constexpr int kRounds = 4;
 int tokens_a_block(int64_t tokens, int64_t heads, int lanes) {
   int block = kMaxTokens;
-  while (block > 1 && (block * heads * lanes > kRounds * kNormThreads || (tokens + block - 1) / block < kLeastBlocks))
+  while (block > 1 && (block * heads * lanes > kRounds * kNormThreads ||
+                       (tokens + block - 1) / block < (block == kMaxTokens ? 2048 : 256)))
     block /= 2;
   return block;
 }
