@@ -750,6 +750,8 @@ typedef struct oscar_quant_step {
   int64_t partials_size;
   int32_t sources; /* ranges of keys that are converted */
   int32_t pages;   /* of 16 keys each */
+  int32_t once;    /* codes are more than the caches hold */
+  int32_t reserved;
 } oscar_quant_step;
 
 int oscar_quant_plan(const int32_t* query_start_loc, const int32_t* seq_lens, int32_t num_requests, int32_t num_heads,

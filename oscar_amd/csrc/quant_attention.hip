@@ -34,6 +34,7 @@ struct Source {
   int32_t table_row, group0, groups, page0;
 };
 static_assert(sizeof(Source) == 16, "item size");
+constexpr int64_t kLastCache = 256ll << 20;      // bytes
 
 struct QuantArgs {
   const uint8_t* k;        // codes
@@ -78,7 +79,7 @@ __device__ __forceinline__ LanePlace code_place(const QuantArgs& a, int lane) {
 }
 
 // 16 keys' codes from `key` on, as load_keys.
-template <int D, bool kV>
+template <int D, bool kV, int kPolicy>
 __device__ __forceinline__ void load_codes(const QuantArgs& a, const Piece& p, int key, int key_in_tile, int page,
                                            int in_page, uint8_t* lds, const LanePlace& at) {
   constexpr int kStep = 1024 / D;           // keys of a load
@@ -93,7 +94,7 @@ __device__ __forceinline__ void load_codes(const QuantArgs& a, const Piece& p, i
     const int first = key_in_tile + n * kStep;
     const int turn = 16 * (kV ? v_code_swizzle<D>(first) : k_code_swizzle<D>(first));
     __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_void*)(lds + first * D), 16,
-                                             at.row + n * kStep * stride + (at.chunk ^ turn), 0, 0, kOnce);
+                                             at.row + n * kStep * stride + (at.chunk ^ turn), 0, 0, kPolicy);
   }
 }
 
@@ -193,7 +194,7 @@ constexpr int code_keys(int d) { return 8192 / d; }
 constexpr int kCodeWgs = 2;                // workgroups a CU
 constexpr int code_lds(int d) { return kWaves * (2 * 8192 + std::max(2 * code_keys(d) * 4, 2 * kTileRows * 4)); }
 
-template <typename T, int D>
+template <typename T, int D, int kPolicy>
 __device__ __forceinline__ void code_piece(const QuantChunkArgs& all, const Piece p, uint8_t* smem) {
   typedef typename Num<T>::V8 V8;
   const ChunkArgs& a = all.wide;
@@ -233,7 +234,7 @@ __device__ __forceinline__ void code_piece(const QuantChunkArgs& all, const Piec
     const LanePlace at = code_place<D, kV>(c, opaque(lane));       // (found anew: registers)
 #pragma unroll
     for (int h = 0; h < kGroups; ++h)
-      load_codes<D, kV>(c, p, p.key0 + t * kKeys + 16 * h, 16 * h, page_of(t, h), in_page(t, h), lds, at);
+      load_codes<D, kV, kPolicy>(c, p, p.key0 + t * kKeys + 16 * h, 16 * h, page_of(t, h), in_page(t, h), lds, at);
   };
   // The powers of keys lane % 32 of the subtiles: K's in the low byte, V's above.  (Their
   // places as scalars: as a choice of the lane the pages would be the lane's for the
@@ -407,10 +408,13 @@ __device__ __forceinline__ void code_piece(const QuantChunkArgs& all, const Piec
 }
 
 // ---------------------------------------------------------------- kernels
-template <typename T, int D>
+// (Codes past the caches, kOnce, where they are more than the last-level cache holds: 32
+// users' token over 2K to 16K keys of 8 heads of 128, 578 MB, 123 us, through them 135; 32
+// users' 4 of one head of 256, 146 MB, 39 us, through them 37; 48 rows over 32 MB 33, 31.)
+template <typename T, int D, int kPolicy>
 __global__ __launch_bounds__(kThreads, kCodeWgs) void code_kernel(QuantChunkArgs a) {
   __shared__ __attribute__((aligned(1024))) uint8_t smem[code_lds(D)];
-  code_piece<T, D>(a, a.wide.pieces[blockIdx.x], smem);
+  code_piece<T, D, kPolicy>(a, a.wide.pieces[blockIdx.x], smem);
 }
 // A step with wide pieces, the narrow ones first where they are few, as mixed_kernel.
 constexpr int kFewNarrow = kCus;
@@ -420,7 +424,7 @@ __global__ __launch_bounds__(kThreads, kWideWgs) void quant_kernel(QuantChunkArg
   const int total = a.wide.narrow + a.wide.wide, lead = a.wide.narrow <= kFewNarrow ? 0 : a.wide.narrow;
   const int at = (int)blockIdx.x + lead, i = at < total ? at : at - total;
   if (i >= a.wide.narrow) wide_piece<T, D>(a.wide, a.wide.pieces[i], smem);
-  else code_piece<T, D>(a, a.wide.pieces[i], smem);
+  else code_piece<T, D, kKept>(a, a.wide.pieces[i], smem);
 }
 
 // The sources' keys as 16-bit pages of 16 keys [K | V][key][head][D], a workgroup each,
@@ -476,8 +480,13 @@ __global__ __launch_bounds__(256) void pages_kernel(PagesArgs a) {
 }
 
 // ---------------------------------------------------------------- host
+// Rows of a request that are computed from codes, at most.  From codes / converted first,
+// us: 8 users' 48 rows over 8000 keys, D = 256, 24 / 41; 4 users' 96 over 16000 30 / 45,
+// 192 over 8000 32 / 39; 16 users' 64 over 4000, D = 128, 8 heads, 55 / 128; 8 users' 256
+// over 2000, D = 64, 4 heads, 33 / 30, 192 of D = 128 72 / 87.
 inline PlanRule quant_rule(int32_t head_size) {
-  return PlanRule{head_size, 3 * kTileRows, {kCus, 2 * kCus}, 1.};
+  const int32_t rows = head_size == 64 ? 96 : 192;
+  return PlanRule{head_size, rows, {kCus, 2 * kCus}, 1.};
 }
 
 // The wide pieces' keys, request by request, and the pieces' table rows in the pages'.
@@ -544,7 +553,8 @@ int launch(const QuantChunkArgs& a, const PagesArgs& pages, const oscar_quant_st
                 "the workgroups of a CU must fit its 160 KiB of LDS");
   if (step.pages > 0) pages_kernel<T><<<step.pages, 256, 0, stream>>>(pages);
   const uint32_t pieces = (uint32_t)(step.chunk.narrow + step.chunk.wide);
-  if (step.chunk.wide == 0) code_kernel<T, D><<<pieces, kThreads, 0, stream>>>(a);
+  if (step.chunk.wide == 0 && step.once != 0) code_kernel<T, D, kOnce><<<pieces, kThreads, 0, stream>>>(a);
+  else if (step.chunk.wide == 0) code_kernel<T, D, kKept><<<pieces, kThreads, 0, stream>>>(a);
   else quant_kernel<T, D><<<pieces, kThreads, 0, stream>>>(a);
   return launch_joins<T, D>(a.wide, step.chunk, stream);
 }
@@ -596,6 +606,11 @@ extern "C" int oscar_quant_plan(const int32_t* query_start_loc, const int32_t* s
     const int64_t packed = s.items_size;
     step->sources = (int32_t)sources.size();
     step->pages = (int32_t)read;
+    int64_t codes = 0;                      // bytes that narrow pieces read
+    for (const Piece& p : plan.narrow)
+      if (p.row0 == 0) codes += 2ll * cache->head_size * (p.key1 - p.key0);
+    step->once = codes > kLastCache;
+    step->reserved = 0;
     step->partials_size = (s.workspace_size + 255) / 256 * 256;
     s.items_size += (int64_t)(sources.size() * sizeof(Source));
     s.workspace_size = read == 0 ? s.workspace_size : step->partials_size + table_bytes(*step) + read * page_bytes(s);

@@ -32,7 +32,8 @@ class ChunkStepArgs(ctypes.Structure):
 
 class QuantStepArgs(ctypes.Structure):
     """struct oscar_quant_step (include/oscar_amd.h)."""
-    _fields_ = [("chunk", ChunkStepArgs), ("partials_size", _i64), ("sources", _i32), ("pages", _i32)]
+    _fields_ = [("chunk", ChunkStepArgs), ("partials_size", _i64), ("sources", _i32), ("pages", _i32),
+                ("once", _i32), ("reserved", _i32)]
 
 
 class ChunkStep:
