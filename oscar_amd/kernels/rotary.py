@@ -229,16 +229,21 @@ def pack_norm(query_weight, key_weight, eps: float, offset: float, d: int, devic
     """struct oscar_head_norm of weights [d] (None: that kind has no norm)."""
     if not 0.0 <= eps < MAX_FLOAT or not -MAX_FLOAT < offset < MAX_FLOAT:
         raise ValueError("eps must be finite and not negative, the offset finite")
-    dtype, at = None, [0, 0]
-    for i, (w, what) in enumerate(((query_weight, "query_weight"), (key_weight, "key_weight"))):
-        if w is None:
-            continue
-        if w.shape != (d,) or w.dtype not in DTYPES or w.device != device or (d > 1 and w.stride(0) != 1):
-            raise ValueError(f"{what} must be a contiguous bf16, fp16 or fp32 [{d}] tensor on the rows' device")
-        if dtype is not None and w.dtype is not dtype:
-            raise ValueError("query_weight and key_weight must be of one type")
-        dtype, at[i] = w.dtype, w.data_ptr()
-    return _pack_norm(*at, DTYPES[dtype] if dtype is not None else 0, eps, offset, 0)
+    q, q_type = _weight(query_weight, d, device, "query_weight")
+    k, k_type = _weight(key_weight, d, device, "key_weight")
+    if q_type is not k_type and q and k:
+        raise ValueError("query_weight and key_weight must be of one type")
+    return _pack_norm(q, k, DTYPES.get(q_type or k_type, 0), eps, offset, 0)
+
+
+def _weight(w, d: int, device, what: str):
+    """(address, type) of a weight; (0, None) without one."""
+    if w is None:
+        return 0, None
+    dtype = w.dtype
+    if w.ndim != 1 or w.shape[0] != d or dtype not in DTYPES or w.device != device or not w.is_contiguous():
+        raise ValueError(f"{what} must be a contiguous bf16, fp16 or fp32 [{d}] tensor on the rows' device")
+    return w.data_ptr(), dtype
 
 
 def norm_rotate(query: torch.Tensor, key: torch.Tensor | None, query_weight: torch.Tensor,
@@ -258,8 +263,9 @@ def norm_rotate(query: torch.Tensor, key: torch.Tensor | None, query_weight: tor
         raise ValueError("norm_rotate takes a weight for queries, and for keys where they are given")
     if key is None:
         key_weight = None
-    leaves = [x for x in (query, key, query_weight, key_weight) if x is not None]
-    if (torch.is_grad_enabled() and any(x.requires_grad for x in leaves) and query_out is None and key_out is None):
+    if (query_out is None and key_out is None and torch.is_grad_enabled()
+            and (query.requires_grad or query_weight.requires_grad
+                 or (key is not None and (key.requires_grad or key_weight.requires_grad)))):
         if key is not None and key.shape[0] > query.shape[0]:
             key = key[:query.shape[0]]
         return _Normed.apply(query, key, query_weight, key_weight, positions, rotary, eps, offset)
