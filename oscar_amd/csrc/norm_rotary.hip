@@ -25,7 +25,8 @@ namespace oscar {
 namespace {
 
 constexpr int kNormThreads = 256;
-constexpr int kMaxTokens = 16;             // of a workgroup at a time
+constexpr int kMaxTokens = 64;             // of a workgroup at a time,
+constexpr int kMaxTurns = 4096;            // and their cosines and sines
 constexpr int kMaxRotary = 256;
 constexpr int64_t kLastCache = 256ll << 20;      // bytes
 constexpr int kBackBlocks = 4096;          // workgroups of the gradient, at most (1024: 30843 tokens' step 357 us for 297)
@@ -236,7 +237,7 @@ __device__ __forceinline__ void turn_part(const float* cs, int half, const Place
 }
 
 struct TokenState {
-  float cs[kMaxTokens * kMaxRotary];       // [token][cos | sin]
+  float cs[kMaxTurns];                     // [token][cos | sin]
   float weight[256];                       // weight + offset
   int64_t at[kMaxTokens], at_e[kMaxTokens];        // byte offsets of the slot and of its power
   int live[kMaxTokens];
@@ -609,14 +610,13 @@ bool pieces_of_16(const oscar_rotary* r, int32_t head_size) { return head_size %
 
 // Tokens of a workgroup of a kind: a power of two, up to kRounds heads a group of lanes (8:
 // 30843 tokens' gradient step 357 us for 303), fewer where that leaves less than 256
-// workgroups (512: 2000 tokens of 7 heads 7.7 us for 6.4), 16 only where there are 2048 of
-// them (where less do: 9256 tokens 17.5 us for 16.1; where none do: a write of 65536 tokens
-// 144 us for 137).
+// workgroups (512: 2000 tokens of 7 heads 7.7 us for 6.4), more than 8 only where there are
+// 2048 of them (where less do: 9256 tokens 17.5 us for 16.1).
 constexpr int kRounds = 4;
-int tokens_a_block(int64_t tokens, int64_t heads, int lanes) {
+int tokens_a_block(int64_t tokens, const NormJob& j, int lanes) {
   int block = kMaxTokens;
-  while (block > 1 && (block * heads * lanes > kRounds * kNormThreads ||
-                       (tokens + block - 1) / block < (block == kMaxTokens ? 2048 : 256)))
+  while (block > 1 && (block * (int64_t)j.heads * lanes > kRounds * kNormThreads || 2 * j.half * block > kMaxTurns ||
+                       (tokens + block - 1) / block < (block > 8 ? 2048 : 256)))
     block /= 2;
   return block;
 }
@@ -712,7 +712,7 @@ int run_norm(const oscar_rotary* r, const oscar_head_norm* n, const int64_t* pos
   int64_t blocks = 0;
   for (int i = 0; i < kJobs; ++i) {
     NormJob& j = a.job[i];
-    j.block_tokens = tokens_a_block(tokens, j.heads, a.lanes);
+    j.block_tokens = tokens_a_block(tokens, j, a.lanes);
     j.first_block = (int32_t)blocks;
     blocks += blocks_of(j, tokens);
     if (blocks > INT32_MAX) return kErrInvalidArgument;
@@ -845,7 +845,7 @@ extern "C" int oscar_norm_rotate_backward(const oscar_rotary* rotary, const osca
   int64_t blocks[2] = {};
   for (int i = 0; i < 2; ++i) {
     NormJob& j = a.job[i];
-    j.block_tokens = tokens_a_block(num_tokens, j.heads, a.lanes);
+    j.block_tokens = tokens_a_block(num_tokens, j, a.lanes);
     blocks[i] = std::min<int64_t>(blocks_of(j, num_tokens), std::max<int64_t>(1, kBackBlocks * j.heads / std::max<int64_t>(1, heads)));
   }
   a.job[kKey].first_block = (int32_t)blocks[0];
