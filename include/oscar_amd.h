@@ -715,7 +715,7 @@ typedef struct oscar_chunk_step {
   int64_t items_size;
   int64_t workspace_size;
   int32_t parts; /* joins of rows that share a prefix */
-  int32_t reserved;
+  int32_t join_rows;
 } oscar_chunk_step;
 
 /* Keys [0, keys) that requests first .. first + requests - 1 of a step begin with, on

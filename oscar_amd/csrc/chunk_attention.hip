@@ -120,7 +120,8 @@ extern "C" int oscar_chunk_attention(const oscar_chunk_step* step, const void* i
   if (step->num_kv_heads != cache->num_kv_heads || step->head_size != cache->head_size ||
       step->block_size != cache->block_size)
     return kErrInvalidArgument;
-  if (step->narrow < 0 || step->wide < 0 || step->few_joins < 0 || step->joins < step->few_joins || step->parts < 0)
+  if (step->narrow < 0 || step->wide < 0 || step->few_joins < 0 || step->joins < step->few_joins || step->parts < 0 ||
+      step->join_rows < 0 || step->join_rows > kTileRows || (step->joins > step->few_joins && step->join_rows == 0))
     return kErrInvalidArgument;
   if (step->narrow + step->wide == 0) return kOk;
   ChunkArgs a{};

@@ -345,9 +345,11 @@ int pack_plan(const Plan& plan, int32_t head_size, void* items, size_t items_siz
   step->wide = (int32_t)plan.wide.size();
   step->joins = (int32_t)plan.joins.size();
   step->parts = (int32_t)plan.parts.size();
-  step->few_joins = (int32_t)std::count_if(plan.joins.begin(), plan.joins.end(), [&](const Join& j) {
-    return j.count + (j.shared > 0 ? plan.parts[j.shared - 1].count : 0) <= kFewParts;
-  });
+  auto few = [&](const Join& j) { return j.count + (j.shared > 0 ? plan.parts[j.shared - 1].count : 0) <= kFewParts; };
+  step->few_joins = (int32_t)std::count_if(plan.joins.begin(), plan.joins.end(), few);
+  step->join_rows = 0;
+  for (const Join& j : plan.joins)
+    if (!few(j)) step->join_rows = std::max(step->join_rows, j.rows);
   const void* const from[4] = {plan.narrow.data(), plan.wide.data(), plan.joins.data(), plan.parts.data()};
   const size_t size[4] = {plan.narrow.size() * sizeof(Piece), plan.wide.size() * sizeof(Piece),
                           plan.joins.size() * sizeof(Join), plan.parts.size() * sizeof(SharedPart)};
@@ -398,6 +400,7 @@ int step_args(const oscar_chunk_step* step, const void* items, const int32_t* bl
   a.narrow = step->narrow;
   a.wide = step->wide;
   a.few_joins = step->few_joins;
+  a.join_rows = step->join_rows;
   a.joins = reinterpret_cast<const Join*>(a.pieces + step->narrow + step->wide);
   a.parts = reinterpret_cast<const SharedPart*>(a.joins + step->joins);
   a.partials = static_cast<float*>(workspace);
@@ -412,7 +415,7 @@ int step_args(const oscar_chunk_step* step, const void* items, const int32_t* bl
 
 template <typename T, int D>
 int launch_joins(const ChunkArgs& a, const oscar_chunk_step& step, hipStream_t stream) {
-  const int64_t blocks = (int64_t)step.few_joins * (D / 32) + (int64_t)(step.joins - step.few_joins) * (kTileRows * D / 64);
+  const int64_t blocks = (int64_t)step.few_joins * (D / 32) + (int64_t)(step.joins - step.few_joins) * (step.join_rows * (D / 64));
   if (blocks > INT32_MAX) return kErrInvalidArgument;
   if (blocks > 0 && step.parts == 0) join_kernel<T, D, false><<<(uint32_t)blocks, 256, 0, stream>>>(a);
   else if (blocks > 0) join_kernel<T, D, true><<<(uint32_t)blocks, 256, 0, stream>>>(a);

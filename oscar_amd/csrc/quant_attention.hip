@@ -638,7 +638,8 @@ extern "C" int oscar_quant_attention(const oscar_quant_step* step, const void* i
       s.num_heads % cache->num_kv_heads || s.num_kv_heads != cache->num_kv_heads || s.head_size != cache->head_size ||
       s.block_size != cache->block_size)
     return kErrInvalidArgument;
-  if (s.narrow < 0 || s.wide < 0 || s.few_joins < 0 || s.joins < s.few_joins || s.parts < 0 || step->sources < 0 ||
+  if (s.narrow < 0 || s.wide < 0 || s.few_joins < 0 || s.joins < s.few_joins || s.parts < 0 || s.join_rows < 0 ||
+      s.join_rows > kTileRows || (s.joins > s.few_joins && s.join_rows == 0) || step->sources < 0 ||
       step->pages < 0 || (s.wide > 0) != (step->sources > 0) || (s.wide > 0) != (step->pages > 0) ||
       step->partials_size < 0)
     return kErrInvalidArgument;

@@ -27,7 +27,7 @@ class ChunkStepArgs(ctypes.Structure):
     _fields_ = [("num_requests", _i32), ("num_tokens", _i32), ("num_heads", _i32), ("window", _i32),
                 ("table_cols", _i32), ("narrow", _i32), ("wide", _i32), ("joins", _i32), ("few_joins", _i32),
                 ("num_kv_heads", _i32), ("head_size", _i32), ("block_size", _i32), ("items_size", _i64),
-                ("workspace_size", _i64), ("parts", _i32), ("reserved", _i32)]
+                ("workspace_size", _i64), ("parts", _i32), ("join_rows", _i32)]
 
 
 class QuantStepArgs(ctypes.Structure):
