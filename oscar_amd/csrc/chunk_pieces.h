@@ -898,6 +898,7 @@ __device__ __forceinline__ void wide_piece(const ChunkArgs& a, const Piece p, ui
 // it (512 wide pieces of D = 128: 43 MB, 9.7 us), or, where there is little, latency:
 // 2.3 to 5 us.
 constexpr int kFewParts = 8;
+constexpr int kManyAtOnce = 4;             // of a thread
 
 // A partial of one row: its slot, and the row's place there.
 struct RowPart {
@@ -953,17 +954,39 @@ __device__ __forceinline__ void join_many(const ChunkArgs& a, const Join j, cons
   __shared__ float red_m[16], red_l[16];
   const int count = kShared ? j.count + p.count : j.count;
   float m = kNone;
-  for (int i = part; i < count; i += 16) {
-    const RowPart at = part_of<D, kShared>(a, j, p, row, i);
-    m = fmaxf(m, at.slot[kTileRows * D + at.row]);
-  }
   floatx4 o{};
   float l = 0.f;
-  for (int i = part; i < count; i += 16) {
-    const RowPart at = part_of<D, kShared>(a, j, p, row, i);
-    const float w = __builtin_amdgcn_exp2f(at.slot[kTileRows * D + at.row] - m);
-    l += w * at.slot[kTileRows * D + kTileRows + at.row];
-    o += w * *reinterpret_cast<const floatx4*>(at.slot + at.row * D + feature);
+  if (count <= 16 * kManyAtOnce) {          // (one round trip to memory; more would have the maximum first)
+    float pm[kManyAtOnce], pl[kManyAtOnce];
+    floatx4 x[kManyAtOnce];
+#pragma unroll
+    for (int s = 0; s < kManyAtOnce; ++s) {
+      const RowPart at = part_of<D, kShared>(a, j, p, row, min(part + 16 * s, count - 1));
+      pm[s] = at.slot[kTileRows * D + at.row];
+      pl[s] = at.slot[kTileRows * D + kTileRows + at.row];
+      x[s] = *reinterpret_cast<const floatx4*>(at.slot + at.row * D + feature);
+    }
+#pragma unroll
+    for (int s = 0; s < kManyAtOnce; ++s)
+      if (part + 16 * s < count) m = fmaxf(m, pm[s]);
+#pragma unroll
+    for (int s = 0; s < kManyAtOnce; ++s)
+      if (part + 16 * s < count) {
+        const float w = __builtin_amdgcn_exp2f(pm[s] - m);
+        l += w * pl[s];
+        o += w * x[s];
+      }
+  } else {
+    for (int i = part; i < count; i += 16) {
+      const RowPart at = part_of<D, kShared>(a, j, p, row, i);
+      m = fmaxf(m, at.slot[kTileRows * D + at.row]);
+    }
+    for (int i = part; i < count; i += 16) {
+      const RowPart at = part_of<D, kShared>(a, j, p, row, i);
+      const float w = __builtin_amdgcn_exp2f(at.slot[kTileRows * D + at.row] - m);
+      l += w * at.slot[kTileRows * D + kTileRows + at.row];
+      o += w * *reinterpret_cast<const floatx4*>(at.slot + at.row * D + feature);
+    }
   }
   *reinterpret_cast<floatx4*>(&red[part][4 * (tid & 15)]) = o;
   if ((tid & 15) == 0) {
