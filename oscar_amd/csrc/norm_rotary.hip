@@ -554,12 +554,13 @@ int make_rows(Rows& s, const oscar_heads* x, int64_t tokens, int size, bool& vec
   if (x == nullptr || x->num_heads == 0) return kOk;
   if (x->data == nullptr || x->num_heads < 0 || x->num_heads > (1 << 16)) return kErrInvalidArgument;
   s.at = static_cast<uint8_t*>(x->data);
-  s.token = tokens > 1 ? x->token_stride * size : 0;
-  s.head = x->num_heads > 1 ? x->head_stride * size : 0;
+  s.token = tokens > 1 ? x->token_stride : 0;
+  s.head = x->num_heads > 1 ? x->head_stride : 0;
   s.heads = x->num_heads;
-  if (x->token_stride > (INT64_MAX >> 3) || x->head_stride > (INT64_MAX >> 3)) return kErrUnsupportedGeometry;
-  for (const int64_t y : {s.token, s.head})
-    if (y < 0 || y > UINT32_MAX) return kErrUnsupportedGeometry;
+  for (int64_t* const y : {&s.token, &s.head}) {
+    if (*y < 0 || *y > UINT32_MAX / size) return kErrUnsupportedGeometry;
+    *y *= size;
+  }
   vec = vec && ((uintptr_t)s.at | (uintptr_t)s.token | (uintptr_t)s.head) % 16 == 0;
   return kOk;
 }

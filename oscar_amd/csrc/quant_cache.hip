@@ -93,11 +93,13 @@ extern "C" int oscar_read_back(const oscar_quant_cache* cache, const int64_t* sl
     a.codes[i] = codes[i];
     a.page[i] = page[i], a.token[i] = token[i], a.head[i] = head[i];
     a.out[i] = static_cast<uint8_t*>(out[i]->data);
-    if (out[i]->token_stride > (INT64_MAX >> 34) || out[i]->head_stride > (INT64_MAX >> 34)) return kErrUnsupportedGeometry;
-    a.out_token[i] = num_tokens > 1 ? size * out[i]->token_stride : 0;       // (of single rows they mean nothing)
-    a.out_head[i] = cache->num_kv_heads > 1 ? size * out[i]->head_stride : 0;
-    if (a.out_token[i] < 0 || a.out_head[i] < 0 ||
-        ((uintptr_t)a.out[i] | (uintptr_t)a.out_token[i] | (uintptr_t)a.out_head[i]) % 16)
+    a.out_token[i] = num_tokens > 1 ? out[i]->token_stride : 0;       // (of single rows they mean nothing)
+    a.out_head[i] = cache->num_kv_heads > 1 ? out[i]->head_stride : 0;
+    for (int64_t* const y : {&a.out_token[i], &a.out_head[i]}) {
+      if (*y < 0 || *y > UINT32_MAX) return kErrUnsupportedGeometry;
+      *y *= size;
+    }
+    if (((uintptr_t)a.out[i] | (uintptr_t)a.out_token[i] | (uintptr_t)a.out_head[i]) % 16)
       return kErrUnsupportedGeometry;
     spans[i] = RowSpan{(uint64_t)(uintptr_t)a.out[i], a.out_token[i], a.out_head[i], num_tokens, cache->num_kv_heads, row};
   }
