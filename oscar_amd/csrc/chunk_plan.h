@@ -35,13 +35,14 @@ struct PlanRule {
   int32_t narrow_rows;     // of a request and kv head, at most
   int32_t resident[2];     // narrow pieces that read at full rate, and that fit the GPU at once
   double key_bytes;        // of a key's features, read
+  int32_t uneven;          // narrow pieces to cut very uneven row tiles to, where they fill the GPU; 0: never
 };
 inline PlanRule plain_rule(int32_t head_size) {
   // Up to 32 rows a request is narrow (28 rows of 16 users over 1000 keys, D = 128: 20.4
   // us, as wide tiles 24.2; 30 of 8 users over 16000, D = 256, 31.1, 30.1), from 33 on
   // wide, where narrow tiles would read its keys twice (48 rows, the same: 24.7 us, as
   // narrow 23.2; 32.2, 36.1; 32 users over 4000 32.5, 49.6).
-  return PlanRule{head_size, kTileRows, {kCus, kCus * narrow_wgs(head_size)}, 2.};
+  return PlanRule{head_size, kTileRows, {kCus, kCus * narrow_wgs(head_size)}, 2., 0};
 }
 
 struct RowTile {
@@ -154,6 +155,13 @@ int32_t pieces_of(const RowTile& x, int64_t per) { return (int32_t)((x.tiles + p
 // 256, 190 us, 5.2 TB/s), but one request that is far longer than the others is then
 // read by one workgroup (300 users of 1000 keys and one of 131072 2.2 ms, where the
 // bytes take 0.09), and by a few where there are just fewer (250 and one: 0.39 ms).
+// `uneven`: row tiles that are as many, the longest of them more than twice a resident
+// piece's mean length and 32 key tiles above it, are cut to that many mean lengths.
+// 8-bit caches, whole / cut to three a CU, us: 64 users over 100 to 16000 keys, D = 128,
+// 8 kv heads, 195 / 107, 128 users 291 / 203, 4 tokens of 128 users, D = 64, 4 heads,
+// 155 / 84; 256 over 100 to 8000, D = 256, 175 / 103; 300 over 1000 and one over 60000
+// 954 / 90; without the second condition 256 over 100 to 800 27 / 32.
+constexpr int32_t kMuchLonger = 32;
 void plan_narrow(const std::vector<RowTile>& rows, const PlanRule& rule, double beside, Plan& plan,
                  std::vector<PrefixRows>& prefixes) {
   int64_t total = 0;
@@ -170,6 +178,8 @@ void plan_narrow(const std::vector<RowTile>& rows, const PlanRule& rule, double 
       for (const RowTile& x : rows) c += pieces_of(x, t);
       return c;
     };
+    if (rule.uneven > 0 && (int64_t)rows.size() >= resident && most > 2 * per && most > per + kMuchLonger)
+      return std::max<int64_t>(kWaves, (total + rule.uneven - 1) / rule.uneven);
     if ((int64_t)rows.size() >= resident || most <= uncut) per = std::max<int64_t>(per, most);
     // (The count falls as pieces get longer.  Step by step the search took 5 ms for 250
     // short rows beside 2^20 keys, and 17 s beside 2^30.)

@@ -147,3 +147,44 @@ def test_step_struct_matches_the_header(tmp_path):
     got = subprocess.run([str(tmp_path / "layout")], check=True, capture_output=True, text=True).stdout.split()
     assert [int(x) for x in got] == [ctypes.sizeof(chunk.QuantStepArgs)] + [getattr(chunk.QuantStepArgs, f).offset
                                                                             for f in fields]
+
+
+@pytest.mark.parametrize("d, hk, group", [(64, 4, 4), (64, 3, 2), (256, 1, 6), (128, 2, 16)])
+@pytest.mark.parametrize("window", [0, 100])
+@pytest.mark.parametrize("reqs", [[(1, 32768)] * 8, [(4, 5000), (0, 7), (12, 4096), (4, 333), (5, 31)],
+                                  [(1, 37 * i) for i in range(300)], [(9, 700)] * 11])
+def test_narrow_pieces_cover_every_row_and_key_once(reqs, window, d, hk, group):
+    """In whatever order they stand; pieces of the same lines 8 apart."""
+    starts, seqs = [0], []
+    for n, h in reqs:
+        starts.append(starts[-1] + n)
+        seqs.append(n + h)
+    args, pieces, _ = plan(starts, seqs, hk * group, quant_cache(d=d, hk=hk), window)
+    assert args.chunk.wide == 0
+    parts = {}
+    for token0, pos0, row, head, row0, rows, key0, key1, *_ in pieces:
+        n, h = reqs[row]
+        assert token0 == starts[row] and pos0 == h and row0 % 32 == 0 and rows == min(32, n * group - row0)
+        parts.setdefault((row, head, row0), []).append((key0, key1))
+    assert len(parts) == sum(hk * -(-n * group // 32) for n, _ in reqs)
+    for (row, _, row0), keys in parts.items():
+        n, h = reqs[row]
+        first, last = h + row0 // group, h + (min(row0 + 32, n * group) - 1) // group
+        keys.sort()
+        lo = max(0, first - window + 1) if window else 0
+        assert keys[0][0] == lo // 32 * 32 and keys[-1][1] == last + 1
+        assert all(a[1] == b[0] for a, b in zip(keys, keys[1:]))
+    if d == 64 and hk == 4 and len({n for n, _ in reqs}) == 1 and not window:
+        at = {p[:8]: i for i, p in enumerate(pieces)}
+        pairs = [at[p[:3] + (p[3] + 1,) + p[4:8]] - i for i, p in enumerate(pieces) if p[3] % 2 == 0 and p[4] == 0]
+        assert all(x > 0 for x in pairs) and sum(x == 8 for x in pairs) >= len(pairs) - 8
+
+
+@pytest.mark.parametrize("d, hk, group", [(64, 4, 4), (256, 2, 6), (128, 8, 4)])
+def test_a_much_longer_request_is_cut_where_the_others_fill_the_gpu(d, hk, group):
+    keys = [1000] * 300 + [60000]
+    args, pieces, _ = plan(list(range(302)), keys, hk * group, quant_cache(d=d, hk=hk))
+    mean = -(-sum(-(-n // 32) for n in keys) * hk // (3 * 256))           # tiles of 32 keys
+    assert max(p[7] - p[6] for p in pieces) <= 32 * mean and args.chunk.narrow <= 301 * hk + 3 * 256 and args.chunk.wide == 0
+    args, pieces, _ = plan(list(range(302)), [100 + 2 * i for i in range(301)], hk * group, quant_cache(d=d, hk=hk))
+    assert args.chunk.narrow == 301 * hk and args.chunk.joins == 0
