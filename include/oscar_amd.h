@@ -662,7 +662,8 @@ typedef struct oscar_quant_cache {
  * power of two is the smallest, of 2^-80 .. 2^100 (bf16) or 2^-15 .. 2^8 (fp16), with
  * which its largest finite magnitude is at most 448 times it; smaller values than the
  * least power reaches round to zero, larger ones than the greatest reaches become 240
- * times it; infinities and NaN become NaN. */
+ * times it; infinities and NaN become NaN.  Slots of a call are distinct: of two tokens
+ * that name one, the row may hold one's codes and the other's power. */
 int oscar_append_quantized(const oscar_rotary* rotary, const oscar_head_norm* norm, const int64_t* positions,
                            int64_t position_axis_stride, int64_t num_tokens, const oscar_heads* query,
                            const oscar_heads* query_out, const oscar_heads* key, const oscar_heads* value,
