@@ -639,7 +639,8 @@ int oscar_append_normed(const oscar_rotary* rotary, const oscar_head_norm* norm,
  * stands for code * 2^(b - 127), b the byte at exponents[((p * num_kv_heads + h) *
  * block_size + t) * 2], of V the byte after it.  Base addresses and strides are
  * multiples of 16 bytes and tokens and heads do not overlap; head_size is a multiple
- * of 16, at most 256.  dtype: of the rows that are written and read (bf16 or fp16). */
+ * of 16, at most 256.  dtype: of the rows that are written and read (bf16 or fp16).  b
+ * is 47 to 227 in bf16 and 112 to 135 in fp16, of codes of zero any. */
 typedef struct oscar_quant_cache {
   void* k;
   void* v;

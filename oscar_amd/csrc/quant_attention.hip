@@ -235,7 +235,9 @@ __device__ __forceinline__ void code_piece(const QuantChunkArgs& all, const Piec
     for (int h = 0; h < kGroups; ++h)
       load_codes<D, kV, kPolicy>(c, p, p.key0 + t * kKeys + 16 * h, 16 * h, page_of(t, h), in_page(t, h), lds, at);
   };
-  // The powers of keys lane % 32 of the subtiles: K's in the low byte, V's above.  (Their
+  // The powers of keys lane % 32 of the subtiles: K's in the low byte, V's above, which is
+  // taken for the type's least where it is less (zeros that no write has left: a weight
+  // over 2^-127 would pass fp32).  (Their
   // places as scalars: as a choice of the lane the pages would be the lane's for the
   // loads to LDS as well, which then loop over descriptors.)
   uint32_t powers[kSubs];
@@ -299,8 +301,10 @@ __device__ __forceinline__ void code_piece(const QuantChunkArgs& all, const Piec
     for (int u = 0; u < kSubs; ++u) {
       k_scale[u] = scale_of(powers[u] & 0xFFu);
       if (here < 32) {
-        v_powers[32 * u + here] = (float)((int)(powers[u] >> 8) - 127);
-        v_scales[32 * u + here] = scale_of(powers[u] >> 8);
+        constexpr uint32_t kLeast = 127 + exponent_range(std::is_same_v<T, __bf16> ? OSCAR_BF16 : OSCAR_FP16).low;
+        const uint32_t v = max(powers[u] >> 8, kLeast);
+        v_powers[32 * u + here] = (float)((int)v - 127);
+        v_scales[32 * u + here] = scale_of(v);
       }
     }
     // (in this order at D = 256, kAhead reads ahead: left to it, the compiler asks for all

@@ -19,7 +19,7 @@ namespace oscar {
 struct ExponentRange {
   int low, high;
 };
-inline ExponentRange exponent_range(int dtype) {
+constexpr ExponentRange exponent_range(int dtype) {
   return dtype == OSCAR_FP16 ? ExponentRange{-15, 8} : ExponentRange{-80, 100};
 }
 

@@ -79,8 +79,9 @@ class QuantCache:
     """A layer's 8-bit K and V pages, checked and packed once: codes [pages,
     block_size, Hk, D] (float8_e4m3fn, or their bytes as uint8) that stand for
     code * 2^(b - 127), b the byte at exponents [pages, Hk, block_size, 2] (uint8,
-    contiguous; K's, then V's).  dtype (bf16 or fp16) is that of the rows that are
-    written and read; the values are exact in it.  Codes may be views as
+    contiguous; K's, then V's): 47 to 227 in bf16, 112 to 135 in fp16, of codes of zero
+    any.  dtype (bf16 or fp16) is that of the rows that are written and read; the values
+    are exact in it.  Codes may be views as
     PagedCache's may; D is a multiple of 16."""
 
     def __init__(self, k_codes: torch.Tensor, v_codes: torch.Tensor, exponents: torch.Tensor, dtype: torch.dtype):

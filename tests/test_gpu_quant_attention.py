@@ -369,3 +369,23 @@ def test_two_graphs_of_a_step(device):
             graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(held, want))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("new", [1, 300])
+def test_rows_of_zeros_whatever_their_power(device, dtype, d, new):
+    """Slots that hold zeros with a power below the type's least, as fresh memory of zeros
+    does, weigh as any key of zeros: alone, and beside keys of large negative scores,
+    where exp2(score - maximum of score + power) would pass fp32 if the power counted."""
+    g = torch.Generator(device=device).manual_seed(d)
+    q, cache, table, starts, seqs = make(g, [(new, 900), (new, 100)], 4, 2, d, 32, dtype)
+    for x in (cache.k_codes, cache.v_codes, cache.exponents):
+        x.zero_()
+    step = chunk.ChunkStep(starts, seqs, table, 4, cache)
+    assert chunk.chunk_attention(q, cache, step, 0.1).eq(0).all()
+    page = table[0, 3].long()               # keys 96 .. 127 of request 0, against the queries
+    q.copy_(q.abs() + 1)
+    cache.k_codes[page], cache.v_codes[page], cache.exponents[page] = 0xF8, 0x70, 127 - 3
+    got = chunk.chunk_attention(q, cache, step, 1.0 / d)
+    check(got, q, cache, table, starts, seqs, 0, 1.0 / d)
