@@ -13,7 +13,8 @@ Of dx = r (u - x^ mean(u x^)), u = R^T(g) w, x^ = r x: each factor is off by at 
 2^-24 (u as y above), the mean by as much again, so 2^-18 of r (|u| + |x^| mean(|u||x^|)),
 |u| taken as (|g1| + |g2|) |w|, and the roundings to the type as above.
 Of dw = sum of h x^: 2^-19 of the terms' magnitudes, and the additions': at most 20 rows
-of heads in a lane, 256 groups, 128 workgroups a thread and 16 threads, 420 * 2^-24."""
+of heads in a lane, 256 groups, 8 workgroups a place, 8 places and 64 threads: 356, taken
+as 420 * 2^-24."""
 import pytest
 import torch
 
@@ -359,3 +360,18 @@ def test_refusals(device):
         rotary.norm_rotate(x[:, :4], None, w, None, pos, turn, query_out=x[:, 2:6])
     with pytest.raises(ValueError, match="device"):
         rotary.norm_rotate(q, None, w.cpu(), None, pos, turn)
+
+
+def test_positions_of_any_kind(device):
+    """int32 and strided positions, rows of a padded batch behind them."""
+    g = torch.Generator(device=device).manual_seed(8)
+    turn = rotary.Rotary(rotary.rotary_table(500, 32).to(device))
+    wq, wk = weights(g, 64, torch.float32, 0.0)
+    q, k = (torch.randn(20, h, 64, generator=g, device=device).bfloat16() for h in (3, 2))
+    positions = torch.randint(0, 500, (17,), generator=g, device=device)
+    want = rotary.norm_rotate(q[:17], k[:17], wq, wk, positions, turn)
+    wide = torch.zeros(17, 3, dtype=torch.int64, device=device)
+    wide[:, 1] = positions
+    for p in (positions.int(), wide[:, 1], wide.int()[:, 1]):
+        for x, y in zip(rotary.norm_rotate(q[:17], k[:17], wq, wk, p, turn), want):
+            assert torch.equal(x, y)

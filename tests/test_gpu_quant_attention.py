@@ -389,3 +389,37 @@ def test_rows_of_zeros_whatever_their_power(device, dtype, d, new):
     cache.k_codes[page], cache.v_codes[page], cache.exponents[page] = 0xF8, 0x70, 127 - 3
     got = chunk.chunk_attention(q, cache, step, 1.0 / d)
     check(got, q, cache, table, starts, seqs, 0, 1.0 / d)
+
+
+def test_a_much_longer_request_among_many(device):
+    """It is cut where the others fill the GPU; nothing else of the step is."""
+    g = torch.Generator(device=device).manual_seed(12)
+    reqs = [(1, 7 * i % 97) for i in range(260)] + [(2, 8000)] + [(1, 50)] * 3
+    for dtype, hq, hk, d, page in ((torch.bfloat16, 6, 2, 256, 128), (torch.float16, 8, 2, 64, 16)):
+        q, cache, table, starts, seqs = make(g, reqs, hq, hk, d, page, dtype)
+        step = chunk.ChunkStep(starts, seqs, table, hq, cache)
+        assert step.args.chunk.joins == hk and step.args.chunk.narrow > len(reqs) * hk + 8
+        got = chunk.chunk_attention(q, cache, step, d ** -0.5)
+        check(got, q, cache, table, starts, seqs, 0, d ** -0.5)
+
+
+def test_two_calls_of_a_step_at_once(device):
+    """On two streams, into the queries themselves: prompts, cut decodes and a prefix."""
+    g = torch.Generator(device=device).manual_seed(13)
+    reqs = [(300, 700), (1, 20000), (4, 3000), (4, 3100), (4, 3050)]
+    q, cache, table, starts, seqs = make(g, reqs, 4, 2, 128, 32, torch.bfloat16)
+    table[3, :93] = table[4, :93] = table[2, :93]
+    step = chunk.ChunkStep(starts, seqs, table, 4, cache, prefixes=[(2, 3, 2976)])
+    want = chunk.chunk_attention(q, cache, step, 0.1)
+    check(want, q, cache, table, starts, seqs, 0, 0.1)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        rows = [q.clone() for _ in streams]
+        torch.cuda.synchronize()
+        for x, stream in zip(rows, streams):
+            with torch.cuda.stream(stream):
+                chunk.chunk_attention(x, cache, step, 0.1, out=x)
+        torch.cuda.synchronize()
+        for x in rows:
+            assert torch.equal(x, want)
