@@ -10,10 +10,19 @@
 //   dx = r (u - x^ sum(u x^) / D),   dw = sum over heads and tokens of h x^.
 // All of it is fp32 arithmetic, one rounding to the rows' type at the end.
 //
+// (The sum is of fp32 squares: of a head whose values pass 1e18 it is an infinity, and the
+// head becomes zeros.)
+//
 // Every value is read once and written once, so memory bounds the kernels, and for a
 // few tokens their latency.  A group of lanes takes a head (16 features a lane in two
 // pieces of 8, pairs that turn together in one lane), so its sums are a few
-// exchanges inside 16 lanes and nothing but the tokens' cosines goes through LDS.
+// exchanges inside 16 lanes; the tokens' cosines and the kind's weights go through LDS
+// (as loads of each lane's own, sixteen for four rows, 9256 tokens take 20.0 us for
+// 17.4, 30843 with the gradient 395 for 356).
+// Measured: one token of 6 + 1 heads of 256 3.8 us; 9256 tokens (66 MB, in the last-level
+// cache) 15.7, 4.2 TB/s; 30843 of 32 + 8 heads of 128 110 (632 MB, 5.7 TB/s), their
+// gradient 181 (947 MB, 5.2 TB/s) and the weights' sums 6.9; the write of 65536 tokens of
+// 6 + 1 + 1 heads of 256 to 8 bits 115 (503 MB, 4.4 TB/s).
 #include "plain_cache.h"
 #include "quant_cache.h"
 #include "row_span.h"
@@ -29,7 +38,8 @@ constexpr int kMaxTokens = 64;             // of a workgroup at a time,
 constexpr int kMaxTurns = 4096;            // and their cosines and sines
 constexpr int kMaxRotary = 256;
 constexpr int64_t kLastCache = 256ll << 20;      // bytes
-constexpr int kBackBlocks = 4096;          // workgroups of the gradient, at most (1024: 30843 tokens' step 357 us for 297)
+// Workgroups of the gradient, at most (1024: 30843 tokens' step 357 us for 297).
+constexpr int kBackBlocks = 4096;
 
 enum Target { kRows, kPlain, kQuant };
 
@@ -359,11 +369,12 @@ template <typename T, int kVec, bool kAdjacent, int kTarget, bool kOnce>
 __global__ __launch_bounds__(kNormThreads) void norm_kernel(NormArgs a) {
   constexpr int kSlots = Part<kVec>::kSlots, kPairs = Part<kVec>::kPairs;
   __shared__ __attribute__((aligned(16))) TokenState st;
-  const int kind = (int)blockIdx.x >= a.job[kValue].first_block ? kValue : (int)blockIdx.x >= a.job[kKey].first_block ? kKey : kQuery;
+  const int block = (int)blockIdx.x;
+  const int kind = block >= a.job[kValue].first_block ? kValue : block >= a.job[kKey].first_block ? kKey : kQuery;
   const NormJob& j = a.job[kind];
   const int tid = (int)threadIdx.x;
   const int group = tid >> a.lane_shift, u0 = tid & (a.lanes - 1), groups = kNormThreads >> a.lane_shift;
-  const int64_t tok0 = (int64_t)((int)blockIdx.x - j.first_block) * j.block_tokens;
+  const int64_t tok0 = (int64_t)(block - j.first_block) * j.block_tokens;
   const int tokens = (int)min((int64_t)j.block_tokens, a.tokens - tok0), count = tokens * j.heads;
   const bool cached = kTarget != kRows && kind != kQuery;
   Place at[kSlots];
@@ -621,15 +632,18 @@ int tokens_a_block(int64_t tokens, const NormJob& j, int lanes) {
     block /= 2;
   return block;
 }
-int64_t blocks_of(const NormJob& j, int64_t tokens) { return j.heads == 0 ? 0 : (tokens + j.block_tokens - 1) / j.block_tokens; }
+int64_t blocks_of(const NormJob& j, int64_t tokens) {
+  return j.heads == 0 ? 0 : (tokens + j.block_tokens - 1) / j.block_tokens;
+}
 
 template <typename T, int kTarget>
 void launch_norm(const NormArgs& a, uint32_t blocks, bool vec, bool once, hipStream_t stream) {
   // (single values of adjacent pairs and of halves differ in their places alone)
-  const auto kernel = !vec            ? &norm_kernel<T, 1, false, kTarget, false>
-                      : a.adjacent    ? once ? &norm_kernel<T, 8, true, kTarget, true> : &norm_kernel<T, 8, true, kTarget, false>
-                      : once          ? &norm_kernel<T, 8, false, kTarget, true>
-                                      : &norm_kernel<T, 8, false, kTarget, false>;
+  const auto kernel = !vec                 ? &norm_kernel<T, 1, false, kTarget, false>
+                      : a.adjacent && once ? &norm_kernel<T, 8, true, kTarget, true>
+                      : a.adjacent         ? &norm_kernel<T, 8, true, kTarget, false>
+                      : once               ? &norm_kernel<T, 8, false, kTarget, true>
+                                           : &norm_kernel<T, 8, false, kTarget, false>;
   kernel<<<blocks, kNormThreads, 0, stream>>>(a);
 }
 
@@ -847,7 +861,8 @@ extern "C" int oscar_norm_rotate_backward(const oscar_rotary* rotary, const osca
   for (int i = 0; i < 2; ++i) {
     NormJob& j = a.job[i];
     j.block_tokens = tokens_a_block(num_tokens, j, a.lanes);
-    blocks[i] = std::min<int64_t>(blocks_of(j, num_tokens), std::max<int64_t>(1, kBackBlocks * j.heads / std::max<int64_t>(1, heads)));
+    const int64_t share = kBackBlocks * j.heads / std::max<int64_t>(1, heads);
+    blocks[i] = std::min<int64_t>(blocks_of(j, num_tokens), std::max<int64_t>(1, share));
   }
   a.job[kKey].first_block = (int32_t)blocks[0];
   if (blocks[0] + blocks[1] > 0) {

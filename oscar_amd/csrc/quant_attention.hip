@@ -189,6 +189,11 @@ __device__ __forceinline__ void add_nan(const ChunkArgs& a, const QuantArgs& c, 
 // K; V's go through LDS to the lanes that hold the keys' scores, as numbers and as powers.
 // A tile is weighed by the maximum as it stands, and only where a weight is too large
 // is the maximum raised and the tile weighed again.
+// Memory bounds it: 32 users' 4 tokens of 6 heads over 2K to 16K keys of 256, 146 MB, 31.3
+// us (4.7 TB/s; 10 to 15 % less without the products: the rest is the start, the first
+// tile's round trips and the waves' joining), 32 users' token over 8 heads of 128, 578 MB, 118
+// (5.0 TB/s); at D = 64, 32 users' 4 tokens of 16 heads on 4, 147 MB, 43 with the join (3.4
+// TB/s; 41 where a head's rows lie together).
 constexpr int code_keys(int d) { return 8192 / d; }
 constexpr int kCodeWgs = 2;                // workgroups a CU
 constexpr int code_lds(int d) { return kWaves * (2 * 8192 + std::max(2 * code_keys(d) * 4, 2 * kTileRows * 4)); }
@@ -252,7 +257,8 @@ __device__ __forceinline__ void code_piece(const QuantChunkArgs& all, const Piec
         at[h] = 2 * (((int64_t)page * c.num_heads + p.kv_head) * c.block_size + from);
       }
       const int at_lane = opaque(lane);
-      powers[u] = *reinterpret_cast<const uint16_t*>(c.exponents + ((at_lane & 16) != 0 ? at[1] : at[0]) + 2 * (at_lane & 15));
+      const int64_t row = (at_lane & 16) != 0 ? at[1] : at[0];
+      powers[u] = *reinterpret_cast<const uint16_t*>(c.exponents + row + 2 * (at_lane & 15));
     }
   };
   float* const v_powers = reinterpret_cast<float*>(smem + kWaves * 2 * kTileBytes) + wave * 2 * kKeys;
@@ -346,7 +352,8 @@ __device__ __forceinline__ void code_piece(const QuantChunkArgs& all, const Piec
 #pragma unroll
     for (int u = 0; u < kSubs; ++u) weigh(x[u], u, w[u], l);
     if constexpr (D == 256) keep_order();
-    ushortx8 most = __builtin_elementwise_max(__builtin_bit_cast(ushortx8, w[0][0]), __builtin_bit_cast(ushortx8, w[0][1]));
+    ushortx8 most = __builtin_bit_cast(ushortx8, w[0][0]);
+    most = __builtin_elementwise_max(most, __builtin_bit_cast(ushortx8, w[0][1]));
 #pragma unroll
     for (int u = 1; u < kSubs; ++u)
 #pragma unroll
@@ -413,7 +420,9 @@ __device__ __forceinline__ void code_piece(const QuantChunkArgs& all, const Piec
 // ---------------------------------------------------------------- kernels
 // (Codes past the caches, kOnce, where they are more than the last-level cache holds: 32
 // users' token over 2K to 16K keys of 8 heads of 128, 578 MB, 123 us, through them 135; 32
-// users' 4 of one head of 256, 146 MB, 39 us, through them 37; 48 rows over 32 MB 33, 31.)
+// users' 4 of one head of 256, 146 MB, 39 us, through them 37; 48 rows over 32 MB 33, 31.
+// At D = 64 neighbouring heads share lines, which L2 keeps for the second: 8 heads of 32
+// users, 297 MB, 88 us, through them 82; of one head, 587 MB, 76 and 81.)
 template <typename T, int D, int kPolicy>
 __global__ __launch_bounds__(kThreads, kCodeWgs) void code_kernel(QuantChunkArgs a) {
   __shared__ __attribute__((aligned(1024))) uint8_t smem[code_lds(D)];
@@ -431,7 +440,9 @@ __global__ __launch_bounds__(kThreads, kWideWgs) void quant_kernel(QuantChunkArg
 }
 
 // The sources' keys as 16-bit pages of 16 keys [K | V][key][head][D], a workgroup each,
-// and the pages' block table.  A thread takes 8 codes at a time, four times at once.
+// and the pages' block table.  A thread takes 8 codes at a time, four times at once.  Memory
+// and a launch bound it: 24579 keys of a head of 256 7.8 us (38 MB, 4.8 TB/s), 12288 of 8
+// heads of 128 15 (75 MB, 5.0 TB/s; the products over them then take 690).
 struct PagesArgs {
   QuantArgs codes;
   const Source* sources;
@@ -528,7 +539,8 @@ void order_pieces(std::vector<Piece>& pieces, int32_t head_size) {
   std::vector<uint32_t> groups{0};          // where they begin in the order
   for (size_t i = 0; i < order.size();) {
     size_t end = i + 1;
-    while (end < order.size() && pieces[end].table_row == pieces[i].table_row && pieces[end].token0 == pieces[i].token0) ++end;
+    auto of_one = [&](const Piece& p) { return p.table_row == pieces[i].table_row && p.token0 == pieces[i].token0; };
+    while (end < order.size() && of_one(pieces[end])) ++end;
     std::sort(order.begin() + (std::ptrdiff_t)i, order.begin() + (std::ptrdiff_t)end);
     for (size_t k = i + 1; k <= end; ++k)
       if (k == end || order[k].first != order[k - 1].first) groups.push_back((uint32_t)k);
@@ -620,7 +632,8 @@ extern "C" int oscar_quant_plan(const int32_t* query_start_loc, const int32_t* s
     int64_t codes = 0;                      // bytes that narrow pieces read
     for (const Piece& p : plan.narrow)
       if (p.row0 == 0) codes += 2ll * cache->head_size * (p.key1 - p.key0);
-    step->once = codes > kLastCache;
+    const bool half_lines = cache->head_size == 64 && cache->num_kv_heads > 1 && cache->k_stride_head == 64;
+    step->once = codes > kLastCache && !half_lines;
     step->reserved = 0;
     step->partials_size = (s.workspace_size + 255) / 256 * 256;
     s.items_size += (int64_t)(sources.size() * sizeof(Source));
