@@ -375,3 +375,36 @@ def test_positions_of_any_kind(device):
     for p in (positions.int(), wide[:, 1], wide.int()[:, 1]):
         for x, y in zip(rotary.norm_rotate(q[:17], k[:17], wq, wk, p, turn), want):
             assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("d, rd", [(256, 64), (128, 128), (192, 64)])
+def test_rows_off_16_bytes(device, dtype, d, rd):
+    """Heads whose rows begin at single values: the outputs, the gradient, the writes."""
+    g = torch.Generator(device=device).manual_seed(d)
+    turn = rotary.Rotary(rotary.rotary_table(500, rd, device=device))
+    n = 37
+    fused = torch.randn(n, 5 * d + 3, generator=g, device=device).to(dtype)[:, 1:1 + 5 * d].unflatten(1, (5, d))
+    q, k, v = fused[:, :3], fused[:, 3:4], fused[:, 4:]
+    wq, wk = weights(g, d, torch.float32, 0.0)
+    pos = torch.randint(0, 500, (n,), generator=g, device=device)
+    out = torch.empty(n, 4 * d + 1, dtype=dtype, device=device)[:, 1:].unflatten(1, (4, d))
+    got = rotary.norm_rotate(q, k, wq, wk, pos, turn, query_out=out[:, :3], key_out=out[:, 3:])
+    for x, y, w in zip(got, (q, k), (wq, wk)):
+        close(x, normed(y, w, pos[None], turn, False, None, 1e-6, 0.0))
+    leaf = fused.detach().requires_grad_()
+    wq.requires_grad_()
+    grad = torch.randn(n, 3 * d + 1, generator=g, device=device).to(dtype)[:, 1:].unflatten(1, (3, d))
+    dx, dw = torch.autograd.grad(rotary.norm_rotate(leaf[:, :3], None, wq, None, pos, turn)[0], (leaf, wq), grad)
+    want = gradients(q.detach(), wq.detach(), grad, pos, turn, False, None, 1e-6, 0.0)
+    close(dx[:, :3], want[0])
+    close(dw, want[1])
+    assert dx[:, 3:].eq(0).all()
+    if dtype == torch.float32:
+        return
+    slots = torch.randperm(64, generator=g, device=device)[:n]
+    caches = [append.quant_cache(4, 16, 1, d, dtype, device) for _ in range(2)]
+    for cache, rows_of in zip(caches, (lambda x: x, lambda x: x.contiguous())):
+        append.append_quantized(None, rows_of(k), rows_of(v), pos, turn, cache, slots)
+    for x in ("k_codes", "v_codes", "exponents"):       # (no norm: the same sums whatever the lanes)
+        assert torch.equal(getattr(caches[0], x), getattr(caches[1], x))
