@@ -153,18 +153,20 @@ __device__ __forceinline__ bool take_out_nan(uint8_t* vt, int lane) {
   }
   return true;
 }
-// NaN among a tile's values, for the rows that see them; what is whole and mapped had
-// them in the product.
-template <typename T, int D>
+// NaN among the values of a tile of kKeys, for the rows that see them.  A tile that is whole
+// and has all its groups of 16 keys, mapped ones below the piece's last, had them in the
+// product; of any other they were taken out, of the groups that are there as well.
+template <typename T, int D, int kKeys>
 __device__ __forceinline__ void add_nan(const ChunkArgs& a, const QuantArgs& c, const Piece& p, int key0, bool whole,
                                         int lane, RowState<T, D>& s) {
   auto page_of = [&](int key) {
     const int page = c.table[(int64_t)p.table_row * c.table_stride + fast_div((uint32_t)key, c.block_div)];
     return page >= 0 && page < c.num_pages ? page : -1;
   };
-  const int end = min(key0 + kTileKeys, p.key1);
-  if (whole && page_of(key0) >= 0 && page_of(end - 1) >= 0) return;
-  for (int key = key0; key < end; ++key) {
+  bool there = whole;
+  for (int key = key0; there && key < key0 + kKeys; key += 16) there = key < p.key1 && page_of(key) >= 0;
+  if (there) return;
+  for (int key = key0; key < min(key0 + kKeys, p.key1); ++key) {
     const int page = page_of(key);
     if (page < 0) continue;
     const uint8_t* row = c.v + (int64_t)p.kv_head * c.v_head + (uint64_t)(uint32_t)page * c.v_page +
@@ -412,7 +414,7 @@ __device__ __forceinline__ void code_piece(const QuantChunkArgs& all, const Piec
   if (__builtin_expect(special, 0))
     for (int t = first; t < last; ++t) {
       const int key0 = p.key0 + t * kKeys;
-      for (int k = key0; k < min(key0 + kKeys, p.key1); k += kTileKeys) add_nan<T, D>(a, c, p, k, whole(key0), lane, s);
+      add_nan<T, D, kKeys>(a, c, p, key0, whole(key0), lane, s);
     }
   combine_waves<T, D, D == 256 ? 2 : 1>(a, p, s, smem, tid, lane, wave);
 }

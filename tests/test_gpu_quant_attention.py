@@ -423,3 +423,42 @@ def test_two_calls_of_a_step_at_once(device):
         torch.cuda.synchronize()
         for x in rows:
             assert torch.equal(x, want)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("reqs, gone, prefixes, window", [
+    ([(1, 3999)], (), (), 0), ([(1, 4099), (3, 4001)], (), (), 0), ([(2, 1030)], (0, 21, 45, 63), (), 0),
+    ([(3, 2000)], (124,), (), 900), ([(1, 1700), (2, 1650), (1, 1633)], (), [(0, 3, 1632)], 0)])
+def test_nan_beside_keys_that_are_not_there(device, dtype, d, reqs, gone, prefixes, window):
+    """One in every 32 keys, a feature each, where pieces end inside a tile of codes and where
+    a page of 16 keys in a tile is outside the cache: each reaches the rows that see it."""
+    g = torch.Generator(device=device).manual_seed(len(reqs) + d)
+    q, cache, table, starts, seqs = make(g, reqs, 4, 2, d, 16, dtype)
+    for first, count, keys in prefixes:
+        table[first:first + count, :keys // 16] = table[first, :keys // 16]
+    for page in gone:
+        table[0, page] = -1
+    step = chunk.ChunkStep(starts, seqs, table, 4, cache, window, prefixes=prefixes)
+    clean = chunk.chunk_attention(q, cache, step, 0.1)
+    assert clean.isfinite().all()
+    held = cache.v_codes.clone()
+    tiles = range(seqs[0] // 32)
+    for at in range(0, len(tiles), d):
+        touched = torch.zeros_like(clean, dtype=torch.bool)
+        for tile in tiles[at:at + d]:
+            feature = tile - at
+            pos = 32 * tile + (7 * tile) % 32
+            page = table[0, pos // 16].long()
+            if page < 0:
+                continue
+            cache.v_codes[page, pos % 16, 1, feature] = 0x7F if tile % 2 else 0xFF
+            for i, (n, h) in enumerate(reqs):
+                if i == 0 or any(pos < keys for _, _, keys in prefixes):
+                    rows = h + torch.arange(n, device=device)
+                    sees = (rows >= pos) & ((rows < pos + window) if window else True)
+                    touched[starts[i]:starts[i + 1], 2:, feature] |= sees[:, None]
+        got = chunk.chunk_attention(q, cache, step, 0.1)
+        assert touched.any()
+        assert torch.equal(got.isnan(), touched) and torch.equal(got[~touched], clean[~touched])
+        cache.v_codes.copy_(held)
