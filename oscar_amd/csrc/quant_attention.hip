@@ -243,8 +243,9 @@ __device__ __forceinline__ void code_piece(const QuantChunkArgs& all, const Piec
       load_codes<D, kV, kPolicy>(c, p, p.key0 + t * kKeys + 16 * h, 16 * h, page_of(t, h), in_page(t, h), lds, at);
   };
   // The powers of keys lane % 32 of the subtiles: K's in the low byte, V's above, which is
-  // taken for the type's least where it is less (zeros that no write has left: a weight
-  // over 2^-127 would pass fp32).  (Their
+  // taken for the type's least where it is outside its range (zeros that no write has left:
+  // below it a weight over 2^-127 would pass fp32, above it the maximum would be theirs and
+  // every other key's weight nothing beside it).  (Their
   // places as scalars: as a choice of the lane the pages would be the lane's for the
   // loads to LDS as well, which then loop over descriptors.)
   uint32_t powers[kSubs];
@@ -309,8 +310,9 @@ __device__ __forceinline__ void code_piece(const QuantChunkArgs& all, const Piec
     for (int u = 0; u < kSubs; ++u) {
       k_scale[u] = scale_of(powers[u] & 0xFFu);
       if (here < 32) {
-        constexpr uint32_t kLeast = 127 + exponent_range(std::is_same_v<T, __bf16> ? OSCAR_BF16 : OSCAR_FP16).low;
-        const uint32_t v = max(powers[u] >> 8, kLeast);
+        constexpr ExponentRange kRange = exponent_range(std::is_same_v<T, __bf16> ? OSCAR_BF16 : OSCAR_FP16);
+        constexpr uint32_t kLeast = 127 + kRange.low, kSpan = kRange.high - kRange.low;
+        const uint32_t byte = powers[u] >> 8, v = byte - kLeast <= kSpan ? byte : kLeast;
         v_powers[32 * u + here] = (float)((int)v - 127);
         v_scales[32 * u + here] = scale_of(v);
       }

@@ -462,3 +462,20 @@ def test_nan_beside_keys_that_are_not_there(device, dtype, d, reqs, gone, prefix
         assert touched.any()
         assert torch.equal(got.isnan(), touched) and torch.equal(got[~touched], clean[~touched])
         cache.v_codes.copy_(held)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("new", [1, 300])
+def test_rows_of_zeros_of_powers_past_the_types(device, dtype, d, new):
+    """Codes of zero are zeros under any power byte: they take no other key's weight away."""
+    g = torch.Generator(device=device).manual_seed(d + new)
+    for byte in (228 if dtype == torch.bfloat16 else 136, 200 if dtype == torch.float16 else 240, 254, 255):
+        q, cache, table, starts, seqs = make(g, [(new, 900), (new, 100)], 4, 2, d, 32, dtype)
+        cache.exponents[..., 1] = torch.randint(-12, 6, cache.exponents.shape[:3], generator=g, device=device) + 127
+        zero = torch.rand(cache.exponents.shape[:3], generator=g, device=device) < 0.4
+        cache.exponents[..., 1] = torch.where(zero, byte, cache.exponents[..., 1].int()).to(torch.uint8)
+        cache.v_codes[zero.transpose(1, 2)] = 0
+        cache.k_codes[3], cache.exponents[3, :, :, 0] = 0, byte          # (keys of zero too)
+        got = chunk.chunk_attention(q, cache, chunk.ChunkStep(starts, seqs, table, 4, cache), d ** -0.5)
+        check(got, q, cache, table, starts, seqs, 0, d ** -0.5)
