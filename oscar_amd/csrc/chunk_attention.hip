@@ -44,7 +44,7 @@ int launch(const ChunkArgs& a, const oscar_chunk_step& step, hipStream_t stream)
   void (*const kernels[3])(ChunkArgs) = {&narrow_kernel<T, D>, &wide_kernel<T, D>, &mixed_kernel<T, D>};
   const int which = step.wide == 0 ? 0 : step.narrow == 0 ? 1 : 2;
   kernels[which]<<<step.narrow + step.wide, kThreads, 0, stream>>>(a);
-  return launch_joins<T, D>(a, step, stream);
+  return launch_joins<T, D, false>(a, step, stream);
 }
 
 template <typename T>

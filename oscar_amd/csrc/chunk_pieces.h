@@ -422,9 +422,21 @@ __device__ __forceinline__ uint8_t* out_row(const ChunkArgs& a, int token0, int 
   return a.out + (int64_t)(token0 + tok) * a.out_token + (int64_t)head * a.out_head;
 }
 
+// `to` and a sum of weights held to a maximum m, `down` = m - (the new maximum).  kPowers: m
+// goes with values' powers of two (the 8-bit cache), of which the sum has the inverse, up to
+// 2^80 for a key: where the factor alone is below fp32's smallest, their product need not be,
+// so it is applied by halves.
+template <bool kPowers>
+__device__ __forceinline__ float add_lowered(float to, float sum, float down) {
+  const float at_once = to + __builtin_amdgcn_exp2f(down) * sum;
+  if constexpr (!kPowers) return at_once;
+  const float half = __builtin_amdgcn_exp2f(0.5f * down);
+  return down > -126.f ? at_once : to + half * sum * half;
+}
+
 // The waves' sums of a narrow piece through LDS, D / kRounds features at a time (16-byte
 // pieces, the row xor-ed in): the rows' outputs, or a partial.
-template <typename T, int D, int kRounds>
+template <typename T, int D, int kRounds, bool kPowers>
 __device__ __forceinline__ void combine_waves(const ChunkArgs& a, const Piece& p, RowState<T, D>& s, uint8_t* smem,
                                               int tid, int lane, int wave) {
   constexpr int kPart = D / kRounds, kTurn = kPart >= 64 ? 15 : kPart / 4 - 1;
@@ -471,7 +483,7 @@ __device__ __forceinline__ void combine_waves(const ChunkArgs& a, const Piece& p
 #pragma unroll
         for (int w = 0; w < kWaves; ++w) {
           const float f = __builtin_amdgcn_exp2f(wm[w] - m[n]);
-          l[n] += f * wl[w];
+          l[n] = add_lowered<kPowers>(l[n], wl[w], wm[w] - m[n]);
           o[n] += f * x[w];
         }
       }
@@ -614,7 +626,7 @@ __device__ __forceinline__ void narrow_piece(const ChunkArgs& a, const Piece p, 
   if (__builtin_expect(special, 0))
     for (int t = first; t < last; ++t) add_special<T, D, kKeys>(a, p, t * kKeys, whole(t * kKeys), lane, s);
 
-  combine_waves<T, D, 32 / kKeys>(a, p, s, smem, tid, lane, wave);
+  combine_waves<T, D, 32 / kKeys, false>(a, p, s, smem, tid, lane, wave);
 }
 
 // ---------------------------------------------------------------- 128 rows
@@ -918,7 +930,7 @@ __device__ __forceinline__ RowPart part_of(const ChunkArgs& a, const Join& j, co
   return RowPart{a.partials + (int64_t)(j.slot0 + i * j.step) * (kTileRows * (D + 2)), row};
 }
 
-template <typename T, int D, int kParts, bool kShared>
+template <typename T, int D, int kParts, bool kShared, bool kPowers>
 __device__ __forceinline__ void join_few(const ChunkArgs& a, const Join j, const SharedPart p, int block) {
   const int i = block * 256 + (int)threadIdx.x, row = i / (D / 4), feature = 4 * (i % (D / 4));
   if (row >= j.rows) return;
@@ -940,14 +952,14 @@ __device__ __forceinline__ void join_few(const ChunkArgs& a, const Join j, const
   for (int s = 0; s < kParts; ++s)
     if (s < count) {
       const float w = __builtin_amdgcn_exp2f(m[s] - top);
-      sum += w * l[s];
+      sum = add_lowered<kPowers>(sum, l[s], m[s] - top);
       o += w * x[s];
     }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   store4<T>(out_row(a, j.token0, j.kv_head, j.row0 + row) + 2 * feature, o * inv);
 }
 
-template <typename T, int D, bool kShared>
+template <typename T, int D, bool kShared, bool kPowers>
 __device__ __forceinline__ void join_many(const ChunkArgs& a, const Join j, const SharedPart p, int row, int part64) {
   const int tid = (int)threadIdx.x, feature = 64 * part64 + 4 * (tid & 15), part = tid >> 4;
   __shared__ float red[16][64 + 4];
@@ -973,7 +985,7 @@ __device__ __forceinline__ void join_many(const ChunkArgs& a, const Join j, cons
     for (int s = 0; s < kManyAtOnce; ++s)
       if (part + 16 * s < count) {
         const float w = __builtin_amdgcn_exp2f(pm[s] - m);
-        l += w * pl[s];
+        l = add_lowered<kPowers>(l, pl[s], pm[s] - m);
         o += w * x[s];
       }
   } else {
@@ -983,8 +995,8 @@ __device__ __forceinline__ void join_many(const ChunkArgs& a, const Join j, cons
     }
     for (int i = part; i < count; i += 16) {
       const RowPart at = part_of<D, kShared>(a, j, p, row, i);
-      const float w = __builtin_amdgcn_exp2f(at.slot[kTileRows * D + at.row] - m);
-      l += w * at.slot[kTileRows * D + kTileRows + at.row];
+      const float down = at.slot[kTileRows * D + at.row] - m, w = __builtin_amdgcn_exp2f(down);
+      l = add_lowered<kPowers>(l, at.slot[kTileRows * D + kTileRows + at.row], down);
       o += w * *reinterpret_cast<const floatx4*>(at.slot + at.row * D + feature);
     }
   }
@@ -1003,7 +1015,7 @@ __device__ __forceinline__ void join_many(const ChunkArgs& a, const Join j, cons
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
     const float w = __builtin_amdgcn_exp2f(red_m[i] - top);
-    lsum += w * red_l[i];
+    lsum = add_lowered<kPowers>(lsum, red_l[i], red_m[i] - top);
     sum += w * *reinterpret_cast<const floatx4*>(&red[i][4 * tid]);
   }
   const float inv = lsum == 0.f ? 0.f : 1.f / lsum;
@@ -1013,7 +1025,7 @@ __device__ __forceinline__ void join_many(const ChunkArgs& a, const Join j, cons
 // Groups of few partials first, D / 32 workgroups each; then join_rows x D / 64 a group
 // (as many rows as some group of many partials has: 8 users' token of 4 heads on one over
 // a prefix of 4096 keys 14.8 us in all, with 32 x D / 64 a group 17.4).
-template <typename T, int D, bool kShared>
+template <typename T, int D, bool kShared, bool kPowers>
 __global__ __launch_bounds__(256) void join_kernel(ChunkArgs a) {
   constexpr int kFewBlocks = D / 32;
   const int block = (int)blockIdx.x, few = a.few_joins * kFewBlocks, many_blocks = a.join_rows * (D / 64);
@@ -1024,12 +1036,12 @@ __global__ __launch_bounds__(256) void join_kernel(ChunkArgs a) {
     if (j.shared > 0) p = a.parts[j.shared - 1];
   if (block < few) {
     const int count = j.count + p.count;
-    if (count <= 2) join_few<T, D, 2, kShared>(a, j, p, block % kFewBlocks);
-    else if (count <= 4) join_few<T, D, 4, kShared>(a, j, p, block % kFewBlocks);
-    else join_few<T, D, kFewParts, kShared>(a, j, p, block % kFewBlocks);
+    if (count <= 2) join_few<T, D, 2, kShared, kPowers>(a, j, p, block % kFewBlocks);
+    else if (count <= 4) join_few<T, D, 4, kShared, kPowers>(a, j, p, block % kFewBlocks);
+    else join_few<T, D, kFewParts, kShared, kPowers>(a, j, p, block % kFewBlocks);
     return;
   }
-  if (at / (D / 64) < j.rows) join_many<T, D, kShared>(a, j, p, at / (D / 64), at % (D / 64));
+  if (at / (D / 64) < j.rows) join_many<T, D, kShared, kPowers>(a, j, p, at / (D / 64), at % (D / 64));
 }
 
 }  // namespace

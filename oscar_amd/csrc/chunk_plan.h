@@ -423,12 +423,12 @@ int step_args(const oscar_chunk_step* step, const void* items, const int32_t* bl
   return kOk;
 }
 
-template <typename T, int D>
+template <typename T, int D, bool kPowers>
 int launch_joins(const ChunkArgs& a, const oscar_chunk_step& step, hipStream_t stream) {
   const int64_t blocks = (int64_t)step.few_joins * (D / 32) + (int64_t)(step.joins - step.few_joins) * (step.join_rows * (D / 64));
   if (blocks > INT32_MAX) return kErrInvalidArgument;
-  if (blocks > 0 && step.parts == 0) join_kernel<T, D, false><<<(uint32_t)blocks, 256, 0, stream>>>(a);
-  else if (blocks > 0) join_kernel<T, D, true><<<(uint32_t)blocks, 256, 0, stream>>>(a);
+  if (blocks > 0 && step.parts == 0) join_kernel<T, D, false, kPowers><<<(uint32_t)blocks, 256, 0, stream>>>(a);
+  else if (blocks > 0) join_kernel<T, D, true, kPowers><<<(uint32_t)blocks, 256, 0, stream>>>(a);
   return hipGetLastError() == hipSuccess ? kOk : kErrLaunch;
 }
 

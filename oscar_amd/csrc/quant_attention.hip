@@ -382,7 +382,7 @@ __device__ __forceinline__ void code_piece(const QuantChunkArgs& all, const Piec
       const float m = over ? top : s.m, f = __builtin_amdgcn_exp2f(s.m - m);
 #pragma unroll
       for (int b = 0; b < kBlocks; ++b) s.acc[b] *= f;
-      s.l *= f;
+      s.l = add_lowered<true>(0.f, s.l, s.m - m);
       s.m = m;
       l = 0.f;
 #pragma unroll
@@ -418,7 +418,7 @@ __device__ __forceinline__ void code_piece(const QuantChunkArgs& all, const Piec
       const int key0 = p.key0 + t * kKeys;
       add_nan<T, D, kKeys>(a, c, p, key0, whole(key0), lane, s);
     }
-  combine_waves<T, D, D == 256 ? 2 : 1>(a, p, s, smem, tid, lane, wave);
+  combine_waves<T, D, D == 256 ? 2 : 1, true>(a, p, s, smem, tid, lane, wave);
 }
 
 // ---------------------------------------------------------------- kernels
@@ -583,7 +583,9 @@ int launch(const QuantChunkArgs& a, const PagesArgs& pages, const oscar_quant_st
   if (step.chunk.wide == 0 && step.once != 0) code_kernel<T, D, kOnce><<<pieces, kThreads, 0, stream>>>(a);
   else if (step.chunk.wide == 0) code_kernel<T, D, kKept><<<pieces, kThreads, 0, stream>>>(a);
   else quant_kernel<T, D><<<pieces, kThreads, 0, stream>>>(a);
-  return launch_joins<T, D>(a.wide, step.chunk, stream);
+  // (wide pieces' maxima are of scores alone: their joins are the plain cache's)
+  return step.chunk.narrow > 0 ? launch_joins<T, D, true>(a.wide, step.chunk, stream)
+                               : launch_joins<T, D, false>(a.wide, step.chunk, stream);
 }
 template <typename T>
 int launch_sized(int d, const QuantChunkArgs& a, const PagesArgs& pages, const oscar_quant_step& step,

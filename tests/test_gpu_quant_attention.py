@@ -479,3 +479,41 @@ def test_rows_of_zeros_of_powers_past_the_types(device, dtype, d, new):
         cache.k_codes[3], cache.exponents[3, :, :, 0] = 0, byte          # (keys of zero too)
         got = chunk.chunk_attention(q, cache, chunk.ChunkStep(starts, seqs, table, 4, cache), d ** -0.5)
         check(got, q, cache, table, starts, seqs, 0, d ** -0.5)
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("n", [40, 260, 1000, 30000])
+@pytest.mark.parametrize("order", ["rising", "falling", "stripes"])
+def test_sums_of_powers_far_apart(device, d, n, order):
+    """Keys of equal scores share the sum of weights alike, whatever the powers of their values:
+    rows of zeros of the least power, as a write leaves them, and rows of 2^60, in one tile of
+    codes or several, one wave or four, one piece or many."""
+    g = torch.Generator(device=device).manual_seed(n)
+    q, cache, table, starts, seqs = make(g, [(1, n - 1)], 4, 2, d, 16, torch.bfloat16)
+    q.zero_()
+    key = torch.arange(n, device=device)
+    large = {"rising": key >= n // 2, "falling": key < n // 2, "stripes": key // 32 % 2 == 1}[order]
+    page, place = table[0][key // 16].long(), key % 16
+    cache.exponents[page, :, place, 1] = torch.where(large, 127 + 60, 127 - 80)[:, None].to(torch.uint8)
+    cache.v_codes[page[~large], place[~large]] = 0
+    got = chunk.chunk_attention(q, cache, chunk.ChunkStep(starts, seqs, table, 4, cache), 0.1)
+    check(got, q, cache, table, starts, seqs, 0, 0.1)
+
+
+def test_sums_of_powers_far_apart_of_a_prefix(device):
+    """A prefix of many rows is computed from converted keys, whose maxima go without powers."""
+    g = torch.Generator(device=device).manual_seed(3)
+    reqs, keys = [(4, 1700 + i) for i in range(40)], 1696
+    for zeros_first in (True, False):
+        q, cache, table, starts, seqs = make(g, reqs, 8, 1, 128, 16, torch.bfloat16)
+        q.zero_()
+        table[:, :keys // 16] = table[0, :keys // 16]
+        own, shared = table[:, keys // 16:].reshape(-1), table[0, :keys // 16]
+        own = own[own >= 0].long()
+        zero, large = (shared.long(), own) if zeros_first else (own, shared.long())
+        cache.exponents[zero, ..., 1], cache.exponents[large, ..., 1] = 127 - 80, 127 + 60
+        cache.v_codes[zero] = 0
+        step = chunk.ChunkStep(starts, seqs, table, 8, cache, prefixes=[(0, 40, keys)])
+        assert step.args.chunk.wide > 0 and step.args.chunk.narrow > 0
+        got = chunk.chunk_attention(q, cache, step, 0.1)
+        check(got, q, cache, table, starts, seqs, 0, 0.1)
