@@ -422,17 +422,21 @@ __device__ __forceinline__ uint8_t* out_row(const ChunkArgs& a, int token0, int 
   return a.out + (int64_t)(token0 + tok) * a.out_token + (int64_t)head * a.out_head;
 }
 
-// `to` and a sum of weights held to a maximum m, `down` = m - (the new maximum).  kPowers: m
-// goes with values' powers of two (the 8-bit cache), of which the sum has the inverse, up to
-// 2^80 for a key: where the factor alone is below fp32's smallest, their product need not be,
-// so it is applied by halves.
+// What a partial's sums are multiplied by as its maximum is raised by `up` (0 or less: from
+// the new one to its own): `all`, its products, and sum_of(l) its weights.  kPowers: the
+// maximum goes with values' powers of two (the 8-bit cache), of which the weights' sum has
+// the inverse, up to 2^80 for a key: where the factor alone is below fp32's smallest,
+// their product need not be, so it is applied by halves.
 template <bool kPowers>
-__device__ __forceinline__ float add_lowered(float to, float sum, float down) {
-  const float at_once = to + __builtin_amdgcn_exp2f(down) * sum;
-  if constexpr (!kPowers) return at_once;
-  const float half = __builtin_amdgcn_exp2f(0.5f * down);
-  return down > -126.f ? at_once : to + half * sum * half;
-}
+struct Lowered {
+  float half, all;
+  __device__ __forceinline__ explicit Lowered(float up)
+      : half(kPowers ? __builtin_amdgcn_exp2f(0.5f * up) : 1.f), all(kPowers ? half * half : __builtin_amdgcn_exp2f(up)) {}
+  __device__ __forceinline__ float add(float to, float l) const {
+    if constexpr (kPowers) return to + half * (half * l);
+    return to + all * l;
+  }
+};
 
 // The waves' sums of a narrow piece through LDS, D / kRounds features at a time (16-byte
 // pieces, the row xor-ed in): the rows' outputs, or a partial.
@@ -482,9 +486,9 @@ __device__ __forceinline__ void combine_waves(const ChunkArgs& a, const Piece& p
         o[n] = floatx4{};
 #pragma unroll
         for (int w = 0; w < kWaves; ++w) {
-          const float f = __builtin_amdgcn_exp2f(wm[w] - m[n]);
-          l[n] = add_lowered<kPowers>(l[n], wl[w], wm[w] - m[n]);
-          o[n] += f * x[w];
+          const Lowered<kPowers> f(wm[w] - m[n]);
+          l[n] = f.add(l[n], wl[w]);
+          o[n] += f.all * x[w];
         }
       }
 #pragma unroll
@@ -951,9 +955,9 @@ __device__ __forceinline__ void join_few(const ChunkArgs& a, const Join j, const
 #pragma unroll
   for (int s = 0; s < kParts; ++s)
     if (s < count) {
-      const float w = __builtin_amdgcn_exp2f(m[s] - top);
-      sum = add_lowered<kPowers>(sum, l[s], m[s] - top);
-      o += w * x[s];
+      const Lowered<kPowers> w(m[s] - top);
+      sum = w.add(sum, l[s]);
+      o += w.all * x[s];
     }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   store4<T>(out_row(a, j.token0, j.kv_head, j.row0 + row) + 2 * feature, o * inv);
@@ -984,9 +988,9 @@ __device__ __forceinline__ void join_many(const ChunkArgs& a, const Join j, cons
 #pragma unroll
     for (int s = 0; s < kManyAtOnce; ++s)
       if (part + 16 * s < count) {
-        const float w = __builtin_amdgcn_exp2f(pm[s] - m);
-        l = add_lowered<kPowers>(l, pl[s], pm[s] - m);
-        o += w * x[s];
+        const Lowered<kPowers> w(pm[s] - m);
+        l = w.add(l, pl[s]);
+        o += w.all * x[s];
       }
   } else {
     for (int i = part; i < count; i += 16) {
@@ -995,9 +999,9 @@ __device__ __forceinline__ void join_many(const ChunkArgs& a, const Join j, cons
     }
     for (int i = part; i < count; i += 16) {
       const RowPart at = part_of<D, kShared>(a, j, p, row, i);
-      const float down = at.slot[kTileRows * D + at.row] - m, w = __builtin_amdgcn_exp2f(down);
-      l = add_lowered<kPowers>(l, at.slot[kTileRows * D + kTileRows + at.row], down);
-      o += w * *reinterpret_cast<const floatx4*>(at.slot + at.row * D + feature);
+      const Lowered<kPowers> w(at.slot[kTileRows * D + at.row] - m);
+      l = w.add(l, at.slot[kTileRows * D + kTileRows + at.row]);
+      o += w.all * *reinterpret_cast<const floatx4*>(at.slot + at.row * D + feature);
     }
   }
   *reinterpret_cast<floatx4*>(&red[part][4 * (tid & 15)]) = o;
@@ -1014,9 +1018,9 @@ __device__ __forceinline__ void join_many(const ChunkArgs& a, const Join j, cons
   float lsum = 0.f;
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
-    const float w = __builtin_amdgcn_exp2f(red_m[i] - top);
-    lsum = add_lowered<kPowers>(lsum, red_l[i], red_m[i] - top);
-    sum += w * *reinterpret_cast<const floatx4*>(&red[i][4 * tid]);
+    const Lowered<kPowers> w(red_m[i] - top);
+    lsum = w.add(lsum, red_l[i]);
+    sum += w.all * *reinterpret_cast<const floatx4*>(&red[i][4 * tid]);
   }
   const float inv = lsum == 0.f ? 0.f : 1.f / lsum;
   store4<T>(out_row(a, j.token0, j.kv_head, j.row0 + row) + 2 * feature, sum * inv);

@@ -379,10 +379,11 @@ __device__ __forceinline__ void code_piece(const QuantChunkArgs& all, const Piec
         }
       top = max_halves(top) - Num<T>::kLift;
       const bool over = max_halves(heaviest > Num<T>::kMostBits ? 1.f : 0.f) != 0.f && top > s.m;
-      const float m = over ? top : s.m, f = __builtin_amdgcn_exp2f(s.m - m);
+      const float m = over ? top : s.m;
+      const Lowered<true> f(s.m - m);
 #pragma unroll
-      for (int b = 0; b < kBlocks; ++b) s.acc[b] *= f;
-      s.l = add_lowered<true>(0.f, s.l, s.m - m);
+      for (int b = 0; b < kBlocks; ++b) s.acc[b] *= f.all;
+      s.l = f.add(0.f, s.l);
       s.m = m;
       l = 0.f;
 #pragma unroll
