@@ -1032,9 +1032,14 @@ __device__ __forceinline__ void join_many(const ChunkArgs& a, const Join j, cons
 template <typename T, int D, bool kShared, bool kPowers>
 __global__ __launch_bounds__(256) void join_kernel(ChunkArgs a) {
   constexpr int kFewBlocks = D / 32;
-  const int block = (int)blockIdx.x, few = a.few_joins * kFewBlocks, many_blocks = a.join_rows * (D / 64);
-  const int many = (block - few) / many_blocks, at = (block - few) % many_blocks;
-  const Join j = a.joins[block < few ? block / kFewBlocks : a.few_joins + many];
+  const int block = (int)blockIdx.x, few = a.few_joins * kFewBlocks;
+  int join = block / kFewBlocks, at = 0;
+  if (block >= few) {                       // (there are none where join_rows is 0)
+    const int many_blocks = a.join_rows * (D / 64);
+    join = a.few_joins + (block - few) / many_blocks;
+    at = (block - few) % many_blocks;
+  }
+  const Join j = a.joins[join];
   SharedPart p{};
   if constexpr (kShared)
     if (j.shared > 0) p = a.parts[j.shared - 1];
