@@ -17,6 +17,7 @@ import ctypes
 import struct
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -155,15 +156,23 @@ def rotate(query: torch.Tensor, key: torch.Tensor | None, positions: torch.Tenso
     strides below 4 GiB.  Returns (query_out, key_out): new tensors, or the ones
     given, each its own input as it stands or apart from all rows of the call.
     New tensors carry a gradient to rows that require one (theirs, turned the
-    other way); a call with a given output records no autograd graph.  A token
-    with a position outside the table is left out: its output rows keep what they
-    held, and its inputs' gradient is zero."""
+    other way); a call with a given output records no autograd graph.  Rows that carry
+    forward mode's tangents are refused.  A token with a position outside the table is
+    left out: its output rows keep what they held, and its inputs' gradient is zero."""
+    _refuse_tangents(query, key)
     if ((query.requires_grad or (key is not None and key.requires_grad)) and torch.is_grad_enabled()
             and query_out is None and key_out is None):
         if key is not None and key.shape[0] > query.shape[0]:
             key = key[:query.shape[0]]
         return _Turned.apply(query, key, positions, rotary, inverse, False)
     return _rotate(query, key, positions, rotary, query_out, key_out, inverse)
+
+
+def _refuse_tangents(*tensors) -> None:
+    """Raise for dual tensors of forward mode, whose tangents a kernel's output would not have."""
+    if getattr(forward_ad, "_current_level", -1) >= 0 and any(
+            x is not None and forward_ad.unpack_dual(x).tangent is not None for x in tensors):
+        raise ValueError("rows and weights carry tangents: there are no forward-mode gradients")
 
 
 class _Turned(torch.autograd.Function):
@@ -256,9 +265,10 @@ def norm_rotate(query: torch.Tensor, key: torch.Tensor | None, query_weight: tor
     for all query heads and one for all key heads; offset 1 is for models that keep
     them around zero.  Rows, positions and outputs are as ``rotate`` takes them.  New
     tensors carry a gradient to rows and weights that require one (a single time); a
-    call with a given output records no autograd graph.  A token with a position
-    outside the table is left out: its output rows keep what they held, and it adds
-    nothing to a gradient."""
+    call with a given output records no autograd graph.  Rows and weights that carry
+    forward mode's tangents are refused.  A token with a position outside the table is
+    left out: its output rows keep what they held, and it adds nothing to a gradient."""
+    _refuse_tangents(query, key, query_weight, key_weight)
     if query_weight is None or (key is not None and key_weight is None):
         raise ValueError("norm_rotate takes a weight for queries, and for keys where they are given")
     if key is None:
