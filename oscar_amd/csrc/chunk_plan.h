@@ -155,12 +155,14 @@ int32_t pieces_of(const RowTile& x, int64_t per) { return (int32_t)((x.tiles + p
 // 256, 190 us, 5.2 TB/s), but one request that is far longer than the others is then
 // read by one workgroup (300 users of 1000 keys and one of 131072 2.2 ms, where the
 // bytes take 0.09), and by a few where there are just fewer (250 and one: 0.39 ms).
-// `uneven`: row tiles that are as many, the longest of them more than twice a resident
-// piece's mean length and 32 key tiles above it, are cut to that many mean lengths.
+// `uneven`: where the longest piece is still more than twice a resident piece's mean length
+// and 32 key tiles above it, as with as many row tiles or nearly as many, all are cut to so
+// many mean lengths.
 // 8-bit caches, whole / cut to three a CU, us: 64 users over 100 to 16000 keys, D = 128,
 // 8 kv heads, 195 / 107, 128 users 291 / 203, 4 tokens of 128 users, D = 64, 4 heads,
 // 155 / 84; 256 over 100 to 8000, D = 256, 175 / 103; 300 over 1000 and one over 60000
-// 954 / 90; without the second condition 256 over 100 to 800 27 / 32.
+// 954 / 90, 508 over 1000 and one 257 / 76, 490 77 / 75; 62 and one of 8 heads, D = 128, 328 /
+// 57; 168 and one beside a prompt of 1200 482 / 56; without the second condition 256 over 100 to 800 27 / 32.
 constexpr int32_t kMuchLonger = 32;
 void plan_narrow(const std::vector<RowTile>& rows, const PlanRule& rule, double beside, Plan& plan,
                  std::vector<PrefixRows>& prefixes) {
@@ -178,8 +180,6 @@ void plan_narrow(const std::vector<RowTile>& rows, const PlanRule& rule, double 
       for (const RowTile& x : rows) c += pieces_of(x, t);
       return c;
     };
-    if (rule.uneven > 0 && (int64_t)rows.size() >= resident && most > 2 * per && most > per + kMuchLonger)
-      return std::max<int64_t>(kWaves, (total + rule.uneven - 1) / rule.uneven);
     if ((int64_t)rows.size() >= resident || most <= uncut) per = std::max<int64_t>(per, most);
     // (The count falls as pieces get longer.  Step by step the search took 5 ms for 250
     // short rows beside 2^20 keys, and 17 s beside 2^30.)
@@ -191,9 +191,16 @@ void plan_narrow(const std::vector<RowTile>& rows, const PlanRule& rule, double 
     return per;
   };
   const bool reading = total * rule.key_bytes > 2 * 240 * beside;
-  int64_t per = fit(beside == 0. ? rule.resident[0] : reading ? 2 * kCus : 2 * kCus / 3);
-  if (beside == 0. && ((int64_t)rows.size() >= rule.resident[0] || 100 * per * rule.resident[0] > 115 * total))
-    per = fit(rule.resident[1]);
+  int64_t resident = beside == 0. ? rule.resident[0] : reading ? 2 * kCus : 2 * kCus / 3;
+  int64_t per = fit(resident);
+  if (beside == 0. && ((int64_t)rows.size() >= rule.resident[0] || 100 * per * rule.resident[0] > 115 * total)) {
+    resident = rule.resident[1];
+    per = fit(resident);
+  }
+  const int64_t mean = std::max<int64_t>(kWaves, (total + resident - 1) / resident);
+  const int64_t longest = std::min<int64_t>(per, most);
+  if (rule.uneven > 0 && longest > 2 * mean && longest > mean + kMuchLonger)
+    per = std::max<int64_t>(kWaves, (total + rule.uneven - 1) / rule.uneven);
   for (const RowTile& x : rows) cut(x, pieces_of(x, per), plan, prefixes, plan.narrow);
 }
 

@@ -188,3 +188,20 @@ def test_a_much_longer_request_is_cut_where_the_others_fill_the_gpu(d, hk, group
     assert max(p[7] - p[6] for p in pieces) <= 32 * mean and args.chunk.narrow <= 301 * hk + 3 * 256 and args.chunk.wide == 0
     args, pieces, _ = plan(list(range(302)), [100 + 2 * i for i in range(301)], hk * group, quant_cache(d=d, hk=hk))
     assert args.chunk.narrow == 301 * hk and args.chunk.joins == 0
+
+
+@pytest.mark.parametrize("d, hk, group", [(64, 1, 6), (128, 1, 6), (256, 1, 6), (256, 2, 4)])
+@pytest.mark.parametrize("prompt", [0, 1200])
+@pytest.mark.parametrize("others", [100, 160, 165, 168, 169, 170, 171, 200, 249, 254, 255, 256, 400, 490, 500, 510, 511, 512,
+                                    600])
+def test_a_much_longer_request_is_cut_however_many_others_there_are(d, hk, group, prompt, others):
+    """Also where they nearly fill the GPU: pieces are at most twice the mean length of those
+    that reside at once, or 32 key tiles above it."""
+    keys = [1000] * (others // hk) + [60000] + ([prompt] if prompt else [])
+    starts = list(range(len(keys) + 1))
+    starts[-1] += max(prompt - 1, 0)
+    args, pieces, _ = plan(starts, keys, hk * group, quant_cache(d=d, hk=hk))
+    assert (args.chunk.wide > 0) == (prompt > 0)
+    tiles = hk * sum(-(-n // 32) for n in keys[:others // hk + 1])
+    mean = max(4, -(-tiles // (170 if prompt else 512)))                 # (the fewest that may reside)
+    assert max(p[7] - p[6] for p in pieces[:args.chunk.narrow]) <= 32 * max(2 * mean, mean + 32)
