@@ -721,8 +721,9 @@ typedef struct oscar_chunk_step {
 } oscar_chunk_step;
 
 /* Keys [0, keys) that requests first .. first + requests - 1 of a step begin with, on
- * pages that hold the same: they are computed once for the rows of all, from the block
- * table row of the first of them that has tokens. */
+ * pages that hold the same: they are read from the block table row of the first of them
+ * that has tokens and computed once for the rows of all, but for prompts that fill the GPU
+ * by themselves (they would only gain partials). */
 typedef struct oscar_prefix {
   int32_t first;
   int32_t requests;

@@ -129,7 +129,9 @@ struct Piece {
   int32_t row0, rows;      // of the request's (token, head) rows
   int32_t key0, key1;
   int32_t slot;            // first partial of 32 rows, -1: rows are finished here
-  int32_t pad[3];
+  int32_t head_keys;       // keys below it (a multiple of 32) are on table row head_row
+  int32_t head_row;
+  int32_t pad;
 };
 // 32 rows whose partials are slots slot0, slot0 + step, ... and, if `shared` > 0, those
 // of a prefix that their request shares: parts[shared - 1].
@@ -226,12 +228,16 @@ __device__ __forceinline__ int k_swizzle(int key) { return D >= 128 ? key & 15 :
 template <int D>
 __device__ __forceinline__ int v_swizzle(int key) { return D >= 128 ? 4 * (key & 3) : 4 * ((key >> 1) & 1); }
 
+__device__ __forceinline__ int64_t table_row_of(const Piece& p, int key) {
+  return key < p.head_keys ? p.head_row : p.table_row;
+}
+
 // Pages of 64 groups of 16 keys from group `base` on, one a lane; -1: unmapped.
 __device__ __forceinline__ int load_pages(const ChunkArgs& a, const Piece& p, int base, int lane) {
   const int key = 16 * (base + lane);
   int page = -1;
   if (key >= 0 && key < p.key1) {
-    page = a.table[(int64_t)p.table_row * a.table_stride + fast_div((uint32_t)key, a.block_div)];
+    page = a.table[table_row_of(p, key) * a.table_stride + fast_div((uint32_t)key, a.block_div)];
     page = page >= 0 && page < a.num_pages ? page : -1;
   }
   return page;
@@ -369,7 +375,7 @@ __device__ __forceinline__ void add_special(const ChunkArgs& a, const Piece& p, 
                                             RowState<T, D>& s) {
   typedef T T4 __attribute__((ext_vector_type(4)));
   auto page_of = [&](int key) {
-    const int page = a.table[(int64_t)p.table_row * a.table_stride + fast_div((uint32_t)key, a.block_div)];
+    const int page = a.table[table_row_of(p, key) * a.table_stride + fast_div((uint32_t)key, a.block_div)];
     return page >= 0 && page < a.num_pages ? page : -1;
   };
   const int end = min(key0 + kKeys, p.key1);

@@ -52,11 +52,16 @@ struct RowTile {
   int32_t with_prefix = -1, prefix_row = 0;      // PrefixRows that its rows go on from, and where they begin there
 };
 
-// The row tiles of a request, `rows` rows each, with the keys that they see from `from`
-// (a multiple of 32) on.  with_prefix: PrefixRows of its first kv head, or -1.
+// What a request has of a prefix: its rows go on from row `row` of PrefixRows `with` (of its
+// first kv head), or, without (-1), it computes the keys itself, on table row `head`.
+struct OfPrefix {
+  int32_t keys = 0, with = -1, row = 0, head = 0;
+};
+
+// The row tiles of a request, `rows` rows each, with the keys that they see, but for those of a
+// prefix that it goes on from.
 void row_tiles(int32_t token0, int32_t n, int32_t seq, int32_t table_row, int32_t group, int32_t kv_heads,
-               int32_t window, int32_t rows, std::vector<RowTile>& out, int32_t from = 0, int32_t with_prefix = -1,
-               int32_t prefix_row = 0) {
+               int32_t window, int32_t rows, const OfPrefix& prefix, std::vector<RowTile>& out) {
   const int32_t all = n * group;
   for (int32_t r = 0; r < all; r += rows) {
     Piece p{};
@@ -66,15 +71,19 @@ void row_tiles(int32_t token0, int32_t n, int32_t seq, int32_t table_row, int32_
     p.row0 = r;
     p.rows = std::min(rows, all - r);
     p.slot = -1;
-    const int32_t lo = window > 0 ? std::max(0, p.pos0 + r / group - window + 1) : from;
+    if (prefix.with < 0 && prefix.head != table_row) {
+      p.head_keys = prefix.keys;
+      p.head_row = prefix.head;
+    }
+    const int32_t lo = window > 0 ? std::max(0, p.pos0 + r / group - window + 1) : prefix.with >= 0 ? prefix.keys : 0;
     p.key0 = lo / kTileKeys * kTileKeys;
     p.key1 = p.pos0 + (r + p.rows - 1) / group + 1;
     for (int32_t h = 0; h < kv_heads; ++h) {
       p.kv_head = h;
       RowTile x{p, (p.key1 - p.key0 + kTileKeys - 1) / kTileKeys};
-      if (with_prefix >= 0) {
-        x.with_prefix = with_prefix + h;
-        x.prefix_row = prefix_row + r;
+      if (prefix.with >= 0) {
+        x.with_prefix = prefix.with + h;
+        x.prefix_row = prefix.row + r;
       }
       out.push_back(x);
     }
@@ -88,7 +97,7 @@ void prefix_tiles(int32_t token0, int32_t tokens, int32_t keys, int32_t table_ro
   const int32_t all = tokens * group;
   for (int32_t r = 0; r < all; r += rows)
     for (int32_t h = 0; h < kv_heads; ++h) {
-      RowTile x{Piece{token0, keys, table_row, h, r, std::min(rows, all - r), 0, keys, -1, {}}, keys / kTileKeys};
+      RowTile x{Piece{token0, keys, table_row, h, r, std::min(rows, all - r), 0, keys, -1, 0, 0, 0}, keys / kTileKeys};
       x.of_prefix = of_prefix + h;
       out.push_back(x);
     }
@@ -271,37 +280,66 @@ double plan_wide(const std::vector<RowTile>& rows, int32_t head_size, Plan& plan
   return best;
 }
 
+// A prefix' requests that fill wide pieces compute its keys themselves, from the first one's
+// table row, where the step has rows for more of those than there are CUs: they are not cut
+// then and bound by the matrix unit, which has the same products to do either way, and
+// sharing would only add partials, to write, read and hold.  Shared / each for itself, us:
+// 8 prompts of 4096 tokens over 1024 keys, 32 heads of 128 on 8, 1933 and 1.09 GB of
+// partials / 1577 and none; 16 of 2048 over 64 1032 / 660; 8 of 300 over 960 79 / 64; 8 of 1200
+// over 4096, 6 heads of 256 on one, 273 / 248; of the 8-bit cache (the keys converted once
+// for all) 32 of 64 over 4096 167 / 145.  With fewer rows they are cut in any case: 8 of 128
+// over 8192 150 / 155, 4 of 512 over 24576, D = 256, 284 / 308, 8 of 300 over 1024 50 / 44; rows
+// that fill no wide tile fill them together: 128 of 10 over 1024 54 / 76, over 64 37 / 17.
+// The requests between them are computed together, as far as they follow each other.
 void make_plan(const int32_t* qsl, const int32_t* seqs, int32_t num_requests, int32_t group, int32_t kv_heads,
                const PlanRule& rule, int32_t window, const std::vector<Prefix>& shared, Plan& plan) {
   std::vector<RowTile> narrow, wide;
   std::vector<PrefixRows> prefixes;
+  auto rows_of = [&](int32_t i) { return (int64_t)(qsl[i + 1] - qsl[i]) * group; };
+  int64_t wide_rows = 0;
+  if (!shared.empty())
+    for (int32_t i = 0; i < num_requests; ++i)
+      if (rows_of(i) > rule.narrow_rows) wide_rows += rows_of(i) * kv_heads;
+  auto alone = [&](int32_t i) {
+    return wide_rows > (int64_t)kCus * kWideRows && rows_of(i) > rule.narrow_rows && rows_of(i) >= kWideRows;
+  };
   auto prefix = shared.begin();
-  int32_t keys = 0, until = 0, first_token = 0;        // of the prefix that request i begins with
+  OfPrefix of;                              // the prefix that request i begins with,
+  int32_t until = 0, together = 0, first_token = 0;    // and its requests up to `together` that share it
   for (int32_t i = 0; i < num_requests; ++i) {
     const int32_t n = qsl[i + 1] - qsl[i];
-    if (i >= until) keys = 0;
+    if (i >= until) of = OfPrefix{};
     if (prefix != shared.end() && i == prefix->first) {
-      keys = prefix->keys;
+      of.keys = prefix->keys;
       until = i + prefix->count;
-      first_token = qsl[i];
-      const int32_t tokens = qsl[until] - qsl[i], at = (int32_t)prefixes.size();
-      int32_t table_row = i;                           // a request's that has tokens
-      while (qsl[table_row + 1] == qsl[table_row]) ++table_row;
-      PrefixRows rows;
-      rows.groups = (tokens * group + kTileRows - 1) / kTileRows;
-      prefixes.insert(prefixes.end(), kv_heads, rows);
-      if (tokens * (int64_t)group <= rule.narrow_rows)
-        prefix_tiles(qsl[i], tokens, keys, table_row, group, kv_heads, kTileRows, at, narrow);
-      else
-        prefix_tiles(qsl[i], tokens, keys, table_row, group, kv_heads, kWideRows, at, wide);
+      together = i;
+      of.head = i;                          // a request's that has tokens
+      while (qsl[of.head + 1] == qsl[of.head]) ++of.head;
       ++prefix;
     }
-    const int32_t with = keys > 0 ? (int32_t)prefixes.size() - kv_heads : -1;
-    const int32_t row = keys > 0 ? (qsl[i] - first_token) * group : 0;
-    if (n * (int64_t)group <= rule.narrow_rows)
-      row_tiles(qsl[i], n, seqs[i], i, group, kv_heads, window, kTileRows, narrow, keys, with, row);
+    if (of.keys > 0 && i >= together) {
+      int32_t members = 0;
+      for (; together < until && !alone(together); ++together) members += qsl[together + 1] > qsl[together];
+      of.with = -1;
+      if (members > 1) {
+        of.with = (int32_t)prefixes.size();
+        first_token = qsl[i];
+        const int32_t tokens = qsl[together] - qsl[i];
+        PrefixRows rows;
+        rows.groups = (tokens * group + kTileRows - 1) / kTileRows;
+        prefixes.insert(prefixes.end(), kv_heads, rows);
+        if (tokens * (int64_t)group <= rule.narrow_rows)
+          prefix_tiles(qsl[i], tokens, of.keys, of.head, group, kv_heads, kTileRows, of.with, narrow);
+        else
+          prefix_tiles(qsl[i], tokens, of.keys, of.head, group, kv_heads, kWideRows, of.with, wide);
+      }
+      together = std::max(together, i + 1);
+    }
+    of.row = of.with >= 0 ? (qsl[i] - first_token) * group : 0;
+    if (rows_of(i) <= rule.narrow_rows)
+      row_tiles(qsl[i], n, seqs[i], i, group, kv_heads, window, kTileRows, of, narrow);
     else
-      row_tiles(qsl[i], n, seqs[i], i, group, kv_heads, window, kWideRows, wide, keys, with, row);
+      row_tiles(qsl[i], n, seqs[i], i, group, kv_heads, window, kWideRows, of, wide);
   }
   const double beside = wide.empty() ? 0. : plan_wide(wide, rule.head_size, plan, prefixes);
   if (!narrow.empty()) plan_narrow(narrow, rule, beside, plan, prefixes);

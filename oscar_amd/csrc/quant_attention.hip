@@ -160,7 +160,7 @@ template <typename T, int D, int kKeys>
 __device__ __forceinline__ void add_nan(const ChunkArgs& a, const QuantArgs& c, const Piece& p, int key0, bool whole,
                                         int lane, RowState<T, D>& s) {
   auto page_of = [&](int key) {
-    const int page = c.table[(int64_t)p.table_row * c.table_stride + fast_div((uint32_t)key, c.block_div)];
+    const int page = c.table[table_row_of(p, key) * c.table_stride + fast_div((uint32_t)key, c.block_div)];
     return page >= 0 && page < c.num_pages ? page : -1;
   };
   bool there = whole;
@@ -218,7 +218,7 @@ __device__ __forceinline__ void code_piece(const QuantChunkArgs& all, const Piec
     const int key = 16 * (group0 + base + lane);
     int page = -1;
     if (key < p.key1) {
-      page = c.table[(int64_t)p.table_row * c.table_stride + fast_div((uint32_t)key, c.block_div)];
+      page = c.table[table_row_of(p, key) * c.table_stride + fast_div((uint32_t)key, c.block_div)];
       page = page >= 0 && page < c.num_pages ? page : -1;
     }
     return page;
@@ -508,25 +508,38 @@ inline PlanRule quant_rule(int32_t head_size) {
   return PlanRule{head_size, rows, {kCus, 2 * kCus}, 1., 3 * kCus};
 }
 
-// The wide pieces' keys, request by request, and the pieces' table rows in the pages'.
+// The wide pieces' keys, table row by table row, and the pieces' table rows in the pages'.
 void make_sources(Plan& plan, std::vector<Source>& sources, int64_t& pages) {
-  std::vector<std::pair<int32_t, size_t>> order;       // table row, piece
-  for (size_t i = 0; i < plan.wide.size(); ++i) order.emplace_back(plan.wide[i].table_row, i);
-  std::sort(order.begin(), order.end());
+  struct Range {
+    int32_t row, from, to;                  // groups of 16 keys
+  };
+  std::vector<Range> ranges;
+  ranges.reserve(plan.wide.size());
+  for (const Piece& p : plan.wide) {
+    if (p.key0 < p.head_keys)
+      ranges.push_back(Range{p.head_row, p.key0 / 16, (std::min(p.key1, p.head_keys) + 15) / 16});
+    if (p.key1 > p.head_keys) ranges.push_back(Range{p.table_row, std::max(p.key0, p.head_keys) / 16, (p.key1 + 15) / 16});
+  }
+  std::sort(ranges.begin(), ranges.end(), [](const Range& x, const Range& y) { return x.row < y.row; });
   pages = 0;
-  for (size_t i = 0; i < order.size();) {
-    const int32_t row = order[i].first;
-    int32_t from = kMostKeys, to = 0;
-    size_t end = i;
-    for (; end < order.size() && order[end].first == row; ++end) {
-      const Piece& p = plan.wide[order[end].second];
-      from = std::min(from, p.key0 / 16);
-      to = std::max(to, (p.key1 + 15) / 16);
+  for (size_t i = 0; i < ranges.size();) {
+    Range all = ranges[i];
+    for (; i < ranges.size() && ranges[i].row == all.row; ++i) {
+      all.from = std::min(all.from, ranges[i].from);
+      all.to = std::max(all.to, ranges[i].to);
     }
-    if (pages + to - from > INT32_MAX) throw 0;
-    for (; i < end; ++i) plan.wide[order[i].second].table_row = (int32_t)pages - from;
-    sources.push_back(Source{row, from, to - from, (int32_t)pages});
-    pages += to - from;
+    if (pages + all.to - all.from > INT32_MAX) throw 0;
+    sources.push_back(Source{all.row, all.from, all.to - all.from, (int32_t)pages});
+    pages += all.to - all.from;
+  }
+  auto base = [&](int32_t row) {            // of a row that none of the piece's keys are on: any
+    const auto at = std::lower_bound(sources.begin(), sources.end(), row,
+                                     [](const Source& x, int32_t y) { return x.table_row < y; });
+    return at == sources.end() ? 0 : at->page0 - at->group0;
+  };
+  for (Piece& p : plan.wide) {
+    p.table_row = base(p.table_row);
+    p.head_row = p.head_keys > 0 ? base(p.head_row) : 0;
   }
 }
 

@@ -111,3 +111,97 @@ def test_graph_and_streams(device):
         torch.cuda.synchronize()
         assert torch.equal(held, want) and torch.equal(other, want)
         check(held, q, caches, table, starts, seqs, 0, 0.1, page)
+
+
+FULL = [
+    ([(0, 900), (4, 1900), (3, 1930), (900, 1900), (2, 1905), (1400, 2000), (1, 1900), (5, 2011)], [(0, 8, 1900)]),
+    ([(1200, 100), (1, 100), (2, 100), (1000, 130), (1, 96)], [(0, 4, 100)]),
+    ([(1, 333), (1300, 333), (1100, 400)], [(0, 3, 333)]),
+]
+
+
+@pytest.mark.parametrize("dtype, bits", [(torch.bfloat16, 16), (torch.float16, 16), (torch.bfloat16, 8), (torch.float16, 8)],
+                         ids=str)
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("case", range(len(FULL)))
+def test_prompts_that_fill_the_gpu(device, dtype, bits, d, case):
+    """They compute the prefix themselves, from the first one's pages too, the last of which may
+    hold other keys in theirs; their own table rows need not hold it."""
+    from tests import test_gpu_quant_attention as quant
+
+    reqs, prefixes = FULL[case]
+    hq, hk, page = 16, 4, 48
+    g = torch.Generator(device=device).manual_seed(10 * case + d)
+    if bits == 8:
+        q, cache, table, starts, seqs = quant.make(g, reqs, hq, hk, d, page, dtype)
+        caches = [cache.k_codes, cache.v_codes, cache.exponents.transpose(1, 2)]
+    else:
+        q, caches, table, starts, seqs = make(g, reqs, hq, hk, d, page, dtype, "joint", spread=2.0)
+        cache = append.PagedCache(*caches)
+    assert sum(n * 4 for n, _ in reqs if n >= 32) * hk > 256 * 128
+    step = chunk.ChunkStep(starts, seqs, table, hq, cache, prefixes=prefixes)
+    assert sum(p[-1] for p in prefixes) >= 100
+    sizes = step.args.chunk if bits == 8 else step.args
+    sharing = [n for n, _ in reqs if 0 < n < 32]
+    assert sizes.wide > 0 and sizes.parts <= len(sharing) * hk
+    first, count, keys = prefixes[0]
+    at = next(i for i in range(first, first + count) if reqs[i][0])
+    whole = keys // 32 * 32
+    # what the others' rows stand for, as a table of their own
+    full = table.clone()
+    full[first:first + count, :whole // page] = table[at, :whole // page]
+    rest = whole % page
+    for i in range(first, first + count):
+        table[i, :whole // page] = table[at, :whole // page] if i == at else -1
+        if rest and i != at and reqs[i][0]:       # (one without tokens has no such page)
+            page_of, own = full[at, whole // page].long(), full[i, whole // page].long()
+            for c in caches:
+                c[own, :rest] = c[page_of, :rest]
+    step = chunk.ChunkStep(starts, seqs, table, hq, cache, prefixes=prefixes)
+    out = torch.full_like(q, 7.0)
+    chunk.chunk_attention(q, cache, step, d ** -0.5, out=out)
+    if bits == 8:
+        quant.check(out, q, cache, full, starts, seqs, 0, d ** -0.5)
+    else:
+        check(out, q, caches, full, starts, seqs, 0, d ** -0.5, page)
+    # the same, whatever their own pages hold in the prefix' places
+    for i in range(first, first + count):
+        if rest and i != at and reqs[i][0]:       # (one without tokens has no such page)
+            for c in caches:
+                c[full[i, whole // page].long(), :rest] = c[full[at, 0].long(), 1:rest + 1].flip(0)
+    assert torch.equal(out, chunk.chunk_attention(q, cache, step, d ** -0.5))
+    assert torch.equal(out, chunk.chunk_attention(q.clone(), cache, step, d ** -0.5, out=q))
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_hidden_values_of_prompts_that_fill_the_gpu(device, d, bits):
+    """NaN in the prefix reaches all rows of its requests; of a request's own keys those that see
+    them; pages outside the cache are no keys."""
+    from tests import test_gpu_quant_attention as quant
+
+    reqs, prefixes, page, hq, hk = [(1200, 200), (1000, 230), (60, 40)], [(0, 2, 200)], 16, 16, 4
+    g = torch.Generator(device=device).manual_seed(d)
+    if bits == 8:
+        q, cache, table, starts, seqs = quant.make(g, reqs, hq, hk, d, page, torch.bfloat16)
+        values, nan = cache.v_codes, 0x7F
+    else:
+        q, caches, table, starts, seqs = make(g, reqs, hq, hk, d, page, torch.bfloat16)
+        cache, values, nan = append.PagedCache(*caches), caches[1], float("nan")
+    table[0, 3] = -1
+    table[1, :12] = -1
+    step = chunk.ChunkStep(starts, seqs, table, hq, cache, prefixes=prefixes)
+    clean = chunk.chunk_attention(q, cache, step, 0.1)
+    assert clean.isfinite().all()
+    marks = [(0, 5, 1), (0, 191, 2), (1, 300, 3), (0, 1399, 4), (1, 195, 5), (0, 50, 6)]   # request, key, feature
+    touched = torch.zeros_like(clean, dtype=torch.bool)
+    for r, key, feature in marks:
+        if table[r, key // page] < 0:
+            continue
+        values[table[r, key // page].long(), key % page, 1, feature] = nan
+        for i in (0, 1) if key < 192 else (r,):
+            n, h = reqs[i]
+            sees = h + torch.arange(n, device=device) >= key
+            touched[starts[i]:starts[i + 1], 4:8, feature] |= sees[:, None]
+    got = chunk.chunk_attention(q, cache, step, 0.1)
+    assert torch.equal(got.isnan(), touched) and torch.equal(got[~touched], clean[~touched])

@@ -166,3 +166,79 @@ def test_a_step_of_a_bad_count_is_refused():
     h = rotary.HeadsArgs(1 << 20, 8 * 128, 128, 8, 0)
     assert _lib.load().oscar_chunk_attention(ctypes.byref(bad), 1 << 20, 1 << 20, 1000, cache.address, ctypes.byref(h),
                                              ctypes.byref(h), 0.1, 1 << 20, args.workspace_size, None) == -1
+
+
+FULL = [
+    ([(4096, 1024)] * 8, [(0, 8, 1024)]),
+    ([(2048, 64)] * 16, [(0, 16, 64)]),
+    ([(0, 900), (4, 1900), (3, 1930), (3000, 1900), (2, 1905), (0, 9), (4000, 2000), (1, 1900), (5, 2011), (1, 1950),
+      (9, 400), (1, 400)], [(0, 10, 1900), (10, 2, 400)]),
+    ([(4000, 500), (1, 500), (2, 500), (4000, 0), (2, 100), (2, 96)], [(0, 3, 500), (4, 2, 96)]),
+    ([(9256, 32), (9256, 32), (1, 70)], [(0, 3, 32)]),
+]
+
+
+@pytest.mark.parametrize("d, hk, group", [(64, 4, 4), (128, 8, 4), (256, 1, 6)])
+@pytest.mark.parametrize("case", range(len(FULL)))
+def test_prompts_that_fill_the_gpu_share_no_sums(case, d, hk, group):
+    """Each computes the prefix itself, on the first one's pages, and leaves no partials for it;
+    the requests between them share theirs.  Every row meets every key once."""
+    reqs, prefixes = FULL[case]
+    starts, seqs = [0], []
+    for n, h in reqs:
+        starts.append(starts[-1] + n)
+        seqs.append(n + h)
+    narrow_rows = 32
+    full = sum(n * group for n, _ in reqs if n * group > narrow_rows) * hk > 256 * WIDE
+    assert full or case == 2 and hk == 1
+    if not full:
+        return
+    alone = [n * group >= WIDE for n, _ in reqs]
+    args, pieces, joins, parts = plan(starts, seqs, hk * group, prefixes, plain_cache(d=d, hk=hk))
+    head, keys_of, run = {}, {}, {}
+    for first, count, keys in prefixes:
+        members = [i for i in range(first, first + count) if reqs[i][0]]
+        runs = [[]]
+        for i in members:
+            head[i], keys_of[i] = members[0], keys // TILE * TILE
+            if alone[i]:
+                runs.append([])
+            else:
+                runs[-1].append(i)
+        for r in runs:
+            run.update({i: r for i in r if len(r) > 1})
+    met = {}                                # (request, kv head, row0): ranges of keys, by table row
+    slots = set()
+    for i, (token0, pos0, row, kv, row0, rows, key0, key1, slot, head_keys, head_row, pad) in enumerate(pieces):
+        request = max(r for r in range(len(reqs)) if starts[r] <= token0 and reqs[r][0])
+        assert rows <= (NARROW if i < args.narrow else WIDE) and pad == 0
+        if slot >= 0:
+            slots.add(slot)
+        if request in run and key1 <= keys_of[request] and pos0 == keys_of[request] and token0 == starts[run[request][0]]:
+            assert row == head[request] and head_keys == 0 and slot >= 0
+            n = sum(reqs[r][0] for r in run[request])
+            at = ("run", run[request][0], kv, row0)
+            assert rows == min(NARROW if i < args.narrow else WIDE, n * group - row0)
+        else:
+            assert token0 == starts[request] and row == request and pos0 == reqs[request][1]
+            at = (request, kv, row0)
+            if request in head and request not in run and head[request] != request:
+                assert (head_keys, head_row) == (keys_of[request], head[request])
+            else:
+                assert head_keys == 0
+            if alone[request] and args.joins == 0:
+                assert slot < 0
+        met.setdefault(at, []).append((key0, key1))
+    for at, keys in met.items():
+        keys.sort()
+        assert all(a[1] == b[0] for a, b in zip(keys, keys[1:]))
+        if at[0] == "run":
+            assert keys[0][0] == 0 and keys[-1][1] == keys_of[at[1]]
+        else:
+            n, h = reqs[at[0]]
+            assert keys[0][0] == (keys_of[at[0]] if at[0] in run else 0) and keys[-1][1] <= n + h
+    assert {a[:2] for a in met if a[0] != "run"} == {(i, kv) for i, (n, _) in enumerate(reqs) if n for kv in range(hk)}
+    assert sum(a[0] == "run" for a in met) > 0 if run else args.parts == 0
+    # partials: of the requests that share, and a bounded number of others
+    own = sum(-(-reqs[i][0] * group // NARROW) for i in run) * hk
+    assert args.parts == own and (run or args.joins == 0 and args.workspace_size == 0)
