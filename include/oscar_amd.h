@@ -640,7 +640,8 @@ int oscar_append_normed(const oscar_rotary* rotary, const oscar_head_norm* norm,
  * block_size + t) * 2], of V the byte after it.  Base addresses and strides are
  * multiples of 16 bytes and tokens and heads do not overlap; head_size is a multiple
  * of 16, at most 256.  dtype: of the rows that are written and read (bf16 or fp16).  b
- * is 47 to 227 in bf16 and 112 to 135 in fp16, of codes of zero any. */
+ * is 47 to 227 in bf16 and 112 to 135 in fp16 (135 with codes up to 240, which are exact
+ * there), of codes of zero any. */
 typedef struct oscar_quant_cache {
   void* k;
   void* v;
@@ -662,8 +663,8 @@ typedef struct oscar_quant_cache {
  * arguments, keys and values rounded to codes (to nearest, ties to even).  A row's
  * power of two is the smallest, of 2^-80 .. 2^100 (bf16) or 2^-15 .. 2^8 (fp16), with
  * which its largest finite magnitude is at most 448 times it; smaller values than the
- * least power reaches round to zero, larger ones than the greatest reaches become 240
- * times it; infinities and NaN become NaN.  Slots of a call are distinct: of two tokens
+ * least power reaches round to zero; under the greatest, values past 240 times it (2^107.9;
+ * 61440) become that; infinities and NaN become NaN.  Slots of a call are distinct: of two tokens
  * that name one, the row may hold one's codes and the other's power. */
 int oscar_append_quantized(const oscar_rotary* rotary, const oscar_head_norm* norm, const int64_t* positions,
                            int64_t position_axis_stride, int64_t num_tokens, const oscar_heads* query,

@@ -13,9 +13,10 @@
 
 namespace oscar {
 
-// e of bf16 rows: 448 2^100 is short of its largest value; a sum of weights over 2^e,
-// which the attention keeps, stays within fp32.  Of fp16 ones: 2^-9 2^-15 is its own
-// smallest step, and 240 2^8 the largest code below 65504.
+// e of bf16 rows: 2^-80 to 2^100, with which a sum of weights over 2^e, which the attention
+// keeps, stays within fp32.  Of fp16 ones: 2^-9 2^-15 is its own smallest step, and 240 2^8
+// the largest value below 65504, so that codes of the greatest power end at 240 (of bf16
+// ones too: past 240 2^100 = 2^107.9).
 struct ExponentRange {
   int low, high;
 };

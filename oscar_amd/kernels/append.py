@@ -79,10 +79,10 @@ class QuantCache:
     """A layer's 8-bit K and V pages, checked and packed once: codes [pages,
     block_size, Hk, D] (float8_e4m3fn, or their bytes as uint8) that stand for
     code * 2^(b - 127), b the byte at exponents [pages, Hk, block_size, 2] (uint8,
-    contiguous; K's, then V's): 47 to 227 in bf16, 112 to 135 in fp16, of codes of zero
-    any.  dtype (bf16 or fp16) is that of the rows that are written and read; the values
-    are exact in it.  Codes may be views as
-    PagedCache's may; D is a multiple of 16."""
+    contiguous; K's, then V's): 47 to 227 in bf16, 112 to 135 in fp16 (135 with codes up
+    to 240), of codes of zero any.  dtype (bf16 or fp16) is that of the rows that are
+    written and read; the values are exact in it.  Codes may be views as PagedCache's may;
+    D is a multiple of 16."""
 
     def __init__(self, k_codes: torch.Tensor, v_codes: torch.Tensor, exponents: torch.Tensor, dtype: torch.dtype):
         if k_codes.ndim != 4 or k_codes.shape != v_codes.shape or min(k_codes.shape) < 1:
@@ -171,7 +171,8 @@ def append_quantized(query: torch.Tensor | None, key: torch.Tensor, value: torch
     weight, and turned; keys and values rounded to e4m3 codes (to nearest, ties to even)
     times a power of two for each token and head, the smallest with which the row's
     largest finite magnitude is at most 448 times it (2^-80 to 2^100 in bf16, 2^-15 to
-    2^8 in fp16).  What is not finite becomes NaN."""
+    2^8 in fp16; under the greatest, values past 240 times it become that).  What is not
+    finite becomes NaN."""
     if not isinstance(cache, QuantCache):
         raise ValueError("append_quantized writes 8-bit caches (append_rotated and append_normed plain ones)")
     norm = _rotary.pack_norm(query_weight if query is not None else None, key_weight, eps, offset, cache.head_size,
