@@ -22,7 +22,8 @@
 // Measured: one token of 6 + 1 heads of 256 3.8 us; 9256 tokens (66 MB, in the last-level
 // cache) 15.7, 4.2 TB/s; 30843 of 32 + 8 heads of 128 110 (632 MB, 5.7 TB/s), their
 // gradient 181 (947 MB, 5.2 TB/s) and the weights' sums 6.9; the write of 65536 tokens of
-// 6 + 1 + 1 heads of 256 to 8 bits 115 (503 MB, 4.4 TB/s).
+// 6 + 1 + 1 heads of 256 to 8 bits 115 (503 MB, 4.4 TB/s), to plain pages 125 (537 MB, 4.3
+// TB/s; turned alone 103).
 #include "plain_cache.h"
 #include "quant_cache.h"
 #include "row_span.h"
@@ -102,7 +103,8 @@ __device__ __forceinline__ float group_max(float x, int lanes) {
 
 // A lane's part of a head: kSlots places, each two pieces of kVec features in the order
 // of memory.  kVec is 8 where rows, strides and pairs are multiples of 16 bytes, else 1
-// (a model's head size and projection decide).  Pairs that turn together are both of one
+// (a model's head size and projection decide: 65536 tokens of 6 + 1 heads of 256 111 us in
+// pieces, 177 off 16 bytes or with rotary_dim 56, 2.65 TB/s; one token 3.9, 4.4).  Pairs that turn together are both of one
 // lane: the pieces' features of one index, or, where pairs are adjacent and kVec is 8,
 // neighbours in a piece.
 template <int kVec>
