@@ -664,8 +664,8 @@ typedef struct oscar_quant_cache {
  * power of two is the smallest, of 2^-80 .. 2^100 (bf16) or 2^-15 .. 2^8 (fp16), with
  * which its largest finite magnitude is at most 448 times it; smaller values than the
  * least power reaches round to zero; under the greatest, values past 240 times it (2^107.9;
- * 61440) become that; infinities and NaN become NaN.  Slots of a call are distinct: of two tokens
- * that name one, the row may hold one's codes and the other's power. */
+ * 61440) become that; infinities and NaN become NaN.  Slots of a call are distinct: of two
+ * tokens that name one, the row may hold one's codes and the other's power. */
 int oscar_append_quantized(const oscar_rotary* rotary, const oscar_head_norm* norm, const int64_t* positions,
                            int64_t position_axis_stride, int64_t num_tokens, const oscar_heads* query,
                            const oscar_heads* query_out, const oscar_heads* key, const oscar_heads* value,
@@ -723,8 +723,8 @@ typedef struct oscar_chunk_step {
 
 /* Keys [0, keys) that requests first .. first + requests - 1 of a step begin with, on
  * pages that hold the same: they are read from the block table row of the first of them
- * that has tokens and computed once for the rows of all, but for prompts that fill the GPU
- * by themselves (they would only gain partials). */
+ * that has tokens and computed once for the rows of all, but for those of long requests in a
+ * step that fills the GPU (they would only gain partials). */
 typedef struct oscar_prefix {
   int32_t first;
   int32_t requests;

@@ -428,16 +428,17 @@ __device__ __forceinline__ uint8_t* out_row(const ChunkArgs& a, int token0, int 
   return a.out + (int64_t)(token0 + tok) * a.out_token + (int64_t)head * a.out_head;
 }
 
-// What a partial's sums are multiplied by as its maximum is raised by `up` (0 or less: from
-// the new one to its own): `all`, its products, and sum_of(l) its weights.  kPowers: the
+// What sums held to one maximum are multiplied by when they are held to a larger one, `down`
+// (0 or less) from it: products by `all`, and a sum of weights as add() does it.  kPowers: the
 // maximum goes with values' powers of two (the 8-bit cache), of which the weights' sum has
 // the inverse, up to 2^80 for a key: where the factor alone is below fp32's smallest,
 // their product need not be, so it is applied by halves.
 template <bool kPowers>
 struct Lowered {
   float half, all;
-  __device__ __forceinline__ explicit Lowered(float up)
-      : half(kPowers ? __builtin_amdgcn_exp2f(0.5f * up) : 1.f), all(kPowers ? half * half : __builtin_amdgcn_exp2f(up)) {}
+  __device__ __forceinline__ explicit Lowered(float down)
+      : half(kPowers ? __builtin_amdgcn_exp2f(0.5f * down) : 1.f),
+        all(kPowers ? half * half : __builtin_amdgcn_exp2f(down)) {}
   __device__ __forceinline__ float add(float to, float l) const {
     if constexpr (kPowers) return to + half * (half * l);
     return to + all * l;

@@ -171,7 +171,8 @@ int32_t pieces_of(const RowTile& x, int64_t per) { return (int32_t)((x.tiles + p
 // 8 kv heads, 195 / 107, 128 users 291 / 203, 4 tokens of 128 users, D = 64, 4 heads,
 // 155 / 84; 256 over 100 to 8000, D = 256, 175 / 103; 300 over 1000 and one over 60000
 // 954 / 90, 508 over 1000 and one 257 / 76, 490 77 / 75; 62 and one of 8 heads, D = 128, 328 /
-// 57; 168 and one beside a prompt of 1200 482 / 56; without the second condition 256 over 100 to 800 27 / 32.
+// 57; 168 and one beside a prompt of 1200 482 / 56; without the second condition 256 over 100
+// to 800 27 / 32.
 constexpr int32_t kMuchLonger = 32;
 void plan_narrow(const std::vector<RowTile>& rows, const PlanRule& rule, double beside, Plan& plan,
                  std::vector<PrefixRows>& prefixes) {
@@ -280,17 +281,21 @@ double plan_wide(const std::vector<RowTile>& rows, int32_t head_size, Plan& plan
   return best;
 }
 
-// A prefix' requests that fill wide pieces compute its keys themselves, from the first one's
-// table row, where the step has rows for more of those than there are CUs: they are not cut
-// then and bound by the matrix unit, which has the same products to do either way, and
-// sharing would only add partials, to write, read and hold.  Shared / each for itself, us:
-// 8 prompts of 4096 tokens over 1024 keys, 32 heads of 128 on 8, 1933 and 1.09 GB of
-// partials / 1577 and none; 16 of 2048 over 64 1032 / 660; 8 of 300 over 960 79 / 64; 8 of 1200
-// over 4096, 6 heads of 256 on one, 273 / 248; of the 8-bit cache (the keys converted once
-// for all) 32 of 64 over 4096 167 / 145.  With fewer rows they are cut in any case: 8 of 128
-// over 8192 150 / 155, 4 of 512 over 24576, D = 256, 284 / 308, 8 of 300 over 1024 50 / 44; rows
-// that fill no wide tile fill them together: 128 of 10 over 1024 54 / 76, over 64 37 / 17.
-// The requests between them are computed together, as far as they follow each other.
+// Where a step has rows for a wide piece a CU, its row tiles are not cut and the matrix unit
+// bounds them.  Of a prefix it then has the same products to do either way, but for the rows
+// that a request's last tile lacks, which the prefix' tiles have; sharing costs partials, of
+// the prefix and of the request's own keys: 16 (D + 2) bytes a row, written and read, take as
+// long at 5 TB/s as 4 D flops a key of 800 keys at 1 PFLOP/s.  So a request whose idle rows
+// times the prefix' keys are less than 800 times its rows computes them itself, from the first
+// one's table row.  Shared / each for itself, us: 8 prompts of 4096 tokens over 1024 keys, 32
+// heads of 128 on 8, 1933 and 1.09 GB of partials / 1571 and none; 16 of 2048 over 64 1032 /
+// 660; 8 of 300 over 960 79 / 65; 32 of 32 over 64 24 / 10.5, over 1024 41 / 29; 128 of 16
+// over 64 44 / 21, but over 1024 72 / 81; 128 of 10 over 1024 55 / 79; 8 of 1200 over 4096, 6
+// heads of 256 on one, 273 / 254; of the 8-bit cache (the keys converted once for all) 32 of 64
+// over 4096 167 / 146.  With fewer rows tiles are cut in any case: 4 of 512 over 24576, D =
+// 256, 292 / 305, 8 of 300 over 1024 52 / 45, 16 of 16 over 8192, D = 128, 52 / 73.
+// The requests between such are computed together, as far as they follow each other.
+constexpr int64_t kKeysOfPartial = 800;
 void make_plan(const int32_t* qsl, const int32_t* seqs, int32_t num_requests, int32_t group, int32_t kv_heads,
                const PlanRule& rule, int32_t window, const std::vector<Prefix>& shared, Plan& plan) {
   std::vector<RowTile> narrow, wide;
@@ -300,12 +305,13 @@ void make_plan(const int32_t* qsl, const int32_t* seqs, int32_t num_requests, in
   if (!shared.empty())
     for (int32_t i = 0; i < num_requests; ++i)
       if (rows_of(i) > rule.narrow_rows) wide_rows += rows_of(i) * kv_heads;
-  auto alone = [&](int32_t i) {
-    return wide_rows > (int64_t)kCus * kWideRows && rows_of(i) > rule.narrow_rows && rows_of(i) >= kWideRows;
-  };
   auto prefix = shared.begin();
   OfPrefix of;                              // the prefix that request i begins with,
   int32_t until = 0, together = 0, first_token = 0;    // and its requests up to `together` that share it
+  auto alone = [&](int32_t i) {
+    const int64_t rows = rows_of(i), idle = (kWideRows - rows % kWideRows) % kWideRows;
+    return wide_rows >= (int64_t)kCus * kWideRows && rows > rule.narrow_rows && of.keys * idle < kKeysOfPartial * rows;
+  };
   for (int32_t i = 0; i < num_requests; ++i) {
     const int32_t n = qsl[i + 1] - qsl[i];
     if (i >= until) of = OfPrefix{};

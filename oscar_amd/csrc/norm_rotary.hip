@@ -104,9 +104,9 @@ __device__ __forceinline__ float group_max(float x, int lanes) {
 // A lane's part of a head: kSlots places, each two pieces of kVec features in the order
 // of memory.  kVec is 8 where rows, strides and pairs are multiples of 16 bytes, else 1
 // (a model's head size and projection decide: 65536 tokens of 6 + 1 heads of 256 111 us in
-// pieces, 177 off 16 bytes or with rotary_dim 56, 2.65 TB/s; one token 3.9, 4.4).  Pairs that turn together are both of one
-// lane: the pieces' features of one index, or, where pairs are adjacent and kVec is 8,
-// neighbours in a piece.
+// pieces, 177 off 16 bytes or with rotary_dim 56, 2.65 TB/s; one token 3.9, 4.4).  Pairs
+// that turn together are both of one lane: the pieces' features of one index, or, where pairs
+// are adjacent and kVec is 8, neighbours in a piece.
 template <int kVec>
 struct Part {
   static constexpr int kSlots = kVec == 8 ? 1 : 2, kPairs = kSlots * kVec;

@@ -11,8 +11,9 @@
 // m the running maximum of x_t + b_t, so that the weights that are rounded for the
 // product are the ones whose size counts, whatever the powers.  The sum below is of fp32
 // weights, not of the rounded ones as over 16-bit pages: those go with 2^b, and keys whose
-// values are far below the heaviest's, rows of zeros too, would be missing from it.  Numerators and sums of pieces relate by 2^m as those over 16-bit pages do,
-// and the same launch joins them.
+// values are far below the heaviest's, rows of zeros too, would be missing from it.
+// Numerators and sums of pieces relate by 2^m as those over 16-bit pages do, and the same
+// launch joins them.
 //
 // Requests of more rows are bounded by the matrix unit, which would wait for the
 // conversions that each of a tile's four waves makes for itself.  Their keys are

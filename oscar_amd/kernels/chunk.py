@@ -50,9 +50,9 @@ class ChunkStep:
     prefixes: (first, requests, keys) of groups of requests, one after the other in the
     step, whose first `keys` keys are the same and come before each one's own tokens (a
     system prompt, samples of one prompt).  They are read from the pages of the group's
-    first request that has tokens, and computed once for all its rows, but for prompts
-    that fill the GPU by themselves; results are within rounding of a step without them.
-    They do not go with a window.
+    first request that has tokens, and computed once for all its rows, but for those of
+    long requests in a step that fills the GPU; results are within rounding of a step
+    without them.  They do not go with a window.
 
     Building copies the step's arrays to the device on the current stream; calls
     on other streams wait for that by themselves.  A step is not built under graph

@@ -175,25 +175,28 @@ FULL = [
       (9, 400), (1, 400)], [(0, 10, 1900), (10, 2, 400)]),
     ([(4000, 500), (1, 500), (2, 500), (4000, 0), (2, 100), (2, 96)], [(0, 3, 500), (4, 2, 96)]),
     ([(9256, 32), (9256, 32), (1, 70)], [(0, 3, 32)]),
+    ([(10, 64)] * 128 + [(2000, 500)] * 6, [(0, 128, 64)]),
+    ([(10, 4096)] * 128 + [(2000, 500)] * 6, [(0, 128, 4096)]),
 ]
 
 
 @pytest.mark.parametrize("d, hk, group", [(64, 4, 4), (128, 8, 4), (256, 1, 6)])
 @pytest.mark.parametrize("case", range(len(FULL)))
 def test_prompts_that_fill_the_gpu_share_no_sums(case, d, hk, group):
-    """Each computes the prefix itself, on the first one's pages, and leaves no partials for it;
-    the requests between them share theirs.  Every row meets every key once."""
+    """Those that gain nothing by sharing compute the prefix themselves, on the first one's pages,
+    and leave no partials for it; the requests between them share theirs.  Every row meets every
+    key once."""
     reqs, prefixes = FULL[case]
     starts, seqs = [0], []
     for n, h in reqs:
         starts.append(starts[-1] + n)
         seqs.append(n + h)
     narrow_rows = 32
-    full = sum(n * group for n, _ in reqs if n * group > narrow_rows) * hk > 256 * WIDE
-    assert full or case == 2 and hk == 1
-    if not full:
-        return
-    alone = [n * group >= WIDE for n, _ in reqs]
+    assert sum(n * group for n, _ in reqs if n * group > narrow_rows) * hk >= 256 * WIDE
+    alone = []
+    for i, (n, _) in enumerate(reqs):
+        keys = sum(k // TILE * TILE for first, count, k in prefixes if first <= i < first + count)
+        alone.append(n * group > narrow_rows and keys * (-n * group % WIDE) < 800 * n * group)
     args, pieces, joins, parts = plan(starts, seqs, hk * group, prefixes, plain_cache(d=d, hk=hk))
     head, keys_of, run = {}, {}, {}
     for first, count, keys in prefixes:
